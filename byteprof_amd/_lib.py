@@ -100,6 +100,14 @@ SIGNATURES: dict[str, tuple] = {
     "bp_decode_argmax_rows_scratch_bytes": (_c_size, [_c_int]),
     "bp_decode_argmax_rows": (_c_int, [_c_vp, _c_int, _c_int, _c_vp, _c_vp, _c_vp]),
     "bp_draft_verify_next": (_c_int, [_c_vp, _c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_vp]),
+    "bp_attn_workspace_bytes": (_c_size, [_c_i64] * 6),
+    "bp_attn_packed": (_c_int, [_c_int] + [_c_vp] * 5 + [_c_int] * 5 + [_c_i64] * 6 + [_c_int, _c_float, _c_vp, _c_size,
+                                                                                       _c_vp]),
+    "bp_attn_paged": (_c_int, [_c_int] + [_c_vp] * 5 + [_c_i64, _c_vp, _c_vp] + [_c_int] * 8 + [_c_i64] * 8 +
+                      [_c_float, _c_vp, _c_size, _c_vp]),
+    "bp_paged_append": (_c_int, [_c_int] + [_c_vp] * 5 + [_c_i64, _c_vp, _c_vp] + [_c_int] * 7 + [_c_i64] * 10 + [_c_vp]),
+    "bp_logprobs_workspace_bytes": (_c_size, [_c_int, _c_i64, _c_i64, _c_int]),
+    "bp_logprobs": (_c_int, [_c_int, _c_vp, _c_i64] + [_c_vp] * 5 + [_c_i64, _c_i64, _c_int, _c_vp, _c_size, _c_vp]),
 }
 
 _LIB: ctypes.CDLL | None = None

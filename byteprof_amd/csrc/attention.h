@@ -1,0 +1,321 @@
+// Attention of several sequences at once: the plan of a launch, which every workgroup makes for itself from the device's
+// offsets and lengths, and the pieces of the kernels that do not depend on where a key lies.
+//
+//   out[i, h] = sum_j p_ij v[j, h / group],  p_i = softmax_j(scale q[i, h] . k[j, h / group]),  j <= limit(i)
+//
+// The rows of a product are (token, query head of the group) pairs of one key head, token-major: row r of a sequence is
+// token r / group, head r % group of the group, so the heads that share keys share the loads of them. The scores are
+// computed transposed, S^T = K Q^T (32 keys x 32 rows a matrix instruction): a lane then holds scores of one row only, its
+// maximum, sum and rescaling are scalars of the lane, and the probabilities, rounded to the tensors' type, are the second
+// product's operand where they lie (O^T = V^T P^T; its key order is the order in which the first product leaves them).
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "common.h"
+
+namespace bp {
+namespace attn {
+
+constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / kWave;
+constexpr int kSmallRows = 64;   // sequences of at most this many rows: 32-row tiles whose waves share the keys
+constexpr int kTileSmall = 32;
+constexpr int kTileLarge = 128;  // 32 rows a wave, all keys
+constexpr int kKeyStep = 128;    // a split's keys are a multiple of this: whole steps of either kind of tile
+
+struct Args {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* out;           // [tokens, hq, d], contiguous
+  const int* cu;       // [seqs + 1]
+  const int* lengths;  // [seqs], or null: as many keys as tokens (packed)
+  const int* table;    // [seqs, max_pages], or null
+  float* ws;           // partials of split tiles, or null: nothing is split
+  int64_t q_t, q_h;            // element strides
+  int64_t k_p, k_t, k_h;       // page (paged), position, head
+  int64_t v_p, v_t, v_h;
+  int64_t table_stride;
+  int tokens, seqs, pool, page, page_shift, max_keys, hq, hk, group, d, causal;
+  int target;     // tiles that splitting aims at
+  int chunk_min;  // least keys of a split
+  int ws_rows;    // rows of a partial's slot
+  int slots;      // slots that ws holds
+  float scale_log2;
+};
+
+// What a sequence asks for.
+struct Seq {
+  int begin, rows, keys, tiles;
+};
+
+__device__ __forceinline__ Seq sequence(const Args& a, int b) {
+  Seq s;
+  s.begin = min(max(a.cu[b], 0), a.tokens);
+  const int end = min(max(a.cu[b + 1], s.begin), a.tokens);
+  s.rows = (end - s.begin) * a.group;
+  s.keys = a.lengths ? min(max(a.lengths[b], 0), a.max_keys) : end - s.begin;
+  s.tiles = s.rows <= kSmallRows ? (s.rows + kTileSmall - 1) / kTileSmall : (s.rows + kTileLarge - 1) / kTileLarge;
+  return s;
+}
+
+// Keys of a split: the whole work in keys x tiles over the tiles that splitting aims at, never under chunk_min. Every
+// workgroup adds the same numbers in the same order, so all of them find the same value.
+__device__ __forceinline__ int split_keys(const Args& a, int lane) {
+  if (a.ws == nullptr) return 0x40000000;
+  float units = 0.f;
+  for (int b = lane; b < a.seqs; b += kWave) {
+    const Seq s = sequence(a, b);
+    units += static_cast<float>(s.tiles) * static_cast<float>(s.keys);
+  }
+  units = xor_butterfly<true>(units, AddOp());
+  const float want = units * static_cast<float>(a.hk) / static_cast<float>(a.target) * 1.001f;
+  const int chunk = want < 1e9f ? static_cast<int>(want) + 1 : 0x3fffff00;
+  return (max(chunk, a.chunk_min) + kKeyStep - 1) / kKeyStep * kKeyStep;
+}
+
+__device__ __forceinline__ int scan_add(int v, int lane) {
+#pragma unroll
+  for (int o = 1; o < kWave; o <<= 1) {
+    const int u = __shfl_up(v, o);
+    if (lane >= o) v += u;
+  }
+  return v;
+}
+
+// One workgroup's part: `rows` rows from row0 of sequence b, key range [key0, key1) of split `split`. divided: the tile's
+// parts go to slots from `slot` on (a tile of fewer keys than its sequence leaves the last of them unwritten; its first it
+// always writes). b < 0: beyond the last tile, `extra` tiles past it.
+struct Item {
+  int b, begin, row0, rows, seq_rows, keys, first, key0, key1, split, splits, slot, extra;
+  bool small, divided;
+};
+
+// The tile of index `index` (per key head). merge: indices count the tiles alone, without their splits.
+__device__ __forceinline__ Item find_item(const Args& a, int index, bool merge) {
+  const int lane = static_cast<int>(threadIdx.x) & 63;
+  const int chunk = split_keys(a, lane);
+  Item it;
+  it.b = -1;
+  int items = 0, slots = 0;
+  for (int b0 = 0; b0 < a.seqs; b0 += kWave) {
+    const int b = b0 + lane;
+    Seq s = {0, 0, 0, 0};
+    if (b < a.seqs) s = sequence(a, b);
+    const int splits = max(1, (s.keys + chunk - 1) / chunk);
+    const int count = s.tiles * (merge ? 1 : splits);
+    const int parts = splits > 1 ? s.tiles * splits : 0;
+    const int upto = scan_add(count, lane), slot_upto = scan_add(parts, lane);
+    const uint64_t over = __ballot(items + upto > index);
+    if (over != 0) {
+      const int l = __builtin_ctzll(over);
+      const int tiles = __builtin_amdgcn_readlane(s.tiles, l);
+      const int at = index - items - __builtin_amdgcn_readlane(upto - count, l);
+      it.b = b0 + l;
+      it.begin = __builtin_amdgcn_readlane(s.begin, l);
+      it.seq_rows = __builtin_amdgcn_readlane(s.rows, l);
+      it.keys = __builtin_amdgcn_readlane(s.keys, l);
+      it.splits = __builtin_amdgcn_readlane(splits, l);
+      const int per = merge ? 1 : it.splits;
+      // the last rows first: under a causal mask they have the most keys
+      const int tile = tiles - 1 - at / per;
+      it.split = at % per;
+      it.divided = it.splits > 1;
+      it.slot = slots + __builtin_amdgcn_readlane(slot_upto - parts, l) + tile * it.splits;
+      it.small = it.seq_rows <= kSmallRows;
+      const int tile_rows = it.small ? kTileSmall : kTileLarge;
+      it.row0 = tile * tile_rows;
+      it.rows = min(tile_rows, it.seq_rows - it.row0);
+      it.first = it.keys - it.seq_rows / a.group;  // the key position of token 0
+      const int last = (it.row0 + it.rows - 1) / a.group;
+      const int end = a.causal ? min(it.keys, max(0, it.first + last + 1)) : it.keys;
+      it.key0 = min(end, it.split * min(chunk, 0x3fffffff));
+      it.key1 = min(end, it.key0 + chunk);
+      if (merge) {
+        it.key0 = 0;
+        it.key1 = end;
+        it.splits = max(1, (end + chunk - 1) / chunk);  // those that had keys
+      }
+      return it;
+    }
+    items += __builtin_amdgcn_readlane(upto, 63);
+    slots += __builtin_amdgcn_readlane(slot_upto, 63);
+  }
+  it.extra = index - items;
+  return it;
+}
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+
+struct Bf16 {
+  static __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ uint32_t pack(float x, float y) {
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2){x, y}, bf16x2));
+  }
+};
+struct F16 {
+  static __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ uint32_t pack(float x, float y) {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, (h2){static_cast<_Float16>(x), static_cast<_Float16>(y)});
+  }
+};
+
+// LDS images of key and value rows: [row][DP / 8] chunks of 16 bytes, the chunk of a row at a place that the row turns, so
+// that 16 rows' equal chunks (the first product's operand) or 4 rows' 64 bytes (the second's) lie in different banks.
+// Chunks past the head's own d / 8 are never loaded; they are zeroed once.
+template <int DP>
+__device__ __forceinline__ int k_place(int row, int chunk) {
+  constexpr int CH = DP / 8;
+  if constexpr (CH == 8) return row * CH + (chunk ^ ((row >> 1) & 7));
+  else if constexpr (CH == 12) return row * CH + (chunk ^ ((row >> 2) & 3));
+  else return row * CH + (chunk ^ (row & 15));
+}
+template <int DP>
+__device__ __forceinline__ int v_place(int row, int chunk) {
+  constexpr int CH = DP / 8;
+  if constexpr (CH == 8) return row * CH + (chunk ^ (4 * ((row >> 1) & 1)));
+  else if constexpr (CH == 12) return row * CH + chunk;
+  else return row * CH + (chunk ^ (4 * (row & 3)));
+}
+// Chunk that lies at `place` of a row (the turns are their own inverses).
+template <int DP, bool V>
+__device__ __forceinline__ int chunk_at(int row, int place) {
+  constexpr int CH = DP / 8;
+  return (V ? v_place<DP>(row, place) : k_place<DP>(row, place)) - row * CH;
+}
+
+// 16 bytes per active lane from `src` to LDS at base + 16 x lane (base: wave-uniform byte address), without a register.
+// (m0 is the compiler's only between instructions that it emits together.) Counted by vmcnt: the wave waits with wait_vm before it, or after a barrier another wave, reads them.
+__device__ __forceinline__ void load_lds16(const void* src, uint32_t base) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(base), "v"(src) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void wait_vm() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
+      (__attribute__((address_space(3))) const void*)(p)));
+}
+
+// S^T of 32 keys x 32 rows over DP / 16 steps: K rows from an LDS image, Q from registers.
+template <class T, int DP>
+__device__ __forceinline__ f32x16 scores(const u32x4* kimg, int row0, const u32x4 (&q)[DP / 16], int lane) {
+  f32x16 s = {};
+  const int row = row0 + (lane & 31), half = lane >> 5;
+#pragma unroll
+  for (int i = 0; i < DP / 16; ++i) s = T::mfma(kimg[k_place<DP>(row, 2 * i + half)], q[i], s);
+  return s;
+}
+
+// O^T += V^T P^T over 32 keys whose probabilities are p (16 per lane, in the order of the scores).
+template <class T, int DP>
+__device__ __forceinline__ void weighted(const u32x4* vimg, int row0, const u32x4 (&p)[2], f32x16 (&o)[DP / 32], int lane) {
+  typedef __attribute__((address_space(3))) s16x4* lds4;
+  const int half = lane >> 5, sub = (lane >> 4) & 1, j = (lane & 15) >> 2, e = lane & 3;
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db) {
+      u32x4 a;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        // a 16-lane group reads 4 keys x 16 columns, 4 columns a lane, and gets them transposed: its column's 4 keys
+        const int key = row0 + 16 * t + 8 * u + 4 * half + j;
+        const int place = v_place<DP>(key, 4 * db + 2 * sub + (e >> 1));
+        const char* at = reinterpret_cast<const char*>(vimg + place) + 8 * (e & 1);
+        const s16x4 r = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(__attribute__((address_space(3))) void*)at);
+        const u32x2 w = __builtin_bit_cast(u32x2, r);
+        a[2 * u] = w[0];
+        a[2 * u + 1] = w[1];
+      }
+      o[db] = T::mfma(a, p[t], o[db]);
+    }
+  }
+}
+
+__device__ __forceinline__ float max_halves(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float add_halves(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// The running softmax of one row (both halves of a wave hold the row's maximum; each its own part of the sum).
+template <int DP>
+struct Running {
+  f32x16 o[DP / 32];
+  float m, l;
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i) o[i] = f32x16{};
+    m = -INFINITY;
+    l = 0.f;
+  }
+};
+
+// One step over NB x 32 keys from position key0: masks past the row's limit, the new maximum, the probabilities.
+template <class T, int DP, int NB>
+__device__ __forceinline__ void softmax_step(f32x16 (&s)[NB], u32x4 (&p)[NB][2], Running<DP>& r, float c, int key0, int limit,
+                                             bool mask, int lane) {
+  if (mask) {
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int key = key0 + 32 * b + 8 * (i / 4) + 4 * (lane >> 5) + i % 4;
+        if (key > limit) s[b][i] = -INFINITY;
+      }
+  }
+  float mx = s[0][0];
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[b][i]);
+  mx = max_halves(mx) * c;
+  const float m = fmaxf(r.m, mx);
+  if (__any(m > r.m)) {
+    // exp2(-inf - m) = 0 clears a row's empty start; a row that has seen nothing keeps m = -inf and scales by 1
+    const float f = m == r.m ? 1.f : __builtin_amdgcn_exp2f(r.m - m);
+    r.m = m;
+    r.l *= f;
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) r.o[d][i] *= f;
+  }
+  const float shift = r.m == -INFINITY ? 0.f : -r.m;
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      s[b][i] = __builtin_amdgcn_exp2f(fmaf(s[b][i], c, shift));
+      r.l += s[b][i];
+    }
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p[b][t][i] = T::pack(s[b][8 * t + 2 * i], s[b][8 * t + 2 * i + 1]);
+}
+
+}  // namespace attn
+}  // namespace bp

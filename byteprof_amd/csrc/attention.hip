@@ -1,0 +1,577 @@
+// Attention of packed prompts and of chunks over a paged cache, and the append to the cache's pages (attention.h: the
+// mathematics and the plan).
+
+#include "attention.h"
+
+#include "byteprof_amd.h"
+
+namespace bp {
+namespace attn {
+namespace {
+
+template <int DP>
+struct Shape {
+  static constexpr int CH = DP / 8;
+  static constexpr int NB = DP <= 128 ? 2 : 1;   // 32-key blocks of a step of a large tile
+  static constexpr int BN = 32 * NB;
+  static constexpr int kLarge = 4 * BN * CH;     // 16-byte chunks: two images of keys and two of values
+  static constexpr bool kShare = DP > 128;       // small tiles: a wave's keys and values take turns in one image
+  static constexpr int kSmall = kWaves * (kShare ? 1 : 2) * 32 * CH;
+  static constexpr int G = DP / 32 < 4 ? DP / 32 : 4;  // 32-column blocks of a round of the waves' merge
+  static constexpr int kMerge = kWaves * G * 8 * 32;
+  static constexpr int kChunks = kLarge > kSmall ? (kLarge > kMerge ? kLarge : kMerge) : (kSmall > kMerge ? kSmall : kMerge);
+};
+
+// Where the keys and values of an item lie.
+template <bool PAGED>
+struct Source {
+  const uint16_t* k;
+  const uint16_t* v;
+  int64_t k_p, k_t, v_p, v_t;
+  const int* pages;
+  int pool, page, page_shift;
+  bool bad;  // a page outside the pool: the item's rows become NaN
+
+  __device__ __forceinline__ Source(const Args& a, const Item& it, int kvh) {
+    const int64_t from = PAGED ? 0 : it.begin;
+    k = static_cast<const uint16_t*>(a.k) + kvh * a.k_h + from * a.k_t;
+    v = static_cast<const uint16_t*>(a.v) + kvh * a.v_h + from * a.v_t;
+    k_p = a.k_p;
+    k_t = a.k_t;
+    v_p = a.v_p;
+    v_t = a.v_t;
+    pages = PAGED ? a.table + static_cast<int64_t>(it.b) * a.table_stride : nullptr;
+    pool = a.pool;
+    page = a.page;
+    page_shift = a.page_shift;
+    bad = false;
+  }
+  // Element offsets of a key's row.
+  __device__ __forceinline__ void at(int key, int64_t& ko, int64_t& vo) {
+    if constexpr (PAGED) {
+      const int n = page_shift >= 0 ? key >> page_shift : key / page;
+      const int slot = key - n * page;
+      int id = pages[n];
+      if (static_cast<unsigned>(id) >= static_cast<unsigned>(pool)) {
+        bad = true;
+        id = 0;
+      }
+      ko = id * k_p + slot * k_t;
+      vo = id * v_p + slot * v_t;
+    } else {
+      ko = key * k_t;
+      vo = key * v_t;
+    }
+  }
+};
+
+// Loads ROWS rows (keys from key0, those past `last` as the row of `last`) with `threads` threads from thread `me`.
+template <int DP, int ROWS, int THREADS, bool K, bool V, bool PAGED>
+__device__ __forceinline__ void load_rows(Source<PAGED>& src, const u32x4* kimg, const u32x4* vimg, int key0, int last, int chunks,
+                                          int me) {
+  constexpr int CH = DP / 8;
+  static_assert(ROWS * CH % THREADS == 0, "whole loads");
+#pragma unroll
+  for (int i = 0; i < ROWS * CH / THREADS; ++i) {
+    const int idx = i * THREADS + me, row = idx / CH, place = idx % CH;
+    int64_t ko, vo;
+    src.at(min(key0 + row, last), ko, vo);
+    const int first = __builtin_amdgcn_readfirstlane(idx);
+    if constexpr (K) {
+      const int c = chunk_at<DP, false>(row, place);
+      if (c < chunks) load_lds16(src.k + ko + 8 * c, __builtin_amdgcn_readfirstlane(lds_address(kimg)) + 16 * first);
+    }
+    if constexpr (V) {
+      const int c = chunk_at<DP, true>(row, place);
+      if (c < chunks) load_lds16(src.v + vo + 8 * c, __builtin_amdgcn_readfirstlane(lds_address(vimg)) + 16 * first);
+    }
+  }
+}
+
+// Rows that belong to no sequence: zeros, dealt to the workgroups past the last tile.
+__device__ void fill_rest(const Args& a, int kvh, int extra, int extras) {
+  const int lo = a.seqs > 0 ? min(max(a.cu[0], 0), a.tokens) : a.tokens;
+  int hi = a.seqs > 0 ? min(max(a.cu[a.seqs], lo), a.tokens) : a.tokens;
+  const int64_t rest = lo + (a.tokens - hi), per = static_cast<int64_t>(a.group) * a.d / 8;
+  for (int64_t i = static_cast<int64_t>(extra) * kThreads + threadIdx.x; i < rest * per;
+       i += static_cast<int64_t>(extras) * kThreads) {
+    const int64_t n = i / per, c = i % per;
+    const int64_t tok = n < lo ? n : hi + (n - lo);
+    uint16_t* at = static_cast<uint16_t*>(a.out) + (tok * a.hq + static_cast<int64_t>(kvh) * a.group) * a.d + 8 * c;
+    *reinterpret_cast<u32x4*>(at) = u32x4{};
+  }
+}
+
+__device__ __forceinline__ uint16_t* out_row(const Args& a, const Item& it, int kvh, int row) {
+  const int64_t tok = it.begin + row / a.group;
+  return static_cast<uint16_t*>(a.out) + (tok * a.hq + static_cast<int64_t>(kvh) * a.group + row % a.group) * a.d;
+}
+
+// A split's slot: [ws_rows][DP] sums, then ws_rows maxima and ws_rows sums of probabilities.
+template <int DP>
+__device__ __forceinline__ float* slot_at(const Args& a, int64_t slot, int kvh) {
+  return a.ws + (slot * a.hk + kvh) * a.ws_rows * (DP + 2);
+}
+
+template <class T, int DP, bool PAGED>
+__device__ __forceinline__ void load_q(const Args& a, const Item& it, int kvh, int row, u32x4 (&q)[DP / 16], int lane) {
+  const int64_t tok = it.begin + row / a.group;
+  const uint16_t* p = static_cast<const uint16_t*>(a.q) + tok * a.q_t + (static_cast<int64_t>(kvh) * a.group + row % a.group) * a.q_h;
+#pragma unroll
+  for (int i = 0; i < DP / 16; ++i) {
+    const int c = 2 * i + (lane >> 5);
+    q[i] = 8 * c < a.d ? *reinterpret_cast<const u32x4*>(p + 8 * c) : u32x4{};
+  }
+}
+
+__device__ __forceinline__ float inverse(float l) { return l == 0.f ? 0.f : 1.f / l; }
+
+// 128 rows, 32 a wave; the keys in steps of BN that all waves share in LDS, two images of each in turn.
+template <class T, int DP, bool PAGED>
+__device__ __forceinline__ void large_tile(const Args& a, const Item& it, int kvh, u32x4* smem) {
+  using S = Shape<DP>;
+  constexpr int BN = S::BN, NB = S::NB, IMG = BN * S::CH;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int top = it.row0 + it.rows - 1;
+  const int row = it.row0 + 32 * wave + (lane & 31);
+  const int mine = min(row, top);
+  const bool active = it.row0 + 32 * wave <= top;
+  u32x4 q[DP / 16];
+  load_q<T, DP, PAGED>(a, it, kvh, mine, q, lane);
+  const int limit = a.causal ? min(it.first + mine / a.group, it.keys - 1) : it.keys - 1;
+  const int least = __builtin_amdgcn_readfirstlane(limit), most = __builtin_amdgcn_readlane(limit, 31);
+  Running<DP> r;
+  r.clear();
+  Source<PAGED> src(a, it, kvh);
+  const int chunks = a.d / 8, last = it.key1 - 1;
+  int buf = 0;
+  if (it.key0 < it.key1)
+    load_rows<DP, BN, kThreads, true, true>(src, smem, smem + 2 * IMG, it.key0, last, chunks, tid);
+  for (int key = it.key0; key < it.key1; key += BN) {
+    wait_vm<0>();
+    __syncthreads();
+    if (key + BN < it.key1)
+      load_rows<DP, BN, kThreads, true, true>(src, smem + (buf ^ 1) * IMG, smem + (2 + (buf ^ 1)) * IMG, key + BN, last, chunks, tid);
+    if (active && key <= most) {
+      f32x16 s[NB];
+      u32x4 p[NB][2];
+#pragma unroll
+      for (int b = 0; b < NB; ++b) s[b] = scores<T, DP>(smem + buf * IMG, 32 * b, q, lane);
+      softmax_step<T, DP, NB>(s, p, r, a.scale_log2, key, min(limit, last), key + BN - 1 > min(least, last), lane);
+#pragma unroll
+      for (int b = 0; b < NB; ++b) weighted<T, DP>(smem + (2 + buf) * IMG, 32 * b, p[b], r.o, lane);
+    }
+    buf ^= 1;
+  }
+  if constexpr (PAGED) {
+    if (__syncthreads_or(src.bad)) r.l = NAN;
+  }
+  if (!active) return;
+  const float l = add_halves(r.l);
+  if (!it.divided) {
+    const float inv = inverse(l);
+    uint16_t* out = out_row(a, it, kvh, mine);
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        // columns 16 i + 4 half + 0..3 and 8 further, as 8 columns a lane: the halves exchange a group of 4
+        u32x2 x, y;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          x[e] = T::pack(r.o[db][8 * i + 2 * e] * inv, r.o[db][8 * i + 2 * e + 1] * inv);
+          y[e] = T::pack(r.o[db][8 * i + 4 + 2 * e] * inv, r.o[db][8 * i + 4 + 2 * e + 1] * inv);
+        }
+        const auto w0 = __builtin_amdgcn_permlane32_swap(x[0], y[0], false, false);
+        const auto w1 = __builtin_amdgcn_permlane32_swap(x[1], y[1], false, false);
+        const int col = 32 * db + 16 * i + 8 * (lane >> 5);
+        if (row <= top && col < a.d) *reinterpret_cast<u32x4*>(out + col) = u32x4{w0[0], w1[0], w0[1], w1[1]};
+      }
+    return;
+  }
+  float* ws = slot_at<DP>(a, it.slot + it.split, kvh);
+  const int at = row - it.row0;
+  if (row > top || it.slot + it.split >= a.slots) return;
+#pragma unroll
+  for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      *reinterpret_cast<f32x4*>(ws + at * DP + 32 * db + 8 * i + 4 * (lane >> 5)) =
+          f32x4{r.o[db][4 * i], r.o[db][4 * i + 1], r.o[db][4 * i + 2], r.o[db][4 * i + 3]};
+  if (lane < 32) {
+    ws[a.ws_rows * DP + at] = r.m;
+    ws[a.ws_rows * (DP + 1) + at] = l;
+  }
+}
+
+// Up to 32 rows: every wave has all rows and takes every fourth block of 32 keys, through images of its own; then the waves'
+// parts are joined.
+template <class T, int DP, bool PAGED>
+__device__ __forceinline__ void small_tile(const Args& a, const Item& it, int kvh, u32x4* smem, float* stats) {
+  using S = Shape<DP>;
+  constexpr int IMG = 32 * S::CH, LOADS = IMG / kWave;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int top = it.row0 + it.rows - 1;
+  const int mine = min(it.row0 + (lane & 31), top);
+  u32x4 q[DP / 16];
+  load_q<T, DP, PAGED>(a, it, kvh, mine, q, lane);
+  const int limit = a.causal ? min(it.first + mine / a.group, it.keys - 1) : it.keys - 1;
+  const int least = __builtin_amdgcn_readfirstlane(limit);
+  Running<DP> r;
+  r.clear();
+  Source<PAGED> src(a, it, kvh);
+  const int chunks = a.d / 8, last = it.key1 - 1;
+  u32x4* kimg = smem + wave * (S::kShare ? 1 : 2) * IMG;
+  u32x4* vimg = S::kShare ? kimg : kimg + IMG;
+  int key = it.key0 + 32 * wave;
+  if (key < it.key1) {
+    load_rows<DP, 32, kWave, true, false>(src, kimg, vimg, key, last, chunks, lane);
+    if constexpr (!S::kShare) load_rows<DP, 32, kWave, false, true>(src, kimg, vimg, key, last, chunks, lane);
+  }
+  for (; key < it.key1; key += 32 * kWaves) {
+    const bool more = key + 32 * kWaves < it.key1;
+    if constexpr (S::kShare) wait_vm<0>();
+    else wait_vm<LOADS>();  // the keys: only the values' loads are younger
+    f32x16 s[1] = {scores<T, DP>(kimg, 0, q, lane)};
+    u32x4 p[1][2];
+    wait_lds();  // the keys are in registers: their image is free
+    if constexpr (S::kShare) load_rows<DP, 32, kWave, false, true>(src, kimg, vimg, key, last, chunks, lane);
+    else if (more) load_rows<DP, 32, kWave, true, false>(src, kimg, vimg, key + 32 * kWaves, last, chunks, lane);
+    softmax_step<T, DP, 1>(s, p, r, a.scale_log2, key, min(limit, last), key + 31 > min(least, last), lane);
+    if (!S::kShare && more) wait_vm<LOADS>();
+    else wait_vm<0>();
+    weighted<T, DP>(vimg, 0, p[0], r.o, lane);
+    wait_lds();
+    if (more) load_rows<DP, 32, kWave, S::kShare, !S::kShare>(src, kimg, vimg, key + 32 * kWaves, last, chunks, lane);
+  }
+  if (PAGED && __any(src.bad)) r.l = NAN;
+  r.l = add_halves(r.l);
+  // stats: [wave][32] maxima, [wave][32] sums, [32] factors of the result
+  if (lane < 32) {
+    stats[32 * wave + lane] = r.m;
+    stats[32 * (kWaves + wave) + lane] = r.l;
+  }
+  __syncthreads();
+  float m = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) m = fmaxf(m, stats[32 * w + (lane & 31)]);
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    const float mw = stats[32 * w + (lane & 31)];
+    l += stats[32 * (kWaves + w) + (lane & 31)] * (mw == m ? 1.f : __builtin_amdgcn_exp2f(mw - m));
+  }
+  const float f = r.m == m ? 1.f : __builtin_amdgcn_exp2f(r.m - m);
+  const bool whole = !it.divided;
+  float* ws = whole ? nullptr : slot_at<DP>(a, it.slot + it.split, kvh);
+  const bool keep = whole || it.slot + it.split < a.slots;
+  if (wave == 0 && lane < 32) {
+    stats[32 * 2 * kWaves + lane] = whole ? inverse(l) : 1.f;
+    if (!whole && keep && lane < it.rows) {
+      ws[a.ws_rows * DP + lane] = m;
+      ws[a.ws_rows * (DP + 1) + lane] = l;
+    }
+  }
+  f32x4* parts = reinterpret_cast<f32x4*>(smem);
+  constexpr int G = S::G;
+#pragma unroll
+  for (int g = 0; g < DP / 32 / G; ++g) {
+    if ((lane & 31) < it.rows) {
+#pragma unroll
+      for (int db = 0; db < G; ++db)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const f32x16& o = r.o[g * G + db];
+          parts[(wave * G * 8 + db * 8 + 2 * i + (lane >> 5)) * 32 + (lane & 31)] =
+              f32x4{o[4 * i] * f, o[4 * i + 1] * f, o[4 * i + 2] * f, o[4 * i + 3] * f};
+        }
+    }
+    __syncthreads();
+    for (int i = tid; i < it.rows * G * 8; i += kThreads) {
+      const int row = i / (G * 8), piece = i % (G * 8), col = 4 * piece + 32 * G * g;
+      f32x4 x = parts[piece * 32 + row];
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) x += parts[(w * G * 8 + piece) * 32 + row];
+      if (whole) {
+        const float inv = stats[32 * 2 * kWaves + row];
+        if (col < a.d)
+          *reinterpret_cast<u32x2*>(out_row(a, it, kvh, it.row0 + row) + col) =
+              u32x2{T::pack(x[0] * inv, x[1] * inv), T::pack(x[2] * inv, x[3] * inv)};
+      } else if (keep) {
+        *reinterpret_cast<f32x4*>(ws + row * DP + col) = x;
+      }
+    }
+    if (g + 1 < DP / 32 / G) __syncthreads();
+  }
+}
+
+template <class T, int DP, bool PAGED>
+__global__ __launch_bounds__(kThreads, 2) void attention_kernel(Args a) {
+  using S = Shape<DP>;
+  __shared__ __align__(16) u32x4 smem[S::kChunks];
+  __shared__ float stats[32 * (2 * kWaves + 1)];
+  const int kvh = blockIdx.x % a.hk, index = blockIdx.x / a.hk;
+  const Item it = find_item(a, index, false);
+  if (it.b < 0) {
+    fill_rest(a, kvh, it.extra, gridDim.x / a.hk - (index - it.extra));
+    return;
+  }
+  if (it.key0 >= it.key1 && it.split > 0) return;
+  if (a.d < DP) {
+    for (int i = threadIdx.x; i < S::kChunks; i += kThreads) smem[i] = u32x4{};
+    __syncthreads();
+  }
+  if (it.small) small_tile<T, DP, PAGED>(a, it, kvh, smem, stats);
+  else large_tile<T, DP, PAGED>(a, it, kvh, smem);
+}
+
+// Joins the partials of split tiles: the parts' sums, each times exp2 of its maximum less the greatest.
+template <class T, int DP>
+__global__ __launch_bounds__(kThreads) void merge_kernel(Args a) {
+  const int kvh = blockIdx.x % a.hk, index = blockIdx.x / a.hk;
+  const Item it = find_item(a, index, true);
+  if (it.b < 0 || !it.divided || it.slot + it.splits > a.slots) return;
+  const int pieces = a.d / 4;
+  for (int i = threadIdx.x; i < it.rows * pieces; i += kThreads) {
+    const int row = i / pieces, col = 4 * (i % pieces);
+    float m = -INFINITY, l = 0.f;
+    f32x4 x = {};
+    for (int s = 0; s < it.splits; ++s) {
+      const float* ws = slot_at<DP>(a, it.slot + s, kvh);
+      const float ms = ws[a.ws_rows * DP + row];
+      const f32x4 xs = *reinterpret_cast<const f32x4*>(ws + row * DP + col);
+      const float to = fmaxf(m, ms);
+      const float fa = m == to ? 1.f : __builtin_amdgcn_exp2f(m - to), fb = ms == to ? 1.f : __builtin_amdgcn_exp2f(ms - to);
+      l = l * fa + ws[a.ws_rows * (DP + 1) + row] * fb;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = x[e] * fa + xs[e] * fb;
+      m = to;
+    }
+    const float inv = inverse(l);
+    *reinterpret_cast<u32x2*>(out_row(a, it, kvh, it.row0 + row) + col) =
+        u32x2{T::pack(x[0] * inv, x[1] * inv), T::pack(x[2] * inv, x[3] * inv)};
+  }
+}
+
+// The append: piece c of head h of token tok goes to the token's place in its sequence's pages.
+struct Append {
+  const void* k;
+  const void* v;
+  void* k_pages;
+  void* v_pages;
+  const int* cu;
+  const int* lengths;
+  const int* table;
+  int64_t k_t, k_h, v_t, v_h, kp_p, kp_t, kp_h, vp_p, vp_t, vp_h, table_stride;  // bytes, table_stride in entries
+  int tokens, seqs, pool, page, page_shift, max_keys, hk, pieces;
+};
+
+// E: a piece, 16 bytes where every row is made of aligned ones, else one element.
+template <class E>
+__global__ __launch_bounds__(kThreads) void append_kernel(Append a) {
+  const int64_t per = static_cast<int64_t>(a.hk) * a.pieces, total = a.tokens * per;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < total;
+       i += static_cast<int64_t>(gridDim.x) * kThreads) {
+    const int tok = static_cast<int>(i / per), rest = static_cast<int>(i - tok * per), h = rest / a.pieces, c = rest % a.pieces;
+    int lo = 0, hi = a.seqs;  // the last sequence that begins at or before tok
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (a.cu[mid] <= tok) lo = mid;
+      else hi = mid;
+    }
+    const int end = a.cu[lo + 1];
+    if (tok < a.cu[lo] || tok >= end) continue;
+    const int64_t at = static_cast<int64_t>(a.lengths[lo]) - (end - tok);
+    if (at < 0 || at >= a.max_keys) continue;
+    const int pos = static_cast<int>(at), n = a.page_shift >= 0 ? pos >> a.page_shift : pos / a.page, slot = pos - n * a.page;
+    const int id = a.table[lo * a.table_stride + n];
+    if (static_cast<unsigned>(id) >= static_cast<unsigned>(a.pool)) continue;
+    const auto from = [&](const void* p, int64_t t, int64_t hs) {
+      return reinterpret_cast<const E*>(static_cast<const char*>(p) + tok * t + h * hs) + c;
+    };
+    const auto to = [&](void* p, int64_t ps, int64_t t, int64_t hs) {
+      return reinterpret_cast<E*>(static_cast<char*>(p) + id * ps + slot * t + h * hs) + c;
+    };
+    *to(a.k_pages, a.kp_p, a.kp_t, a.kp_h) = *from(a.k, a.k_t, a.k_h);
+    *to(a.v_pages, a.vp_p, a.vp_t, a.vp_h) = *from(a.v, a.v_t, a.v_h);
+  }
+}
+
+constexpr int kTarget = 1024;   // tiles that splitting aims at: two workgroups a CU, twice over
+constexpr int kChunkMin = 256;  // least keys of a split
+
+int page_shift_of(int page) {
+  int s = 0;
+  while ((1 << s) < page && s < 30) ++s;
+  return (1 << s) == page ? s : -1;
+}
+
+// Row tiles of a key head that any offsets can give: sequences of up to 64 rows have 32-row tiles.
+int64_t tiles_bound(int64_t tokens, int64_t seqs, int64_t group) {
+  const int64_t rows = tokens * group, some = seqs < tokens ? seqs : tokens;
+  const int64_t a = rows / kTileLarge + 2 * some, b = rows / kTileSmall + some;
+  return a < b ? a : b;
+}
+
+bool may_split(int64_t max_keys) { return max_keys > kChunkMin; }
+
+int padded_dim(int d) { return d <= 64 ? 64 : d <= 96 ? 96 : d <= 128 ? 128 : 256; }
+
+int slot_rows(int64_t tokens, int64_t group) { return tokens * group <= kSmallRows ? kTileSmall : kTileLarge; }
+
+// Partials that any offsets can give. A sequence is divided where its keys exceed a split's, and a split's keys are at least
+// the whole work over the target: the parts are fewer than twice the target; nor are they more than every tile's most.
+int64_t slots_bound(int64_t tokens, int64_t seqs, int64_t group, int64_t hk, int64_t max_keys) {
+  const int64_t most = tiles_bound(tokens, seqs, group) * hk * ((max_keys + kChunkMin - 1) / kChunkMin);
+  const int64_t aim = 2 * kTarget + hk;
+  return most < aim ? most : aim;
+}
+
+template <class T, int DP, bool PAGED>
+int launch(const Args& a, int64_t index, int64_t merges, hipStream_t st) {
+  attention_kernel<T, DP, PAGED><<<static_cast<unsigned>(index * a.hk), kThreads, 0, st>>>(a);
+  hipError_t e = hipGetLastError();
+  if (e == hipSuccess && merges > 0) {
+    merge_kernel<T, DP><<<static_cast<unsigned>(merges * a.hk), kThreads, 0, st>>>(a);
+    e = hipGetLastError();
+  }
+  return e == hipSuccess ? BP_OK : static_cast<int>(e);
+}
+
+template <class T, bool PAGED>
+int launch_dim(const Args& a, int64_t index, int64_t merges, hipStream_t st) {
+  switch (padded_dim(a.d)) {
+    case 64: return launch<T, 64, PAGED>(a, index, merges, st);
+    case 96: return launch<T, 96, PAGED>(a, index, merges, st);
+    case 128: return launch<T, 128, PAGED>(a, index, merges, st);
+    default: return launch<T, 256, PAGED>(a, index, merges, st);
+  }
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+size_t workspace_bytes(int64_t tokens, int64_t seqs, int64_t hq, int64_t hk, int64_t d, int64_t max_keys) {
+  if (tokens <= 0 || seqs <= 0 || hk <= 0 || hq % hk != 0 || d <= 0 || d > 256 || !may_split(max_keys)) return 0;
+  const int64_t group = hq / hk;
+  return static_cast<size_t>(slots_bound(tokens, seqs, group, hk, max_keys)) * slot_rows(tokens, group) *
+         (padded_dim(static_cast<int>(d)) + 2) * sizeof(float);
+}
+
+int run(int dtype, Args& a, bool paged, size_t ws_bytes, hipStream_t st) {
+  if (dtype != BP_DT_BF16 && dtype != BP_DT_F16) return BP_E_UNSUPPORTED;
+  if (a.tokens < 0 || a.seqs < 0 || a.hk <= 0 || a.hq <= 0 || a.hq % a.hk != 0 || !(a.scale_log2 > 0.f) || a.max_keys < 0)
+    return BP_E_INVALID_ARG;
+  if (a.d <= 0 || a.d % 8 != 0 || a.d > 256) return BP_E_UNSUPPORTED;
+  if (a.tokens == 0) return BP_OK;
+  if (a.q == nullptr || a.out == nullptr || (a.seqs > 0 && a.cu == nullptr)) return BP_E_INVALID_ARG;
+  if (!aligned16(a.q) || !aligned16(a.k) || !aligned16(a.v) || !aligned16(a.out) ||
+      ((a.q_t | a.q_h | a.k_p | a.k_t | a.k_h | a.v_p | a.v_t | a.v_h) & 7) != 0)
+    return BP_E_INVALID_ARG;
+  a.group = a.hq / a.hk;
+  // rows of a sequence, and keys plus a split, in 32 bits
+  if (static_cast<int64_t>(a.tokens) * a.hq >= (1ll << 30) || a.max_keys >= (1 << 29)) return BP_E_UNSUPPORTED;
+  const int64_t tiles = tiles_bound(a.tokens, a.seqs, a.group);
+  a.target = kTarget;
+  a.chunk_min = kChunkMin;
+  a.ws_rows = slot_rows(a.tokens, a.group);
+  int64_t index = tiles, merges = 0;
+  const size_t need = workspace_bytes(a.tokens, a.seqs, a.hq, a.hk, a.d, a.max_keys);
+  if (need > 0) {
+    if (a.ws == nullptr || ws_bytes < need || !aligned16(a.ws)) return BP_E_WORKSPACE;
+    a.slots = static_cast<int>(slots_bound(a.tokens, a.seqs, a.group, a.hk, a.max_keys) / a.hk);
+    const int64_t most = tiles * ((a.max_keys + kChunkMin - 1) / kChunkMin - 1), aim = kTarget / a.hk + 1;
+    index += most < aim ? most : aim;
+    merges = tiles;
+  } else {
+    a.ws = nullptr;
+    a.slots = 0;
+  }
+  index += 1;  // rows of no sequence
+  if (index * a.hk >= (1ll << 31)) return BP_E_UNSUPPORTED;
+  if (dtype == BP_DT_BF16)
+    return paged ? launch_dim<Bf16, true>(a, index, merges, st) : launch_dim<Bf16, false>(a, index, merges, st);
+  return paged ? launch_dim<F16, true>(a, index, merges, st) : launch_dim<F16, false>(a, index, merges, st);
+}
+
+}  // namespace
+}  // namespace attn
+}  // namespace bp
+
+extern "C" {
+
+size_t bp_attn_workspace_bytes(int64_t tokens, int64_t seqs, int64_t hq, int64_t hk, int64_t head_dim, int64_t max_keys) {
+  return bp::attn::workspace_bytes(tokens, seqs, hq, hk, head_dim, max_keys);
+}
+
+int bp_attn_packed(int dtype, const void* q, const void* k, const void* v, void* out, const int32_t* cu, int tokens, int seqs,
+                   int hq, int hk, int head_dim, int64_t q_t, int64_t q_h, int64_t k_t, int64_t k_h, int64_t v_t, int64_t v_h,
+                   int causal, float scale, void* workspace, size_t workspace_bytes, void* stream) {
+  bp::attn::Args a = {};
+  if (tokens > 0 && (k == nullptr || v == nullptr)) return BP_E_INVALID_ARG;
+  a.q = q, a.k = k, a.v = v, a.out = out, a.cu = cu;
+  a.ws = static_cast<float*>(workspace);
+  a.q_t = q_t, a.q_h = q_h, a.k_t = k_t, a.k_h = k_h, a.v_t = v_t, a.v_h = v_h;
+  a.tokens = tokens, a.seqs = seqs, a.hq = hq, a.hk = hk, a.d = head_dim, a.causal = causal != 0;
+  a.max_keys = tokens;
+  a.page = 1;
+  a.scale_log2 = scale * 1.44269504088896340736f;
+  return bp::attn::run(dtype, a, false, workspace_bytes, static_cast<hipStream_t>(stream));
+}
+
+int bp_attn_paged(int dtype, const void* q, const void* k_pages, const void* v_pages, void* out, const int32_t* table,
+                  int64_t table_stride, const int32_t* lengths, const int32_t* cu, int tokens, int seqs, int pool, int page,
+                  int max_pages, int hq, int hk, int head_dim, int64_t q_t, int64_t q_h, int64_t k_p, int64_t k_t, int64_t k_h,
+                  int64_t v_p, int64_t v_t, int64_t v_h, float scale, void* workspace, size_t workspace_bytes, void* stream) {
+  if (page <= 0 || pool < 0 || max_pages < 0 || static_cast<int64_t>(page) * max_pages >= (1ll << 29)) return BP_E_INVALID_ARG;
+  if (tokens > 0 && seqs > 0 &&
+      (lengths == nullptr || (max_pages > 0 && (table == nullptr || k_pages == nullptr || v_pages == nullptr || pool == 0))))
+    return BP_E_INVALID_ARG;
+  bp::attn::Args a = {};
+  a.q = q, a.k = k_pages, a.v = v_pages, a.out = out, a.cu = cu, a.lengths = lengths, a.table = table;
+  a.ws = static_cast<float*>(workspace);
+  a.q_t = q_t, a.q_h = q_h, a.k_p = k_p, a.k_t = k_t, a.k_h = k_h, a.v_p = v_p, a.v_t = v_t, a.v_h = v_h;
+  a.table_stride = table_stride;
+  a.tokens = tokens, a.seqs = seqs, a.hq = hq, a.hk = hk, a.d = head_dim, a.causal = 1;
+  a.pool = pool, a.page = page, a.page_shift = bp::attn::page_shift_of(page), a.max_keys = page * max_pages;
+  a.scale_log2 = scale * 1.44269504088896340736f;
+  return bp::attn::run(dtype, a, true, workspace_bytes, static_cast<hipStream_t>(stream));
+}
+
+int bp_paged_append(int element_bytes, const void* k, const void* v, void* k_pages, void* v_pages, const int32_t* table,
+                    int64_t table_stride, const int32_t* lengths, const int32_t* cu, int tokens, int seqs, int pool, int page,
+                    int max_pages, int hk, int head_dim, int64_t k_t, int64_t k_h, int64_t v_t, int64_t v_h, int64_t kp_p,
+                    int64_t kp_t, int64_t kp_h, int64_t vp_p, int64_t vp_t, int64_t vp_h, void* stream) {
+  if ((element_bytes != 1 && element_bytes != 2 && element_bytes != 4) || tokens < 0 || seqs < 0 || pool < 0 || page <= 0 ||
+      max_pages < 0 || static_cast<int64_t>(page) * max_pages >= (1ll << 29) || hk < 0 || head_dim < 0)
+    return BP_E_INVALID_ARG;
+  if (tokens == 0 || seqs == 0 || pool == 0 || max_pages == 0 || hk == 0 || head_dim == 0) return BP_OK;
+  if (k == nullptr || v == nullptr || k_pages == nullptr || v_pages == nullptr || table == nullptr || lengths == nullptr ||
+      cu == nullptr)
+    return BP_E_INVALID_ARG;
+  const int64_t row = static_cast<int64_t>(head_dim) * element_bytes;
+  if (hk * row >= (1ll << 31)) return BP_E_UNSUPPORTED;
+  bp::attn::Append a = {};
+  a.k = k, a.v = v, a.k_pages = k_pages, a.v_pages = v_pages, a.cu = cu, a.lengths = lengths, a.table = table;
+  a.k_t = k_t * element_bytes, a.k_h = k_h * element_bytes, a.v_t = v_t * element_bytes, a.v_h = v_h * element_bytes;
+  a.kp_p = kp_p * element_bytes, a.kp_t = kp_t * element_bytes, a.kp_h = kp_h * element_bytes;
+  a.vp_p = vp_p * element_bytes, a.vp_t = vp_t * element_bytes, a.vp_h = vp_h * element_bytes;
+  a.table_stride = table_stride;
+  a.tokens = tokens, a.seqs = seqs, a.pool = pool, a.page = page, a.page_shift = bp::attn::page_shift_of(page);
+  a.max_keys = page * max_pages, a.hk = hk;
+  const bool wide = bp::attn::aligned16(k) && bp::attn::aligned16(v) && bp::attn::aligned16(k_pages) &&
+                    bp::attn::aligned16(v_pages) && row % 16 == 0 &&
+                    ((a.k_t | a.k_h | a.v_t | a.v_h | a.kp_p | a.kp_t | a.kp_h | a.vp_p | a.vp_t | a.vp_h) & 15) == 0;
+  a.pieces = wide ? static_cast<int>(row / 16) : head_dim;
+  const int64_t total = static_cast<int64_t>(tokens) * hk * a.pieces;
+  int64_t blocks = (total + bp::attn::kThreads - 1) / bp::attn::kThreads;
+  if (blocks > 16384) blocks = 16384;
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  const dim3 grid(static_cast<unsigned>(blocks));
+  if (wide) bp::attn::append_kernel<bp::u32x4><<<grid, bp::attn::kThreads, 0, st>>>(a);
+  else if (element_bytes == 1) bp::attn::append_kernel<uint8_t><<<grid, bp::attn::kThreads, 0, st>>>(a);
+  else if (element_bytes == 2) bp::attn::append_kernel<uint16_t><<<grid, bp::attn::kThreads, 0, st>>>(a);
+  else bp::attn::append_kernel<uint32_t><<<grid, bp::attn::kThreads, 0, st>>>(a);
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? BP_OK : static_cast<int>(e);
+}
+
+}  // extern "C"

@@ -414,6 +414,56 @@ int bp_decode_argmax_next(const void* logits, int vocab, int64_t* tok, int64_t* 
 size_t bp_decode_argmax_rows_scratch_bytes(int rows);
 int bp_decode_argmax_rows(const void* logits, int vocab, int rows, int64_t* tok, void* scratch, void* stream);
 
+/*
+ * Attention of several sequences in one call; the softmax in fp32, the probabilities rounded to the tensors' type before the
+ * product with the values (both sums in fp32), the result rounded once. dtype BP_DT_BF16 or BP_DT_F16 for q, k, v and out;
+ * head_dim a multiple of 8 up to 256 (else BP_E_UNSUPPORTED); hq a multiple of hk (query head h reads key head
+ * h / (hq / hk)); every base 16-byte aligned, every stride (in elements; the innermost is 1) a multiple of 8; out
+ * [tokens, hq, head_dim] contiguous. cu [seqs + 1] (int32): sequence b's tokens are cu[b] .. cu[b + 1] - 1; what of them lies
+ * outside [0, tokens) is left out. Rows of no sequence become zeros, so do rows that see no key.
+ * packed: keys and values of the tokens themselves; with causal, token i sees those of its sequence up to i, else all.
+ * paged:  caches [pool, page, hk, head_dim] (any strides between pages, positions and heads). Sequence b has lengths[b]
+ *         (int32) positions, position p in page table[b, p / page] (int32, table_stride entries a row), at p % page; its
+ *         tokens are the last of them, their keys and values in the cache already; the token at position p sees 0 .. p.
+ *         lengths are taken up to page x max_pages. Rows of a sequence that has to read a page outside [0, pool) become NaN.
+ * The offsets, lengths and table are read on the device only: a captured graph serves whatever they hold at a replay.
+ * workspace: bp_attn_workspace_bytes(tokens, seqs, hq, hk, head_dim, max_keys) bytes, 16-byte aligned, for the partial sums of
+ * divided keys (max_keys: tokens, or page x max_pages for the cache); nothing in it outlives the call.
+ * No counterpart in the reference (batch 1, one contiguous cache).
+ */
+size_t bp_attn_workspace_bytes(int64_t tokens, int64_t seqs, int64_t hq, int64_t hk, int64_t head_dim, int64_t max_keys);
+int bp_attn_packed(int dtype, const void* q, const void* k, const void* v, void* out, const int32_t* cu, int tokens, int seqs,
+                   int hq, int hk, int head_dim, int64_t q_t, int64_t q_h, int64_t k_t, int64_t k_h, int64_t v_t, int64_t v_h,
+                   int causal, float scale, void* workspace, size_t workspace_bytes, void* stream);
+int bp_attn_paged(int dtype, const void* q, const void* k_pages, const void* v_pages, void* out, const int32_t* table,
+                  int64_t table_stride, const int32_t* lengths, const int32_t* cu, int tokens, int seqs, int pool, int page,
+                  int max_pages, int hq, int hk, int head_dim, int64_t q_t, int64_t q_h, int64_t k_p, int64_t k_t, int64_t k_h,
+                  int64_t v_p, int64_t v_t, int64_t v_h, float scale, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * The keys and values k, v [tokens, hk, head_dim] (element_bytes 1, 2 or 4) into the cache of bp_attn_paged: token i of
+ * sequence b (of c_b tokens) to position lengths[b] - c_b + i. A position below 0 or at or past page x max_pages, a page
+ * outside [0, pool) and a token of no sequence are left out. Strides in elements. 16 bytes at a time where all rows allow.
+ * No counterpart in the reference.
+ */
+int bp_paged_append(int element_bytes, const void* k, const void* v, void* k_pages, void* v_pages, const int32_t* table,
+                    int64_t table_stride, const int32_t* lengths, const int32_t* cu, int tokens, int seqs, int pool, int page,
+                    int max_pages, int hk, int head_dim, int64_t k_t, int64_t k_h, int64_t v_t, int64_t v_h, int64_t kp_p,
+                    int64_t kp_t, int64_t kp_h, int64_t vp_p, int64_t vp_t, int64_t vp_h, void* stream);
+
+/*
+ * Of every row of logits [rows, vocab] (BP_DT_BF16 / F16 / F32, row_stride elements apart, rows contiguous): logprob [rows] =
+ * log softmax at targets [rows] (targets NULL: none; a target outside the row: NaN), entropy [rows] (in nats), and the `top`
+ * (0 .. 32, at most vocab) most likely tokens, top_ids, top_logprobs [rows, top], in order of logit, equal ones in order of
+ * index. fp32 results. A row with a NaN or +inf, and one of nothing but -inf, has NaN for every probability; NaN counts as
+ * greatest in the order. workspace: bp_logprobs_workspace_bytes(dtype, rows, vocab, top).
+ * No counterpart in the reference.
+ */
+size_t bp_logprobs_workspace_bytes(int dtype, int64_t rows, int64_t vocab, int top);
+int bp_logprobs(int dtype, const void* logits, int64_t row_stride, const int64_t* targets, float* logprob, float* entropy,
+                int64_t* top_ids, float* top_logprobs, int64_t rows, int64_t vocab, int top, void* workspace,
+                size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
