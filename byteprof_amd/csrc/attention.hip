@@ -22,17 +22,31 @@ struct Shape {
   static constexpr int kChunks = kLarge > kSmall ? (kLarge > kMerge ? kLarge : kMerge) : (kSmall > kMerge ? kSmall : kMerge);
 };
 
-// Where the keys and values of an item lie.
+// Rows of a load instruction: whole rows, a power of two of them, so that a page that is a multiple of it holds all of them.
+template <int DP>
+struct Load {
+  static constexpr int CH = DP / 8;
+  static constexpr int ROWS = CH == 8 ? 8 : CH == 32 ? 2 : 4;
+};
+
+// Where the keys and values of an item lie. Paged: a wave keeps two blocks of 64 entries of the item's page table in LDS, the
+// one in use and the next, which it loads a tile ahead and in the order of the tiles' own loads: no address waits for the
+// table. Pages of fewer than 4 positions, of which a tile may need more than a block, are looked up in memory.
+constexpr int kBlock = 64;
+constexpr int kRing = 2 * kBlock;
+
 template <bool PAGED>
 struct Source {
   const uint16_t* k;
   const uint16_t* v;
   int64_t k_p, k_t, v_p, v_t;
   const int* pages;
-  int pool, page, page_shift;
+  const int* ring;
+  int pool, loaded, last, last_page;
+  Div page;
   bool bad;  // a page outside the pool: the item's rows become NaN
 
-  __device__ __forceinline__ Source(const Args& a, const Item& it, int kvh) {
+  __device__ __forceinline__ Source(const Args& a, const Item& it, int kvh, const int* wave_ring) {
     const int64_t from = PAGED ? 0 : it.begin;
     k = static_cast<const uint16_t*>(a.k) + kvh * a.k_h + from * a.k_t;
     v = static_cast<const uint16_t*>(a.v) + kvh * a.v_h + from * a.v_t;
@@ -40,18 +54,36 @@ struct Source {
     k_t = a.k_t;
     v_p = a.v_p;
     v_t = a.v_t;
-    pages = PAGED ? a.table + static_cast<int64_t>(it.b) * a.table_stride : nullptr;
     pool = a.pool;
     page = a.page;
-    page_shift = a.page_shift;
+    last = it.key1 - 1;
     bad = false;
-  }
-  // Element offsets of a key's row.
-  __device__ __forceinline__ void at(int key, int64_t& ko, int64_t& vo) {
     if constexpr (PAGED) {
-      const int n = page_shift >= 0 ? key >> page_shift : key / page;
-      const int slot = key - n * page;
-      int id = pages[n];
+      pages = a.table + static_cast<int64_t>(it.b) * a.table_stride;
+      ring = wave_ring;
+      last_page = page(last);
+      loaded = -1;
+    }
+  }
+  // Loads the blocks of the table up to the one of `key`, of a tile that begins at `first`.
+  __device__ __forceinline__ void reach(int first, int key, int lane) {
+    if constexpr (PAGED) {
+      if (page.d < 4) return;
+      const int to = min(page(key), last_page) / kBlock;
+      if (loaded < 0) loaded = page(first) / kBlock - 1;
+      while (loaded < to) {
+        ++loaded;
+        load_lds4(pages + min(loaded * kBlock + lane, last_page),
+                  __builtin_amdgcn_readfirstlane(lds_address(ring)) + 4 * (loaded * kBlock % kRing));
+      }
+    }
+  }
+  // Element offsets of the row of a lane's key.
+  __device__ __forceinline__ void at(int key, int64_t& ko, int64_t& vo) {
+    key = min(key, last);
+    if constexpr (PAGED) {
+      const int n = page(key), slot = key - n * page.d;
+      int id = page.d < 4 ? pages[n] : ring[n % kRing];
       if (static_cast<unsigned>(id) >= static_cast<unsigned>(pool)) {
         bad = true;
         id = 0;
@@ -65,25 +97,39 @@ struct Source {
   }
 };
 
-// Loads ROWS rows (keys from key0, those past `last` as the row of `last`) with `threads` threads from thread `me`.
-template <int DP, int ROWS, int THREADS, bool K, bool V, bool PAGED>
-__device__ __forceinline__ void load_rows(Source<PAGED>& src, const u32x4* kimg, const u32x4* vimg, int key0, int last, int chunks,
-                                          int me) {
-  constexpr int CH = DP / 8;
-  static_assert(ROWS * CH % THREADS == 0, "whole loads");
+__device__ __forceinline__ int64_t lane_value(int64_t v, int lane) {
+  const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(v), lane);
+  const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(v >> 32), lane);
+  return static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
+}
+
+// Loads ROWS rows from key0, of keys or of values, with the waves' instructions in turn; row r's element offset is lane r's
+// `off`. Whole tiles whose load instructions each stay inside a page have a wave-uniform address and the lanes' offsets, which
+// do not change from tile to tile; the others (a sequence's last tile, pages of odd sizes) an address a lane.
+template <int DP, int ROWS, int WAVES, bool V, bool FULL, bool PAGED>
+__device__ __forceinline__ void load_rows(const Source<PAGED>& src, const u32x4* img, int key0, int64_t off, int chunks, int wave,
+                                          int lane) {
+  constexpr int CH = DP / 8, R = Load<DP>::ROWS;
+  static_assert(ROWS % (R * WAVES) == 0, "whole loads");
+  const int sub = lane / CH, place = lane % CH;
+  const uint16_t* from = V ? src.v : src.k;
+  const int64_t stride = V ? src.v_t : src.k_t;
+  const uint32_t base = __builtin_amdgcn_readfirstlane(lds_address(img));
+  const bool mine = R * CH == kWave || sub < R;
+  if (key0 + ROWS - 1 <= src.last && (!PAGED || src.page.d % R == 0)) {
 #pragma unroll
-  for (int i = 0; i < ROWS * CH / THREADS; ++i) {
-    const int idx = i * THREADS + me, row = idx / CH, place = idx % CH;
-    int64_t ko, vo;
-    src.at(min(key0 + row, last), ko, vo);
-    const int first = __builtin_amdgcn_readfirstlane(idx);
-    if constexpr (K) {
-      const int c = chunk_at<DP, false>(row, place);
-      if (c < chunks) load_lds16(src.k + ko + 8 * c, __builtin_amdgcn_readfirstlane(lds_address(kimg)) + 16 * first);
+    for (int i = 0; i < ROWS / (R * WAVES); ++i) {
+      const int row0 = (i * WAVES + wave) * R, c = chunk_at<DP, V>(row0 + sub, place);
+      const int64_t o = PAGED ? lane_value(off, row0) : (key0 + row0) * stride;
+      const uint32_t rest = 2 * (static_cast<uint32_t>(sub) * static_cast<uint32_t>(stride) + 8u * c);
+      if (mine && (FULL || c < chunks)) load_lds16(from + o, rest, base + 16 * row0 * CH);
     }
-    if constexpr (V) {
-      const int c = chunk_at<DP, true>(row, place);
-      if (c < chunks) load_lds16(src.v + vo + 8 * c, __builtin_amdgcn_readfirstlane(lds_address(vimg)) + 16 * first);
+  } else {
+#pragma unroll
+    for (int i = 0; i < ROWS / (R * WAVES); ++i) {
+      const int row0 = (i * WAVES + wave) * R, c = chunk_at<DP, V>(row0 + sub, place);
+      const int64_t o = __shfl(off, row0 + sub);
+      if (mine && (FULL || c < chunks)) load_lds16(from + o + 8 * c, base + 16 * row0 * CH);
     }
   }
 }
@@ -92,43 +138,45 @@ __device__ __forceinline__ void load_rows(Source<PAGED>& src, const u32x4* kimg,
 __device__ void fill_rest(const Args& a, int kvh, int extra, int extras) {
   const int lo = a.seqs > 0 ? min(max(a.cu[0], 0), a.tokens) : a.tokens;
   int hi = a.seqs > 0 ? min(max(a.cu[a.seqs], lo), a.tokens) : a.tokens;
-  const int64_t rest = lo + (a.tokens - hi), per = static_cast<int64_t>(a.group) * a.d / 8;
+  const int64_t rest = lo + (a.tokens - hi), per = static_cast<int64_t>(a.group.d) * a.d / 8;
   for (int64_t i = static_cast<int64_t>(extra) * kThreads + threadIdx.x; i < rest * per;
        i += static_cast<int64_t>(extras) * kThreads) {
     const int64_t n = i / per, c = i % per;
     const int64_t tok = n < lo ? n : hi + (n - lo);
-    uint16_t* at = static_cast<uint16_t*>(a.out) + (tok * a.hq + static_cast<int64_t>(kvh) * a.group) * a.d + 8 * c;
+    uint16_t* at = static_cast<uint16_t*>(a.out) + (tok * a.hq + static_cast<int64_t>(kvh) * a.group.d) * a.d + 8 * c;
     *reinterpret_cast<u32x4*>(at) = u32x4{};
   }
 }
 
 __device__ __forceinline__ uint16_t* out_row(const Args& a, const Item& it, int kvh, int row) {
-  const int64_t tok = it.begin + row / a.group;
-  return static_cast<uint16_t*>(a.out) + (tok * a.hq + static_cast<int64_t>(kvh) * a.group + row % a.group) * a.d;
+  const int n = a.group(row);
+  const int64_t head = static_cast<int64_t>(it.begin + n) * a.hq + kvh * a.group.d + (row - n * a.group.d);
+  return static_cast<uint16_t*>(a.out) + head * a.d;
 }
 
 // A split's slot: [ws_rows][DP] sums, then ws_rows maxima and ws_rows sums of probabilities.
 template <int DP>
 __device__ __forceinline__ float* slot_at(const Args& a, int64_t slot, int kvh) {
-  return a.ws + (slot * a.hk + kvh) * a.ws_rows * (DP + 2);
+  return a.ws + (slot * a.hk.d + kvh) * a.ws_rows * (DP + 2);
 }
 
-template <class T, int DP, bool PAGED>
+template <class T, int DP, bool FULL>
 __device__ __forceinline__ void load_q(const Args& a, const Item& it, int kvh, int row, u32x4 (&q)[DP / 16], int lane) {
-  const int64_t tok = it.begin + row / a.group;
-  const uint16_t* p = static_cast<const uint16_t*>(a.q) + tok * a.q_t + (static_cast<int64_t>(kvh) * a.group + row % a.group) * a.q_h;
+  const int n = a.group(row);
+  const uint16_t* p = static_cast<const uint16_t*>(a.q) + static_cast<int64_t>(it.begin + n) * a.q_t +
+                      static_cast<int64_t>(kvh * a.group.d + row - n * a.group.d) * a.q_h;
 #pragma unroll
   for (int i = 0; i < DP / 16; ++i) {
     const int c = 2 * i + (lane >> 5);
-    q[i] = 8 * c < a.d ? *reinterpret_cast<const u32x4*>(p + 8 * c) : u32x4{};
+    q[i] = FULL || 8 * c < a.d ? *reinterpret_cast<const u32x4*>(p + 8 * c) : u32x4{};
   }
 }
 
 __device__ __forceinline__ float inverse(float l) { return l == 0.f ? 0.f : 1.f / l; }
 
 // 128 rows, 32 a wave; the keys in steps of BN that all waves share in LDS, two images of each in turn.
-template <class T, int DP, bool PAGED>
-__device__ __forceinline__ void large_tile(const Args& a, const Item& it, int kvh, u32x4* smem) {
+template <class T, int DP, bool PAGED, bool FULL>
+__device__ __forceinline__ void large_tile(const Args& a, const Item& it, int kvh, u32x4* smem, const int* ring) {
   using S = Shape<DP>;
   constexpr int BN = S::BN, NB = S::NB, IMG = BN * S::CH;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -137,30 +185,51 @@ __device__ __forceinline__ void large_tile(const Args& a, const Item& it, int kv
   const int mine = min(row, top);
   const bool active = it.row0 + 32 * wave <= top;
   u32x4 q[DP / 16];
-  load_q<T, DP, PAGED>(a, it, kvh, mine, q, lane);
-  const int limit = a.causal ? min(it.first + mine / a.group, it.keys - 1) : it.keys - 1;
+  load_q<T, DP, FULL>(a, it, kvh, mine, q, lane);
+  const int limit = a.causal ? min(it.first + a.group(mine), it.keys - 1) : it.keys - 1;
   const int least = __builtin_amdgcn_readfirstlane(limit), most = __builtin_amdgcn_readlane(limit, 31);
   Running<DP> r;
   r.clear();
-  Source<PAGED> src(a, it, kvh);
+  Source<PAGED> src(a, it, kvh, ring);
   const int chunks = a.d / 8, last = it.key1 - 1;
   int buf = 0;
-  if (it.key0 < it.key1)
-    load_rows<DP, BN, kThreads, true, true>(src, smem, smem + 2 * IMG, it.key0, last, chunks, tid);
-  for (int key = it.key0; key < it.key1; key += BN) {
+  const auto load = [&](int key, int to) {
+    int64_t ko, vo;
+    src.at(key + lane % BN, ko, vo);
+    load_rows<DP, BN, kWaves, false, FULL>(src, smem + to * IMG, key, ko, chunks, wave, lane);
+    load_rows<DP, BN, kWaves, true, FULL>(src, smem + (2 + to) * IMG, key, vo, chunks, wave, lane);
+  };
+  if (it.key0 < it.key1) {
+    src.reach(it.key0, it.key0 + 2 * BN - 1, lane);
+    if constexpr (PAGED) wait_vm<0>();
+    load(it.key0, 0);
+  }
+  wait_vm<0>();  // the queries, too
+  const auto next = [&](int key) {
     wait_vm<0>();
     __syncthreads();
-    if (key + BN < it.key1)
-      load_rows<DP, BN, kThreads, true, true>(src, smem + (buf ^ 1) * IMG, smem + (2 + (buf ^ 1)) * IMG, key + BN, last, chunks, tid);
-    if (active && key <= most) {
-      f32x16 s[NB];
-      u32x4 p[NB][2];
-#pragma unroll
-      for (int b = 0; b < NB; ++b) s[b] = scores<T, DP>(smem + buf * IMG, 32 * b, q, lane);
-      softmax_step<T, DP, NB>(s, p, r, a.scale_log2, key, min(limit, last), key + BN - 1 > min(least, last), lane);
-#pragma unroll
-      for (int b = 0; b < NB; ++b) weighted<T, DP>(smem + (2 + buf) * IMG, 32 * b, p[b], r.o, lane);
+    if (key + BN < it.key1) {
+      src.reach(key, key + 3 * BN - 1, lane);
+      load(key + BN, buf ^ 1);
     }
+  };
+  // The steps that hold a key for this wave, then those that only the other waves need (two loops: with one and a condition
+  // the sums went to other registers and back in every step).
+  int key = it.key0;
+  const int mine_end = active ? min(it.key1, most + 1) : it.key0;
+  for (; key < mine_end; key += BN) {
+    next(key);
+    f32x16 s[NB];
+    u32x4 p[NB][2];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) s[b] = scores<T, DP>(smem + buf * IMG, 32 * b, q, lane);
+    softmax_step<T, DP, NB>(s, p, r, a.scale_log2, key, min(limit, last), key + BN - 1 > min(least, last), lane);
+#pragma unroll
+    for (int b = 0; b < NB; ++b) weighted<T, DP>(smem + (2 + buf) * IMG, 32 * b, p[b], r.o, lane);
+    buf ^= 1;
+  }
+  for (; key < it.key1; key += BN) {
+    next(key);
     buf ^= 1;
   }
   if constexpr (PAGED) {
@@ -206,43 +275,56 @@ __device__ __forceinline__ void large_tile(const Args& a, const Item& it, int kv
 
 // Up to 32 rows: every wave has all rows and takes every fourth block of 32 keys, through images of its own; then the waves'
 // parts are joined.
-template <class T, int DP, bool PAGED>
-__device__ __forceinline__ void small_tile(const Args& a, const Item& it, int kvh, u32x4* smem, float* stats) {
+template <class T, int DP, bool PAGED, bool FULL>
+__device__ __forceinline__ void small_tile(const Args& a, const Item& it, int kvh, u32x4* smem, float* stats, const int* ring) {
   using S = Shape<DP>;
-  constexpr int IMG = 32 * S::CH, LOADS = IMG / kWave;
+  constexpr int IMG = 32 * S::CH, LOADS = 32 / Load<DP>::ROWS;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int top = it.row0 + it.rows - 1;
   const int mine = min(it.row0 + (lane & 31), top);
   u32x4 q[DP / 16];
-  load_q<T, DP, PAGED>(a, it, kvh, mine, q, lane);
-  const int limit = a.causal ? min(it.first + mine / a.group, it.keys - 1) : it.keys - 1;
+  load_q<T, DP, FULL>(a, it, kvh, mine, q, lane);
+  const int limit = a.causal ? min(it.first + a.group(mine), it.keys - 1) : it.keys - 1;
   const int least = __builtin_amdgcn_readfirstlane(limit);
   Running<DP> r;
   r.clear();
-  Source<PAGED> src(a, it, kvh);
+  Source<PAGED> src(a, it, kvh, ring);
   const int chunks = a.d / 8, last = it.key1 - 1;
   u32x4* kimg = smem + wave * (S::kShare ? 1 : 2) * IMG;
   u32x4* vimg = S::kShare ? kimg : kimg + IMG;
+  constexpr int STEP = 32 * kWaves;
   int key = it.key0 + 32 * wave;
+  int64_t ko, vo;
+  if (key < it.key1) src.reach(key, key + STEP + 31, lane);
+  if constexpr (PAGED) wait_vm<0>();  // the table and the queries
   if (key < it.key1) {
-    load_rows<DP, 32, kWave, true, false>(src, kimg, vimg, key, last, chunks, lane);
-    if constexpr (!S::kShare) load_rows<DP, 32, kWave, false, true>(src, kimg, vimg, key, last, chunks, lane);
+    src.at(key + lane % 32, ko, vo);
+    load_rows<DP, 32, 1, false, FULL>(src, kimg, key, ko, chunks, 0, lane);
+    if constexpr (!S::kShare) load_rows<DP, 32, 1, true, FULL>(src, vimg, key, vo, chunks, 0, lane);
   }
-  for (; key < it.key1; key += 32 * kWaves) {
-    const bool more = key + 32 * kWaves < it.key1;
+  if constexpr (!PAGED) wait_vm<0>();  // the queries
+  for (; key < it.key1; key += STEP) {
+    const bool more = key + STEP < it.key1;
     if constexpr (S::kShare) wait_vm<0>();
     else wait_vm<LOADS>();  // the keys: only the values' loads are younger
     f32x16 s[1] = {scores<T, DP>(kimg, 0, q, lane)};
     u32x4 p[1][2];
     wait_lds();  // the keys are in registers: their image is free
-    if constexpr (S::kShare) load_rows<DP, 32, kWave, false, true>(src, kimg, vimg, key, last, chunks, lane);
-    else if (more) load_rows<DP, 32, kWave, true, false>(src, kimg, vimg, key + 32 * kWaves, last, chunks, lane);
+    if constexpr (S::kShare) load_rows<DP, 32, 1, true, FULL>(src, vimg, key, vo, chunks, 0, lane);
+    if (more) {
+      src.reach(key, key + 2 * STEP + 31, lane);
+      src.at(key + STEP + lane % 32, ko, vo);
+      if constexpr (!S::kShare) load_rows<DP, 32, 1, false, FULL>(src, kimg, key + STEP, ko, chunks, 0, lane);
+    }
     softmax_step<T, DP, 1>(s, p, r, a.scale_log2, key, min(limit, last), key + 31 > min(least, last), lane);
     if (!S::kShare && more) wait_vm<LOADS>();
     else wait_vm<0>();
     weighted<T, DP>(vimg, 0, p[0], r.o, lane);
     wait_lds();
-    if (more) load_rows<DP, 32, kWave, S::kShare, !S::kShare>(src, kimg, vimg, key + 32 * kWaves, last, chunks, lane);
+    if (more) {
+      if constexpr (S::kShare) load_rows<DP, 32, 1, false, FULL>(src, kimg, key + STEP, ko, chunks, 0, lane);
+      else load_rows<DP, 32, 1, true, FULL>(src, vimg, key + STEP, vo, chunks, 0, lane);
+    }
   }
   if (PAGED && __any(src.bad)) r.l = NAN;
   r.l = add_halves(r.l);
@@ -304,51 +386,110 @@ __device__ __forceinline__ void small_tile(const Args& a, const Item& it, int kv
   }
 }
 
-template <class T, int DP, bool PAGED>
-__global__ __launch_bounds__(kThreads, 2) void attention_kernel(Args a) {
+// 256 columns: a wave's sums alone are 128 registers, so one workgroup a CU with all of them.
+template <class T, int DP, bool PAGED, bool FULL>
+__global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void attention_kernel(Args a) {
   using S = Shape<DP>;
   __shared__ __align__(16) u32x4 smem[S::kChunks];
   __shared__ float stats[32 * (2 * kWaves + 1)];
-  const int kvh = blockIdx.x % a.hk, index = blockIdx.x / a.hk;
-  const Item it = find_item(a, index, false);
+  __shared__ int rings[PAGED ? kWaves * kRing : 1];
+  const int* ring = rings + (PAGED ? threadIdx.x / kWave * kRing : 0);
+  const int index = a.hk(blockIdx.x), kvh = blockIdx.x - index * a.hk.d;
+  const Item it = find_item<false>(a, index);
   if (it.b < 0) {
-    fill_rest(a, kvh, it.extra, gridDim.x / a.hk - (index - it.extra));
+    fill_rest(a, kvh, it.extra, a.hk(gridDim.x) - (index - it.extra));
     return;
   }
   if (it.key0 >= it.key1 && it.split > 0) return;
-  if (a.d < DP) {
+  if constexpr (!FULL) {
     for (int i = threadIdx.x; i < S::kChunks; i += kThreads) smem[i] = u32x4{};
     __syncthreads();
   }
-  if (it.small) small_tile<T, DP, PAGED>(a, it, kvh, smem, stats);
-  else large_tile<T, DP, PAGED>(a, it, kvh, smem);
+  if (it.small) small_tile<T, DP, PAGED, FULL>(a, it, kvh, smem, stats, ring);
+  else large_tile<T, DP, PAGED, FULL>(a, it, kvh, smem, ring);
 }
 
-// Joins the partials of split tiles: the parts' sums, each times exp2 of its maximum less the greatest.
+// Joins the partials of a unit's rows: the parts' sums, each times exp2 of its maximum less the greatest. Few parts: a thread
+// has 4 columns of a row and loads all parts at once. Many: the workgroup has one row, whose parts its groups of
+// d / 4 threads share (one thread after another part took 30 us for 80 parts of 36 rows).
 template <class T, int DP>
 __global__ __launch_bounds__(kThreads) void merge_kernel(Args a) {
-  const int kvh = blockIdx.x % a.hk, index = blockIdx.x / a.hk;
-  const Item it = find_item(a, index, true);
-  if (it.b < 0 || !it.divided || it.slot + it.splits > a.slots) return;
-  const int pieces = a.d / 4;
-  for (int i = threadIdx.x; i < it.rows * pieces; i += kThreads) {
-    const int row = i / pieces, col = 4 * (i % pieces);
-    float m = -INFINITY, l = 0.f;
-    f32x4 x = {};
-    for (int s = 0; s < it.splits; ++s) {
-      const float* ws = slot_at<DP>(a, it.slot + s, kvh);
-      const float ms = ws[a.ws_rows * DP + row];
-      const f32x4 xs = *reinterpret_cast<const f32x4*>(ws + row * DP + col);
-      const float to = fmaxf(m, ms);
-      const float fa = m == to ? 1.f : __builtin_amdgcn_exp2f(m - to), fb = ms == to ? 1.f : __builtin_amdgcn_exp2f(ms - to);
-      l = l * fa + ws[a.ws_rows * (DP + 1) + row] * fb;
+  __shared__ float red[kWaves];
+  __shared__ f32x4 sums[kThreads];
+  __shared__ float total[kThreads];
+  const int index = a.hk(blockIdx.x), kvh = blockIdx.x - index * a.hk.d;
+  const int tid = threadIdx.x, pieces = a.d / 4;
+  const int64_t step = static_cast<int64_t>(a.hk.d) * a.ws_rows * (DP + 2);
+  for (int unit = index;; unit += a.hk(gridDim.x)) {
+    const Item it = find_item<true>(a, unit);
+    if (it.b < 0) return;
+    if (it.slot + it.splits > a.slots) continue;
+    const float* ws = slot_at<DP>(a, it.slot, kvh);
+    if (it.splits <= kMergeParts) {
+      for (int i = tid; i < it.rows * pieces; i += kThreads) {
+        const int row = it.split + i / pieces, col = 4 * (i % pieces);
+        float m[kMergeParts], l[kMergeParts];
+        f32x4 x[kMergeParts];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = x[e] * fa + xs[e] * fb;
-      m = to;
+        for (int s = 0; s < kMergeParts; ++s) {
+          const float* p = ws + (s < it.splits ? s : 0) * step;
+          m[s] = s < it.splits ? p[a.ws_rows * DP + row] : -INFINITY;
+          l[s] = p[a.ws_rows * (DP + 1) + row];
+          x[s] = *reinterpret_cast<const f32x4*>(p + row * DP + col);
+        }
+        float top = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int s = 0; s < kMergeParts; ++s) top = fmaxf(top, m[s]);
+        f32x4 o = {};
+#pragma unroll
+        for (int s = 0; s < kMergeParts; ++s) {
+          if (s >= it.splits) break;
+          const float f = m[s] == top ? 1.f : __builtin_amdgcn_exp2f(m[s] - top);
+          sum += l[s] * f;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[e] += x[s][e] * f;
+        }
+        const float inv = inverse(sum);
+        *reinterpret_cast<u32x2*>(out_row(a, it, kvh, it.row0 + row) + col) =
+            u32x2{T::pack(o[0] * inv, o[1] * inv), T::pack(o[2] * inv, o[3] * inv)};
+      }
+      continue;
     }
-    const float inv = inverse(l);
-    *reinterpret_cast<u32x2*>(out_row(a, it, kvh, it.row0 + row) + col) =
-        u32x2{T::pack(x[0] * inv, x[1] * inv), T::pack(x[2] * inv, x[3] * inv)};
+    const int row = it.split;
+    const float* stats = ws + a.ws_rows * DP + row;
+    float top = -INFINITY;
+    for (int s = tid; s < it.splits; s += kThreads) top = fmaxf(top, stats[s * step]);
+    top = xor_butterfly<true>(top, MaxOp());
+    __syncthreads();  // the last unit's sums are read
+    if ((tid & 63) == 0) red[tid / kWave] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    const int groups = kThreads / pieces, g = tid / pieces, piece = tid - g * pieces;
+    float sum = 0.f;
+    f32x4 o = {};
+    if (g < groups) {
+#pragma unroll 8
+      for (int s = g; s < it.splits; s += groups) {
+        const float ms = stats[s * step];
+        const f32x4 xs = *reinterpret_cast<const f32x4*>(ws + s * step + row * DP + 4 * piece);
+        const float f = ms == top ? 1.f : __builtin_amdgcn_exp2f(ms - top);
+        sum += stats[s * step + a.ws_rows] * f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] += xs[e] * f;
+      }
+      sums[tid] = o;
+      total[tid] = sum;
+    }
+    __syncthreads();
+    if (g == 0) {
+      for (int n = 1; n < groups; ++n) {
+        sum += total[n * pieces + piece];
+        o += sums[n * pieces + piece];
+      }
+      const float inv = inverse(sum);
+      *reinterpret_cast<u32x2*>(out_row(a, it, kvh, it.row0 + row) + 4 * piece) =
+          u32x2{T::pack(o[0] * inv, o[1] * inv), T::pack(o[2] * inv, o[3] * inv)};
+    }
   }
 }
 
@@ -362,7 +503,8 @@ struct Append {
   const int* lengths;
   const int* table;
   int64_t k_t, k_h, v_t, v_h, kp_p, kp_t, kp_h, vp_p, vp_t, vp_h, table_stride;  // bytes, table_stride in entries
-  int tokens, seqs, pool, page, page_shift, max_keys, hk, pieces;
+  Div page;
+  int tokens, seqs, pool, max_keys, hk, pieces;
 };
 
 // E: a piece, 16 bytes where every row is made of aligned ones, else one element.
@@ -382,7 +524,7 @@ __global__ __launch_bounds__(kThreads) void append_kernel(Append a) {
     if (tok < a.cu[lo] || tok >= end) continue;
     const int64_t at = static_cast<int64_t>(a.lengths[lo]) - (end - tok);
     if (at < 0 || at >= a.max_keys) continue;
-    const int pos = static_cast<int>(at), n = a.page_shift >= 0 ? pos >> a.page_shift : pos / a.page, slot = pos - n * a.page;
+    const int pos = static_cast<int>(at), n = a.page(pos), slot = pos - n * a.page.d;
     const int id = a.table[lo * a.table_stride + n];
     if (static_cast<unsigned>(id) >= static_cast<unsigned>(a.pool)) continue;
     const auto from = [&](const void* p, int64_t t, int64_t hs) {
@@ -396,14 +538,9 @@ __global__ __launch_bounds__(kThreads) void append_kernel(Append a) {
   }
 }
 
-constexpr int kTarget = 1024;   // tiles that splitting aims at: two workgroups a CU, twice over
-constexpr int kChunkMin = 256;  // least keys of a split
-
-int page_shift_of(int page) {
-  int s = 0;
-  while ((1 << s) < page && s < 30) ++s;
-  return (1 << s) == page ? s : -1;
-}
+constexpr int kTarget = 1024;    // parts that splitting aims at where they are more than the card holds at once
+constexpr int kChunkMin = 256;   // least keys of a split
+constexpr int kMergeGrid = 1024;  // workgroups of a merge launch; each takes every such unit  // least keys of a split
 
 // Row tiles of a key head that any offsets can give: sequences of up to 64 rows have 32-row tiles.
 int64_t tiles_bound(int64_t tokens, int64_t seqs, int64_t group) {
@@ -428,10 +565,12 @@ int64_t slots_bound(int64_t tokens, int64_t seqs, int64_t group, int64_t hk, int
 
 template <class T, int DP, bool PAGED>
 int launch(const Args& a, int64_t index, int64_t merges, hipStream_t st) {
-  attention_kernel<T, DP, PAGED><<<static_cast<unsigned>(index * a.hk), kThreads, 0, st>>>(a);
+  const unsigned grid = static_cast<unsigned>(index * a.hk.d);
+  if (a.d == DP) attention_kernel<T, DP, PAGED, true><<<grid, kThreads, 0, st>>>(a);
+  else attention_kernel<T, DP, PAGED, false><<<grid, kThreads, 0, st>>>(a);
   hipError_t e = hipGetLastError();
   if (e == hipSuccess && merges > 0) {
-    merge_kernel<T, DP><<<static_cast<unsigned>(merges * a.hk), kThreads, 0, st>>>(a);
+    merge_kernel<T, DP><<<static_cast<unsigned>(merges * a.hk.d), kThreads, 0, st>>>(a);
     e = hipGetLastError();
   }
   return e == hipSuccess ? BP_OK : static_cast<int>(e);
@@ -457,8 +596,9 @@ size_t workspace_bytes(int64_t tokens, int64_t seqs, int64_t hq, int64_t hk, int
 }
 
 int run(int dtype, Args& a, bool paged, size_t ws_bytes, hipStream_t st) {
+  const int hk = a.hk.d;
   if (dtype != BP_DT_BF16 && dtype != BP_DT_F16) return BP_E_UNSUPPORTED;
-  if (a.tokens < 0 || a.seqs < 0 || a.hk <= 0 || a.hq <= 0 || a.hq % a.hk != 0 || !(a.scale_log2 > 0.f) || a.max_keys < 0)
+  if (a.tokens < 0 || a.seqs < 0 || hk <= 0 || a.hq <= 0 || a.hq % hk != 0 || !(a.scale_log2 > 0.f) || a.max_keys < 0)
     return BP_E_INVALID_ARG;
   if (a.d <= 0 || a.d % 8 != 0 || a.d > 256) return BP_E_UNSUPPORTED;
   if (a.tokens == 0) return BP_OK;
@@ -466,27 +606,35 @@ int run(int dtype, Args& a, bool paged, size_t ws_bytes, hipStream_t st) {
   if (!aligned16(a.q) || !aligned16(a.k) || !aligned16(a.v) || !aligned16(a.out) ||
       ((a.q_t | a.q_h | a.k_p | a.k_t | a.k_h | a.v_p | a.v_t | a.v_h) & 7) != 0)
     return BP_E_INVALID_ARG;
-  a.group = a.hq / a.hk;
-  // rows of a sequence, and keys plus a split, in 32 bits
-  if (static_cast<int64_t>(a.tokens) * a.hq >= (1ll << 30) || a.max_keys >= (1 << 29)) return BP_E_UNSUPPORTED;
-  const int64_t tiles = tiles_bound(a.tokens, a.seqs, a.group);
+  // rows of a sequence, keys plus a split, and the byte offsets inside a load instruction, in 32 bits
+  if (static_cast<int64_t>(a.tokens) * a.hq >= (1ll << 30) || a.max_keys >= (1 << 29) || a.k_t < 0 || a.v_t < 0 ||
+      a.k_t >= (1 << 28) || a.v_t >= (1 << 28))
+    return BP_E_UNSUPPORTED;
+  const int group = a.hq / hk, some = a.seqs < a.tokens ? a.seqs : a.tokens;
+  a.hk = Div::of(hk);
+  a.group = Div::of(group);
+  a.tile_tokens = Div::of(group < kTileLarge ? kTileLarge / group : 1);
   a.target = kTarget;
   a.chunk_min = kChunkMin;
-  a.ws_rows = slot_rows(a.tokens, a.group);
+  a.ws_rows = slot_rows(a.tokens, group);
+  const int64_t tiles = tiles_bound(a.tokens, a.seqs, group);
   int64_t index = tiles, merges = 0;
-  const size_t need = workspace_bytes(a.tokens, a.seqs, a.hq, a.hk, a.d, a.max_keys);
+  const size_t need = workspace_bytes(a.tokens, a.seqs, a.hq, hk, a.d, a.max_keys);
   if (need > 0) {
     if (a.ws == nullptr || ws_bytes < need || !aligned16(a.ws)) return BP_E_WORKSPACE;
-    a.slots = static_cast<int>(slots_bound(a.tokens, a.seqs, a.group, a.hk, a.max_keys) / a.hk);
-    const int64_t most = tiles * ((a.max_keys + kChunkMin - 1) / kChunkMin - 1), aim = kTarget / a.hk + 1;
+    a.slots = static_cast<int>(slots_bound(a.tokens, a.seqs, group, hk, a.max_keys) / hk);
+    const int64_t most = tiles * ((a.max_keys + kChunkMin - 1) / kChunkMin - 1), aim = kTarget / hk + 1;
     index += most < aim ? most : aim;
-    merges = tiles;
+    const int64_t units = static_cast<int64_t>(a.tokens) * group, wanted = kMergeGrid / hk + 1;
+    merges = units < wanted ? units : wanted;
   } else {
     a.ws = nullptr;
     a.slots = 0;
   }
   index += 1;  // rows of no sequence
-  if (index * a.hk >= (1ll << 31)) return BP_E_UNSUPPORTED;
+  if (index * hk >= (1ll << 30)) return BP_E_UNSUPPORTED;
+  // one sequence's tiles come in this order by themselves, and with a workgroup's place for every tile none is needed
+  a.order = a.seqs > 1 && a.seqs <= kWave && index * hk > kResident;
   if (dtype == BP_DT_BF16)
     return paged ? launch_dim<Bf16, true>(a, index, merges, st) : launch_dim<Bf16, false>(a, index, merges, st);
   return paged ? launch_dim<F16, true>(a, index, merges, st) : launch_dim<F16, false>(a, index, merges, st);
@@ -510,9 +658,9 @@ int bp_attn_packed(int dtype, const void* q, const void* k, const void* v, void*
   a.q = q, a.k = k, a.v = v, a.out = out, a.cu = cu;
   a.ws = static_cast<float*>(workspace);
   a.q_t = q_t, a.q_h = q_h, a.k_t = k_t, a.k_h = k_h, a.v_t = v_t, a.v_h = v_h;
-  a.tokens = tokens, a.seqs = seqs, a.hq = hq, a.hk = hk, a.d = head_dim, a.causal = causal != 0;
+  a.tokens = tokens, a.seqs = seqs, a.hq = hq, a.hk.d = hk, a.d = head_dim, a.causal = causal != 0;
   a.max_keys = tokens;
-  a.page = 1;
+  a.page = bp::attn::Div::of(1);
   a.scale_log2 = scale * 1.44269504088896340736f;
   return bp::attn::run(dtype, a, false, workspace_bytes, static_cast<hipStream_t>(stream));
 }
@@ -530,8 +678,9 @@ int bp_attn_paged(int dtype, const void* q, const void* k_pages, const void* v_p
   a.ws = static_cast<float*>(workspace);
   a.q_t = q_t, a.q_h = q_h, a.k_p = k_p, a.k_t = k_t, a.k_h = k_h, a.v_p = v_p, a.v_t = v_t, a.v_h = v_h;
   a.table_stride = table_stride;
-  a.tokens = tokens, a.seqs = seqs, a.hq = hq, a.hk = hk, a.d = head_dim, a.causal = 1;
-  a.pool = pool, a.page = page, a.page_shift = bp::attn::page_shift_of(page), a.max_keys = page * max_pages;
+  a.tokens = tokens, a.seqs = seqs, a.hq = hq, a.hk.d = hk, a.d = head_dim, a.causal = 1;
+  a.pool = pool, a.page = bp::attn::Div::of(page);
+  a.max_keys = page * max_pages;
   a.scale_log2 = scale * 1.44269504088896340736f;
   return bp::attn::run(dtype, a, true, workspace_bytes, static_cast<hipStream_t>(stream));
 }
@@ -555,7 +704,7 @@ int bp_paged_append(int element_bytes, const void* k, const void* v, void* k_pag
   a.kp_p = kp_p * element_bytes, a.kp_t = kp_t * element_bytes, a.kp_h = kp_h * element_bytes;
   a.vp_p = vp_p * element_bytes, a.vp_t = vp_t * element_bytes, a.vp_h = vp_h * element_bytes;
   a.table_stride = table_stride;
-  a.tokens = tokens, a.seqs = seqs, a.pool = pool, a.page = page, a.page_shift = bp::attn::page_shift_of(page);
+  a.tokens = tokens, a.seqs = seqs, a.pool = pool, a.page = bp::attn::Div::of(page);
   a.max_keys = page * max_pages, a.hk = hk;
   const bool wide = bp::attn::aligned16(k) && bp::attn::aligned16(v) && bp::attn::aligned16(k_pages) &&
                     bp::attn::aligned16(v_pages) && row % 16 == 0 &&

@@ -22,16 +22,22 @@ from .. import _lib
 MAX_HEAD_DIM = 256
 
 
-def _same_device(what: str, device: torch.device, *tensors: torch.Tensor | None) -> None:
-    if device.type != "cuda":
+_FLOATS = {torch.bfloat16: _lib.DT_BF16, torch.float16: _lib.DT_F16}
+
+
+def _same_device(what: str, x: torch.Tensor, *tensors: torch.Tensor | None) -> int:
+    """The index of the GPU that all tensors are on."""
+    index = x.get_device()
+    if index < 0:
         raise ValueError(f"{what}: the tensors must be on a GPU (there is no CPU path)")
     for t in tensors:
-        if t is not None and t.device != device:
-            raise ValueError(f"{what}: all tensors must be on {device}, got {t.device}")
+        if t is not None and t.get_device() != index:
+            raise ValueError(f"{what}: all tensors must be on {x.device}, got {t.device}")
+    return index
 
 
-def _no_grad(what: str, *tensors: torch.Tensor) -> None:
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+def _no_backward(what: str) -> None:
+    if torch.is_grad_enabled():
         raise ValueError(f"{what} has no backward pass: detach its inputs or use torch.no_grad()")
 
 
@@ -41,12 +47,12 @@ def _ints(what: str, name: str, t: torch.Tensor, dims: int) -> None:
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
-    """t itself where the kernel's 16-byte loads can take it as it lies, else a contiguous copy."""
-    st = t.stride()
-    if st[-1] == 1 and t.data_ptr() % 16 == 0 and all(s % 8 == 0 for s in st[:-1]):
+    """t [.., .., D] itself where the kernel's 16-byte loads can take it as it lies, else a contiguous copy."""
+    s0, s1, s2 = t.stride()
+    if s2 == 1 and not (t.data_ptr() & 15 or (s0 | s1) & 7):
         return t
     t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+    return t.clone() if t.data_ptr() & 15 else t
 
 
 def _scale(what: str, scale: float | None, d: int) -> float:
@@ -56,19 +62,24 @@ def _scale(what: str, scale: float | None, d: int) -> float:
     return scale
 
 
-def _heads(what: str, q: torch.Tensor, hk: int, d: int, *others: torch.Tensor) -> None:
-    if q.dtype not in (torch.bfloat16, torch.float16) or any(t.dtype != q.dtype for t in others):
+def _dtype(what: str, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> int:
+    code = _FLOATS.get(q.dtype)
+    if code is None or k.dtype != q.dtype or v.dtype != q.dtype:
         raise ValueError(f"{what}: q, keys and values must share one dtype, bfloat16 or float16")
-    if hk < 1 or q.shape[1] < 1 or q.shape[1] % hk:
-        raise ValueError(f"{what}: {q.shape[1]} query heads are no multiple of {hk} key heads")
-    if q.shape[2] != d or d < 8 or d > MAX_HEAD_DIM or d % 8:
+    return code
+
+
+def _heads(what: str, hq: int, hk: int, d: int, dk: int) -> None:
+    if hk < 1 or hq < 1 or hq % hk:
+        raise ValueError(f"{what}: {hq} query heads are no multiple of {hk} key heads")
+    if d != dk or d < 8 or d > MAX_HEAD_DIM or d % 8:
         raise ValueError(f"{what}: head_dim must be the same everywhere, a multiple of 8 up to {MAX_HEAD_DIM}")
 
 
 def _output(what: str, q: torch.Tensor, out: torch.Tensor | None) -> torch.Tensor:
     if out is None:
-        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    if out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous() or out.data_ptr() % 16:
+        return torch.empty_like(q, memory_format=torch.contiguous_format)
+    if out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous() or out.data_ptr() & 15:
         raise ValueError(f"{what}: out must be a contiguous 16-byte aligned {tuple(q.shape)} {q.dtype} tensor")
     return out
 
@@ -78,12 +89,14 @@ def _workspace(tokens: int, seqs: int, hq: int, hk: int, d: int, max_keys: int, 
     return (torch.empty(need, dtype=torch.uint8, device=device), need) if need else (None, 0)
 
 
-def _launch(device: torch.device, name: str, *args) -> None:
-    """One call of the library on torch's current stream of `device`."""
-    if device.index != torch.cuda.current_device():
-        with torch.cuda.device(device):
-            return _launch(device, name, *args)
-    _lib.check(getattr(_lib.lib(), name)(*args, _lib.stream_ptr(device)), name)
+def _launch(index: int, name: str, *args) -> None:
+    """One call of the library on torch's current stream of GPU `index`."""
+    if index != torch._C._cuda_getDevice():
+        with torch.cuda.device(index):
+            return _launch(index, name, *args)
+    status = getattr(_lib.lib(), name)(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status:
+        _lib.check(status, name)
 
 
 def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu: torch.Tensor, *, causal: bool = True,
@@ -96,39 +109,48 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu: torc
     if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape or k.shape[0] != q.shape[0]:
         raise ValueError(f"{what}: q must be [tokens, Hq, D] and k, v [tokens, Hk, D]")
     tokens, hq, d = q.shape
-    hk = k.shape[1]
-    _heads(what, q, hk, k.shape[2], k, v)
+    _, hk, dk = k.shape
+    dtype = _dtype(what, q, k, v)
+    _heads(what, hq, hk, d, dk)
     _ints(what, "cu", cu, 1)
-    if cu.shape[0] < 1:
+    seqs = cu.shape[0] - 1
+    if seqs < 0:
         raise ValueError(f"{what}: cu needs at least one entry")
-    _same_device(what, q.device, k, v, cu, out)
-    _no_grad(what, q, k, v)
+    index = _same_device(what, q, k, v, cu, out)
+    if q.requires_grad or k.requires_grad or v.requires_grad:
+        _no_backward(what)
     scale = _scale(what, scale, d)
     q, k, v = _rows(q), _rows(k), _rows(v)
     y = _output(what, q, out)
     if tokens == 0:
         return y
-    seqs = cu.shape[0] - 1
     ws, need = _workspace(tokens, seqs, hq, hk, d, tokens, q.device)
-    _launch(q.device, "bp_attn_packed", _lib.TORCH_DT[q.dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(), y.data_ptr(),
-            cu.data_ptr(), tokens, seqs, hq, hk, d, q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0),
-            v.stride(1), int(causal), scale, _lib.ptr(ws), need)
+    q_t, q_h, _ = q.stride()
+    k_t, k_h, _ = k.stride()
+    v_t, v_h, _ = v.stride()
+    _launch(index, "bp_attn_packed", dtype, q.data_ptr(), k.data_ptr(), v.data_ptr(), y.data_ptr(), cu.data_ptr(), tokens,
+            seqs, hq, hk, d, q_t, q_h, k_t, k_h, v_t, v_h, causal, scale, _lib.ptr(ws), need)
     return y
 
 
 def _pages(what: str, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor,
-           cu: torch.Tensor) -> None:
-    if k_pages.dim() != 4 or v_pages.shape != k_pages.shape or k_pages.shape[1] < 1:
+           cu: torch.Tensor) -> tuple:
+    """(pages, page size, Hk, D), the caches' strides, the sequences and the table's width and stride."""
+    shape = k_pages.shape
+    if len(shape) != 4 or v_pages.shape != shape or shape[1] < 1:
         raise ValueError(f"{what}: the caches must be [pages, page size, Hk, D], keys and values alike")
-    if k_pages.stride(3) != 1 or v_pages.stride(3) != 1:
+    kst, vst = k_pages.stride(), v_pages.stride()
+    if kst[3] != 1 or vst[3] != 1:
         raise ValueError(f"{what}: the caches must be contiguous in the head dimension")
     _ints(what, "table", table, 2)
     _ints(what, "lengths", lengths, 1)
     _ints(what, "cu", cu, 1)
-    if cu.shape[0] < 1 or lengths.shape[0] != cu.shape[0] - 1 or table.shape[0] != lengths.shape[0]:
+    seqs, most = table.shape
+    if lengths.shape[0] != seqs or cu.shape[0] != seqs + 1:
         raise ValueError(f"{what}: table [sequences, pages], lengths [sequences] and cu [sequences + 1] disagree")
-    if table.shape[1] * k_pages.shape[1] >= 1 << 29:
+    if most * shape[1] >= 1 << 29:
         raise ValueError(f"{what}: a sequence may have fewer than 2 ** 29 positions")
+    return shape, kst, vst, seqs, most, table.stride(0)
 
 
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor,
@@ -142,26 +164,26 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     what = "paged_attention"
     if q.dim() != 3:
         raise ValueError(f"{what}: q must be [tokens, Hq, D]")
-    _pages(what, k_pages, v_pages, table, lengths, cu)
+    (pool, page, hk, dk), kst, vst, seqs, most, row = _pages(what, k_pages, v_pages, table, lengths, cu)
     tokens, hq, d = q.shape
-    pool, page, hk, _ = k_pages.shape
-    _heads(what, q, hk, k_pages.shape[3], k_pages, v_pages)
-    for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
-        if t.data_ptr() % 16 or any(s % 8 for s in t.stride()[:3]):
-            raise ValueError(f"{what}: {name} must be 16-byte aligned, with strides of whole multiples of 8 elements")
-    _same_device(what, q.device, k_pages, v_pages, table, lengths, cu, out)
-    _no_grad(what, q, k_pages, v_pages)
+    dtype = _dtype(what, q, k_pages, v_pages)
+    _heads(what, hq, hk, d, dk)
+    k_ptr, v_ptr = k_pages.data_ptr(), v_pages.data_ptr()
+    if (k_ptr | v_ptr) & 15 or (kst[0] | kst[1] | kst[2] | vst[0] | vst[1] | vst[2]) & 7:
+        raise ValueError(f"{what}: the caches must be 16-byte aligned, with strides of whole multiples of 8 elements")
+    index = _same_device(what, q, k_pages, v_pages, table, lengths, cu, out)
+    if q.requires_grad or k_pages.requires_grad or v_pages.requires_grad:
+        _no_backward(what)
     scale = _scale(what, scale, d)
     q = _rows(q)
     y = _output(what, q, out)
     if tokens == 0:
         return y
-    seqs, most = table.shape
     ws, need = _workspace(tokens, seqs, hq, hk, d, page * most, q.device)
-    kst, vst = k_pages.stride(), v_pages.stride()
-    _launch(q.device, "bp_attn_paged", _lib.TORCH_DT[q.dtype], q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
-            y.data_ptr(), table.data_ptr(), table.stride(0), lengths.data_ptr(), cu.data_ptr(), tokens, seqs, pool, page, most,
-            hq, hk, d, q.stride(0), q.stride(1), kst[0], kst[1], kst[2], vst[0], vst[1], vst[2], scale, _lib.ptr(ws), need)
+    q_t, q_h, _ = q.stride()
+    _launch(index, "bp_attn_paged", dtype, q.data_ptr(), k_ptr, v_ptr, y.data_ptr(), table.data_ptr(), row, lengths.data_ptr(),
+            cu.data_ptr(), tokens, seqs, pool, page, most, hq, hk, d, q_t, q_h, kst[0], kst[1], kst[2], vst[0], vst[1], vst[2],
+            scale, _lib.ptr(ws), need)
     return y
 
 
@@ -173,20 +195,22 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     what = "paged_append"
     if k.dim() != 3 or v.shape != k.shape:
         raise ValueError(f"{what}: k and v must be [tokens, Hk, D]")
-    _pages(what, k_pages, v_pages, table, lengths, cu)
-    pool, page, hk, d = k_pages.shape
-    if k.shape[1:] != (hk, d):
-        raise ValueError(f"{what}: the caches hold {hk} heads of {d}, k and v {k.shape[1]} of {k.shape[2]}")
-    if k.dtype != v.dtype or k_pages.dtype != k.dtype or v_pages.dtype != k.dtype or k.element_size() not in (1, 2, 4):
+    (pool, page, hk, d), kst, vst, seqs, most, row = _pages(what, k_pages, v_pages, table, lengths, cu)
+    tokens, heads, dim = k.shape
+    if heads != hk or dim != d:
+        raise ValueError(f"{what}: the caches hold {hk} heads of {d}, k and v {heads} of {dim}")
+    dtype, size = k.dtype, k.element_size()
+    if v.dtype != dtype or k_pages.dtype != dtype or v_pages.dtype != dtype or size not in (1, 2, 4):
         raise ValueError(f"{what}: k, v and the caches must share one dtype of 1, 2 or 4 bytes")
-    if k.numel() and (k.stride(2) != 1 or v.stride(2) != 1):
+    k_t, k_h, k_d = k.stride()
+    v_t, v_h, v_d = v.stride()
+    if (k_d != 1 or v_d != 1) and k.numel():
         raise ValueError(f"{what}: k and v must be contiguous in the head dimension")
-    _same_device(what, k.device, v, k_pages, v_pages, table, lengths, cu)
-    _no_grad(what, k, v, k_pages, v_pages)
-    if k.numel() == 0:
+    index = _same_device(what, k, v, k_pages, v_pages, table, lengths, cu)
+    if k.requires_grad or v.requires_grad or k_pages.requires_grad or v_pages.requires_grad:
+        _no_backward(what)
+    if tokens == 0 or hk == 0 or d == 0:
         return
-    seqs, most = table.shape
-    kst, vst = k_pages.stride(), v_pages.stride()
-    _launch(k.device, "bp_paged_append", k.element_size(), k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
-            table.data_ptr(), table.stride(0), lengths.data_ptr(), cu.data_ptr(), k.shape[0], seqs, pool, page, most, hk, d,
-            k.stride(0), k.stride(1), v.stride(0), v.stride(1), kst[0], kst[1], kst[2], vst[0], vst[1], vst[2])
+    _launch(index, "bp_paged_append", size, k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
+            table.data_ptr(), row, lengths.data_ptr(), cu.data_ptr(), tokens, seqs, pool, page, most, hk, d, k_t, k_h, v_t, v_h,
+            kst[0], kst[1], kst[2], vst[0], vst[1], vst[2])

@@ -8,7 +8,7 @@ from typing import NamedTuple
 import torch
 
 from .. import _lib
-from .attention import _launch, _no_grad, _same_device
+from .attention import _launch, _no_backward, _same_device
 
 MAX_TOP = 32
 
@@ -30,10 +30,14 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, *,
     NaN or +inf has NaN probabilities (NaN counts as greatest in the order), and so has a row of nothing but -inf. Forward
     only: logits that require a gradient are refused."""
     what = "token_logprobs"
-    if logits.dim() != 2 or (logits.numel() and (logits.stride(1) != 1 or logits.stride(0) < 0)):
+    if logits.dim() != 2:
         raise ValueError(f"{what}: logits must be [rows, vocab], each row contiguous")
     rows, vocab = logits.shape
-    if logits.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+    row, inner = logits.stride()
+    if (inner != 1 and vocab > 1) or row < 0:
+        raise ValueError(f"{what}: logits must be [rows, vocab], each row contiguous")
+    dtype = _lib.TORCH_DT.get(logits.dtype, _lib.DT_I8)
+    if dtype == _lib.DT_I8:
         raise ValueError(f"{what}: logits must be bfloat16, float16 or float32")
     if not 0 <= top <= MAX_TOP or (rows and top > vocab):
         raise ValueError(f"{what}: top must be 0..{MAX_TOP} and at most the vocabulary, got {top}")
@@ -41,19 +45,22 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, *,
         raise ValueError(f"{what}: the vocabulary must have 1 to 2 ** 30 - 1 tokens")
     if targets is not None and (targets.dtype != torch.int64 or targets.shape != (rows,)):
         raise ValueError(f"{what}: targets must be int64 [rows]")
-    _same_device(what, logits.device, targets)
-    _no_grad(what, logits)
-    dev = logits.device
-    f32 = lambda *shape: torch.empty(*shape, dtype=torch.float32, device=dev)  # noqa: E731
-    out = TokenLogprobs(None if targets is None else f32(rows), f32(rows),
-                        torch.empty(rows, top, dtype=torch.int64, device=dev), f32(rows, top))
+    index = _same_device(what, logits, targets)
+    if logits.requires_grad:
+        _no_backward(what)
+    # one allocation for all results and the partial sums, 8-byte aligned parts first
+    need = _lib.lib().bp_logprobs_workspace_bytes(dtype, rows, vocab, top)
+    words = rows * (3 * top + 2)
+    buf = torch.empty(words + need // 4, dtype=torch.float32, device=logits.device)
+    ids = buf[:2 * rows * top].view(torch.int64).view(rows, top)
+    tops, entropy, logprob = buf[2 * rows * top:3 * rows * top].view(rows, top), buf[words - 2 * rows:words - rows], \
+        buf[words - rows:words]
+    out = TokenLogprobs(None if targets is None else logprob, entropy, ids, tops)
     if rows == 0:
         return out
-    if targets is not None:
+    if targets is not None and rows > 1:
         targets = targets.contiguous()
-    dt = _lib.TORCH_DT[logits.dtype]
-    need = _lib.lib().bp_logprobs_workspace_bytes(dt, rows, vocab, top)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    _launch(dev, "bp_logprobs", dt, logits.data_ptr(), logits.stride(0), _lib.ptr(targets), _lib.ptr(out.logprob),
-            out.entropy.data_ptr(), out.top_ids.data_ptr(), out.top_logprobs.data_ptr(), rows, vocab, top, _lib.ptr(ws), need)
+    at = buf.data_ptr()
+    _launch(index, "bp_logprobs", dtype, logits.data_ptr(), row, _lib.ptr(targets), at + 4 * (words - rows),
+            at + 4 * (words - 2 * rows), at, at + 8 * rows * top, rows, vocab, top, at + 4 * words, need)
     return out

@@ -111,6 +111,36 @@ def test_packed(lens, hq, hk, d, dtype, causal, pad, fused):
     assert not got[off[-1]:].any()
 
 
+@pytest.mark.parametrize("causal", [True, False])
+def test_packed_many_tiles_in_order(causal):
+    """More tiles than the card holds at once, of 2 to 64 sequences: they run longest first, whatever sequence they are of."""
+    g = torch.Generator(device=DEV).manual_seed(20)
+    lens = [(37 * i * i + 11) % 620 for i in range(64)]
+    off = offsets(lens)
+    q, k, v = (randn(g, off[-1] + 3, n, 64, dtype=BF) for n in (6, 3, 3))
+    print(f"\n[order] packed {off[-1]} causal={causal}", flush=True)
+    got = A.packed_attention(q, k, v, ints(off), causal=causal)
+    for a, b in zip(off, off[1:]):
+        want, bound = reference(q[a:b], k[a:b], v[a:b], 0 if causal else None, 64 ** -0.5)
+        check(got[a:b], want, bound, f"sequence at {a}")
+    assert not got[off[-1]:].any()
+
+
+def test_paged_many_tiles_in_order():
+    g = torch.Generator(device=DEV).manual_seed(21)
+    lens = [(53 * i * i + 7) % 700 for i in range(50)]
+    chunks = [min(n, (29 * i) % 300 if i % 3 else 1) for i, n in enumerate(lens)]
+    lens[7], chunks[7] = 20, 250  # the first 230 rows see nothing
+    print("\n[order] paged", flush=True)
+    kp, vp, table, ks, vs = paged_state(lens, 16, 4, 64, FP, g)
+    off = offsets(chunks)
+    q = randn(g, off[-1], 8, 64, dtype=FP)
+    got = A.paged_attention(q, kp, vp, table, ints(lens), ints(off))
+    for b, (a, z) in enumerate(zip(off, off[1:])):
+        want, bound = reference(q[a:z], ks[b], vs[b], lens[b] - chunks[b], 64 ** -0.5)
+        check(got[a:z], want, bound, f"sequence {b}")
+
+
 def test_packed_rows_before_the_first_sequence_and_a_scale():
     g = torch.Generator(device=DEV).manual_seed(2)
     q, k, v = randn(g, 90, 4, 64, dtype=BF), randn(g, 90, 2, 64, dtype=BF), randn(g, 90, 2, 64, dtype=BF)
