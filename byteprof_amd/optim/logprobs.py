@@ -51,7 +51,7 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, *,
     # one allocation for all results and the partial sums, 8-byte aligned parts first
     need = _lib.lib().bp_logprobs_workspace_bytes(dtype, rows, vocab, top)
     words = rows * (3 * top + 2)
-    buf = torch.empty(words + need // 4, dtype=torch.float32, device=logits.device)
+    buf = torch.empty(words + words % 2 + need // 4, dtype=torch.float32, device=logits.device)
     ids = buf[:2 * rows * top].view(torch.int64).view(rows, top)
     tops, entropy, logprob = buf[2 * rows * top:3 * rows * top].view(rows, top), buf[words - 2 * rows:words - rows], \
         buf[words - rows:words]
@@ -62,5 +62,5 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, *,
         targets = targets.contiguous()
     at = buf.data_ptr()
     _launch(index, "bp_logprobs", dtype, logits.data_ptr(), row, _lib.ptr(targets), at + 4 * (words - rows),
-            at + 4 * (words - 2 * rows), at, at + 8 * rows * top, rows, vocab, top, at + 4 * words, need)
+            at + 4 * (words - 2 * rows), at, at + 8 * rows * top, rows, vocab, top, at + 4 * (words + words % 2), need)
     return out

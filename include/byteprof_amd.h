@@ -456,7 +456,8 @@ int bp_paged_append(int element_bytes, const void* k, const void* v, void* k_pag
  * log softmax at targets [rows] (targets NULL: none; a target outside the row: NaN), entropy [rows] (in nats), and the `top`
  * (0 .. 32, at most vocab) most likely tokens, top_ids, top_logprobs [rows, top], in order of logit, equal ones in order of
  * index. fp32 results. A row with a NaN or +inf, and one of nothing but -inf, has NaN for every probability; NaN counts as
- * greatest in the order. workspace: bp_logprobs_workspace_bytes(dtype, rows, vocab, top).
+ * greatest in the order. workspace: bp_logprobs_workspace_bytes(dtype, rows, vocab, top)
+ * bytes, 8-byte aligned.
  * No counterpart in the reference.
  */
 size_t bp_logprobs_workspace_bytes(int dtype, int64_t rows, int64_t vocab, int top);
