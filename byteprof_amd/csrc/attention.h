@@ -24,6 +24,7 @@ constexpr int kSmallRows = 64;   // sequences of at most this many rows: 32-row 
 constexpr int kTileSmall = 32;
 constexpr int kTileLarge = 128;  // 32 rows a wave, all keys
 constexpr int kResident = 512;   // workgroups that the card holds at once (two a CU)
+constexpr int kSharedMin = 512;  // least keys of a split where the parts are more than that
 constexpr int kKeyStep = 128;    // a split's keys are a multiple of this: whole steps of either kind of tile
 
 // n / d for n below 2^30 without a division: magic = floor(2^(32 + shift) / d) + 1 with 2^shift < d <= 2^(shift + 1).
@@ -100,10 +101,10 @@ __device__ __forceinline__ int scan_add(int v) {
 // than those; else over `target`, so that ragged parts share the card evenly; never under chunk_min. (A verify round of 36 rows
 // over 41k keys: 39 us in 480 parts, 53 in 660; a decode batch of 64 ragged sequences: 219 us by the first rule, 204 to 210 by
 // the second.) Every workgroup adds the same numbers in the same order, so all of them find the same value.
-__device__ __forceinline__ int split_keys(const Args& a, int lane) {
+__device__ __forceinline__ int split_keys(const Args& a, const Seq& own, int lane) {
   float units = 0.f;
   for (int b = lane; b < a.seqs; b += kWave) {
-    const Seq s = sequence(a, b);
+    const Seq s = b < kWave ? own : sequence(a, b);
     units += static_cast<float>(s.tiles) * static_cast<float>(s.keys);
   }
   units = xor_butterfly<true>(units, AddOp()) * static_cast<float>(a.hk.d) * 1.001f;
@@ -115,10 +116,10 @@ __device__ __forceinline__ int split_keys(const Args& a, int lane) {
   const int chunk = chunk_of(kResident);
   int items = 0;
   for (int b = lane; b < a.seqs; b += kWave) {
-    const Seq s = sequence(a, b);
-    items += s.tiles * static_cast<int>(static_cast<unsigned>(s.keys + chunk - 1) / static_cast<unsigned>(chunk));
+    const Seq s = b < kWave ? own : sequence(a, b);
+    items += s.tiles * max(1, static_cast<int>(static_cast<unsigned>(s.keys + chunk / 2) / static_cast<unsigned>(chunk)));
   }
-  return wave_sum(items) <= kResident / a.hk.d ? chunk : chunk_of(a.target);
+  return wave_sum(items) <= kResident / a.hk.d ? chunk : max(chunk_of(a.target), kSharedMin);
 }
 
 // One workgroup's part: `rows` rows from row0 of sequence b, key range [key0, key1) of split `split` of `splits`. divided: the
@@ -139,18 +140,20 @@ constexpr int kUndivided = 0x3fffffff;
 template <bool MERGE>
 __device__ __forceinline__ Item find_item(const Args& a, int index) {
   const int lane = static_cast<int>(threadIdx.x) & 63;
+  Seq own = {0, 0, 0, 0, 0};  // the lane's of the first 64 sequences: read once
+  if (lane < a.seqs) own = sequence(a, lane);
   const bool divide = a.ws != nullptr;
-  const int chunk = divide ? split_keys(a, lane) : 0;
+  const int chunk = divide ? split_keys(a, own, lane) : 0;
   Item it;
   it.b = -1;
   int items = 0, slots = 0;
   for (int b0 = 0; b0 < a.seqs; b0 += kWave) {
     const int b = b0 + lane;
-    Seq s = {0, 0, 0, 0, 0};
-    if (b < a.seqs) s = sequence(a, b);
+    Seq s = own;
+    if (b0 > 0) s = b < a.seqs ? sequence(a, b) : Seq{0, 0, 0, 0, 0};
     int splits = 1, part = kUndivided, parts = 0, slot_upto = 0;
     if (divide) {
-      splits = max(1u, static_cast<unsigned>(s.keys + chunk - 1) / static_cast<unsigned>(chunk));
+      splits = max(1u, static_cast<unsigned>(s.keys + chunk / 2) / static_cast<unsigned>(chunk));
       if (splits > 1) {
         // the sequence's own splits: all alike, of whole steps
         part = (static_cast<unsigned>(s.keys + splits - 1) / static_cast<unsigned>(splits) + kKeyStep - 1) / kKeyStep * kKeyStep;

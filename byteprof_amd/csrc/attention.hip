@@ -432,14 +432,18 @@ __global__ __launch_bounds__(kThreads) void merge_kernel(Args a) {
         f32x4 x[kMergeParts];
 #pragma unroll
         for (int s = 0; s < kMergeParts; ++s) {
-          const float* p = ws + (s < it.splits ? s : 0) * step;
-          m[s] = s < it.splits ? p[a.ws_rows * DP + row] : -INFINITY;
+          if (s >= it.splits) break;
+          const float* p = ws + s * step;
+          m[s] = p[a.ws_rows * DP + row];
           l[s] = p[a.ws_rows * (DP + 1) + row];
           x[s] = *reinterpret_cast<const f32x4*>(p + row * DP + col);
         }
         float top = -INFINITY, sum = 0.f;
 #pragma unroll
-        for (int s = 0; s < kMergeParts; ++s) top = fmaxf(top, m[s]);
+        for (int s = 0; s < kMergeParts; ++s) {
+          if (s >= it.splits) break;
+          top = fmaxf(top, m[s]);
+        }
         f32x4 o = {};
 #pragma unroll
         for (int s = 0; s < kMergeParts; ++s) {

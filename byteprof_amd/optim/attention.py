@@ -42,7 +42,7 @@ def _no_backward(what: str) -> None:
 
 
 def _ints(what: str, name: str, t: torch.Tensor, dims: int) -> None:
-    if t.dtype != torch.int32 or t.dim() != dims or (t.numel() > 0 and t.stride(-1) != 1):
+    if t.dtype is not torch.int32 or t.dim() != dims or (t.stride(-1) != 1 and t.shape[-1] > 1):
         raise ValueError(f"{what}: {name} must be an int32 tensor of {dims} dimension(s), contiguous in the last")
 
 

@@ -48,19 +48,19 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, *,
     index = _same_device(what, logits, targets)
     if logits.requires_grad:
         _no_backward(what)
-    # one allocation for all results and the partial sums, 8-byte aligned parts first
-    need = _lib.lib().bp_logprobs_workspace_bytes(dtype, rows, vocab, top)
-    words = rows * (3 * top + 2)
-    buf = torch.empty(words + words % 2 + need // 4, dtype=torch.float32, device=logits.device)
-    ids = buf[:2 * rows * top].view(torch.int64).view(rows, top)
-    tops, entropy, logprob = buf[2 * rows * top:3 * rows * top].view(rows, top), buf[words - 2 * rows:words - rows], \
-        buf[words - rows:words]
-    out = TokenLogprobs(None if targets is None else logprob, entropy, ids, tops)
+    dev = logits.device
+    f32 = torch.float32
+    logprob = None if targets is None else torch.empty_strided((rows,), (1,), dtype=f32, device=dev)
+    entropy = torch.empty_strided((rows,), (1,), dtype=f32, device=dev)
+    ids = torch.empty_strided((rows, top), (top, 1), dtype=torch.int64, device=dev)
+    tops = torch.empty_strided((rows, top), (top, 1), dtype=f32, device=dev)
+    out = TokenLogprobs(logprob, entropy, ids, tops)
     if rows == 0:
         return out
     if targets is not None and rows > 1:
         targets = targets.contiguous()
-    at = buf.data_ptr()
-    _launch(index, "bp_logprobs", dtype, logits.data_ptr(), row, _lib.ptr(targets), at + 4 * (words - rows),
-            at + 4 * (words - 2 * rows), at, at + 8 * rows * top, rows, vocab, top, at + 4 * (words + words % 2), need)
+    need = _lib.lib().bp_logprobs_workspace_bytes(dtype, rows, vocab, top)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    _launch(index, "bp_logprobs", dtype, logits.data_ptr(), row, _lib.ptr(targets), _lib.ptr(logprob), entropy.data_ptr(),
+            ids.data_ptr(), tops.data_ptr(), rows, vocab, top, _lib.ptr(ws), need)
     return out
