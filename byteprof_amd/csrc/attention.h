@@ -23,7 +23,6 @@ constexpr int kWaves = kThreads / kWave;
 constexpr int kSmallRows = 64;   // sequences of at most this many rows: 32-row tiles whose waves share the keys
 constexpr int kTileSmall = 32;
 constexpr int kTileLarge = 128;  // 32 rows a wave, all keys
-constexpr int kResident = 512;   // workgroups that the card holds at once (two a CU)
 constexpr int kSharedMin = 512;  // least keys of a split where the parts are more than that
 constexpr int kKeyStep = 128;    // a split's keys are a multiple of this: whole steps of either kind of tile
 
@@ -58,7 +57,8 @@ struct Args {
   Div hk, group, page, tile_tokens;
   int tokens, seqs, pool, max_keys, hq, d, causal;
   int order;      // the longest tiles first, over all sequences (up to 64 of them)
-  int target;     // tiles that splitting aims at
+  int resident;   // workgroups that the card holds at once
+  int target;     // parts that splitting aims at where they are more
   int chunk_min;  // least keys of a split
   int ws_rows;    // rows of a partial's slot
   int slots;      // slots of a key head that ws holds
@@ -113,13 +113,13 @@ __device__ __forceinline__ int split_keys(const Args& a, const Seq& own, int lan
     const int chunk = want < 1e9f ? static_cast<int>(want) + 1 : 0x3fffff00;
     return __builtin_amdgcn_readfirstlane((max(chunk, a.chunk_min) + kKeyStep - 1) / kKeyStep * kKeyStep);
   };
-  const int chunk = chunk_of(kResident);
+  const int chunk = chunk_of(a.resident);
   int items = 0;
   for (int b = lane; b < a.seqs; b += kWave) {
     const Seq s = b < kWave ? own : sequence(a, b);
     items += s.tiles * max(1, static_cast<int>(static_cast<unsigned>(s.keys + chunk / 2) / static_cast<unsigned>(chunk)));
   }
-  return wave_sum(items) <= kResident / a.hk.d ? chunk : max(chunk_of(a.target), kSharedMin);
+  return wave_sum(items) <= a.resident / a.hk.d ? chunk : max(chunk_of(a.target), kSharedMin);
 }
 
 // One workgroup's part: `rows` rows from row0 of sequence b, key range [key0, key1) of split `split` of `splits`. divided: the

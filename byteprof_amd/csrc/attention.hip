@@ -542,7 +542,8 @@ __global__ __launch_bounds__(kThreads) void append_kernel(Append a) {
   }
 }
 
-constexpr int kTarget = 1024;    // parts that splitting aims at where they are more than the card holds at once
+constexpr int kCus = 256;
+constexpr int kTarget = 1024;    // most parts that splitting aims at: twice the workgroups that the card holds at once
 constexpr int kChunkMin = 256;   // least keys of a split
 constexpr int kMergeGrid = 1024;  // workgroups of a merge launch; each takes every such unit  // least keys of a split
 
@@ -557,13 +558,18 @@ bool may_split(int64_t max_keys) { return max_keys > kChunkMin; }
 
 int padded_dim(int d) { return d <= 64 ? 64 : d <= 96 ? 96 : d <= 128 ? 128 : 256; }
 
+// By the registers of attention_kernel: 256 columns leave one wave a SIMD, 128 two (fewer columns three, but planning for three
+// made heads of 96 no faster and cached ones slower, 97 us against 90).
+int workgroups_a_cu(int padded) { return padded > 128 ? 1 : 2; }
+
 int slot_rows(int64_t tokens, int64_t group) { return tokens * group <= kSmallRows ? kTileSmall : kTileLarge; }
 
-// Partials that any offsets can give. A sequence is divided where its keys exceed a split's, and a split's keys are at least
-// the whole work over the target: the parts are fewer than twice the target; nor are they more than every tile's most.
+// Partials that any offsets can give. A split's keys are at least the whole work over the target, and a sequence is divided
+// into as many parts as its keys come to, rounded to the nearest, from 1.5 on: at most a third more parts than the target. Nor
+// are they more than every tile's most.
 int64_t slots_bound(int64_t tokens, int64_t seqs, int64_t group, int64_t hk, int64_t max_keys) {
   const int64_t most = tiles_bound(tokens, seqs, group) * hk * ((max_keys + kChunkMin - 1) / kChunkMin);
-  const int64_t aim = 2 * kTarget + hk;
+  const int64_t aim = kTarget + kTarget / 3 + 1 + hk;
   return most < aim ? most : aim;
 }
 
@@ -618,7 +624,8 @@ int run(int dtype, Args& a, bool paged, size_t ws_bytes, hipStream_t st) {
   a.hk = Div::of(hk);
   a.group = Div::of(group);
   a.tile_tokens = Div::of(group < kTileLarge ? kTileLarge / group : 1);
-  a.target = kTarget;
+  a.resident = kCus * workgroups_a_cu(padded_dim(a.d));
+  a.target = 2 * a.resident;
   a.chunk_min = kChunkMin;
   a.ws_rows = slot_rows(a.tokens, group);
   const int64_t tiles = tiles_bound(a.tokens, a.seqs, group);
@@ -638,7 +645,7 @@ int run(int dtype, Args& a, bool paged, size_t ws_bytes, hipStream_t st) {
   index += 1;  // rows of no sequence
   if (index * hk >= (1ll << 30)) return BP_E_UNSUPPORTED;
   // one sequence's tiles come in this order by themselves, and with a workgroup's place for every tile none is needed
-  a.order = a.seqs > 1 && a.seqs <= kWave && index * hk > kResident;
+  a.order = a.seqs > 1 && a.seqs <= kWave && index * hk > a.resident;
   if (dtype == BP_DT_BF16)
     return paged ? launch_dim<Bf16, true>(a, index, merges, st) : launch_dim<Bf16, false>(a, index, merges, st);
   return paged ? launch_dim<F16, true>(a, index, merges, st) : launch_dim<F16, false>(a, index, merges, st);
