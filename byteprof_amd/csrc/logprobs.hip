@@ -428,8 +428,9 @@ __global__ __launch_bounds__(kThreads, 4) void logprobs_kernel(Args a) {
   finish<E>(a, r, s, best, count, lane);
 }
 
-// Joins a row's parts, lane p part p: the `top`-th greatest of the parts' best is a threshold, and what reaches it goes into one
-// list that is put in order.
+// Joins a row's parts, lane p part p. Where n parts have r entries each that reach a value, n r >= top, it is a threshold: the
+// n-th greatest of the parts' r-th entries, with the least r that the number of parts allows; so is every part's last entry.
+// What reaches them goes into one list that is put in order.
 template <class E>
 __global__ __launch_bounds__(kWave) void merge_kernel(Args a) {
   __shared__ __align__(16) Key list[kCap + kPad];
@@ -439,10 +440,11 @@ __global__ __launch_bounds__(kWave) void merge_kernel(Args a) {
   const int words = kStatWords + 2 * a.top;
   const float* ws = a.ws + r * a.parts * static_cast<int64_t>(words);
   Stats s = {-INFINITY, 0.f, 0.f};
+  const int deep = max(1, (a.top + a.parts - 1) / a.parts);
   uint32_t head = 0;
   if (lane < a.parts) {
     s = Stats{ws[lane * words], ws[lane * words + 1], ws[lane * words + 2]};
-    if (a.top > 0) head = static_cast<uint32_t>(*reinterpret_cast<const Key*>(ws + lane * words + kStatWords) >> 32);
+    if (a.top > 0) head = static_cast<uint32_t>(reinterpret_cast<const Key*>(ws + lane * words + kStatWords)[deep - 1] >> 32);
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) s = join(s, Stats{__shfl_xor(s.m, o), __shfl_xor(s.z, o), __shfl_xor(s.w, o)});
@@ -452,16 +454,31 @@ __global__ __launch_bounds__(kWave) void merge_kernel(Args a) {
     int rank = 0;
 #pragma unroll 16
     for (int l = 0; l < kWave; ++l) rank += static_cast<int>(static_cast<uint32_t>(__builtin_amdgcn_readlane(head, l)) > head);
-    const int nth = __builtin_ctzll(__ballot(rank == a.top - 1));
+    const int nth = __builtin_ctzll(__ballot(rank == (a.top + deep - 1) / deep - 1));
     Key threshold = static_cast<Key>(static_cast<uint32_t>(__builtin_amdgcn_readlane(head, nth)) & ~63u) << 32;
-    for (int i0 = 0; i0 < a.parts * a.top; i0 += kWave) {
-      const int i = i0 + lane, p = i / a.top, k = i - p * a.top;
-      Key e = 0;
-      if (p < a.parts) e = reinterpret_cast<const Key*>(ws + p * words + kStatWords)[k];
-      append(list, count, e > threshold, e);
-      if (count > kFull) {
-        count = cut(list, out, count, a.top, lane);
-        threshold = list[a.top - 1];
+    // nor can an entry below a part's last one be among the best, if the part has as many as are asked for
+    Key tail = lane < a.parts ? reinterpret_cast<const Key*>(ws + lane * words + kStatWords)[a.top - 1] : 0;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+      const Key other = __shfl_xor(tail, o);
+      tail = other > tail ? other : tail;
+    }
+    if (tail > threshold) threshold = tail - 1;
+    constexpr int kAhead = 4;  // entries of a lane loaded together
+    for (int i0 = 0; i0 < a.parts * a.top; i0 += kAhead * kWave) {
+      Key e[kAhead];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int i = i0 + u * kWave + lane, p = i / a.top, k = i - p * a.top;
+        e[u] = p < a.parts ? reinterpret_cast<const Key*>(ws + p * words + kStatWords)[k] : 0;
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        append(list, count, e[u] > threshold, e[u]);
+        if (count > kFull) {
+          count = cut(list, out, count, a.top, lane);
+          threshold = list[a.top - 1];
+        }
       }
     }
     count = cut(list, out, count, a.top, lane);
@@ -470,11 +487,11 @@ __global__ __launch_bounds__(kWave) void merge_kernel(Args a) {
 }
 
 constexpr int kTarget = 1024;    // workgroups that splitting rows aims at
-constexpr int kLeastPart = 256;  // least pieces of a part: one a thread
+constexpr int kLeastPart = 1024;  // least pieces of a part: a batch of every thread (with a quarter of it 126 rows of 23908 took 25 us, so 17)
 
 int parts_of(int64_t rows, int64_t vocab, int per) {
   const int64_t pieces = (vocab + per - 1) / per + 1;  // + 1: a row that begins inside a piece
-  int64_t parts = (kTarget + rows - 1) / rows;
+  int64_t parts = kTarget / rows;  // no more than the card holds at once
   const int64_t most = (pieces + kLeastPart - 1) / kLeastPart;
   parts = parts < most ? parts : most;
   return static_cast<int>(parts < 1 ? 1 : parts < kMaxParts ? parts : kMaxParts);
