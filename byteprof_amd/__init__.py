@@ -9,6 +9,12 @@ product, fused multi-step mLSTM recurrence) as hand-written gfx950 (MI355X) HIP 
   byteprof_amd.quant.select         olmo_should_quantize, ...             (byteprof/quant/select.py)
   byteprof_amd.quant.accounting     linear_bytes                          (byteprof/quant/accounting.py)
   byteprof_amd.optim.draft_fused    multistep_fw                          (byteprof/optim/draft_fused.py)
+
+and, for several sequences at once (no counterpart in the reference):
+
+  byteprof_amd.optim.attention      packed_attention, paged_append, paged_attention
+  byteprof_amd.optim.logprobs       token_logprobs
+  byteprof_amd.optim.olmo_batch     OlmoBatch
 """
 
 __version__ = "0.1.0"

@@ -367,6 +367,9 @@ __device__ __forceinline__ void finish(const Args& a, int64_t r, Stats s, const 
   if (nan && a.top > 0) order_with_nan<E>(row, a.vocab, a.top, a.top_ids + r * a.top, lane);
 }
 
+// Bound by memory without alternatives (2048 rows of 100352 in bf16: 76 us, 5.4 TB/s), by the vector unit with them (20: 106 us;
+// a logit costs about seven instructions, a quarter of the time goes to thresholds and lists). Four 16-byte pieces a thread in
+// flight while the four before are worked on: with two and six workgroups a CU 113 us.
 template <class E>
 __global__ __launch_bounds__(kThreads, 4) void logprobs_kernel(Args a) {
   __shared__ __align__(16) Key lists[kWaves][kCap + kPad];
