@@ -85,6 +85,8 @@ PACKED = [
     ([1500, 900], 2, 1, 128, BF, True, 0, False),  # long, few heads: the keys of a tile are divided
     ([1500], 1, 1, 256, FP, False, 0, False),
     ([700] * 3 + [0] * 70 + [5] * 70, 1, 1, 64, BF, True, 0, False),  # more sequences than a wave's lanes
+    ([3, 40, 1], 200, 1, 64, BF, True, 2, False),  # more query heads to a key head than a tile has rows
+    ([9, 30], 129, 3, 72, FP, False, 0, False),
 ]
 
 
@@ -197,6 +199,11 @@ PAGED = [
     ([2049], [2], 16, 1, 1, 256, FP),
     ([4, 0, 2], [4, 0, 2], 16, 2, 1, 64, BF),
     ([40 + i for i in range(130)], [1 + i % 3 for i in range(130)], 16, 2, 1, 64, FP),
+    ([600 + i for i in range(70)], [1 + 40 * (i % 2) for i in range(70)], 16, 2, 1, 64, BF),  # divided, more than 64 sequences
+    ([300, 77, 129], [1, 70, 129], 2, 3, 1, 128, BF),  # pages smaller than a load instruction's rows, and than a block's share
+    ([300, 77, 700], [1, 70, 65], 5, 4, 2, 256, BF),
+    ([260, 900], [3, 40], 3, 160, 1, 64, FP),
+    ([4000, 3900, 10], [1, 1, 1], 12, 4, 1, 72, BF),
 ]
 
 
