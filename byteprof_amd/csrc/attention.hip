@@ -551,7 +551,7 @@ __global__ __launch_bounds__(kThreads) void append_kernel(Append a) {
 
 constexpr int kCus = 256;
 constexpr int kTarget = 1024;    // most parts that splitting aims at: twice the workgroups that the card holds at once
-constexpr int kChunkMin = 256;   // least keys of a split
+constexpr int kChunkMin = BP_ATTN_UNDIVIDED_KEYS;  // least keys of a split
 constexpr int kMergeGrid = 1024;  // workgroups of a merge launch; each takes every such unit  // least keys of a split
 
 // Row tiles of a key head that any offsets can give: sequences of up to 64 rows have 32-row tiles.

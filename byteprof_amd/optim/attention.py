@@ -20,6 +20,7 @@ import torch
 from .. import _lib
 
 MAX_HEAD_DIM = 256
+UNDIVIDED_KEYS = 256  # a sequence's keys up to here are never divided: no workspace
 
 
 _FLOATS = {torch.bfloat16: _lib.DT_BF16, torch.float16: _lib.DT_F16}
@@ -42,7 +43,7 @@ def _no_backward(what: str) -> None:
 
 
 def _ints(what: str, name: str, t: torch.Tensor, dims: int) -> None:
-    if t.dtype is not torch.int32 or t.dim() != dims or (t.stride(-1) != 1 and t.shape[-1] > 1):
+    if t.dtype is not torch.int32 or t.dim() != dims or not (t.is_contiguous() or t.stride(-1) == 1):
         raise ValueError(f"{what}: {name} must be an int32 tensor of {dims} dimension(s), contiguous in the last")
 
 
@@ -85,6 +86,8 @@ def _output(what: str, q: torch.Tensor, out: torch.Tensor | None) -> torch.Tenso
 
 
 def _workspace(tokens: int, seqs: int, hq: int, hk: int, d: int, max_keys: int, device: torch.device):
+    if max_keys <= UNDIVIDED_KEYS:
+        return None, 0
     need = _lib.lib().bp_attn_workspace_bytes(tokens, seqs, hq, hk, d, max_keys)
     return (torch.empty(need, dtype=torch.uint8, device=device), need) if need else (None, 0)
 
@@ -145,12 +148,12 @@ def _pages(what: str, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch
     _ints(what, "table", table, 2)
     _ints(what, "lengths", lengths, 1)
     _ints(what, "cu", cu, 1)
-    seqs, most = table.shape
+    (seqs, most), (row, _) = table.shape, table.stride()
     if lengths.shape[0] != seqs or cu.shape[0] != seqs + 1:
         raise ValueError(f"{what}: table [sequences, pages], lengths [sequences] and cu [sequences + 1] disagree")
     if most * shape[1] >= 1 << 29:
         raise ValueError(f"{what}: a sequence may have fewer than 2 ** 29 positions")
-    return shape, kst, vst, seqs, most, table.stride(0)
+    return shape, kst, vst, seqs, most, row
 
 
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor,

@@ -431,6 +431,7 @@ int bp_decode_argmax_rows(const void* logits, int vocab, int rows, int64_t* tok,
  * divided keys (max_keys: tokens, or page x max_pages for the cache); nothing in it outlives the call.
  * No counterpart in the reference (batch 1, one contiguous cache).
  */
+#define BP_ATTN_UNDIVIDED_KEYS 256 /* up to this many keys a sequence is never divided: no workspace */
 size_t bp_attn_workspace_bytes(int64_t tokens, int64_t seqs, int64_t hq, int64_t hk, int64_t head_dim, int64_t max_keys);
 int bp_attn_packed(int dtype, const void* q, const void* k, const void* v, void* out, const int32_t* cu, int tokens, int seqs,
                    int hq, int hk, int head_dim, int64_t q_t, int64_t q_h, int64_t k_t, int64_t k_h, int64_t v_t, int64_t v_h,

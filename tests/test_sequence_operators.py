@@ -4,6 +4,8 @@ entries. CPU only: every call here returns or raises before anything is enqueued
 from __future__ import annotations
 
 import ctypes
+import re
+from pathlib import Path
 
 import pytest
 import torch
@@ -170,7 +172,10 @@ def test_logprobs_entry_refuses_before_any_launch(L):
 
 def test_workspace_of_attention(L):
     """None where no sequence can have more keys than a split; within a bound of the target elsewhere."""
-    assert L.bp_attn_workspace_bytes(64, 64, 32, 8, 128, 256) == 0
+    text = (Path(__file__).resolve().parent.parent / "include" / "byteprof_amd.h").read_text()
+    assert int(re.search(r"#define BP_ATTN_UNDIVIDED_KEYS (\d+)", text).group(1)) == A.UNDIVIDED_KEYS
+    assert L.bp_attn_workspace_bytes(64, 64, 32, 8, 128, A.UNDIVIDED_KEYS) == 0
+    assert L.bp_attn_workspace_bytes(64, 64, 32, 8, 128, A.UNDIVIDED_KEYS + 1) > 0
     assert L.bp_attn_workspace_bytes(0, 1, 8, 8, 128, 10000) == 0
     small = L.bp_attn_workspace_bytes(1, 1, 16, 16, 128, 512)  # 16 heads, 2 parts, 32 rows
     assert small == 16 * 2 * 32 * (128 + 2) * 4
