@@ -130,7 +130,7 @@ struct Item {
   bool small, divided;
 };
 
-constexpr int kMergeRows = 32;    // rows of a unit of the merge where there are at most kMergeParts parts, else one
+constexpr int kMergeRows = 32;  // rows of a unit of the merge; of up to 64 rows with more than kMergeParts parts, one
 constexpr int kMergeParts = 8;
 constexpr int kLevel = 128;  // keys of a level, of which the order of the tiles is made
 constexpr int kUndivided = 0x3fffffff;
@@ -189,7 +189,8 @@ __device__ __forceinline__ Item find_item(const Args& a, int index) {
       at = from - __builtin_amdgcn_readlane(upto - count, l);
       above = __builtin_amdgcn_readlane(before, l);
     } else {
-      const int count = !MERGE ? all : splits == 1 ? 0 : splits > kMergeParts ? s.rows : (s.rows + kMergeRows - 1) / kMergeRows;
+      const bool single = splits > kMergeParts && s.rows <= kSmallRows;
+      const int count = !MERGE ? all : splits == 1 ? 0 : single ? s.rows : (s.rows + kMergeRows - 1) / kMergeRows;
       const int upto = scan_add(count);
       const uint64_t over = __ballot(items + upto > index);
       if (over == 0) {
@@ -211,7 +212,7 @@ __device__ __forceinline__ Item find_item(const Args& a, int index) {
     const int tile_rows = it.small ? kTileSmall : kTileLarge;
     // the last rows first: under a causal mask they have the most keys
     const int done = it.divided && !MERGE ? static_cast<unsigned>(at) / static_cast<unsigned>(it.splits) : at;
-    const int unit = MERGE && it.splits <= kMergeParts ? kMergeRows : 1;
+    const int unit = MERGE && (it.splits <= kMergeParts || !it.small) ? kMergeRows : 1;
     const int tile = MERGE ? at * unit / tile_rows : tiles - 1 - above - done;
     it.split = it.divided ? at - done * it.splits : 0;
     it.slot = slots + __builtin_amdgcn_readlane(slot_upto - parts, l) + tile * it.splits;

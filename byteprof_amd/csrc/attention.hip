@@ -415,8 +415,8 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void attention_kernel(A
   else large_tile<T, DP, PAGED, FULL>(a, it, kvh, smem, ring);
 }
 
-// Joins the partials of a unit's rows: the parts' sums, each times exp2 of its maximum less the greatest. Few parts: a thread
-// has 4 columns of a row and loads all parts at once. Many: the workgroup has one row, whose parts its groups of
+// Joins the partials of a unit's rows: the parts' sums, each times exp2 of its maximum less the greatest. Few parts or many rows: a thread
+// has 4 columns of a row and loads 8 parts at once. Few rows of many parts: the workgroup has one row, whose parts its groups of
 // d / 4 threads share (one thread after another part took 30 us for 80 parts of 36 rows).
 template <class T, int DP>
 __global__ __launch_bounds__(kThreads) void merge_kernel(Args a) {
@@ -431,33 +431,41 @@ __global__ __launch_bounds__(kThreads) void merge_kernel(Args a) {
     if (it.b < 0) return;
     if (it.slot + it.splits > a.slots) continue;
     const float* ws = slot_at<DP>(a, it.slot, kvh);
-    if (it.splits <= kMergeParts) {
+    if (it.splits <= kMergeParts || !it.small) {
       for (int i = tid; i < it.rows * pieces; i += kThreads) {
         const int row = it.split + i / pieces, col = 4 * (i % pieces);
-        float m[kMergeParts], l[kMergeParts];
-        f32x4 x[kMergeParts];
-#pragma unroll
-        for (int s = 0; s < kMergeParts; ++s) {
-          if (s >= it.splits) break;
-          const float* p = ws + s * step;
-          m[s] = p[a.ws_rows * DP + row];
-          l[s] = p[a.ws_rows * (DP + 1) + row];
-          x[s] = *reinterpret_cast<const f32x4*>(p + row * DP + col);
-        }
         float top = -INFINITY, sum = 0.f;
-#pragma unroll
-        for (int s = 0; s < kMergeParts; ++s) {
-          if (s >= it.splits) break;
-          top = fmaxf(top, m[s]);
-        }
         f32x4 o = {};
+        for (int s0 = 0; s0 < it.splits; s0 += kMergeParts) {
+          float m[kMergeParts], l[kMergeParts];
+          f32x4 x[kMergeParts];
 #pragma unroll
-        for (int s = 0; s < kMergeParts; ++s) {
-          if (s >= it.splits) break;
-          const float f = m[s] == top ? 1.f : __builtin_amdgcn_exp2f(m[s] - top);
-          sum += l[s] * f;
+          for (int s = 0; s < kMergeParts; ++s) {
+            if (s0 + s >= it.splits) break;
+            const float* p = ws + (s0 + s) * step;
+            m[s] = p[a.ws_rows * DP + row];
+            l[s] = p[a.ws_rows * (DP + 1) + row];
+            x[s] = *reinterpret_cast<const f32x4*>(p + row * DP + col);
+          }
+          float now = top;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[e] += x[s][e] * f;
+          for (int s = 0; s < kMergeParts; ++s) {
+            if (s0 + s >= it.splits) break;
+            now = fmaxf(now, m[s]);
+          }
+          const float before = top == now ? 1.f : __builtin_amdgcn_exp2f(top - now);
+          top = now;
+          sum *= before;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[e] *= before;
+#pragma unroll
+          for (int s = 0; s < kMergeParts; ++s) {
+            if (s0 + s >= it.splits) break;
+            const float f = m[s] == top ? 1.f : __builtin_amdgcn_exp2f(m[s] - top);
+            sum += l[s] * f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] += x[s][e] * f;
+          }
         }
         const float inv = inverse(sum);
         *reinterpret_cast<u32x2*>(out_row(a, it, kvh, it.row0 + row) + col) =

@@ -204,6 +204,7 @@ PAGED = [
     ([300, 77, 700], [1, 70, 65], 5, 4, 2, 256, BF),
     ([260, 900], [3, 40], 3, 160, 1, 64, FP),
     ([4000, 3900, 10], [1, 1, 1], 12, 4, 1, 72, BF),
+    ([6000], [150], 16, 1, 1, 64, BF),  # large tiles of many parts
 ]
 
 
