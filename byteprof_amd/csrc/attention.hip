@@ -1,5 +1,5 @@
 // Attention of packed prompts and of chunks over a paged cache, and the append to the cache's pages (attention.h: the
-// mathematics and the plan).
+// mathematics; attention_plan.h: the plan).
 
 #include "attention.h"
 
@@ -571,68 +571,30 @@ __global__ __launch_bounds__(kThreads) void append_kernel(Append a) {
   }
 }
 
-constexpr int kCus = 256;
-constexpr int kTarget = 1024;    // most parts that splitting aims at: twice the workgroups that the card holds at once
-constexpr int kChunkMin = BP_ATTN_UNDIVIDED_KEYS;  // least keys of a split
-constexpr int kMergeGrid = 1024;  // workgroups of a merge launch; each takes every such unit  // least keys of a split
-
-// Row tiles of a key head that any offsets can give: sequences of up to 64 rows have 32-row tiles.
-int64_t tiles_bound(int64_t tokens, int64_t seqs, int64_t group) {
-  const int64_t rows = tokens * group, some = seqs < tokens ? seqs : tokens;
-  const int64_t a = rows / kTileLarge + 2 * some, b = rows / kTileSmall + some;
-  return a < b ? a : b;
-}
-
-bool may_split(int64_t max_keys) { return max_keys > kChunkMin; }
-
-int padded_dim(int d) { return d <= 64 ? 64 : d <= 96 ? 96 : d <= 128 ? 128 : 256; }
-
-// By the registers of attention_kernel: 256 columns leave one wave a SIMD, 128 two (fewer columns three, but planning for three
-// made heads of 96 no faster and cached ones slower, 97 us against 90).
-int workgroups_a_cu(int padded) { return padded > 128 ? 1 : 2; }
-
-int slot_rows(int64_t tokens, int64_t group) { return tokens * group <= kSmallRows ? kTileSmall : kTileLarge; }
-
-// Partials that any offsets can give. A split's keys are at least the whole work over the target, and a sequence is divided
-// into as many parts as its keys come to, rounded to the nearest, from 1.5 on: at most a third more parts than the target. Nor
-// are they more than every tile's most.
-int64_t slots_bound(int64_t tokens, int64_t seqs, int64_t group, int64_t hk, int64_t max_keys) {
-  const int64_t most = tiles_bound(tokens, seqs, group) * hk * ((max_keys + kChunkMin - 1) / kChunkMin);
-  const int64_t aim = kTarget + kTarget / 3 + 1 + hk;
-  return most < aim ? most : aim;
-}
-
 template <class T, int DP, bool PAGED>
-int launch(const Args& a, int64_t index, int64_t merges, hipStream_t st) {
-  const unsigned grid = static_cast<unsigned>(index * a.hk.d);
+int launch(const Args& a, const Launch& n, hipStream_t st) {
+  const unsigned grid = static_cast<unsigned>(n.index * a.hk.d);
   if (a.d == DP) attention_kernel<T, DP, PAGED, true><<<grid, kThreads, 0, st>>>(a);
   else attention_kernel<T, DP, PAGED, false><<<grid, kThreads, 0, st>>>(a);
   hipError_t e = hipGetLastError();
-  if (e == hipSuccess && merges > 0) {
-    merge_kernel<T, DP><<<static_cast<unsigned>(merges * a.hk.d), kThreads, 0, st>>>(a);
+  if (e == hipSuccess && n.merges > 0) {
+    merge_kernel<T, DP><<<static_cast<unsigned>(n.merges * a.hk.d), kThreads, 0, st>>>(a);
     e = hipGetLastError();
   }
   return e == hipSuccess ? BP_OK : static_cast<int>(e);
 }
 
 template <class T, bool PAGED>
-int launch_dim(const Args& a, int64_t index, int64_t merges, hipStream_t st) {
+int launch_dim(const Args& a, const Launch& n, hipStream_t st) {
   switch (padded_dim(a.d)) {
-    case 64: return launch<T, 64, PAGED>(a, index, merges, st);
-    case 96: return launch<T, 96, PAGED>(a, index, merges, st);
-    case 128: return launch<T, 128, PAGED>(a, index, merges, st);
-    default: return launch<T, 256, PAGED>(a, index, merges, st);
+    case 64: return launch<T, 64, PAGED>(a, n, st);
+    case 96: return launch<T, 96, PAGED>(a, n, st);
+    case 128: return launch<T, 128, PAGED>(a, n, st);
+    default: return launch<T, 256, PAGED>(a, n, st);
   }
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-
-size_t workspace_bytes(int64_t tokens, int64_t seqs, int64_t hq, int64_t hk, int64_t d, int64_t max_keys) {
-  if (tokens <= 0 || seqs <= 0 || hk <= 0 || hq % hk != 0 || d <= 0 || d > 256 || !may_split(max_keys)) return 0;
-  const int64_t group = hq / hk;
-  return static_cast<size_t>(slots_bound(tokens, seqs, group, hk, max_keys)) * slot_rows(tokens, group) *
-         (padded_dim(static_cast<int>(d)) + 2) * sizeof(float);
-}
 
 int run(int dtype, Args& a, bool paged, size_t ws_bytes, hipStream_t st) {
   const int hk = a.hk.d;
@@ -649,35 +611,13 @@ int run(int dtype, Args& a, bool paged, size_t ws_bytes, hipStream_t st) {
   if (static_cast<int64_t>(a.tokens) * a.hq >= (1ll << 30) || a.max_keys >= (1 << 29) || a.k_t < 0 || a.v_t < 0 ||
       a.k_t >= (1 << 28) || a.v_t >= (1 << 28))
     return BP_E_UNSUPPORTED;
-  const int group = a.hq / hk, some = a.seqs < a.tokens ? a.seqs : a.tokens;
-  a.hk = Div::of(hk);
-  a.group = Div::of(group);
-  a.tile_tokens = Div::of(group < kTileLarge ? kTileLarge / group : 1);
-  a.resident = kCus * workgroups_a_cu(padded_dim(a.d));
-  a.target = 2 * a.resident;
-  a.chunk_min = kChunkMin;
-  a.ws_rows = slot_rows(a.tokens, group);
-  const int64_t tiles = tiles_bound(a.tokens, a.seqs, group);
-  int64_t index = tiles, merges = 0;
-  const size_t need = workspace_bytes(a.tokens, a.seqs, a.hq, hk, a.d, a.max_keys);
-  if (need > 0) {
-    if (a.ws == nullptr || ws_bytes < need || !aligned16(a.ws)) return BP_E_WORKSPACE;
-    a.slots = static_cast<int>(slots_bound(a.tokens, a.seqs, group, hk, a.max_keys) / hk);
-    const int64_t most = tiles * ((a.max_keys + kChunkMin - 1) / kChunkMin - 1), aim = kTarget / hk + 1;
-    index += most < aim ? most : aim;
-    const int64_t units = static_cast<int64_t>(a.tokens) * group, wanted = kMergeGrid / hk + 1;
-    merges = units < wanted ? units : wanted;
-  } else {
-    a.ws = nullptr;
-    a.slots = 0;
-  }
-  index += 1;  // rows of no sequence
-  if (index * hk >= (1ll << 30)) return BP_E_UNSUPPORTED;
-  // one sequence's tiles come in this order by themselves, and with a workgroup's place for every tile none is needed
-  a.order = a.seqs > 1 && a.seqs <= kWave && index * hk > a.resident;
+  Launch n;
+  if (!plan_launch(a, n)) return BP_E_UNSUPPORTED;
+  if (n.workspace > 0 && (a.ws == nullptr || ws_bytes < n.workspace || !aligned16(a.ws))) return BP_E_WORKSPACE;
+  if (n.workspace == 0) a.ws = nullptr;
   if (dtype == BP_DT_BF16)
-    return paged ? launch_dim<Bf16, true>(a, index, merges, st) : launch_dim<Bf16, false>(a, index, merges, st);
-  return paged ? launch_dim<F16, true>(a, index, merges, st) : launch_dim<F16, false>(a, index, merges, st);
+    return paged ? launch_dim<Bf16, true>(a, n, st) : launch_dim<Bf16, false>(a, n, st);
+  return paged ? launch_dim<F16, true>(a, n, st) : launch_dim<F16, false>(a, n, st);
 }
 
 }  // namespace
