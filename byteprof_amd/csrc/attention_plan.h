@@ -46,7 +46,7 @@ struct Args {
   int64_t k_p, k_t, k_h;       // page (paged), position, head
   int64_t v_p, v_t, v_h;
   int64_t table_stride;
-  Div hk, group, page, tile_tokens;
+  Div hk, group, page;
   int tokens, seqs, pool, max_keys, hq, d, causal;
   int order;      // the longest tiles first, over all sequences (up to 64 of them)
   int resident;   // workgroups that the card holds at once
@@ -157,13 +157,16 @@ __device__ __forceinline__ Item find_item(const Args& a, int index) {
     int l, at, above = 0;  // the sequence's lane, the place among its items, the tiles of it that come earlier
     if (!MERGE && a.order) {
       // Tiles by level, the number of keys in steps, from the greatest down; within a level by sequence. later(x): how many
-      // tiles of the lane's sequence have level x or more. A causal tile's level grows with its place, others' are alike.
+      // tiles of the lane's sequence have level x or more. A causal tile's level grows with its place, others' are alike. No
+      // tile has level hi: a causal one has it only if its sequence's last token is that far, whatever the rows of a token.
       const bool ladder = a.causal && s.rows > kSmallRows && splits == 1;
-      const int flat = min(s.keys, part) / kLevel, first = max(s.keys - s.count, 0), step = a.tile_tokens.d;
+      const int flat = min(s.keys, part) / kLevel, first = max(s.keys - s.count, 0);
       const auto later = [&](int x) {
         if (!ladder) return flat >= x ? s.tiles : 0;
-        const int need = x * kLevel - first;
-        return s.tiles - min(s.tiles, need <= 0 ? 0 : max(a.tile_tokens(need + step - 1) - 1, 0));
+        const int need = x * kLevel - first;  // tokens of the sequence up to the level's first
+        if (need > s.count) return 0;
+        if (need <= 0) return s.tiles;
+        return s.tiles + 1 - static_cast<int>((static_cast<unsigned>(need * a.group.d) + kTileLarge - 1) / kTileLarge);
       };
       if (wave_sum(all) <= index) {
         items = wave_sum(all);
@@ -275,7 +278,6 @@ inline bool plan_launch(Args& a, Launch& n) {
   const int hk = a.hk.d, group = a.hq / hk;
   a.hk = Div::of(hk);
   a.group = Div::of(group);
-  a.tile_tokens = Div::of(group < kTileLarge ? kTileLarge / group : 1);
   a.resident = kCus * workgroups_a_cu(padded_dim(a.d));
   a.target = 2 * a.resident;
   a.chunk_min = kChunkMin;

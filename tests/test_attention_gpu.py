@@ -421,3 +421,30 @@ def test_gpu_refusals():
         A.paged_attention(q, odd, kp, table, lens, cu)
     with pytest.raises(ValueError, match="out must be"):
         A.packed_attention(q, q, q, cu, out=torch.zeros(4, 2, 64, dtype=FP, device=DEV))
+
+
+@pytest.mark.parametrize("counts,lens,hq,hk,d,dtype", [
+    ([100, 1000], None, 200, 1, 64, BF),
+    ([0, 700, 3], None, 160, 1, 96, FP),
+    ([30, 500], None, 387, 3, 256, BF),
+    ([0, 40, 500], [0, 900, 500], 400, 2, 64, BF),
+    ([3, 600, 2], [3, 600, 200], 129, 1, 128, FP),
+])
+def test_more_query_heads_than_a_tile_has_rows_in_order(counts, lens, hq, hk, d, dtype):
+    """More than 128 query heads to a key head and more tiles than the card holds at once, the long sequence not the first."""
+    print(f"\n[heads] {counts} {lens} {hq}/{hk} x {d} {dtype}", flush=True)
+    g = torch.Generator(device=DEV).manual_seed(30)
+    off = offsets(counts)
+    q = randn(g, off[-1], hq, d, dtype=dtype)
+    out = torch.full_like(q, math.nan)
+    if lens is None:
+        k, v = randn(g, off[-1], hk, d, dtype=dtype), randn(g, off[-1], hk, d, dtype=dtype)
+        A.packed_attention(q, k, v, ints(off), out=out)
+        ks, vs, firsts = [k[a:z] for a, z in zip(off, off[1:])], [v[a:z] for a, z in zip(off, off[1:])], [0] * len(counts)
+    else:
+        kp, vp, table, ks, vs = paged_state(lens, 16, hk, d, dtype, g)
+        A.paged_attention(q, kp, vp, table, ints(lens), ints(off), out=out)
+        firsts = [n - c for n, c in zip(lens, counts)]
+    for b, (a, z) in enumerate(zip(off, off[1:])):
+        want, bound = reference(q[a:z], ks[b], vs[b], firsts[b], d ** -0.5)
+        check(out[a:z], want, bound, f"sequence {b}")

@@ -70,3 +70,13 @@ def test_every_part_once(plan):
     rng = random.Random(1)
     answers = plan([draw(rng, (1, 1, 2, 3, 4, 5, 7, 8, 16, 28, 40, 64, 100, 127, 128)) for _ in range(80)])
     assert sum("ordered 1" in a for a in answers) >= 15 and sum(not a.endswith("divided 0") for a in answers) >= 15
+
+
+def test_more_query_heads_than_a_tile_has_rows(plan):
+    """A token's rows are more than one tile: long sequences behind short ones and behind empty ones, in the order of the tiles."""
+    cases = [packed([10, 4000], 160, 1), packed([0, 3000], 200, 1), packed([100, 1000], 200, 1), packed([5, 300], 256, 1),
+             packed([30, 900], 192, 1, 128), paged([0, 40, 700], [0, 9000, 700], 400, 2, 256), packed([4, 0, 900, 3], 512, 1),
+             paged([3, 600, 2], [3, 600, 2], 129, 1)]
+    assert all("ordered 1" in a for a in plan(cases))
+    rng = random.Random(2)
+    plan([draw(rng, (129, 160, 192, 200, 255, 256, 300, 512)) for _ in range(40)])
