@@ -5,15 +5,16 @@
 // in units of log2: d = x log2(e) - m2 is one fused multiply-add, with m2 = m log2(e) rounded once and used everywhere. A wave
 // keeps one running m2 (all lanes the same) and its lanes' own z and w relative to it; a batch of logits that holds a greater
 // one rescales them: z' = f z, w' = f (w + dm z) with f = exp2(dm), dm = m2 - m2'. Held in fp32: logits as they are,
-// exponentials, sums.
+// exponentials, sums. m2 starts at -kFar: what lies far below it (masked tokens, whatever value masks them) adds nothing.
 //
 // The most likely tokens, greater logit first, then lower index: a wave appends the batch's logits above its threshold to a
 // list in LDS; a full list is cut to its best `top`, whose last is the new threshold, and every wave uses the greatest
 // threshold of its workgroup (`top` entries reach each of them, so no answer depends on which it saw).
 //
-// Two kinds of rows are done again by plain passes over memory: those whose z is NaN (a NaN or +inf among the logits makes
-// every log probability NaN, as log softmax does; NaN counts as greatest in the order), and those whose greatest logit is so
-// low that its product with log2(e) passes the type's range.
+// Two kinds of rows are done again by plain passes over memory: the order of those whose z is NaN (a NaN or +inf among the
+// logits makes every log probability NaN, as log softmax does; NaN counts as greatest in the order), and the statistics of those
+// whose m2 is kFar = 2^24 or more either way. There a step of m2 is more than 1: what its rounding leaves goes into the exponent
+// of every term, and from 2^31 on out of exp2's range. Those take the difference of the logits first.
 
 #include "byteprof_amd.h"
 #include "common.h"
@@ -33,6 +34,7 @@ constexpr int kMaxParts = 64;  // workgroups of a row: one lane each in the merg
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
 constexpr int kNoIndex = 0x7fffffff;
+constexpr float kFar = 16777216.f;
 
 struct Args {
   const void* logits;
@@ -133,9 +135,8 @@ struct Stats {
 __device__ __forceinline__ Stats join(const Stats& a, const Stats& b) {
   Stats r;
   r.m = fmaxf(a.m, b.m);
-  const float base = r.m == -INFINITY ? 0.f : r.m;
   const auto part = [&](const Stats& s, float& z, float& w) {
-    const float dm = s.m == r.m ? 0.f : s.m - base;  // s.m = -inf: nothing in it, z = w = 0
+    const float dm = s.m == r.m ? 0.f : s.m - r.m;  // (both may be +inf)
     const float f = s.m == r.m ? 1.f : __builtin_amdgcn_exp2f(dm);
     z += f * s.z;
     w += f == 0.f ? 0.f * s.z : f * (s.w + dm * s.z);
@@ -211,7 +212,7 @@ struct Pass {
 
   // The batches from `first` on. lanes: LDS for the workgroup's first maxima; shared: for the waves' thresholds.
   __device__ __forceinline__ void run(int first, uint32_t* lanes, volatile uint32_t* shared, int wave) {
-    s = Stats{-INFINITY, 0.f, 0.f};
+    s = Stats{-kFar, 0.f, 0.f};
     raise(0);
     count = 0;
     least = head > 0 ? 1 : 0;
@@ -243,17 +244,14 @@ struct Pass {
       if (p0 + kThreads * kVectors < last) fetch(p0 + kThreads * kVectors, raw);  // while this batch is worked on
       if (__any(best * kLog2e > s.m)) {
         const float m = wave_max(best) * kLog2e;
-        if (s.m != -INFINITY) {
-          const float dm = s.m - m, f = __builtin_amdgcn_exp2f(dm);
-          s.w = f == 0.f ? 0.f * s.z : f * (s.w + dm * s.z);
-          s.z *= f;
-        }
+        const float dm = s.m - m, f = __builtin_amdgcn_exp2f(dm);
+        s.w = f == 0.f ? 0.f * s.z : f * (s.w + dm * s.z);
+        s.z *= f;
         s.m = m;
       }
-      const float shift = s.m == -INFINITY ? 0.f : -s.m;
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const float d = fmaf(x[i], kLog2e, shift), e = __builtin_amdgcn_exp2f(d);
+        const float d = fmaf(x[i], kLog2e, -s.m), e = __builtin_amdgcn_exp2f(d);
         s.z += e;
         s.w += e * fmaxf(d, -256.f);  // 0 at -inf
       }
@@ -318,10 +316,10 @@ __device__ void order_with_nan(const E* row, int vocab, int top, int64_t* ids, i
   }
 }
 
-// A row whose greatest logit times log2(e) passes the range: the statistics again, with the difference taken first. Relative to
-// m = 0 in the form that finish() takes: the greatest logit itself comes back in `greatest`.
+// A row whose m2 is kFar or more: the statistics again, with the difference taken first. Relative to m = 0 in the form that
+// finish() takes: the greatest logit itself comes back in `greatest`.
 template <class E>
-__device__ Stats lowest_row(const E* row, int vocab, float& greatest, int lane) {
+__device__ Stats far_row(const E* row, int vocab, float& greatest, int lane) {
   float m = -INFINITY, z = 0.f, w = 0.f;
   for (int i = lane; i < vocab; i += kWave) m = fmaxf(m, Type<E>::value(as_global(row)[i]));
   m = wave_max(m);
@@ -339,12 +337,7 @@ template <class E>
 __device__ __forceinline__ void finish(const Args& a, int64_t r, Stats s, const Key* list, int count, int lane) {
   const E* row = static_cast<const E*>(a.logits) + r * a.stride;
   float base = 0.f;
-  // every logit -inf: z = 0 and all results NaN
-  if (s.m == -INFINITY && s.z == 0.f) {
-    float greatest;
-    const Stats again = lowest_row(row, a.vocab, greatest, lane);
-    if (greatest != -INFINITY) s = again, base = greatest;
-  }
+  if (!(fabsf(s.m) < kFar)) s = far_row(row, a.vocab, base, lane);
   const float lz = log2f(s.z);
   const auto logprob = [&](float x) {
     const float d = x - base;  // next to the type's lowest value the product would pass its range
@@ -442,7 +435,7 @@ __global__ __launch_bounds__(kWave) void merge_kernel(Args a) {
   const int64_t r = blockIdx.x;
   const int words = kStatWords + 2 * a.top;
   const float* ws = a.ws + r * a.parts * static_cast<int64_t>(words);
-  Stats s = {-INFINITY, 0.f, 0.f};
+  Stats s = {-kFar, 0.f, 0.f};
   const int deep = max(1, (a.top + a.parts - 1) / a.parts);
   uint32_t head = 0;
   if (lane < a.parts) {

@@ -159,3 +159,59 @@ def test_gpu_refusals():
         token_logprobs(x, torch.zeros(2, dtype=torch.int64))
     with pytest.raises(ValueError, match="no backward"):
         token_logprobs(x.clone().requires_grad_())
+
+
+def far_rows(dt, vocab, g):
+    """Rows whose greatest logit is far from zero, alone, alike, in ties and next to the nearest number; rows whose masked tokens
+    have such a value and leave few others, all in one place."""
+    rows = []
+    ordinary = torch.randn(vocab, generator=g, device=DEV)
+    for far in (1e10, -1e10, 1e30, -1e30, 3e38, -3e38, torch.finfo(dt).max, -1.5e9, 1.2e7, -1.2e7, 1.1e7):
+        top = torch.tensor(far, dtype=dt, device=DEV)
+        below = torch.nextafter(top, torch.tensor(-math.inf, dtype=dt, device=DEV))
+        x = ordinary.to(dt) if far > 0 else torch.full((vocab,), torch.finfo(dt).min, dtype=dt, device=DEV)
+        x[vocab // 3] = top
+        rows.append(x)
+        rows.append(top.expand(vocab).clone())
+        y = below.expand(vocab).clone()
+        y[torch.tensor([1, vocab // 2, vocab - 1], device=DEV)] = top
+        rows.append(y)
+    for mask in (-1e9, -1e10, -1e20, -1e30, torch.finfo(dt).min, -math.inf):
+        for first in (0, vocab // 2, vocab - 20):
+            x = torch.full((vocab,), mask, dtype=dt, device=DEV)
+            x[first:first + 20] = ordinary[:20].to(dt)
+            rows.append(x)
+    rows.append(ordinary.to(dt))
+    return torch.stack(rows)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("vocab", [3001, 30011])
+@pytest.mark.parametrize("top", [0, 8])
+def test_logits_far_from_zero(dtype, vocab, top):
+    """Against float64, rounded to float32 (what does not fit becomes -inf there, too). A lane of the pass that takes differences
+    first adds vocab / 64 terms."""
+    print(f"\n[far] {dtype} {vocab} {top}", flush=True)
+    g = torch.Generator(device=DEV).manual_seed(5)
+    x = far_rows(DTYPES[dtype], vocab, g)
+    targets = x.float().argmax(-1)
+    targets[1::2] = torch.randint(0, vocab, (len(targets[1::2]),), generator=g, device=DEV)
+    lp, ent, _, _ = reference(x, targets, 0)
+    # the order is the logits' own: 1e30 less, float64 would have them all alike
+    ids = torch.sort(x.double().cpu() + 0.0, dim=-1, descending=True, stable=True).indices[:, :top]
+    tlp = torch.stack([reference(x, ids[:, k], 0)[0] for k in range(top)], 1) if top else torch.empty(len(x), 0).double()
+    tol = (vocab / 64 + 64) * 2.0 ** -23
+
+    def alike(got, want):
+        got, want = got.double().cpu(), want.float().double()
+        return ((got == want) | ((got - want).abs() <= tol * (1 + want.abs()))).all()
+
+    many = x.repeat(20, 1)  # one workgroup a row
+    for r in range(len(x) + 2):
+        whole = r >= len(x)
+        out = token_logprobs(many if r > len(x) else x if whole else x[r:r + 1], targets.repeat(20) if r > len(x) else targets if
+                             whole else targets[r:r + 1], top=top)
+        of = slice(None) if whole else slice(r, r + 1)
+        out = [t[-len(x):] for t in out] if whole else out
+        assert torch.equal(out[2].cpu(), ids[of]), r
+        assert alike(out[0], lp[of]) and alike(out[1], ent[of]) and alike(out[3], tlp[of]), r
