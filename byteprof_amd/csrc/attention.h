@@ -158,7 +158,19 @@ __device__ __forceinline__ float add_halves(float v) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// The running softmax of one row (both halves of a wave hold the row's maximum; each its own part of the sum).
+// Exponents are fma(score, c, -M) with M = m c rounded once, m the row's greatest score and c = scale log2(e); the sums are
+// relative to M. From kFar on a step of M is more than 1: what its rounding leaves goes into the exponents, past fp16's range from
+// 2^28 on and past exp2's from 2^31. There the difference of the scores is taken first, and the sums are relative to m itself.
+constexpr float kFar = 16777216.f;
+
+// What sums relative to the maximum `from` are multiplied by when `to`, no less, takes its place.
+__device__ __forceinline__ float rescaled(float from, float to, float c) {
+#pragma clang fp contract(off)
+  const float a = from * c, b = to * c;
+  return from == to ? 1.f : __builtin_amdgcn_exp2f(fabsf(b) < kFar ? a - b : (from - to) * c);
+}
+
+// The running softmax of one row (both halves of a wave hold the row's maximum, unscaled; each its own part of the sum).
 template <int DP>
 struct Running {
   f32x16 o[DP / 32];
@@ -189,11 +201,10 @@ __device__ __forceinline__ void softmax_step(f32x16 (&s)[NB], u32x4 (&p)[NB][2],
   for (int b = 0; b < NB; ++b)
 #pragma unroll
     for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[b][i]);
-  mx = max_halves(mx) * c;
-  const float m = fmaxf(r.m, mx);
+  const float m = fmaxf(r.m, max_halves(mx));
   if (__any(m > r.m)) {
     // exp2(-inf - m) = 0 clears a row's empty start; a row that has seen nothing keeps m = -inf and scales by 1
-    const float f = m == r.m ? 1.f : __builtin_amdgcn_exp2f(r.m - m);
+    const float f = rescaled(r.m, m, c);
     r.m = m;
     r.l *= f;
 #pragma unroll
@@ -201,7 +212,15 @@ __device__ __forceinline__ void softmax_step(f32x16 (&s)[NB], u32x4 (&p)[NB][2],
 #pragma unroll
       for (int i = 0; i < 16; ++i) r.o[d][i] *= f;
   }
-  const float shift = r.m == -INFINITY ? 0.f : -r.m;
+  float shift = r.m == -INFINITY ? 0.f : -(r.m * c);
+  if (__any(!(fabsf(shift) < kFar))) {
+    const float less = fabsf(shift) < kFar ? 0.f : r.m;
+    shift = fabsf(shift) < kFar ? shift : 0.f;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[b][i] -= less;
+  }
 #pragma unroll
   for (int b = 0; b < NB; ++b)
 #pragma unroll

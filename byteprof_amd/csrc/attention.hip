@@ -346,9 +346,9 @@ __device__ __forceinline__ void small_tile(const Args& a, const Item& it, int kv
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) {
     const float mw = stats[32 * w + (lane & 31)];
-    l += stats[32 * (kWaves + w) + (lane & 31)] * (mw == m ? 1.f : __builtin_amdgcn_exp2f(mw - m));
+    l += stats[32 * (kWaves + w) + (lane & 31)] * rescaled(mw, m, a.scale_log2);
   }
-  const float f = r.m == m ? 1.f : __builtin_amdgcn_exp2f(r.m - m);
+  const float f = rescaled(r.m, m, a.scale_log2);
   const bool whole = !it.divided;
   float* ws = whole ? nullptr : slot_at<DP>(a, it.slot + it.split, kvh);
   const bool keep = whole || it.slot + it.split < a.slots;
@@ -442,7 +442,7 @@ __device__ __forceinline__ void merge_rows(const Args& a, const Item& it, int kv
         now = fmaxf(now, m[s]);
       }
       if constexpr (MORE) {
-        const float before = top == now ? 1.f : __builtin_amdgcn_exp2f(top - now);
+        const float before = rescaled(top, now, a.scale_log2);
         sum *= before;
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[e] *= before;
@@ -451,7 +451,7 @@ __device__ __forceinline__ void merge_rows(const Args& a, const Item& it, int kv
 #pragma unroll
       for (int s = 0; s < kMergeParts; ++s) {
         if (s0 + s >= it.splits) break;
-        const float f = m[s] == top ? 1.f : __builtin_amdgcn_exp2f(m[s] - top);
+        const float f = rescaled(m[s], top, a.scale_log2);
         sum += l[s] * f;
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[e] += x[s][e] * f;
@@ -504,7 +504,7 @@ __global__ __launch_bounds__(kThreads) void merge_kernel(Args a) {
       for (int s = g; s < it.splits; s += groups) {
         const float ms = stats[s * step];
         const f32x4 xs = *reinterpret_cast<const f32x4*>(ws + s * step + row * DP + 4 * piece);
-        const float f = ms == top ? 1.f : __builtin_amdgcn_exp2f(ms - top);
+        const float f = rescaled(ms, top, a.scale_log2);
         sum += stats[s * step + a.ws_rows] * f;
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[e] += xs[e] * f;

@@ -448,3 +448,55 @@ def test_more_query_heads_than_a_tile_has_rows_in_order(counts, lens, hq, hk, d,
     for b, (a, z) in enumerate(zip(off, off[1:])):
         want, bound = reference(q[a:z], ks[b], vs[b], firsts[b], d ** -0.5)
         check(out[a:z], want, bound, f"sequence {b}")
+
+
+def one_hot_reference(q, k, v, first, scale, dtype):
+    """(out, bound) in float64 where every score and every difference of scores is exact in float32 and each row's probabilities
+    are 0 or shares of 1 (or ordinary scores of a few units): what is left is the rounding of the probabilities and of the
+    result, and a few float32 steps."""
+    h = torch.finfo(dtype).eps / 2
+    s = q[:, 0].double().cpu() @ k[:, 0].double().cpu().T * scale
+    seen = torch.arange(len(k))[None, :] <= first + torch.arange(len(q))[:, None]
+    s = torch.where(seen, s, -math.inf)
+    p = torch.softmax(s, -1)
+    v = v[:, 0].double().cpu()
+    o, a = p @ v, p @ v.abs()
+    tiny = 2.0 ** -25 if dtype == FP else 0.0
+    return o, h * o.abs() * 1.01 + (h * 1.01 + 2.0 ** -18) * a + tiny * (seen.double() @ v.abs())
+
+
+FAR = [(BF, 2.0 ** 12, 2.0 ** 12, 1.0), (BF, 2.0 ** 15, 2.0 ** 15, 1.0), (BF, 2.0 ** 16, 2.0 ** 16, None), (BF, 2.0 ** 17, 2.0 ** 17, 0.75),
+       (BF, 2.0 ** 50, 2.0 ** 50, 1.0), (BF, 2.0 ** 63, 2.0 ** 63, 1.5), (BF, 2.0 ** 63, 2.0 ** 63, 16.0),
+       (FP, 2.0 ** 13, 2.0 ** 13, 1.0), (FP, 2.0 ** 14, 2.0 ** 14, 1.0), (FP, 2.0 ** 15, 2.0 ** 15, 1.0), (FP, 2.0 ** 15, 2.0 ** 15, 4.0),
+       (FP, 2.0 ** 15, 2.0 ** 14, 64.0)]
+
+
+@pytest.mark.parametrize("dtype,a,b,scale", FAR)
+def test_scores_far_from_zero(dtype, a, b, scale):
+    """Finite scores from 2^24 up to float32's range and past it with the scale, positive and negative, tied, beside rows of
+    ordinary scores: large tiles, whole and divided, and small ones."""
+    print(f"\n[far] {dtype} {a} {b} {scale}", flush=True)
+    g = torch.Generator(device=DEV).manual_seed(40)
+    d = 64
+    for n, rows, hq in ((160, 160, 1), (1500, 1500, 1), (5000, 1, 1), (900, 9, 4), (33, 2, 1)):
+        k = torch.zeros(n, 1, d, device=DEV)
+        k[:, 0, 5] = b * (1.0 + torch.randint(0, 128, (n,), generator=g, device=DEV) / 128.0)
+        q = torch.zeros(rows, hq, d, device=DEV)
+        kind = torch.randint(0, 4, (rows, hq), generator=g, device=DEV)
+        q[..., 5] = torch.tensor([a, -a, 2.0 / b, 0.0], device=DEV)[kind]  # the third: ordinary scores of 2 scale to 4 scale
+        if dtype == FP:
+            q[..., 5] = torch.where(kind == 2, 0.0, q[..., 5])
+        v = torch.randn(n, 1, d, generator=g, device=DEV)
+        q, k, v = q.to(dtype), k.to(dtype), v.to(dtype)
+        s = d ** -0.5 if scale is None else scale
+        if rows == n:
+            got = A.packed_attention(q, k, v, ints([0, n]), scale=scale)
+        else:
+            order = torch.randperm(-(-n // 16) + 2, generator=g, device=DEV)[:-(-n // 16)].to(torch.int32)
+            kp, vp = (torch.zeros(len(order) + 2, 16, 1, d, dtype=dtype, device=DEV) for _ in range(2))
+            at = torch.arange(n, device=DEV)
+            kp[order.long()[at // 16], at % 16], vp[order.long()[at // 16], at % 16] = k, v
+            got = A.paged_attention(q, kp, vp, order[None], ints([n]), ints([0, rows]), scale=scale)
+        for h in range(hq):
+            want, bound = one_hot_reference(q[:, h:h + 1], k, v, n - rows, s, dtype)
+            check(got[:, h], want, bound, f"{n} keys, {rows} rows, head {h}")
