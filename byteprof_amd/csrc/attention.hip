@@ -555,9 +555,9 @@ __global__ __launch_bounds__(kThreads) void append_kernel(Append a) {
     }
     const int end = a.cu[lo + 1];
     if (tok < a.cu[lo] || tok >= end) continue;
-    const int64_t at = static_cast<int64_t>(a.lengths[lo]) - (end - tok);
-    if (at < 0 || at >= a.max_keys) continue;
-    const int pos = static_cast<int>(at), n = a.page(pos), slot = pos - n * a.page.d;
+    const int pos = max(a.lengths[lo], 0) - (min(end, a.tokens) - tok);  // offsets are cut as the attention cuts them
+    if (static_cast<unsigned>(pos) >= static_cast<unsigned>(a.max_keys)) continue;
+    const int n = a.page(pos), slot = pos - n * a.page.d;
     const int id = a.table[lo * a.table_stride + n];
     if (static_cast<unsigned>(id) >= static_cast<unsigned>(a.pool)) continue;
     const auto from = [&](const void* p, int64_t t, int64_t hs) {

@@ -194,7 +194,8 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
                  lengths: torch.Tensor, cu: torch.Tensor) -> None:
     """The chunks' keys and values k, v [tokens, Hk, D] (any strides with the last dimension contiguous) into the caches, at
     the last positions of each sequence: token i of a chunk of c at position lengths[b] - c + i. Tokens of no chunk, positions
-    outside the table and pages outside the cache are left out. Any dtype of 1, 2 or 4 bytes; the caches' dtype is k's."""
+    outside the table (also where lengths[b] is past it, which paged_attention takes as the table's end) and pages outside the
+    cache are left out. Any dtype of 1, 2 or 4 bytes; the caches' dtype is k's."""
     what = "paged_append"
     if k.dim() != 3 or v.shape != k.shape:
         raise ValueError(f"{what}: k and v must be [tokens, Hk, D]")

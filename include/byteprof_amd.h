@@ -444,7 +444,8 @@ int bp_attn_paged(int dtype, const void* q, const void* k_pages, const void* v_p
 /*
  * The keys and values k, v [tokens, hk, head_dim] (element_bytes 1, 2 or 4) into the cache of bp_attn_paged: token i of
  * sequence b (of c_b tokens) to position lengths[b] - c_b + i. A position below 0 or at or past page x max_pages, a page
- * outside [0, pool) and a token of no sequence are left out. Strides in elements. 16 bytes at a time where all rows allow.
+ * outside [0, pool) and a token of no sequence are left out. cu as in bp_attn_paged; lengths are not cut to page x max_pages
+ * here (a longer sequence's tokens keep their positions, and those past the table are left out). Strides in elements. 16 bytes at a time where all rows allow.
  * No counterpart in the reference.
  */
 int bp_paged_append(int element_bytes, const void* k, const void* v, void* k_pages, void* v_pages, const int32_t* table,

@@ -500,3 +500,23 @@ def test_scores_far_from_zero(dtype, a, b, scale):
         for h in range(hq):
             want, bound = one_hot_reference(q[:, h:h + 1], k, v, n - rows, s, dtype)
             check(got[:, h], want, bound, f"{n} keys, {rows} rows, head {h}")
+
+
+def test_append_and_attention_agree_on_offsets_past_the_tokens():
+    """Offsets before the first token and past the last: both take the tokens that there are, at the same positions."""
+    g = torch.Generator(device=DEV).manual_seed(41)
+    tokens, page, d = 6, 16, 64
+    table, lengths, cu = ints([[3, 0], [1, 4]]), ints([20, 30]), ints([-2, 3, 900])
+    k, v, q = (randn(g, tokens, 1, d, dtype=BF) for _ in range(3))
+    old = [randn(g, 30, 1, d, dtype=BF) for _ in range(4)]  # keys, values of either sequence
+    kp, vp = (torch.zeros(5, page, 1, d, dtype=BF, device=DEV) for _ in range(2))
+    for b, n in enumerate((17, 27)):
+        at = torch.arange(n, device=DEV)
+        where = (table[b].long()[at // page], at % page)
+        kp[where], vp[where] = old[2 * b][:n], old[2 * b + 1][:n]
+    A.paged_append(k, v, kp, vp, table, lengths, cu)
+    got = A.paged_attention(q, kp, vp, table, lengths, cu)
+    for b, (n, a) in enumerate(((17, 0), (27, 3))):
+        ks, vs = torch.cat([old[2 * b][:n], k[a:a + 3]]), torch.cat([old[2 * b + 1][:n], v[a:a + 3]])
+        want, bound = reference(q[a:a + 3], ks, vs, n, d ** -0.5)
+        check(got[a:a + 3], want, bound, f"sequence {b}")
