@@ -604,6 +604,12 @@ int run(int dtype, Args& a, bool paged, size_t ws_bytes, hipStream_t st) {
   if (a.d <= 0 || a.d % 8 != 0 || a.d > 256) return BP_E_UNSUPPORTED;
   if (a.tokens == 0) return BP_OK;
   if (a.q == nullptr || a.out == nullptr || (a.seqs > 0 && a.cu == nullptr)) return BP_E_INVALID_ARG;
+  // a stride that nothing is multiplied with may be anything
+  if (a.tokens == 1) a.q_t = 0;
+  if (a.hq == 1) a.q_h = 0;
+  if (hk == 1) a.k_h = a.v_h = 0;
+  if (paged ? a.page.d == 1 : a.tokens == 1) a.k_t = a.v_t = 0;
+  if (a.pool == 1) a.k_p = a.v_p = 0;
   if (!aligned16(a.q) || !aligned16(a.k) || !aligned16(a.v) || !aligned16(a.out) ||
       ((a.q_t | a.q_h | a.k_p | a.k_t | a.k_h | a.v_p | a.v_t | a.v_h) & 7) != 0)
     return BP_E_INVALID_ARG;

@@ -172,7 +172,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     dtype = _dtype(what, q, k_pages, v_pages)
     _heads(what, hq, hk, d, dk)
     k_ptr, v_ptr = k_pages.data_ptr(), v_pages.data_ptr()
-    if (k_ptr | v_ptr) & 15 or (kst[0] | kst[1] | kst[2] | vst[0] | vst[1] | vst[2]) & 7:
+    if (k_ptr | v_ptr) & 15 or (kst[0] | kst[1] | kst[2] | vst[0] | vst[1] | vst[2]) & 7 and any(
+            n > 1 and (a | b) & 7 for n, a, b in zip((pool, page, hk), kst, vst)):
         raise ValueError(f"{what}: the caches must be 16-byte aligned, with strides of whole multiples of 8 elements")
     index = _same_device(what, q, k_pages, v_pages, table, lengths, cu, out)
     if q.requires_grad or k_pages.requires_grad or v_pages.requires_grad:

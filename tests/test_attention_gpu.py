@@ -520,3 +520,29 @@ def test_append_and_attention_agree_on_offsets_past_the_tokens():
         ks, vs = torch.cat([old[2 * b][:n], k[a:a + 3]]), torch.cat([old[2 * b + 1][:n], v[a:a + 3]])
         want, bound = reference(q[a:a + 3], ks, vs, n, d ** -0.5)
         check(got[a:a + 3], want, bound, f"sequence {b}")
+
+
+def test_strides_of_dimensions_of_one_entry_do_not_count():
+    """One token or one head in a wider buffer whose rows are no multiple of 8: the same as from a tensor of its own."""
+    g = torch.Generator(device=DEV).manual_seed(42)
+    wide = randn(g, 1, 1, 67, dtype=BF)
+    q, k, v = wide[..., :64], randn(g, 1, 1, 65, dtype=BF)[..., :64], randn(g, 1, 1, 71, dtype=BF)[..., :64]
+    assert q.stride()[0] % 8 and q.is_contiguous()
+    own = [t.clone(memory_format=torch.contiguous_format).view(1, 1, 64) for t in (q, k, v)]
+    assert torch.equal(A.packed_attention(q, k, v, ints([0, 1])), A.packed_attention(*own, ints([0, 1])))
+    q3, k3 = randn(g, 3, 1, 64, dtype=BF), randn(g, 3, 1, 64, dtype=BF)  # many tokens, one head with any stride
+    odd = lambda t: t.as_strided(t.shape, (64, 13, 1))  # noqa: E731
+    assert torch.equal(A.packed_attention(odd(q3), odd(k3), odd(k3), ints([0, 3])), A.packed_attention(q3, k3, k3, ints([0, 3])))
+
+    pool = randn(g, 16, 64, dtype=BF)  # one page of 16 positions, one head; then 16 pages of one position
+    table, lengths, cu = ints([[0]]), ints([11]), ints([0, 1])
+    plain = pool.view(1, 16, 1, 64)
+    page = pool.as_strided((1, 16, 1, 64), (17, 64, 3, 1))
+    want = A.paged_attention(q, plain, plain, table, lengths, cu)
+    assert torch.equal(A.paged_attention(q, page, page, table, lengths, cu), want)
+    single = pool.as_strided((16, 1, 1, 64), (64, 5, 3, 1))
+    table = torch.arange(16, dtype=torch.int32, device=DEV)[None]
+    assert torch.equal(A.paged_attention(q, single, single, table, lengths, cu), want)
+    with pytest.raises(ValueError, match="multiples of 8"):
+        two = randn(g, 40, 64, dtype=BF).as_strided((2, 16, 1, 64), (65 * 16 + 1, 64, 64, 1))
+        A.paged_attention(q, two, two, ints([[0]]), lengths, cu)
