@@ -3,6 +3,8 @@
 
 #include "attention.h"
 
+#include <float.h>
+
 #include "byteprof_amd.h"
 
 namespace bp {
@@ -599,7 +601,8 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 int run(int dtype, Args& a, bool paged, size_t ws_bytes, hipStream_t st) {
   const int hk = a.hk.d;
   if (dtype != BP_DT_BF16 && dtype != BP_DT_F16) return BP_E_UNSUPPORTED;
-  if (a.tokens < 0 || a.seqs < 0 || hk <= 0 || a.hq <= 0 || a.hq % hk != 0 || !(a.scale_log2 > 0.f) || a.max_keys < 0)
+  if (a.tokens < 0 || a.seqs < 0 || hk <= 0 || a.hq <= 0 || a.hq % hk != 0 || !(a.scale_log2 > 0.f && a.scale_log2 <= FLT_MAX) ||
+      a.max_keys < 0)
     return BP_E_INVALID_ARG;
   if (a.d <= 0 || a.d % 8 != 0 || a.d > 256) return BP_E_UNSUPPORTED;
   if (a.tokens == 0) return BP_OK;

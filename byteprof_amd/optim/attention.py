@@ -15,6 +15,9 @@ read, so it has to be finite; what lies past a sequence's length or in other seq
 
 from __future__ import annotations
 
+import ctypes
+import math
+
 import torch
 
 from .. import _lib
@@ -57,9 +60,12 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 
 
 def _scale(what: str, scale: float | None, d: int) -> float:
-    scale = d ** -0.5 if scale is None else float(scale)
-    if not 0.0 < scale < float("inf"):
-        raise ValueError(f"{what}: scale must be positive and finite")
+    if scale is None:
+        return d ** -0.5
+    scale = float(scale)
+    # the kernels multiply by scale log2(e) in float32; a scale that vanishes there would be no scale
+    if not 0.0 < ctypes.c_float(ctypes.c_float(scale).value * math.log2(math.e)).value < math.inf:
+        raise ValueError(f"{what}: scale must be positive and finite, and so must scale log2(e) in float32")
     return scale
 
 

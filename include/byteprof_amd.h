@@ -422,6 +422,7 @@ int bp_decode_argmax_rows(const void* logits, int vocab, int rows, int64_t* tok,
  * a dimension of more than one entry a multiple of 8; out
  * [tokens, hq, head_dim] contiguous. cu [seqs + 1] (int32): sequence b's tokens are cu[b] .. cu[b + 1] - 1; what of them lies
  * outside [0, tokens) is left out. Rows of no sequence become zeros, so do rows that see no key.
+ * scale: positive, and scale log2(e) finite in fp32.
  * packed: keys and values of the tokens themselves; with causal, token i sees those of its sequence up to i, else all.
  * paged:  caches [pool, page, hk, head_dim] (any strides between pages, positions and heads). Sequence b has lengths[b]
  *         (int32) positions, position p in page table[b, p / page] (int32, table_stride entries a row), at p % page; its

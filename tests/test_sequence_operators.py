@@ -180,3 +180,16 @@ def test_workspace_of_attention(L):
     small = L.bp_attn_workspace_bytes(1, 1, 16, 16, 128, 512)  # 16 heads, 2 parts, 32 rows
     assert small == 16 * 2 * 32 * (128 + 2) * 4
     assert L.bp_attn_workspace_bytes(1 << 14, 64, 32, 8, 128, 1 << 20) <= 1400 * 128 * 130 * 4
+
+
+def test_a_scale_that_leaves_the_range_of_float32_is_refused(L):
+    for scale in (1e39, 3e38, 1e-60):
+        with pytest.raises(ValueError, match="scale must be"):
+            A._scale("x", scale, 64)
+    assert A._scale("x", 2e38, 64) == 2e38 and A._scale("x", 1e-37, 64) == 1e-37
+    p = ctypes.c_void_p(64)  # never dereferenced
+
+    def packed(scale):
+        return L.bp_attn_packed(0, p, p, p, p, p, 1000, 1, 2, 1, 64, 128, 64, 64, 64, 64, 64, 1, scale, None, 0, None)
+
+    assert packed(3e38) == -1 and packed(float("inf")) == -1 and packed(2e38) == -3  # the last: no workspace
