@@ -8,9 +8,10 @@ cache in pages, with the append that writes it.
 
 Offsets, lengths and page tables are int32 tensors on the GPU that the kernels read: the calls neither copy nor synchronise,
 and one captured graph serves whatever the tensors hold when it is replayed. bf16 or fp16, softmax and sums in fp32; any
-number of query heads to a key head; head_dim a multiple of 8 up to 256. Forward only: a tensor that requires a gradient is
-refused. A key or value that a row may not see (past its causal limit) still takes part with probability 0 where its tile is
-read, so it has to be finite; what lies past a sequence's length or in other sequences is never read.
+number of query heads to a key head; head_dim a multiple of 8 up to 256. Forward only: a tensor that requires a gradient or
+carries a forward-mode tangent is refused. A key or value that a row may not see (past its causal limit) still takes part with
+probability 0 where its tile is read, so it has to be finite; what lies past a sequence's length or in other sequences is
+never read.
 """
 
 from __future__ import annotations
@@ -19,6 +20,7 @@ import ctypes
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _lib
 
@@ -40,9 +42,13 @@ def _same_device(what: str, x: torch.Tensor, *tensors: torch.Tensor | None) -> i
     return index
 
 
-def _no_backward(what: str) -> None:
-    if torch.is_grad_enabled():
-        raise ValueError(f"{what} has no backward pass: detach its inputs or use torch.no_grad()")
+def _no_derivative(what: str, *tensors: torch.Tensor) -> None:
+    """Refuses tensors that a gradient or (inside a forward-mode level) a tangent would have to be taken through."""
+    for t in tensors:
+        if t.requires_grad and torch.is_grad_enabled():
+            raise ValueError(f"{what} has no backward pass: detach its inputs or use torch.no_grad()")
+        if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+            raise ValueError(f"{what} has no forward-mode derivative: pass the primal (torch.autograd.forward_ad.unpack_dual)")
 
 
 def _ints(what: str, name: str, t: torch.Tensor, dims: int) -> None:
@@ -126,8 +132,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu: torc
     if seqs < 0:
         raise ValueError(f"{what}: cu needs at least one entry")
     index = _same_device(what, q, k, v, cu, out)
-    if q.requires_grad or k.requires_grad or v.requires_grad:
-        _no_backward(what)
+    if q.requires_grad or k.requires_grad or v.requires_grad or forward_ad._current_level >= 0:
+        _no_derivative(what, q, k, v)
     scale = _scale(what, scale, d)
     q, k, v = _rows(q), _rows(k), _rows(v)
     y = _output(what, q, out)
@@ -182,8 +188,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
             n > 1 and (a | b) & 7 for n, a, b in zip((pool, page, hk), kst, vst)):
         raise ValueError(f"{what}: the caches must be 16-byte aligned, with strides of whole multiples of 8 elements")
     index = _same_device(what, q, k_pages, v_pages, table, lengths, cu, out)
-    if q.requires_grad or k_pages.requires_grad or v_pages.requires_grad:
-        _no_backward(what)
+    if q.requires_grad or k_pages.requires_grad or v_pages.requires_grad or forward_ad._current_level >= 0:
+        _no_derivative(what, q, k_pages, v_pages)
     scale = _scale(what, scale, d)
     q = _rows(q)
     y = _output(what, q, out)
@@ -218,8 +224,8 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     if (k_d != 1 or v_d != 1) and k.numel():
         raise ValueError(f"{what}: k and v must be contiguous in the head dimension")
     index = _same_device(what, k, v, k_pages, v_pages, table, lengths, cu)
-    if k.requires_grad or v.requires_grad or k_pages.requires_grad or v_pages.requires_grad:
-        _no_backward(what)
+    if k.requires_grad or v.requires_grad or k_pages.requires_grad or v_pages.requires_grad or forward_ad._current_level >= 0:
+        _no_derivative(what, k, v, k_pages, v_pages)
     if tokens == 0 or hk == 0 or d == 0:
         return
     _launch(index, "bp_paged_append", size, k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),

@@ -6,9 +6,10 @@ from __future__ import annotations
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _lib
-from .attention import _launch, _no_backward, _same_device
+from .attention import _launch, _no_derivative, _same_device
 
 MAX_TOP = 32
 
@@ -28,7 +29,7 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, *,
     softmax at each row's target (NaN for one outside the vocabulary), the entropy of the row, and its `top` (up to MAX_TOP)
     most likely tokens in order; equal logits in order of their ids. -inf logits are tokens that cannot come. A row with a
     NaN or +inf has NaN probabilities (NaN counts as greatest in the order), and so has a row of nothing but -inf. Forward
-    only: logits that require a gradient are refused."""
+    only: logits that require a gradient or carry a forward-mode tangent are refused."""
     what = "token_logprobs"
     if logits.dim() != 2:
         raise ValueError(f"{what}: logits must be [rows, vocab], each row contiguous")
@@ -46,8 +47,8 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, *,
     if targets is not None and (targets.dtype != torch.int64 or targets.shape != (rows,)):
         raise ValueError(f"{what}: targets must be int64 [rows]")
     index = _same_device(what, logits, targets)
-    if logits.requires_grad:
-        _no_backward(what)
+    if logits.requires_grad or forward_ad._current_level >= 0:
+        _no_derivative(what, logits)
     dev = logits.device
     f32 = torch.float32
     logprob = None if targets is None else torch.empty_strided((rows,), (1,), dtype=f32, device=dev)

@@ -546,3 +546,25 @@ def test_strides_of_dimensions_of_one_entry_do_not_count():
     with pytest.raises(ValueError, match="multiples of 8"):
         two = randn(g, 40, 64, dtype=BF).as_strided((2, 16, 1, 64), (65 * 16 + 1, 64, 64, 1))
         A.paged_attention(q, two, two, ints([[0]]), lengths, cu)
+
+
+def test_tangents_are_refused():
+    """A dual tensor of forward-mode differentiation, whose tangent a launch would drop; its primal and other tensors run."""
+    from torch.autograd import forward_ad
+
+    from byteprof_amd.optim.logprobs import token_logprobs
+
+    g = torch.Generator(device=DEV).manual_seed(43)
+    q, t = randn(g, 4, 1, 64, dtype=BF), randn(g, 4, 1, 64, dtype=BF)
+    pages, table, lens, cu = torch.zeros(1, 16, 1, 64, dtype=BF, device=DEV), ints([[0]]), ints([4]), ints([0, 4])
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(q, t)
+        for call in (lambda x: A.packed_attention(x, q, q, cu), lambda x: A.packed_attention(q, q, x, cu),
+                     lambda x: A.paged_attention(x, pages, pages, table, lens, cu),
+                     lambda x: A.paged_append(q, x, pages, pages, table, lens, cu), lambda x: token_logprobs(x[:, 0])):
+            with pytest.raises(ValueError, match="forward-mode"):
+                call(dual)
+            with torch.no_grad(), pytest.raises(ValueError, match="forward-mode"):
+                call(dual)
+            call(q)
+            call(forward_ad.unpack_dual(dual).primal)
