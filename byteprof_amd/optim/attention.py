@@ -21,6 +21,7 @@ import math
 
 import torch
 from torch.autograd import forward_ad
+from torch.autograd.graph import increment_version
 
 from .. import _lib
 
@@ -94,6 +95,7 @@ def _output(what: str, q: torch.Tensor, out: torch.Tensor | None) -> torch.Tenso
         return torch.empty_like(q, memory_format=torch.contiguous_format)
     if out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous() or out.data_ptr() & 15:
         raise ValueError(f"{what}: out must be a contiguous 16-byte aligned {tuple(q.shape)} {q.dtype} tensor")
+    increment_version(out)  # a graph that has saved it for its backward pass finds out
     return out
 
 
@@ -231,3 +233,4 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     _launch(index, "bp_paged_append", size, k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
             table.data_ptr(), row, lengths.data_ptr(), cu.data_ptr(), tokens, seqs, pool, page, most, hk, d, k_t, k_h, v_t, v_h,
             kst[0], kst[1], kst[2], vst[0], vst[1], vst[2])
+    increment_version((k_pages, v_pages))

@@ -568,3 +568,23 @@ def test_tangents_are_refused():
                 call(dual)
             call(q)
             call(forward_ad.unpack_dual(dual).primal)
+
+
+def test_written_tensors_count_as_changed():
+    """The caches of an append and the output of an attention, saved by another graph before: its backward pass refuses."""
+    g = torch.Generator(device=DEV).manual_seed(44)
+    q = randn(g, 4, 1, 64, dtype=BF)
+    kp, vp = torch.zeros(1, 16, 1, 64, dtype=BF, device=DEV), torch.zeros(1, 16, 1, 64, dtype=BF, device=DEV)
+    out, w = torch.zeros_like(q), torch.ones(1, device=DEV, requires_grad=True)
+    table, lens, cu = ints([[0]]), ints([4]), ints([0, 4])
+    for saved, call in ((kp, lambda: A.paged_append(q, q, kp, vp, table, lens, cu)), (vp, lambda: A.paged_append(q, q, kp, vp, table, lens, cu)),
+                        (out, lambda: A.packed_attention(q, q, q, cu, out=out)),
+                        (out, lambda: A.paged_attention(q, kp, vp, table, lens, cu, out=out))):
+        loss = (saved * w).sum()
+        call()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    with torch.inference_mode():
+        pages = torch.zeros(1, 16, 1, 64, dtype=BF, device=DEV)  # has no version
+        A.paged_append(q, q, pages, pages.clone(), table, lens, cu)
+        A.packed_attention(q, q, q, cu, out=torch.empty_like(q))
