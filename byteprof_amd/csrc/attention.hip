@@ -624,6 +624,16 @@ int run(int dtype, Args& a, bool paged, size_t ws_bytes, hipStream_t st) {
   if (!plan_launch(a, n)) return BP_E_UNSUPPORTED;
   if (n.workspace > 0 && (a.ws == nullptr || ws_bytes < n.workspace || !aligned16(a.ws))) return BP_E_WORKSPACE;
   if (n.workspace == 0) a.ws = nullptr;
+  // A row of q is read by the tile that writes its result and by no other, so out may be q itself.
+  const auto bytes = [&](int64_t n0, int64_t s0, int64_t n1, int64_t s1, int64_t n2, int64_t s2) {
+    return n0 > 0 ? 2 * ((n0 - 1) * s0 + (n1 - 1) * s1 + (n2 - 1) * s2 + a.d) : 0;
+  };
+  const int64_t dense = static_cast<int64_t>(a.hq) * a.d, out = 2 * dense * a.tokens, keys = paged ? a.page.d : a.tokens;
+  const bool in_place = a.out == a.q && (a.tokens == 1 || a.q_t == dense) && (a.hq == 1 || a.q_h == a.d);
+  if ((!in_place && ranges_overlap(a.out, out, a.q, bytes(a.tokens, a.q_t, a.hq, a.q_h, 1, 0))) ||
+      ranges_overlap(a.out, out, a.k, bytes(paged ? a.pool : 1, a.k_p, keys, a.k_t, hk, a.k_h)) ||
+      ranges_overlap(a.out, out, a.v, bytes(paged ? a.pool : 1, a.v_p, keys, a.v_t, hk, a.v_h)))
+    return BP_E_INVALID_ARG;
   if (dtype == BP_DT_BF16)
     return paged ? launch_dim<Bf16, true>(a, n, st) : launch_dim<Bf16, false>(a, n, st);
   return paged ? launch_dim<F16, true>(a, n, st) : launch_dim<F16, false>(a, n, st);

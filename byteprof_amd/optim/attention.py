@@ -90,11 +90,22 @@ def _heads(what: str, hq: int, hk: int, d: int, dk: int) -> None:
         raise ValueError(f"{what}: head_dim must be the same everywhere, a multiple of 8 up to {MAX_HEAD_DIM}")
 
 
-def _output(what: str, q: torch.Tensor, out: torch.Tensor | None) -> torch.Tensor:
+def _span(t: torch.Tensor) -> tuple[int, int]:
+    """The bytes that t reaches over, first and one past the last."""
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride())) if t.numel() else -1
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def _output(what: str, q: torch.Tensor, out: torch.Tensor | None, *read: torch.Tensor) -> torch.Tensor:
     if out is None:
         return torch.empty_like(q, memory_format=torch.contiguous_format)
     if out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous() or out.data_ptr() & 15:
         raise ValueError(f"{what}: out must be a contiguous 16-byte aligned {tuple(q.shape)} {q.dtype} tensor")
+    first, end = _span(out)
+    for t in read if out.data_ptr() == q.data_ptr() and q.is_contiguous() else (q, *read):
+        a, b = _span(t)
+        if first < b and a < end:
+            raise ValueError(f"{what}: out must not overlap what the call reads (but it may be q itself)")
     increment_version(out)  # a graph that has saved it for its backward pass finds out
     return out
 
@@ -121,7 +132,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu: torc
     """Attention of sequences packed one after another: q [tokens, Hq, D], k, v [tokens, Hk, D] (slices of one projection
     may be passed as they lie), cu [sequences + 1] int32 on the GPU with the sequences' first tokens and the end of the last.
     A token sees the tokens of its own sequence, with `causal` those up to itself. scale: D ** -0.5 by default. Rows that no
-    sequence covers (a batch padded to a fixed size) come out as zeros. Returns [tokens, Hq, D], in `out` when given."""
+    sequence covers (a batch padded to a fixed size) come out as zeros. Returns [tokens, Hq, D], in `out` when given:
+    q itself or a tensor apart from q, k and v."""
     what = "packed_attention"
     if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape or k.shape[0] != q.shape[0]:
         raise ValueError(f"{what}: q must be [tokens, Hq, D] and k, v [tokens, Hk, D]")
@@ -138,7 +150,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu: torc
         _no_derivative(what, q, k, v)
     scale = _scale(what, scale, d)
     q, k, v = _rows(q), _rows(k), _rows(v)
-    y = _output(what, q, out)
+    y = _output(what, q, out, k, v)
     if tokens == 0:
         return y
     ws, need = _workspace(tokens, seqs, hq, hk, d, tokens, q.device)
@@ -177,7 +189,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     table[b, p // page size]; entries past its length are not read), lengths [sequences]: a sequence's positions in the
     cache, its chunk's among them (append first). A chunk's tokens are the last positions; each sees all up to its own. Rows
     that no chunk covers come out as zeros; rows of a sequence with a page id outside the cache below its length as NaN.
-    Returns [tokens, Hq, D], in `out` when given."""
+    Returns [tokens, Hq, D], in `out` when given: q itself or a tensor apart from q and the caches."""
     what = "paged_attention"
     if q.dim() != 3:
         raise ValueError(f"{what}: q must be [tokens, Hq, D]")
@@ -194,7 +206,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         _no_derivative(what, q, k_pages, v_pages)
     scale = _scale(what, scale, d)
     q = _rows(q)
-    y = _output(what, q, out)
+    y = _output(what, q, out, k_pages, v_pages)
     if tokens == 0:
         return y
     ws, need = _workspace(tokens, seqs, hq, hk, d, page * most, q.device)

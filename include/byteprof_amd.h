@@ -418,10 +418,10 @@ int bp_decode_argmax_rows(const void* logits, int vocab, int rows, int64_t* tok,
  * Attention of several sequences in one call; the softmax in fp32, the probabilities rounded to the tensors' type before the
  * product with the values (both sums in fp32), the result rounded once. dtype BP_DT_BF16 or BP_DT_F16 for q, k, v and out;
  * head_dim a multiple of 8 up to 256 (else BP_E_UNSUPPORTED); hq a multiple of hk (query head h reads key head
- * h / (hq / hk)); every base 16-byte aligned, every stride (in elements; the innermost is 1) of
- * a dimension of more than one entry a multiple of 8; out
- * [tokens, hq, head_dim] contiguous. cu [seqs + 1] (int32): sequence b's tokens are cu[b] .. cu[b + 1] - 1; what of them lies
- * outside [0, tokens) is left out. Rows of no sequence become zeros, so do rows that see no key.
+ * h / (hq / hk)); every base 16-byte aligned, every stride (in elements; the innermost is 1) of a dimension of more than one
+ * entry a multiple of 8; out [tokens, hq, head_dim] contiguous, either q itself or apart from q and the keys and values (else
+ * BP_E_INVALID_ARG). cu [seqs + 1] (int32): sequence b's tokens are cu[b] .. cu[b + 1] - 1; what of them lies outside
+ * [0, tokens) is left out. Rows of no sequence become zeros, so do rows that see no key.
  * scale: positive, and scale log2(e) finite in fp32.
  * packed: keys and values of the tokens themselves; with causal, token i sees those of its sequence up to i, else all.
  * paged:  caches [pool, page, hk, head_dim] (any strides between pages, positions and heads). Sequence b has lengths[b]

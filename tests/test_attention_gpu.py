@@ -588,3 +588,15 @@ def test_written_tensors_count_as_changed():
         pages = torch.zeros(1, 16, 1, 64, dtype=BF, device=DEV)  # has no version
         A.paged_append(q, q, pages, pages.clone(), table, lens, cu)
         A.packed_attention(q, q, q, cu, out=torch.empty_like(q))
+
+
+def test_in_place():
+    """out = q, in whole and divided tiles, small and large, with rows of no sequence."""
+    g = torch.Generator(device=DEV).manual_seed(45)
+    q, k, v = randn(g, 1600, 4, 64, dtype=BF), randn(g, 1600, 1, 64, dtype=BF), randn(g, 1600, 1, 64, dtype=BF)
+    for cu in ([0, 1500], [0, 10, 13, 333, 1400], [3, 14]):
+        x = q.clone()
+        want = A.packed_attention(x, k, v, ints(cu))
+        assert A.packed_attention(x, k, v, ints(cu), out=x) is x and torch.equal(x, want)
+    with pytest.raises(ValueError, match="overlap"):
+        A.packed_attention(k, k, v, ints([0, 1600]), out=v)

@@ -193,3 +193,36 @@ def test_a_scale_that_leaves_the_range_of_float32_is_refused(L):
         return L.bp_attn_packed(0, p, p, p, p, p, 1000, 1, 2, 1, 64, 128, 64, 64, 64, 64, 64, 1, scale, None, 0, None)
 
     assert packed(3e38) == -1 and packed(float("inf")) == -1 and packed(2e38) == -3  # the last: no workspace
+
+
+def test_attention_entries_refuse_an_output_that_overlaps_what_they_read(L):
+    """out over k or v, or over another part of q; nothing is dereferenced, the places are numbers."""
+    kb = 4 * 64 * 2  # bytes of 4 tokens of one head of 64
+
+    def packed(out, q=1 << 20, k=2 << 20, v=3 << 20, q_t=128, k_t=64):
+        ptr = ctypes.c_void_p
+        return L.bp_attn_packed(0, ptr(q), ptr(k), ptr(v), ptr(out), ptr(64), 4, 1, 2, 1, 64, q_t, 64, k_t, 64, k_t, 64, 1, 0.1,
+                                None, 0, None)
+
+    assert packed(2 << 20) == -1 and packed(3 << 20) == -1 and packed((2 << 20) + kb - 16) == -1
+    assert packed((3 << 20) - 2 * kb + 16) == -1 and packed((1 << 20) + 128) == -1 and packed(1 << 20, q_t=256) == -1
+    assert packed((2 << 20) + 3 * 1024 * 2, k_t=1024) == -1  # the last of k's rows
+
+    def paged(out, pool=3, page=16):
+        ptr = ctypes.c_void_p
+        return L.bp_attn_paged(0, ptr(1 << 20), ptr(2 << 20), ptr(3 << 20), ptr(out), ptr(64), 4, ptr(64), ptr(64), 4, 1, pool,
+                               page, 4, 2, 1, 64, 128, 64, 1024, 64, 64, 1024, 64, 64, 0.1, None, 0, None)
+
+    assert paged(2 << 20) == -1 and paged((3 << 20) + 2 * (3 * 16 * 64) - 16) == -1 and paged((1 << 20) + 16) == -1
+
+
+def test_out_has_to_be_apart():
+    q, k, v = z(4, 2, 64), z(4, 2, 64), z(4, 2, 64)
+    both = z(2, 4, 2, 64)
+    assert A._output("x", q, q, k, v) is q and A._output("x", both[0], both[1], k, v) is not None
+    for out, read in ((k, (k, v)), (v, (k, v)), (both[0], (both[1], both)), (both[1], (both.transpose(0, 1)[:, 1], v))):
+        with pytest.raises(ValueError, match="overlap"):
+            A._output("x", q, out, *read)
+    wide = z(5, 2, 64)
+    with pytest.raises(ValueError, match="overlap"):
+        A._output("x", wide[1:], wide[:4], k, v)
