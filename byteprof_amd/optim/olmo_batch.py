@@ -19,7 +19,7 @@ import torch
 from .. import _lib
 from . import skinny as S
 from .attention import packed_attention, paged_append, paged_attention
-from .logprobs import TokenLogprobs, token_logprobs
+from .logprobs import MAX_TOP, TokenLogprobs, token_logprobs
 from .olmo import OlmoDecoder, OptimizeError
 
 
@@ -49,7 +49,9 @@ class OlmoBatch:
     def _ints(self, xs: list) -> torch.Tensor:
         return torch.tensor(xs, dtype=torch.int32, device=self.dec.device)
 
-    def _prompts(self, prompts: list[torch.Tensor]) -> list[list[int]]:
+    def _prompts(self, prompts: list[torch.Tensor], top: int) -> list[list[int]]:
+        if not 0 <= top <= min(MAX_TOP, self.dec.cfg.vocab):
+            raise ValueError(f"top must be 0..{MAX_TOP} and at most the vocabulary, got {top}")
         ids = [p.reshape(-1).tolist() for p in prompts]
         if not ids or min(len(i) for i in ids) < 1:
             raise OptimizeError("need at least one prompt, each of at least one token")
@@ -106,7 +108,7 @@ class OlmoBatch:
     @torch.no_grad()
     def score(self, prompts: list[torch.Tensor], top: int = 0) -> list[TokenLogprobs]:
         """Of every prompt, the log probabilities of its tokens after the first, given those before ([L - 1] each)."""
-        ids = self._prompts(prompts)
+        ids = self._prompts(prompts, top)
         flat, positions, cu = self._pack(ids)
         logits = self._forward(flat, positions, lambda i, q, k, v: packed_attention(q, k, v, cu))
         # row t of a prompt predicts its token t + 1; a prompt's last row (whose target is the next prompt's) is dropped
@@ -121,7 +123,7 @@ class OlmoBatch:
     def generate(self, prompts: list[torch.Tensor], max_new_tokens: int, eos_token_id=None, top: int = 0) -> list[Generated]:
         """The greedy continuation of every prompt: one packed pass over the prompts, then one step for all sequences at a
         time until every one has ended."""
-        ids = self._prompts(prompts)
+        ids = self._prompts(prompts, top)
         if max_new_tokens < 1:
             raise OptimizeError("need at least one new token")
         eos = {eos_token_id} if isinstance(eos_token_id, int) else set(eos_token_id or ())

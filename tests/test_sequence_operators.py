@@ -226,3 +226,21 @@ def test_out_has_to_be_apart():
     wide = z(5, 2, 64)
     with pytest.raises(ValueError, match="overlap"):
         A._output("x", wide[1:], wide[:4], k, v)
+
+
+def test_a_batch_refuses_its_arguments_before_any_pass(monkeypatch):
+    from types import SimpleNamespace
+
+    from byteprof_amd.optim.olmo import OlmoConfig
+    from byteprof_amd.optim.olmo_batch import OlmoBatch
+
+    dec = SimpleNamespace(cfg=OlmoConfig(hidden=64, ffn=64, layers=1, heads=1, vocab=20), device=torch.device("cpu"))
+    batch = OlmoBatch(dec, pages=4)
+    monkeypatch.setattr(batch, "_forward", lambda *a, **k: pytest.fail("a pass ran"))
+    ids = [torch.tensor([1, 2, 3])]
+    for top in (33, 21, -1):
+        with pytest.raises(ValueError, match="top must be"):
+            batch.generate(ids, max_new_tokens=2, top=top)
+        with pytest.raises(ValueError, match="top must be"):
+            batch.score(ids, top=top)
+    assert len(batch.free) == 4
