@@ -106,3 +106,40 @@ def test_refusals():
         batch.generate(prompts((3,)), max_new_tokens=0)
     with pytest.raises(ValueError, match="at least one page"):
         OlmoBatch(dec, pages=0)
+
+
+def test_every_generated_token_against_the_oracle():
+    """The oracle's decode steps over what the batch generated: every token is its best but for the logits' error, every log
+    probability and entropy its own. Sequences of all lengths in one batch, through pages of 4."""
+    W = OG.random_weights(CFG, DEV, seed=10)
+    batch = OlmoBatch(OG.OlmoDecoder(CFG, W), pages=60, page=4)
+    ps = prompts((5, 23, 1, 40, 8), seed=6)
+    for p, got in zip(ps, batch.generate(ps, max_new_tokens=20, top=2)):
+        whole = torch.cat([p, got.tokens.cpu()]).tolist()
+        rows = oracle_rows(W, whole[:-1])[len(p) - 1:].astype(np.float64)
+        tol = 2 * LOGITS_TOL * np.abs(rows).max()  # an error of e in every logit moves a log probability by 2 e at most
+        lp = rows - (np.log(np.exp(rows - rows.max(-1, keepdims=True)).sum(-1, keepdims=True)) + rows.max(-1, keepdims=True))
+        mine = lp[np.arange(20), got.tokens.cpu().numpy()]
+        assert (mine >= lp.max(-1) - tol).all()
+        assert np.abs(got.logprobs.cpu().numpy() - mine).max() <= tol
+        assert np.abs(got.top_logprobs.cpu().numpy() - np.take_along_axis(lp, got.top_ids.cpu().numpy(), 1)).max() <= tol
+        ent = -(np.exp(lp) * lp).sum(-1)
+        # its derivative in a logit is -p (lp + H): errors of e move it by e sum p |lp + H| <= 2 e H at most, and as much again
+        assert (np.abs(got.entropy.cpu().numpy() - ent) <= 2 * tol * (1 + ent)).all()
+
+
+@pytest.mark.parametrize("kind", ["bf16", "int8", "int4"])
+def test_the_single_loops_tokens_are_the_batchs_choice(kind):
+    """Every token of the single-sequence loop, scored by the batch behind the same tokens: the batch's own choice there but for
+    the two paths' errors in the logits."""
+    dec = OG.OlmoDecoder(CFG, OG.random_weights(CFG, DEV, seed=8), kind)
+    batch = OlmoBatch(dec, pages=1)
+    ps = prompts((5, 23, 1, 70), seed=4)
+    wholes = [OG.make_generate(dec)(p[None], max_new_tokens=20)[0].cpu() for p in ps]
+    for p, got in zip(ps, batch.score(wholes, top=1)):
+        new = slice(len(p) - 1, None)
+        best = got.top_logprobs[new, 0]
+        assert len(best) == 20
+        # |logit| <= 8, four standard deviations (a normed row times a head row of std 2 / sqrt(hidden)): an error of e in each of
+        # the two paths' logits lets a token be chosen that lies 4 e below the other's best
+        assert (got.logprob[new] >= best - 4 * LOGITS_TOL * 8.0).all()
