@@ -70,11 +70,12 @@ __device__ __forceinline__ int chunk_at(int row, int place) {
   return (V ? v_place<DP>(row, place) : k_place<DP>(row, place)) - row * CH;
 }
 
-// 16 bytes per active lane from `src` to LDS at base + 16 x lane (base: wave-uniform byte address, in m0), without a register.
-// Counted by vmcnt: the wave waits with wait_vm before it, or after a barrier another wave, reads them.
+// 16 bytes per active lane from `src` to LDS at base + 16 x lane (base: wave-uniform byte address), without a register.
+// (m0 is the compiler's only between instructions that it emits together.) Counted by vmcnt: the wave waits with wait_vm before
+// it, or after a barrier another wave, reads them.
 __device__ __forceinline__ void load_lds16(const void* src, uint32_t base) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(base)), "v"(src)
-               : "memory", "m0");
+               : "memory");
 }
 // The same from a wave-uniform address plus a lane's own unsigned byte offset (a scalar that a vector instruction wrote, such
 // as a lane's value, may be an address five states later at the earliest).
@@ -84,12 +85,12 @@ __device__ __forceinline__ void load_lds16(const void* src, uint32_t offset, uin
   const uint64_t hi = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(p >> 32)));
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(base)),
                "v"(offset), "s"(hi << 32 | lo)
-               : "memory", "m0");
+               : "memory");
 }
 // 4 bytes per active lane, to base + 4 x lane.
 __device__ __forceinline__ void load_lds4(const void* src, uint32_t base) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(__builtin_amdgcn_readfirstlane(base)), "v"(src)
-               : "memory", "m0");
+               : "memory");
 }
 // Waits until at most N of the wave's vector-memory loads are outstanding; wait_lds until no LDS access is. As builtins and not
 // as asm: the compiler then knows that its own earlier loads have arrived too. Not knowing, it waited in every step for the
