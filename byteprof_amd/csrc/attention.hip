@@ -178,9 +178,9 @@ __device__ __forceinline__ float inverse(float l) { return l == 0.f ? 0.f : 1.f 
 
 // 128 rows, 32 a wave; the keys in steps of BN that all waves share in LDS, two images of each in turn. Bound by the matrix
 // instructions with the softmax beside them (two workgroups a CU fill each other's gaps): a causal document of 16384 tokens, 16
-// heads of 128, 1.1 ms or 990 TFLOP/s, where a large library matrix product reaches 1212; heads of 64, whose softmax is the same
-// for half the products, 620. With few tiles a step waits for its loads (about 2.5 us a step of one workgroup alone), which is
-// what dividing the keys is for.
+// heads of 128, 1.09 to 1.14 ms or 965 to 1008 TFLOP/s, where a large library matrix product reaches 1206; heads of 64, whose
+// softmax is the same for half the products, 820 (fp16) and 878 (bf16). With few tiles a step waits for its loads (about 2.5 us a
+// step of one workgroup alone), which is what dividing the keys is for.
 template <class T, int DP, bool PAGED, bool FULL>
 __device__ __forceinline__ void large_tile(const Args& a, const Item& it, int kvh, u32x4* smem, const int* ring) {
   using S = Shape<DP>;
@@ -418,7 +418,8 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void attention_kernel(A
 }
 
 // A unit's rows, a thread 4 columns of one, whose parts it loads kMergeParts at a time. MORE: there are more parts than that (the
-// form without the running sums is 5 us faster where there are not: heads of 64 in two parts, 45 us in all against 40).
+// form without the running sums is 5 us faster where there are not: prompts of 2047 and 1300 tokens, heads of 64, in 3 and 2 parts
+// a tile, 45 us in all against 40).
 template <class T, int DP, bool MORE>
 __device__ __forceinline__ void merge_rows(const Args& a, const Item& it, int kvh, const float* ws, int64_t step) {
   const int pieces = a.d / 4;

@@ -229,7 +229,8 @@ __device__ __forceinline__ Item find_item(const Args& a, int index) {
 }
 
 constexpr int kCus = 256;
-constexpr int kTarget = 1024;    // most parts that splitting aims at: twice the workgroups that the card holds at once
+constexpr int kTarget = 1024;    // bound of what splitting aims at (twice the workgroups that the card holds at once: 1024, for 256
+                                 // columns 512)
 constexpr int kChunkMin = BP_ATTN_UNDIVIDED_KEYS;  // least keys of a split
 constexpr int kMergeGrid = 1024;  // workgroups of a merge launch; each takes every such unit
 

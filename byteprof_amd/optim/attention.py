@@ -188,7 +188,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     [sequences + 1]), caches [pages, page size, Hk, D], table [sequences, most pages] (position p of sequence b in page
     table[b, p // page size]; entries past its length are not read), lengths [sequences]: a sequence's positions in the
     cache, its chunk's among them (append first). A chunk's tokens are the last positions; each sees all up to its own. Rows
-    that no chunk covers come out as zeros; rows of a sequence with a page id outside the cache below its length as NaN.
+    that no chunk covers come out as zeros. A row that sees a position whose page id is outside the cache is NaN; so may other
+    rows of its chunk be.
     Returns [tokens, Hq, D], in `out` when given: q itself or a tensor apart from q and the caches."""
     what = "paged_attention"
     if q.dim() != 3:

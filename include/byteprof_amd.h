@@ -427,7 +427,8 @@ int bp_decode_argmax_rows(const void* logits, int vocab, int rows, int64_t* tok,
  * paged:  caches [pool, page, hk, head_dim] (any strides between pages, positions and heads). Sequence b has lengths[b]
  *         (int32) positions, position p in page table[b, p / page] (int32, table_stride entries a row), at p % page; its
  *         tokens are the last of them, their keys and values in the cache already; the token at position p sees 0 .. p.
- *         lengths are taken up to page x max_pages. Rows of a sequence that has to read a page outside [0, pool) become NaN.
+ *         lengths are taken up to page x max_pages. Rows that see a position whose page is outside [0, pool) become NaN; so
+ *         may the other rows of their sequence (those that share a tile with them).
  * The offsets, lengths and table are read on the device only: a captured graph serves whatever they hold at a replay.
  * workspace: bp_attn_workspace_bytes(tokens, seqs, hq, hk, head_dim, max_keys) bytes, 16-byte aligned, for the partial sums of
  * divided keys (max_keys: tokens, or page x max_pages for the cache); nothing in it outlives the call.
