@@ -1,9 +1,11 @@
 // Attention of packed prompts and of chunks over a paged cache, and the append to the cache's pages (attention.h: the
 // mathematics; attention_plan.h: the plan).
 
-#include "attention.h"
+#include "attention_rows.h"
 
 #include <float.h>
+
+#include <type_traits>
 
 #include "byteprof_amd.h"
 
@@ -136,46 +138,6 @@ __device__ __forceinline__ void load_rows(const Source<PAGED>& src, const u32x4*
   }
 }
 
-// Rows that belong to no sequence: zeros, dealt to the workgroups past the last tile.
-__device__ void fill_rest(const Args& a, int kvh, int extra, int extras) {
-  const int lo = a.seqs > 0 ? min(max(a.cu[0], 0), a.tokens) : a.tokens;
-  int hi = a.seqs > 0 ? min(max(a.cu[a.seqs], lo), a.tokens) : a.tokens;
-  const int64_t rest = lo + (a.tokens - hi), per = static_cast<int64_t>(a.group.d) * a.d / 8;
-  for (int64_t i = static_cast<int64_t>(extra) * kThreads + threadIdx.x; i < rest * per;
-       i += static_cast<int64_t>(extras) * kThreads) {
-    const int64_t n = i / per, c = i % per;
-    const int64_t tok = n < lo ? n : hi + (n - lo);
-    uint16_t* at = static_cast<uint16_t*>(a.out) + (tok * a.hq + static_cast<int64_t>(kvh) * a.group.d) * a.d + 8 * c;
-    *reinterpret_cast<u32x4*>(at) = u32x4{};
-  }
-}
-
-__device__ __forceinline__ uint16_t* out_row(const Args& a, const Item& it, int kvh, int row) {
-  const int n = a.group(row);
-  const int64_t head = static_cast<int64_t>(it.begin + n) * a.hq + kvh * a.group.d + (row - n * a.group.d);
-  return static_cast<uint16_t*>(a.out) + head * a.d;
-}
-
-// A split's slot: [ws_rows][DP] sums, then ws_rows maxima and ws_rows sums of probabilities.
-template <int DP>
-__device__ __forceinline__ float* slot_at(const Args& a, int64_t slot, int kvh) {
-  return a.ws + (slot * a.hk.d + kvh) * a.ws_rows * (DP + 2);
-}
-
-template <class T, int DP, bool FULL>
-__device__ __forceinline__ void load_q(const Args& a, const Item& it, int kvh, int row, u32x4 (&q)[DP / 16], int lane) {
-  const int n = a.group(row);
-  const uint16_t* p = static_cast<const uint16_t*>(a.q) + static_cast<int64_t>(it.begin + n) * a.q_t +
-                      static_cast<int64_t>(kvh * a.group.d + row - n * a.group.d) * a.q_h;
-#pragma unroll
-  for (int i = 0; i < DP / 16; ++i) {
-    const int c = 2 * i + (lane >> 5);
-    q[i] = FULL || 8 * c < a.d ? *reinterpret_cast<const u32x4*>(p + 8 * c) : u32x4{};
-  }
-}
-
-__device__ __forceinline__ float inverse(float l) { return l == 0.f ? 0.f : 1.f / l; }
-
 // 128 rows, 32 a wave; the keys in steps of BN that all waves share in LDS, two images of each in turn. Bound by the matrix
 // instructions with the softmax beside them (two workgroups a CU fill each other's gaps): a causal document of 16384 tokens, 16
 // heads of 128, 1.09 to 1.14 ms or 965 to 1008 TFLOP/s, where a large library matrix product reaches 1206; heads of 64, whose
@@ -241,42 +203,7 @@ __device__ __forceinline__ void large_tile(const Args& a, const Item& it, int kv
   if constexpr (PAGED) {
     if (__syncthreads_or(src.bad)) r.l = NAN;
   }
-  if (!active) return;
-  const float l = add_halves(r.l);
-  if (!it.divided) {
-    const float inv = inverse(l);
-    uint16_t* out = out_row(a, it, kvh, mine);
-#pragma unroll
-    for (int db = 0; db < DP / 32; ++db)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        // columns 16 i + 4 half + 0..3 and 8 further, as 8 columns a lane: the halves exchange a group of 4
-        u32x2 x, y;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          x[e] = T::pack(r.o[db][8 * i + 2 * e] * inv, r.o[db][8 * i + 2 * e + 1] * inv);
-          y[e] = T::pack(r.o[db][8 * i + 4 + 2 * e] * inv, r.o[db][8 * i + 4 + 2 * e + 1] * inv);
-        }
-        const auto w0 = __builtin_amdgcn_permlane32_swap(x[0], y[0], false, false);
-        const auto w1 = __builtin_amdgcn_permlane32_swap(x[1], y[1], false, false);
-        const int col = 32 * db + 16 * i + 8 * (lane >> 5);
-        if (row <= top && col < a.d) *reinterpret_cast<u32x4*>(out + col) = u32x4{w0[0], w1[0], w0[1], w1[1]};
-      }
-    return;
-  }
-  float* ws = slot_at<DP>(a, it.slot + it.split, kvh);
-  const int at = row - it.row0;
-  if (row > top || it.slot + it.split >= a.slots) return;
-#pragma unroll
-  for (int db = 0; db < DP / 32; ++db)
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      *reinterpret_cast<f32x4*>(ws + at * DP + 32 * db + 8 * i + 4 * (lane >> 5)) =
-          f32x4{r.o[db][4 * i], r.o[db][4 * i + 1], r.o[db][4 * i + 2], r.o[db][4 * i + 3]};
-  if (lane < 32) {
-    ws[a.ws_rows * DP + at] = r.m;
-    ws[a.ws_rows * (DP + 1) + at] = l;
-  }
+  if (active) write_rows<T, DP>(a, it, kvh, row, r, lane);
 }
 
 // Up to 32 rows: every wave has all rows and takes every fourth block of 32 keys, through images of its own; then the waves'
@@ -335,63 +262,7 @@ __device__ __forceinline__ void small_tile(const Args& a, const Item& it, int kv
     }
   }
   if (PAGED && __any(src.bad)) r.l = NAN;
-  r.l = add_halves(r.l);
-  // stats: [wave][32] maxima, [wave][32] sums, [32] factors of the result
-  if (lane < 32) {
-    stats[32 * wave + lane] = r.m;
-    stats[32 * (kWaves + wave) + lane] = r.l;
-  }
-  __syncthreads();
-  float m = -INFINITY, l = 0.f;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) m = fmaxf(m, stats[32 * w + (lane & 31)]);
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    const float mw = stats[32 * w + (lane & 31)];
-    l += stats[32 * (kWaves + w) + (lane & 31)] * rescaled(mw, m, a.scale_log2);
-  }
-  const float f = rescaled(r.m, m, a.scale_log2);
-  const bool whole = !it.divided;
-  float* ws = whole ? nullptr : slot_at<DP>(a, it.slot + it.split, kvh);
-  const bool keep = whole || it.slot + it.split < a.slots;
-  if (wave == 0 && lane < 32) {
-    stats[32 * 2 * kWaves + lane] = whole ? inverse(l) : 1.f;
-    if (!whole && keep && lane < it.rows) {
-      ws[a.ws_rows * DP + lane] = m;
-      ws[a.ws_rows * (DP + 1) + lane] = l;
-    }
-  }
-  f32x4* parts = reinterpret_cast<f32x4*>(smem);
-  constexpr int G = S::G;
-#pragma unroll
-  for (int g = 0; g < DP / 32 / G; ++g) {
-    if ((lane & 31) < it.rows) {
-#pragma unroll
-      for (int db = 0; db < G; ++db)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const f32x16& o = r.o[g * G + db];
-          parts[(wave * G * 8 + db * 8 + 2 * i + (lane >> 5)) * 32 + (lane & 31)] =
-              f32x4{o[4 * i] * f, o[4 * i + 1] * f, o[4 * i + 2] * f, o[4 * i + 3] * f};
-        }
-    }
-    __syncthreads();
-    for (int i = tid; i < it.rows * G * 8; i += kThreads) {
-      const int row = i / (G * 8), piece = i % (G * 8), col = 4 * piece + 32 * G * g;
-      f32x4 x = parts[piece * 32 + row];
-#pragma unroll
-      for (int w = 1; w < kWaves; ++w) x += parts[(w * G * 8 + piece) * 32 + row];
-      if (whole) {
-        const float inv = stats[32 * 2 * kWaves + row];
-        if (col < a.d)
-          *reinterpret_cast<u32x2*>(out_row(a, it, kvh, it.row0 + row) + col) =
-              u32x2{T::pack(x[0] * inv, x[1] * inv), T::pack(x[2] * inv, x[3] * inv)};
-      } else if (keep) {
-        *reinterpret_cast<f32x4*>(ws + row * DP + col) = x;
-      }
-    }
-    if (g + 1 < DP / 32 / G) __syncthreads();
-  }
+  join_waves<T, DP, S::G>(a, it, kvh, r, smem, stats);
 }
 
 // 256 columns: a wave's sums alone are 128 registers, so one workgroup a CU with all of them.
@@ -579,12 +450,9 @@ int launch(const Args& a, const Launch& n, hipStream_t st) {
   const unsigned grid = static_cast<unsigned>(n.index * a.hk.d);
   if (a.d == DP) attention_kernel<T, DP, PAGED, true><<<grid, kThreads, 0, st>>>(a);
   else attention_kernel<T, DP, PAGED, false><<<grid, kThreads, 0, st>>>(a);
-  hipError_t e = hipGetLastError();
-  if (e == hipSuccess && n.merges > 0) {
-    merge_kernel<T, DP><<<static_cast<unsigned>(n.merges * a.hk.d), kThreads, 0, st>>>(a);
-    e = hipGetLastError();
-  }
-  return e == hipSuccess ? BP_OK : static_cast<int>(e);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return static_cast<int>(e);
+  return n.merges > 0 ? launch_merge(std::is_same<T, Bf16>::value ? BP_DT_BF16 : BP_DT_F16, a, n, st) : BP_OK;
 }
 
 template <class T, bool PAGED>
@@ -641,6 +509,20 @@ int run(int dtype, Args& a, bool paged, size_t ws_bytes, hipStream_t st) {
 }
 
 }  // namespace
+
+int launch_merge(int dtype, const Args& a, const Launch& n, hipStream_t st) {
+  const unsigned grid = static_cast<unsigned>(n.merges * a.hk.d);
+  const bool bf16 = dtype == BP_DT_BF16;
+  switch (padded_dim(a.d)) {
+    case 64: bf16 ? merge_kernel<Bf16, 64><<<grid, kThreads, 0, st>>>(a) : merge_kernel<F16, 64><<<grid, kThreads, 0, st>>>(a); break;
+    case 96: bf16 ? merge_kernel<Bf16, 96><<<grid, kThreads, 0, st>>>(a) : merge_kernel<F16, 96><<<grid, kThreads, 0, st>>>(a); break;
+    case 128: bf16 ? merge_kernel<Bf16, 128><<<grid, kThreads, 0, st>>>(a) : merge_kernel<F16, 128><<<grid, kThreads, 0, st>>>(a); break;
+    default: bf16 ? merge_kernel<Bf16, 256><<<grid, kThreads, 0, st>>>(a) : merge_kernel<F16, 256><<<grid, kThreads, 0, st>>>(a);
+  }
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? BP_OK : static_cast<int>(e);
+}
+
 }  // namespace attn
 }  // namespace bp
 
