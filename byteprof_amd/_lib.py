@@ -23,7 +23,7 @@ BP_E_INVALID_ARG = -1
 BP_E_UNSUPPORTED = -2
 BP_E_WORKSPACE = -3
 
-DT_BF16, DT_F16, DT_F32, DT_I8 = 0, 1, 2, 3
+DT_BF16, DT_F16, DT_F32, DT_I8, DT_E4M3 = 0, 1, 2, 3, 4
 TORCH_DT = {torch.bfloat16: DT_BF16, torch.float16: DT_F16, torch.float32: DT_F32, torch.int8: DT_I8}
 
 _c_i64, _c_int, _c_size, _c_vp, _c_float = ctypes.c_int64, ctypes.c_int, ctypes.c_size_t, ctypes.c_void_p, ctypes.c_float
@@ -106,6 +106,11 @@ SIGNATURES: dict[str, tuple] = {
     "bp_attn_paged": (_c_int, [_c_int] + [_c_vp] * 5 + [_c_i64, _c_vp, _c_vp] + [_c_int] * 8 + [_c_i64] * 8 +
                       [_c_float, _c_vp, _c_size, _c_vp]),
     "bp_paged_append": (_c_int, [_c_int] + [_c_vp] * 5 + [_c_i64, _c_vp, _c_vp] + [_c_int] * 7 + [_c_i64] * 10 + [_c_vp]),
+    "bp_paged_append8": (_c_int, [_c_int, _c_int] + [_c_vp] * 7 + [_c_i64, _c_vp, _c_vp] + [_c_int] * 8 + [_c_i64] * 16 + [_c_vp]),
+    "bp_attn_paged8": (_c_int, [_c_int, _c_int] + [_c_vp] * 7 + [_c_i64, _c_vp, _c_vp] + [_c_int] * 9 + [_c_i64] * 14 +
+                       [_c_float, _c_vp, _c_size, _c_vp]),
+    "bp_paged_read": (_c_int, [_c_int, _c_int] + [_c_vp] * 7 + [_c_i64, _c_vp, _c_vp] + [_c_int] * 8 + [_c_i64] * 12 + [_c_vp]),
+    "bp_rotary": (_c_int, [_c_int] + [_c_vp] * 5 + [_c_int, _c_vp, _c_i64] + [_c_int] * 5 + [_c_float] + [_c_i64] * 8 + [_c_vp]),
     "bp_logprobs_workspace_bytes": (_c_size, [_c_int, _c_i64, _c_i64, _c_int]),
     "bp_logprobs": (_c_int, [_c_int, _c_vp, _c_i64] + [_c_vp] * 5 + [_c_i64, _c_i64, _c_int, _c_vp, _c_size, _c_vp]),
 }

@@ -1,0 +1,401 @@
+// Attention of chunks of new tokens over a paged cache held in 8 bits (cache8.h: the codes; attention.h: the mathematics of the
+// tiles; attention_plan.h: the plan). A position's codes become values of the queries' type, exactly, on their way to the matrix
+// instructions; from there on everything is as over a cache in 16 bits.
+
+#include "attention_rows.h"
+#include "cache8.h"
+
+#include <float.h>
+
+#include <type_traits>
+
+#include "byteprof_amd.h"
+
+namespace bp {
+namespace attn {
+
+// The launch's arguments: those of the 16-bit kernels (k, v: the codes) and the scales' places.
+struct Args8 : Args {
+  const uint8_t* ks;  // [pool, blocks of a page, hk]
+  const uint8_t* vs;
+  int64_t ks_p, ks_b, ks_h, vs_p, vs_b, vs_h;
+  Div block;
+  int wide;  // 16 codes at a time: all rows lie on 16 bytes and are made of them
+};
+
+namespace {
+
+// The cache as an item sees it. Ids of pages are looked up ahead of the loads that need them.
+struct Cache {
+  const uint8_t* k;
+  const uint8_t* v;
+  const uint8_t* ks;
+  const uint8_t* vs;
+  const int* pages;
+  int last;  // the item's last key
+  bool bad;  // a page outside the pool: the item's rows become NaN
+
+  __device__ __forceinline__ Cache(const Args8& a, const Item& it, int kvh) {
+    k = static_cast<const uint8_t*>(a.k) + kvh * a.k_h;
+    v = static_cast<const uint8_t*>(a.v) + kvh * a.v_h;
+    ks = a.ks + kvh * a.ks_h;
+    vs = a.vs + kvh * a.vs_h;
+    pages = a.table + static_cast<int64_t>(it.b) * a.table_stride;
+    last = it.key1 - 1;
+    bad = false;
+  }
+  __device__ __forceinline__ int id(const Args8& a, int key) const { return pages[a.page(min(key, last))]; }
+  // Where a key's row of codes and its scales lie; n: what id() gave for it.
+  __device__ __forceinline__ void at(const Args8& a, int key, int n, int64_t& ko, int64_t& vo, int64_t& kso, int64_t& vso) {
+    key = min(key, last);
+    const int slot = key - a.page(key) * a.page.d, blk = a.block(slot);
+    if (static_cast<unsigned>(n) >= static_cast<unsigned>(a.pool)) {
+      bad = true;
+      n = 0;
+    }
+    ko = n * a.k_p + slot * a.k_t;
+    vo = n * a.v_p + slot * a.v_t;
+    kso = n * a.ks_p + blk * a.ks_b;
+    vso = n * a.vs_p + blk * a.vs_b;
+  }
+};
+
+// 16 codes from column 16 c of a row; of heads that are not whole tiles, zeros past the head's own columns.
+template <bool FULL>
+__device__ __forceinline__ u32x4 codes16(const Args8& a, const uint8_t* row, int c) {
+  if (FULL || (a.wide && 16 * c < a.d)) return *reinterpret_cast<const u32x4*>(row + 16 * c);
+  u32x4 r = {};
+  if (!a.wide) {
+    if (16 * c < a.d) {
+      const u32x2 x = *reinterpret_cast<const u32x2*>(row + 16 * c);
+      r[0] = x[0], r[1] = x[1];
+    }
+    if (16 * c + 8 < a.d) {
+      const u32x2 x = *reinterpret_cast<const u32x2*>(row + 16 * c + 8);
+      r[2] = x[0], r[3] = x[1];
+    }
+  }
+  return r;
+}
+
+// Place of 16-code chunk `chunk` of a row in a wave's image of 32 value rows: turned, so that 8 rows written and the 8 rows that
+// a transposed read takes (4 and 4, 8 apart) lie in different banks.
+template <int DP>
+__device__ __forceinline__ int place8(int row, int chunk) {
+  constexpr int CH = DP / 16;
+  const int turn = (row & 7) ^ ((row >> 3 & 1) << 2);
+  if constexpr (CH == 4) return row * CH + (chunk ^ ((row >> 2 & 1) | (row >> 2 & 2)));
+  else if constexpr (CH == 8) return row * CH + (chunk ^ turn);
+  else if constexpr (CH == 16) return row * CH + (chunk ^ 2 * turn);
+  else return row * CH + chunk;
+}
+
+template <int DP>
+struct Shape8 {
+  static constexpr int BN = DP <= 128 ? 64 : 32;  // keys of a step of a large tile
+  static constexpr int kLarge = 4 * BN * DP / 8;  // 16-byte chunks: two images of keys and two of values, as values
+  static constexpr int kSmall = kWaves * 32 * DP / 16;  // a wave's value codes
+  static constexpr int G = DP / 32 < 4 ? DP / 32 : 4;
+  static constexpr int kMerge = kWaves * G * 8 * 32;
+  static constexpr int kChunks = kLarge > kSmall ? (kLarge > kMerge ? kLarge : kMerge) : (kSmall > kMerge ? kSmall : kMerge);
+};
+
+// O^T += V^T P^T over 32 keys whose codes lie in a wave's image; scale: the lane's key's.
+template <class T, class C, int DP>
+__device__ __forceinline__ void weighted8(const u32x4* img, int scale, const u32x4 (&p)[2], f32x16 (&o)[DP / 32], int lane) {
+  typedef int i32x2 __attribute__((ext_vector_type(2)));
+  typedef __attribute__((address_space(3))) i32x2* lds2;
+  const int half = lane >> 5, sub = (lane >> 4) & 1, j = (lane & 15) >> 1, e = lane & 1;
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    // a scale holds for aligned groups of 4 keys at least
+    const typename C::Scale s0 = C::scale(__shfl(scale, 16 * t + 4 * half)), s1 = C::scale(__shfl(scale, 16 * t + 8 + 4 * half));
+    const int key = 16 * t + 8 * (j >> 2) + 4 * half + (j & 3);
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db) {
+      // a 16-lane group reads 8 keys x 16 columns, 8 columns a lane, and gets them transposed: its column's 8 keys
+      const char* at = reinterpret_cast<const char*>(img + place8<DP>(key, 2 * db + sub)) + 8 * e;
+      const i32x2 r = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds2)(__attribute__((address_space(3))) void*)at);
+      const u32x2 x = C::four(r[0], s0), y = C::four(r[1], s1);
+      o[db] = T::mfma(u32x4{x[0], x[1], y[0], y[1]}, p[t], o[db]);
+    }
+  }
+}
+
+// Up to 32 rows: every wave has all rows and takes every fourth block of 32 keys; then the waves' parts are joined. Keys go from
+// memory to registers, 16 codes a lane of the lane's own key, and become the first product's operand there (its order of the
+// columns is the queries', too); values go through an image in LDS, which is read transposed. A block's loads are sent as soon as
+// the last block's registers are free.
+template <class T, class C, int DP, bool FULL>
+__device__ __forceinline__ void small_tile8(const Args8& a, const Item& it, int kvh, u32x4* smem, float* stats) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
+  const int top = it.row0 + it.rows - 1;
+  const int mine = min(it.row0 + (lane & 31), top);
+  u32x4 q[DP / 16];
+  {
+    const int n = a.group(mine);
+    const uint16_t* p = static_cast<const uint16_t*>(a.q) + static_cast<int64_t>(it.begin + n) * a.q_t +
+                        static_cast<int64_t>(kvh * a.group.d + mine - n * a.group.d) * a.q_h;
+#pragma unroll
+    for (int i = 0; i < DP / 16; ++i) {
+      const int col = 32 * (i / 2) + 16 * half + 8 * (i % 2);
+      q[i] = FULL || col < a.d ? *reinterpret_cast<const u32x4*>(p + col) : u32x4{};
+    }
+  }
+  const int limit = min(it.first + a.group(mine), it.keys - 1);
+  const int least = __builtin_amdgcn_readfirstlane(limit);
+  Running<DP> r;
+  r.clear();
+  Cache cache(a, it, kvh);
+  u32x4* img = smem + wave * 32 * (DP / 16);
+  constexpr int STEP = 32 * kWaves;
+  u32x4 kc[DP / 32], vc[DP / 32];
+  int ks = 0, vs = 0, next = 0;
+  const auto load = [&](int key) {
+    int64_t ko, vo, kso, vso;
+    cache.at(a, key, next, ko, vo, kso, vso);
+    ks = cache.ks[kso];
+#pragma unroll
+    for (int c = 0; c < DP / 32; ++c) kc[c] = codes16<FULL>(a, cache.k + ko, 2 * c + half);
+    vs = cache.vs[vso];
+#pragma unroll
+    for (int c = 0; c < DP / 32; ++c) vc[c] = codes16<FULL>(a, cache.v + vo, 2 * c + half);
+    next = cache.id(a, key + STEP);
+  };
+  int key = it.key0 + 32 * wave;
+  const int sub = lane & 31;
+  if (key < it.key1) {
+    next = cache.id(a, key + sub);
+    load(key + sub);
+  }
+  for (; key < it.key1; key += STEP) {
+    f32x16 s[1] = {};
+    const typename C::Scale kscale = C::scale(ks);
+#pragma unroll
+    for (int c = 0; c < DP / 32; ++c) {
+      s[0] = T::mfma(cache8::eight<C>(kc[c][0], kc[c][1], kscale), q[2 * c], s[0]);
+      s[0] = T::mfma(cache8::eight<C>(kc[c][2], kc[c][3], kscale), q[2 * c + 1], s[0]);
+    }
+#pragma unroll
+    for (int c = 0; c < DP / 32; ++c) img[place8<DP>(sub, 2 * c + half)] = vc[c];
+    const int now = vs;
+    if (key + STEP < it.key1) load(key + STEP + sub);
+    u32x4 p[1][2];
+    softmax_step<T, DP, 1>(s, p, r, a.scale_log2, key, min(limit, cache.last), key + 31 > min(least, cache.last), lane);
+    weighted8<T, C, DP>(img, now, p[0], r.o, lane);
+  }
+  if (__any(cache.bad)) r.l = NAN;
+  join_waves<T, DP, Shape8<DP>::G>(a, it, kvh, r, smem, stats);
+}
+
+// 128 rows, 32 a wave; the keys in steps of BN that all waves share. The workgroup turns a step's codes into values once, in
+// registers, and writes them to the images that the 16-bit kernel's tiles have (two of each in turn); their loads are sent a step
+// before.
+template <class T, class C, int DP, bool FULL>
+__device__ __forceinline__ void large_tile8(const Args8& a, const Item& it, int kvh, u32x4* smem) {
+  using S = Shape8<DP>;
+  constexpr int BN = S::BN, NB = BN / 32, CH = DP / 16, IMG = BN * DP / 8;
+  constexpr int N = (BN * CH + kThreads - 1) / kThreads;  // 16-code pieces of a thread
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int top = it.row0 + it.rows - 1;
+  const int row = it.row0 + 32 * wave + (lane & 31);
+  const int mine = min(row, top);
+  const bool active = it.row0 + 32 * wave <= top;
+  u32x4 q[DP / 16];
+  load_q<T, DP, FULL>(a, it, kvh, mine, q, lane);
+  const int limit = min(it.first + a.group(mine), it.keys - 1);
+  const int least = __builtin_amdgcn_readfirstlane(limit), most = __builtin_amdgcn_readlane(limit, 31);
+  Running<DP> r;
+  r.clear();
+  Cache cache(a, it, kvh);
+  u32x4 kc[N], vc[N];
+  int ks[N], vs[N], next[N];
+  const auto mine_of = [&](int n) { return BN * CH % kThreads == 0 || tid + n * kThreads < BN * CH; };
+  const auto look = [&](int key) {
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+      if (mine_of(n)) next[n] = cache.id(a, key + (tid + n * kThreads) / CH);
+  };
+  const auto load = [&](int key) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      if (!mine_of(n)) continue;
+      const int i = tid + n * kThreads;
+      int64_t ko, vo, kso, vso;
+      cache.at(a, key + i / CH, next[n], ko, vo, kso, vso);
+      ks[n] = cache.ks[kso];
+      vs[n] = cache.vs[vso];
+      kc[n] = codes16<FULL>(a, cache.k + ko, i % CH);
+      vc[n] = codes16<FULL>(a, cache.v + vo, i % CH);
+    }
+  };
+  const auto turn = [&](int to) {
+    u32x4* kimg = smem + to * IMG;
+    u32x4* vimg = smem + (2 + to) * IMG;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      if (!mine_of(n)) continue;
+      const int i = tid + n * kThreads, rw = i / CH, c = i % CH;
+      const typename C::Scale sk = C::scale(ks[n]), sv = C::scale(vs[n]);
+      kimg[k_place<DP>(rw, 2 * c)] = cache8::eight<C>(kc[n][0], kc[n][1], sk);
+      kimg[k_place<DP>(rw, 2 * c + 1)] = cache8::eight<C>(kc[n][2], kc[n][3], sk);
+      vimg[v_place<DP>(rw, 2 * c)] = cache8::eight<C>(vc[n][0], vc[n][1], sv);
+      vimg[v_place<DP>(rw, 2 * c + 1)] = cache8::eight<C>(vc[n][2], vc[n][3], sv);
+    }
+  };
+  int buf = 0;
+  if (it.key0 < it.key1) {
+    look(it.key0);
+    load(it.key0);
+    look(it.key0 + BN);
+    turn(0);
+    if (it.key0 + BN < it.key1) load(it.key0 + BN);
+    look(it.key0 + 2 * BN);
+  }
+  // The image of this step is written; so is, behind the barrier, that of the next, whose loads were sent a step ago.
+  const auto step = [&](int key) {
+    __syncthreads();
+    if (key + BN < it.key1) {
+      turn(buf ^ 1);
+      if (key + 2 * BN < it.key1) {
+        load(key + 2 * BN);
+        look(key + 3 * BN);
+      }
+    }
+  };
+  int key = it.key0;
+  const int mine_end = active ? min(it.key1, most + 1) : it.key0;
+  for (; key < mine_end; key += BN) {
+    step(key);
+    f32x16 s[NB];
+    u32x4 p[NB][2];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) s[b] = scores<T, DP>(smem + buf * IMG, 32 * b, q, lane);
+    softmax_step<T, DP, NB>(s, p, r, a.scale_log2, key, min(limit, cache.last), key + BN - 1 > min(least, cache.last), lane);
+#pragma unroll
+    for (int b = 0; b < NB; ++b) weighted<T, DP>(smem + (2 + buf) * IMG, 32 * b, p[b], r.o, lane);
+    buf ^= 1;
+  }
+  for (; key < it.key1; key += BN) {
+    step(key);
+    buf ^= 1;
+  }
+  if (__syncthreads_or(cache.bad)) r.l = NAN;
+  if (active) write_rows<T, DP>(a, it, kvh, row, r, lane);
+}
+
+template <class T, class C, int DP, bool FULL>
+__global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void attention8_kernel(Args8 a) {
+  __shared__ __align__(16) u32x4 smem[Shape8<DP>::kChunks];
+  __shared__ float stats[32 * (2 * kWaves + 1)];
+  if constexpr (std::is_same<T, F16>::value) cache8::saturate_f16();
+  const int index = a.hk(blockIdx.x), kvh = blockIdx.x - index * a.hk.d;
+  const Item it = find_item<false>(a, index);
+  if (it.b < 0) {
+    fill_rest(a, kvh, it.extra, a.hk(gridDim.x) - (index - it.extra));
+    return;
+  }
+  if (it.key0 >= it.key1 && it.split > 0) return;
+  if (it.small) small_tile8<T, C, DP, FULL>(a, it, kvh, smem, stats);
+  else large_tile8<T, C, DP, FULL>(a, it, kvh, smem);
+}
+
+template <class T, int KIND, int DP>
+int launch8(const Args8& a, const Launch& n, hipStream_t st) {
+  constexpr bool bf16 = std::is_same<T, Bf16>::value;
+  using C = cache8::Codes<KIND, bf16>;
+  const unsigned grid = static_cast<unsigned>(n.index * a.hk.d);
+  if (a.d == DP && a.wide) attention8_kernel<T, C, DP, true><<<grid, kThreads, 0, st>>>(a);
+  else attention8_kernel<T, C, DP, false><<<grid, kThreads, 0, st>>>(a);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return static_cast<int>(e);
+  return n.merges > 0 ? launch_merge(bf16 ? BP_DT_BF16 : BP_DT_F16, a, n, st) : BP_OK;
+}
+
+template <class T, int KIND>
+int launch8_dim(const Args8& a, const Launch& n, hipStream_t st) {
+  switch (padded_dim(a.d)) {
+    case 64: return launch8<T, KIND, 64>(a, n, st);
+    case 96: return launch8<T, KIND, 96>(a, n, st);
+    case 128: return launch8<T, KIND, 128>(a, n, st);
+    default: return launch8<T, KIND, 256>(a, n, st);
+  }
+}
+
+bool aligned(const void* p, int n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+int run8(int dtype, int kind, Args8& a, size_t ws_bytes, hipStream_t st) {
+  const int hk = a.hk.d;
+  if ((dtype != BP_DT_BF16 && dtype != BP_DT_F16) || (kind != BP_DT_E4M3 && kind != BP_DT_I8)) return BP_E_UNSUPPORTED;
+  if (a.tokens < 0 || a.seqs < 0 || hk <= 0 || a.hq <= 0 || a.hq % hk != 0 || !(a.scale_log2 > 0.f && a.scale_log2 <= FLT_MAX))
+    return BP_E_INVALID_ARG;
+  if (a.d <= 0 || a.d % 8 != 0 || a.d > 256) return BP_E_UNSUPPORTED;
+  if (a.tokens == 0) return BP_OK;
+  if (a.q == nullptr || a.out == nullptr || (a.seqs > 0 && a.cu == nullptr)) return BP_E_INVALID_ARG;
+  // a stride that nothing is multiplied with may be anything
+  const int blocks = a.page.d / a.block.d;
+  if (a.tokens == 1) a.q_t = 0;
+  if (a.hq == 1) a.q_h = 0;
+  if (hk == 1) a.k_h = a.v_h = a.ks_h = a.vs_h = 0;
+  if (a.page.d == 1) a.k_t = a.v_t = 0;
+  if (blocks == 1) a.ks_b = a.vs_b = 0;
+  if (a.pool == 1) a.k_p = a.v_p = a.ks_p = a.vs_p = 0;
+  const int64_t strides = a.k_p | a.k_t | a.k_h | a.v_p | a.v_t | a.v_h;
+  if (!aligned(a.q, 16) || !aligned(a.out, 16) || ((a.q_t | a.q_h) & 7) != 0 || !aligned(a.k, 8) || !aligned(a.v, 8) ||
+      (strides & 7) != 0)
+    return BP_E_INVALID_ARG;
+  a.wide = aligned(a.k, 16) && aligned(a.v, 16) && (strides & 15) == 0 && a.d % 16 == 0;
+  // rows of a sequence, and keys plus a split, in 32 bits
+  if (static_cast<int64_t>(a.tokens) * a.hq >= (1ll << 30) || a.max_keys >= (1 << 29)) return BP_E_UNSUPPORTED;
+  Launch n;
+  if (!plan_launch(a, n)) return BP_E_UNSUPPORTED;
+  if (n.workspace > 0 && (a.ws == nullptr || ws_bytes < n.workspace || !aligned(a.ws, 16))) return BP_E_WORKSPACE;
+  if (n.workspace == 0) a.ws = nullptr;
+  // A row of q is read by the tile that writes its result and by no other, so out may be q itself.
+  const auto reach = [](int size, int64_t n0, int64_t s0, int64_t n1, int64_t s1, int64_t n2, int64_t s2, int64_t last) {
+    return n0 > 0 ? size * ((n0 - 1) * s0 + (n1 - 1) * s1 + (n2 - 1) * s2 + last) : 0;
+  };
+  const int64_t dense = static_cast<int64_t>(a.hq) * a.d, out = 2 * dense * a.tokens;
+  const bool in_place = a.out == a.q && (a.tokens == 1 || a.q_t == dense) && (a.hq == 1 || a.q_h == a.d);
+  if ((!in_place && ranges_overlap(a.out, out, a.q, reach(2, a.tokens, a.q_t, a.hq, a.q_h, 1, 0, a.d))) ||
+      ranges_overlap(a.out, out, a.k, reach(1, a.pool, a.k_p, a.page.d, a.k_t, hk, a.k_h, a.d)) ||
+      ranges_overlap(a.out, out, a.v, reach(1, a.pool, a.v_p, a.page.d, a.v_t, hk, a.v_h, a.d)) ||
+      ranges_overlap(a.out, out, a.ks, reach(1, a.pool, a.ks_p, blocks, a.ks_b, hk, a.ks_h, 1)) ||
+      ranges_overlap(a.out, out, a.vs, reach(1, a.pool, a.vs_p, blocks, a.vs_b, hk, a.vs_h, 1)))
+    return BP_E_INVALID_ARG;
+  const bool e4m3 = kind == BP_DT_E4M3;
+  if (dtype == BP_DT_BF16)
+    return e4m3 ? launch8_dim<Bf16, cache8::kE4m3>(a, n, st) : launch8_dim<Bf16, cache8::kInt8>(a, n, st);
+  return e4m3 ? launch8_dim<F16, cache8::kE4m3>(a, n, st) : launch8_dim<F16, cache8::kInt8>(a, n, st);
+}
+
+}  // namespace
+}  // namespace attn
+}  // namespace bp
+
+extern "C" int bp_attn_paged8(int dtype, int cache_dtype, const void* q, const void* k_pages, const void* v_pages,
+                              const uint8_t* k_scales, const uint8_t* v_scales, void* out, const int32_t* table,
+                              int64_t table_stride, const int32_t* lengths, const int32_t* cu, int tokens, int seqs, int pool,
+                              int page, int block, int max_pages, int hq, int hk, int head_dim, int64_t q_t, int64_t q_h,
+                              int64_t k_p, int64_t k_t, int64_t k_h, int64_t v_p, int64_t v_t, int64_t v_h, int64_t ks_p,
+                              int64_t ks_b, int64_t ks_h, int64_t vs_p, int64_t vs_b, int64_t vs_h, float scale, void* workspace,
+                              size_t workspace_bytes, void* stream) {
+  if (page <= 0 || pool < 0 || max_pages < 0 || static_cast<int64_t>(page) * max_pages >= (1ll << 29)) return BP_E_INVALID_ARG;
+  if (block <= 0 || block % 4 != 0 || page % block != 0) return BP_E_INVALID_ARG;
+  if (tokens > 0 && seqs > 0 &&
+      (lengths == nullptr || (max_pages > 0 && (table == nullptr || k_pages == nullptr || v_pages == nullptr ||
+                                                k_scales == nullptr || v_scales == nullptr || pool == 0))))
+    return BP_E_INVALID_ARG;
+  bp::attn::Args8 a = {};
+  a.q = q, a.k = k_pages, a.v = v_pages, a.out = out, a.cu = cu, a.lengths = lengths, a.table = table;
+  a.ks = k_scales, a.vs = v_scales;
+  a.ws = static_cast<float*>(workspace);
+  a.q_t = q_t, a.q_h = q_h, a.k_p = k_p, a.k_t = k_t, a.k_h = k_h, a.v_p = v_p, a.v_t = v_t, a.v_h = v_h;
+  a.ks_p = ks_p, a.ks_b = ks_b, a.ks_h = ks_h, a.vs_p = vs_p, a.vs_b = vs_b, a.vs_h = vs_h;
+  a.table_stride = table_stride;
+  a.tokens = tokens, a.seqs = seqs, a.hq = hq, a.hk.d = hk, a.d = head_dim, a.causal = 1;
+  a.pool = pool, a.page = bp::attn::Div::of(page), a.block = bp::attn::Div::of(block);
+  a.max_keys = page * max_pages;
+  a.scale_log2 = scale * 1.44269504088896340736f;
+  return bp::attn::run8(dtype, cache_dtype, a, workspace_bytes, static_cast<hipStream_t>(stream));
+}

@@ -1,0 +1,422 @@
+// The append to a paged cache held in 8 bits, and the way back: positions of a cache of either kind as values.
+
+#include "cache8.h"
+
+#include <type_traits>
+
+#include "attention_plan.h"
+
+namespace bp {
+namespace cache8 {
+namespace {
+
+constexpr int kThreads = 256;
+
+// Types of the values.
+struct Bf16 {
+  typedef uint16_t Bits;
+  static constexpr uint32_t kAbs = 0x7fff, kInf = 0x7f80;
+  static __device__ __forceinline__ float value(uint32_t b) { return bf16_bits_to_float(b); }
+  static __device__ __forceinline__ uint32_t bits(float f) { return float_to_bf16_bits(f); }
+};
+struct F16 {
+  typedef uint16_t Bits;
+  static constexpr uint32_t kAbs = 0x7fff, kInf = 0x7c00;
+  static __device__ __forceinline__ float value(uint32_t b) {
+    return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(b)));
+  }
+  static __device__ __forceinline__ uint32_t bits(float f) { return __builtin_bit_cast(uint16_t, static_cast<_Float16>(f)); }
+};
+struct F32 {
+  typedef uint32_t Bits;
+  static constexpr uint32_t kAbs = 0x7fffffff, kInf = 0x7f800000;
+  static __device__ __forceinline__ float value(uint32_t b) { return __uint_as_float(b); }
+  static __device__ __forceinline__ uint32_t bits(float f) { return __float_as_uint(f); }
+};
+
+// The exponent byte of the least power of two s with amax <= Q s, Q = 1.75 2^8 (e4m3) or 1.984375 2^6 (int8): amax's own exponent
+// less Q's, one more where its significand is the greater (the addition then carries into the exponent).
+template <int KIND>
+__device__ __forceinline__ uint32_t scale_byte(float amax) {
+  const uint32_t b = __float_as_uint(amax);
+  const int e = KIND == kE4m3 ? static_cast<int>((b + 0x1fffffu) >> 23) - 8 : static_cast<int>((b + 0x01ffffu) >> 23) - 6;
+  return max(e, 0);
+}
+
+// x / s to the nearest code, ties to even; infinities to the greatest, NaN to NaN (e4m3) or 0 (int8). Two of them.
+template <int KIND>
+__device__ __forceinline__ uint32_t encode2(float x, float y) {
+  if constexpr (KIND == kE4m3) {
+    x = fabsf(x) > 448.f ? copysignf(448.f, x) : x;
+    y = fabsf(y) > 448.f ? copysignf(448.f, y) : y;
+    return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(x, y, 0, false)) & 0xffffu;
+  } else {
+    const auto one = [](float v) {
+      v = fabsf(v) > 127.f ? copysignf(127.f, v) : v;
+      return static_cast<uint32_t>(static_cast<int>(rintf(v != v ? 0.f : v))) & 0xffu;
+    };
+    return one(x) | one(y) << 8;
+  }
+}
+
+template <int KIND>
+__device__ __forceinline__ float decode(uint32_t code) {
+  if constexpr (KIND == kE4m3) return __builtin_amdgcn_cvt_f32_fp8(static_cast<int>(code), 0);
+  else return static_cast<float>(static_cast<int8_t>(code));
+}
+
+struct Append {
+  const void* in[2];  // keys, values [tokens, hk, d]
+  uint8_t* pages[2];
+  uint8_t* scales[2];
+  const int* cu;
+  const int* lengths;
+  const int* table;
+  int64_t in_t[2], in_h[2], p_p[2], p_t[2], p_h[2], s_p[2], s_b[2], s_h[2], table_stride;  // elements
+  attn::Div page, block, heads, row;  // row: pieces of a row
+  int tokens, seqs, pool, max_keys, hk, d, units;
+};
+
+// Units of a launch are numbered ahead of what the offsets hold: sequence b's begin at cu[b] / block + 2 b, which leaves every
+// sequence as many as its tokens can touch (tokens / block, rounded down, and 2).
+__device__ __forceinline__ int first_unit(const Append& a, int b) { return a.block(min(max(a.cu[b], 0), a.tokens)) + 2 * b; }
+
+// The last sequence whose units begin at or before u: a wave asks 64 sequences at a time.
+__device__ __forceinline__ int sequence_of(const Append& a, int u, int lane) {
+  int lo = 0, n = a.seqs;
+  while (true) {
+    const int step = (n + kWave - 1) / kWave, at = lane * step;
+    const uint64_t below = __ballot(at < n && first_unit(a, lo + min(at, n - 1)) <= u);
+    const int l = below ? 63 - __builtin_clzll(below) : 0;
+    lo += l * step;
+    n = min(step, n - l * step);
+    if (step == 1) return lo;
+  }
+}
+
+// A unit: the new tokens of one sequence in one block of one head, of keys or of values. G threads (a wave, or the workgroup where
+// a block has more pieces than a wave holds) take the greatest magnitude, then write the codes; what of the tokens they can hold
+// (8 pieces of V elements a thread) is read once. Where the block holds tokens from before the chunk and the scale grows, their
+// codes are rounded to it.
+template <class T, int KIND, int V, int G>
+__global__ __launch_bounds__(kThreads) void append8_kernel(Append a) {
+  constexpr int HELD = 8, BYTES = V * static_cast<int>(sizeof(typename T::Bits)), WORDS = BYTES > 4 ? BYTES / 4 : 1;
+  __shared__ float red[kThreads / kWave];
+  const int lane = static_cast<int>(threadIdx.x) & 63, tid = static_cast<int>(threadIdx.x) % G;
+  const int index = blockIdx.x * (kThreads / G) + __builtin_amdgcn_readfirstlane(threadIdx.x / G);
+  const int kv = index & 1, hu = index >> 1, u = a.heads(hu), h = hu - u * a.hk;
+  if (u >= a.units) return;
+  const int b = sequence_of(a, u, lane);
+  const int begin = min(max(a.cu[b], 0), a.tokens), end = min(max(a.cu[b + 1], begin), a.tokens);
+  const int length = max(a.lengths[b], 0), start = length - (end - begin);
+  if (u < first_unit(a, b) || end == begin || start >= a.max_keys) return;
+  // the block's first position, and the rows of it that are new
+  const int64_t at0 = (a.block(max(start, 0)) + static_cast<int64_t>(u - first_unit(a, b))) * a.block.d;
+  if (at0 >= min(length, a.max_keys)) return;
+  const int at = static_cast<int>(at0);
+  const int lo = max(start - at, 0), hi = min(length - at, a.block.d);
+  const int n = a.page(at), slot = at - n * a.page.d;
+  const int id = a.table[b * a.table_stride + n];
+  if (lo >= hi || static_cast<unsigned>(id) >= static_cast<unsigned>(a.pool)) return;
+  const typename T::Bits* in = static_cast<const typename T::Bits*>(a.in[kv]) + (end - length + at) * a.in_t[kv] + h * a.in_h[kv];
+  uint8_t* out = a.pages[kv] + id * a.p_p[kv] + slot * a.p_t[kv] + h * a.p_h[kv];
+  uint8_t* scale = a.scales[kv] + id * a.s_p[kv] + a.block(slot) * a.s_b[kv] + h * a.s_h[kv];
+  const bool held = start > at;  // tokens from before the chunk
+  const uint32_t had = held ? *scale : 0;
+
+  uint32_t x[HELD][WORDS];
+  const int pieces = (hi - lo) * a.row.d;
+  const auto load = [&](int i, uint32_t (&w)[WORDS]) {
+    const int r = a.row(i), c = i - r * a.row.d;
+    const typename T::Bits* p = in + (lo + r) * a.in_t[kv] + c * V;
+    if constexpr (V == 1) w[0] = *p;
+    else {
+#pragma unroll
+      for (int j = 0; j < WORDS / 4; ++j) {
+        const u32x4 q = reinterpret_cast<const u32x4*>(p)[j];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[4 * j + e] = q[e];
+      }
+    }
+  };
+  const auto element = [](const uint32_t (&w)[WORDS], int e) -> uint32_t {
+    if constexpr (sizeof(typename T::Bits) == 4) return w[e];
+    else return V == 1 ? w[0] : (w[e / 2] >> (16 * (e % 2))) & 0xffffu;
+  };
+  uint32_t top = 0;
+  const auto widen = [&](const uint32_t (&w)[WORDS]) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const uint32_t m = element(w, e) & T::kAbs;
+      top = max(top, m < T::kInf ? m : 0u);
+    }
+  };
+#pragma unroll
+  for (int j = 0; j < HELD; ++j)
+    if (tid + j * G < pieces) load(tid + j * G, x[j]);
+#pragma unroll
+  for (int j = 0; j < HELD; ++j)
+    if (tid + j * G < pieces) widen(x[j]);
+  for (int i = tid + HELD * G; i < pieces; i += G) {
+    uint32_t w[WORDS];
+    load(i, w);
+    widen(w);
+  }
+  float amax = xor_butterfly<true>(T::value(top), MaxOp());
+  if constexpr (G > kWave) {
+    if (lane == 0) red[threadIdx.x / kWave] = amax;
+    __syncthreads();
+    amax = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  }
+  const uint32_t byte = max(had, scale_byte<KIND>(amax));
+  const int inv_byte = 254 - static_cast<int>(byte);
+  const float inv = inv_byte < 0 ? 0.f : scale_value(inv_byte);
+  const auto store = [&](int i, const uint32_t (&w)[WORDS]) {
+    const int r = a.row(i), c = i - r * a.row.d;
+    uint8_t* p = out + (lo + r) * a.p_t[kv] + c * V;
+    if constexpr (V == 1) {
+      *p = static_cast<uint8_t>(encode2<KIND>(T::value(w[0]) * inv, 0.f));
+    } else {
+      u32x2 y;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        uint32_t half[2];
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+          half[g] = encode2<KIND>(T::value(element(w, 4 * e + 2 * g)) * inv, T::value(element(w, 4 * e + 2 * g + 1)) * inv);
+        y[e] = half[0] | half[1] << 16;
+      }
+      *reinterpret_cast<u32x2*>(p) = y;
+    }
+  };
+#pragma unroll
+  for (int j = 0; j < HELD; ++j)
+    if (tid + j * G < pieces) store(tid + j * G, x[j]);
+  for (int i = tid + HELD * G; i < pieces; i += G) {
+    uint32_t w[WORDS];
+    load(i, w);
+    store(i, w);
+  }
+  if (held && byte > had) {
+    const int less = static_cast<int>(byte - had);  // a code times 2^-less; from 126 on nothing is left of it
+    const float f = less < 126 ? scale_value(127 - less) : 0.f;
+    for (int i = tid; i < lo * a.row.d; i += G) {
+      const int r = a.row(i), c = i - r * a.row.d;
+      uint8_t* p = out + r * a.p_t[kv] + c * V;
+      if constexpr (V == 1) {
+        *p = static_cast<uint8_t>(encode2<KIND>(decode<KIND>(*p) * f, 0.f));
+      } else {
+        u32x2 y = *reinterpret_cast<const u32x2*>(p);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          uint32_t w = 0;
+#pragma unroll
+          for (int g = 0; g < 2; ++g)
+            w |= encode2<KIND>(decode<KIND>(y[e] >> (16 * g) & 0xff) * f, decode<KIND>(y[e] >> (16 * g + 8) & 0xff) * f) << (16 * g);
+          y[e] = w;
+        }
+        *reinterpret_cast<u32x2*>(p) = y;
+      }
+    }
+  }
+  if (tid == 0) *scale = static_cast<uint8_t>(byte);
+}
+
+struct Read {
+  const uint8_t* pages[2];
+  const uint8_t* scales[2];  // null: the cache holds values
+  void* out[2];              // [tokens, hk, d], contiguous
+  const int* cu;
+  const int* lengths;
+  const int* table;
+  int64_t p_p[2], p_t[2], p_h[2], s_p[2], s_b[2], s_h[2], table_stride;  // p: bytes
+  attn::Div page, block, row, token;  // pieces of a row, of a token
+  int tokens, seqs, pool, max_keys;
+};
+
+// A piece of 8 columns of a token's head, of keys and of values: codes times their scale in T (KIND e4m3, int8), or the cache's own
+// 16 bits. Positions that the table does not have are zeros, a page outside the pool gives NaN.
+template <class T, int KIND>
+__global__ __launch_bounds__(kThreads) void read_kernel(Read a) {
+  constexpr int kCopy = 2;
+  if constexpr (std::is_same<T, F16>::value) saturate_f16();
+  const int total = a.tokens * a.token.d;
+  for (int i = blockIdx.x * kThreads + threadIdx.x; i < total; i += gridDim.x * kThreads) {
+    const int tok = a.token(i), rest = i - tok * a.token.d, h = a.row(rest), c = rest - h * a.row.d;
+    int lo = 0, hi = a.seqs;  // the last sequence that begins at or before tok
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (a.cu[mid] <= tok) lo = mid;
+      else hi = mid;
+    }
+    bool seen = a.seqs > 0, bad = false;
+    int id = 0, slot = 0;
+    if (seen) {
+      const int end = a.cu[lo + 1], pos = max(a.lengths[lo], 0) - (min(end, a.tokens) - tok);
+      seen = tok >= a.cu[lo] && tok < end && static_cast<unsigned>(pos) < static_cast<unsigned>(a.max_keys);
+      if (seen) {
+        const int n = a.page(pos);
+        slot = pos - n * a.page.d;
+        id = a.table[lo * a.table_stride + n];
+        bad = static_cast<unsigned>(id) >= static_cast<unsigned>(a.pool);
+      }
+    }
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) {
+      typename T::Bits* out = static_cast<typename T::Bits*>(a.out[kv]) + static_cast<int64_t>(i) * 8;
+      if (!seen || bad) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) out[e] = seen ? T::bits(NAN) : 0;
+        continue;
+      }
+      const uint8_t* p = a.pages[kv] + id * a.p_p[kv] + slot * a.p_t[kv] + h * a.p_h[kv];
+      if constexpr (KIND == kCopy) {
+        *reinterpret_cast<u32x4*>(out) = reinterpret_cast<const u32x4*>(p)[c];
+      } else {
+        const uint32_t byte = a.scales[kv][id * a.s_p[kv] + a.block(slot) * a.s_b[kv] + h * a.s_h[kv]];
+        const u32x2 w = reinterpret_cast<const u32x2*>(p)[c];
+        if constexpr (std::is_same<T, F32>::value) {
+          const float s = scale_value(byte);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) out[e] = T::bits(decode<KIND>(w[e / 4] >> (8 * (e % 4)) & 0xff) * s);
+        } else {
+          using C = Codes<KIND, std::is_same<T, Bf16>::value>;
+          *reinterpret_cast<u32x4*>(out) = eight<C>(w[0], w[1], C::scale(byte));
+        }
+      }
+    }
+  }
+}
+
+bool aligned(const void* p, int n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+template <class T, int KIND, int V>
+void append_launch(const Append& a, hipStream_t st) {
+  const int64_t pieces = static_cast<int64_t>(a.block.d) * a.row.d, waves = 2ll * a.units * a.hk;
+  // a wave holds 512 pieces; past those a workgroup takes the unit
+  if (pieces <= 8 * kWave)
+    append8_kernel<T, KIND, V, kWave><<<static_cast<unsigned>((waves + 3) / 4), kThreads, 0, st>>>(a);
+  else append8_kernel<T, KIND, V, kThreads><<<static_cast<unsigned>(waves), kThreads, 0, st>>>(a);
+}
+
+template <class T, int KIND>
+void append_vector(const Append& a, bool wide, hipStream_t st) {
+  if (wide) append_launch<T, KIND, 8>(a, st);
+  else append_launch<T, KIND, 1>(a, st);
+}
+
+template <class T>
+void append_kind(const Append& a, int kind, bool wide, hipStream_t st) {
+  if (kind == BP_DT_E4M3) append_vector<T, kE4m3>(a, wide, st);
+  else append_vector<T, kInt8>(a, wide, st);
+}
+
+template <class T>
+void read_kind(const Read& a, int kind, unsigned grid, hipStream_t st) {
+  if (kind == BP_DT_E4M3) read_kernel<T, kE4m3><<<grid, kThreads, 0, st>>>(a);
+  else if (kind == BP_DT_I8) read_kernel<T, kInt8><<<grid, kThreads, 0, st>>>(a);
+  else read_kernel<T, 2><<<grid, kThreads, 0, st>>>(a);
+}
+
+bool cache_sizes(int tokens, int seqs, int pool, int page, int max_pages, int hk, int head_dim) {
+  return tokens >= 0 && seqs >= 0 && pool >= 0 && page > 0 && max_pages >= 0 &&
+         static_cast<int64_t>(page) * max_pages < (1ll << 29) && hk >= 0 && head_dim >= 0;
+}
+
+}  // namespace
+}  // namespace cache8
+}  // namespace bp
+
+extern "C" {
+
+int bp_paged_append8(int dtype, int cache_dtype, const void* k, const void* v, void* k_pages, void* v_pages, uint8_t* k_scales,
+                     uint8_t* v_scales, const int32_t* table, int64_t table_stride, const int32_t* lengths, const int32_t* cu,
+                     int tokens, int seqs, int pool, int page, int block, int max_pages, int hk, int head_dim, int64_t k_t,
+                     int64_t k_h, int64_t v_t, int64_t v_h, int64_t kp_p, int64_t kp_t, int64_t kp_h, int64_t vp_p, int64_t vp_t,
+                     int64_t vp_h, int64_t ks_p, int64_t ks_b, int64_t ks_h, int64_t vs_p, int64_t vs_b, int64_t vs_h,
+                     void* stream) {
+  using namespace bp::cache8;
+  if ((dtype != BP_DT_BF16 && dtype != BP_DT_F16 && dtype != BP_DT_F32) || (cache_dtype != BP_DT_E4M3 && cache_dtype != BP_DT_I8))
+    return BP_E_UNSUPPORTED;
+  if (!cache_sizes(tokens, seqs, pool, page, max_pages, hk, head_dim) || block <= 0 || page % block != 0) return BP_E_INVALID_ARG;
+  if (tokens == 0 || seqs == 0 || pool == 0 || max_pages == 0 || hk == 0 || head_dim == 0) return BP_OK;
+  if (k == nullptr || v == nullptr || k_pages == nullptr || v_pages == nullptr || k_scales == nullptr || v_scales == nullptr ||
+      table == nullptr || lengths == nullptr || cu == nullptr)
+    return BP_E_INVALID_ARG;
+  Append a = {};
+  a.in[0] = k, a.in[1] = v;
+  a.pages[0] = static_cast<uint8_t*>(k_pages), a.pages[1] = static_cast<uint8_t*>(v_pages);
+  a.scales[0] = k_scales, a.scales[1] = v_scales;
+  a.cu = cu, a.lengths = lengths, a.table = table, a.table_stride = table_stride;
+  a.in_t[0] = k_t, a.in_t[1] = v_t, a.in_h[0] = k_h, a.in_h[1] = v_h;
+  a.p_p[0] = kp_p, a.p_p[1] = vp_p, a.p_t[0] = kp_t, a.p_t[1] = vp_t, a.p_h[0] = kp_h, a.p_h[1] = vp_h;
+  a.s_p[0] = ks_p, a.s_p[1] = vs_p, a.s_b[0] = ks_b, a.s_b[1] = vs_b, a.s_h[0] = ks_h, a.s_h[1] = vs_h;
+  a.page = bp::attn::Div::of(page), a.block = bp::attn::Div::of(block), a.heads = bp::attn::Div::of(hk);
+  a.tokens = tokens, a.seqs = seqs, a.pool = pool, a.max_keys = page * max_pages, a.hk = hk, a.d = head_dim;
+  const int size = dtype == BP_DT_F32 ? 4 : 2;
+  const bool wide = head_dim % 8 == 0 && aligned(k, 16) && aligned(v, 16) && aligned(k_pages, 8) && aligned(v_pages, 8) &&
+                    ((k_t | k_h | v_t | v_h) * size & 15) == 0 && ((kp_p | kp_t | kp_h | vp_p | vp_t | vp_h) & 7) == 0;
+  a.row = bp::attn::Div::of(wide ? head_dim / 8 : head_dim);
+  const int64_t units = tokens / block + 2ll * seqs;
+  // a unit's pieces, the units with their heads, and positions in 32 bits
+  if (static_cast<int64_t>(block) * head_dim >= (1ll << 30) || 2 * units * hk >= (1ll << 30) || tokens >= (1 << 30))
+    return BP_E_UNSUPPORTED;
+  a.units = static_cast<int>(units);
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  if (dtype == BP_DT_BF16) append_kind<Bf16>(a, cache_dtype, wide, st);
+  else if (dtype == BP_DT_F16) append_kind<F16>(a, cache_dtype, wide, st);
+  else append_kind<F32>(a, cache_dtype, wide, st);
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? BP_OK : static_cast<int>(e);
+}
+
+int bp_paged_read(int dtype, int cache_dtype, const void* k_pages, const void* v_pages, const uint8_t* k_scales,
+                  const uint8_t* v_scales, void* k, void* v, const int32_t* table, int64_t table_stride, const int32_t* lengths,
+                  const int32_t* cu, int tokens, int seqs, int pool, int page, int block, int max_pages, int hk, int head_dim,
+                  int64_t kp_p, int64_t kp_t, int64_t kp_h, int64_t vp_p, int64_t vp_t, int64_t vp_h, int64_t ks_p, int64_t ks_b,
+                  int64_t ks_h, int64_t vs_p, int64_t vs_b, int64_t vs_h, void* stream) {
+  using namespace bp::cache8;
+  const bool codes = cache_dtype == BP_DT_E4M3 || cache_dtype == BP_DT_I8;
+  if (dtype != BP_DT_BF16 && dtype != BP_DT_F16 && dtype != BP_DT_F32) return BP_E_UNSUPPORTED;
+  if (!codes && (cache_dtype != dtype || dtype == BP_DT_F32)) return BP_E_UNSUPPORTED;
+  if (!cache_sizes(tokens, seqs, pool, page, max_pages, hk, head_dim) || (codes && (block <= 0 || page % block != 0)))
+    return BP_E_INVALID_ARG;
+  if (head_dim % 8 != 0) return BP_E_UNSUPPORTED;
+  if (tokens == 0 || hk == 0 || head_dim == 0) return BP_OK;
+  const bool empty = seqs == 0 || pool == 0 || max_pages == 0;
+  if (k == nullptr || v == nullptr || (seqs > 0 && (lengths == nullptr || cu == nullptr)) ||
+      (!empty && (k_pages == nullptr || v_pages == nullptr || table == nullptr ||
+                  (codes && (k_scales == nullptr || v_scales == nullptr)))))
+    return BP_E_INVALID_ARG;
+  const int size = codes ? 1 : 2, unit = 8 * size;
+  // a stride that nothing is multiplied with may be anything
+  if (pool == 1) kp_p = vp_p = 0;
+  if (page == 1) kp_t = vp_t = 0;
+  if (hk == 1) kp_h = vp_h = 0;
+  if (!aligned(k, 16) || !aligned(v, 16) || !aligned(k_pages, unit) || !aligned(v_pages, unit) ||
+      ((kp_p | kp_t | kp_h | vp_p | vp_t | vp_h) & 7) != 0)
+    return BP_E_INVALID_ARG;
+  if (static_cast<int64_t>(tokens) * hk * (head_dim / 8) >= (1ll << 30)) return BP_E_UNSUPPORTED;
+  Read a = {};
+  a.pages[0] = static_cast<const uint8_t*>(k_pages), a.pages[1] = static_cast<const uint8_t*>(v_pages);
+  a.scales[0] = k_scales, a.scales[1] = v_scales;
+  a.out[0] = k, a.out[1] = v;
+  a.cu = cu, a.lengths = lengths, a.table = table, a.table_stride = table_stride;
+  a.p_p[0] = kp_p * size, a.p_p[1] = vp_p * size, a.p_t[0] = kp_t * size, a.p_t[1] = vp_t * size;
+  a.p_h[0] = kp_h * size, a.p_h[1] = vp_h * size;
+  a.s_p[0] = ks_p, a.s_p[1] = vs_p, a.s_b[0] = ks_b, a.s_b[1] = vs_b, a.s_h[0] = ks_h, a.s_h[1] = vs_h;
+  a.page = bp::attn::Div::of(page), a.block = bp::attn::Div::of(codes ? block : page);
+  a.row = bp::attn::Div::of(head_dim / 8), a.token = bp::attn::Div::of(hk * (head_dim / 8));
+  a.tokens = tokens, a.seqs = seqs, a.pool = pool, a.max_keys = page * max_pages;
+  const int64_t total = static_cast<int64_t>(tokens) * a.token.d, blocks = (total + kThreads - 1) / kThreads;
+  const unsigned grid = static_cast<unsigned>(blocks < 16384 ? blocks : 16384);
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  if (dtype == BP_DT_BF16) read_kind<Bf16>(a, cache_dtype, grid, st);
+  else if (dtype == BP_DT_F16) read_kind<F16>(a, cache_dtype, grid, st);
+  else if (cache_dtype == BP_DT_E4M3) read_kernel<F32, kE4m3><<<grid, kThreads, 0, st>>>(a);
+  else read_kernel<F32, kInt8><<<grid, kThreads, 0, st>>>(a);
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? BP_OK : static_cast<int>(e);
+}
+
+}  // extern "C"

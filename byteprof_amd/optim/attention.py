@@ -1,10 +1,17 @@
 """Attention of several sequences on gfx950 (through libbyteprof_amd.so): packed prompts, and chunks of new tokens over a
-cache in pages, with the append that writes it.
+cache in pages, with the append that writes it and the way back.
 
   packed_attention  whole sequences one after another in [tokens, heads, head_dim]
   paged_append      a chunk's keys and values into the pages
   paged_attention   a chunk of each sequence (one token in a decode step, drafts in a verify round, a part of a prompt) over
                     everything its sequence has in the cache
+  paged_read        the last positions of each sequence out of the pages, packed
+
+The cache holds 16-bit values, or (with k_scales and v_scales) 8 bits: pages of float8_e4m3fn or int8 codes, and for each block of
+a page's positions and each head a power of two, float8_e8m0fnu [pages, blocks of a page, Hk]; a value is code x scale. The append
+takes the least power of two that all new values of a block fit under (448 times it for e4m3, 127 times it for int8); where a
+block holds earlier positions it never lowers their scale, and rounds their codes again when it grows. int8 holds normally
+distributed keys and values about three times as exactly as e4m3 does; e4m3 holds small values beside large ones.
 
 Offsets, lengths and page tables are int32 tensors on the GPU that the kernels read: the calls neither copy nor synchronise,
 and one captured graph serves whatever the tensors hold when it is replayed. bf16 or fp16, softmax and sums in fp32; any
@@ -30,6 +37,8 @@ UNDIVIDED_KEYS = 256  # a sequence's keys up to here are never divided: no works
 
 
 _FLOATS = {torch.bfloat16: _lib.DT_BF16, torch.float16: _lib.DT_F16}
+_VALUES = {**_FLOATS, torch.float32: _lib.DT_F32}
+_CODES = {torch.float8_e4m3fn: _lib.DT_E4M3, torch.int8: _lib.DT_I8}
 
 
 def _same_device(what: str, x: torch.Tensor, *tensors: torch.Tensor | None) -> int:
@@ -182,15 +191,42 @@ def _pages(what: str, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch
     return shape, kst, vst, seqs, most, row
 
 
+def _codes(what: str, k_pages: torch.Tensor, v_pages: torch.Tensor, k_scales: torch.Tensor | None,
+           v_scales: torch.Tensor | None) -> tuple:
+    """Of an 8-bit cache: the code of its dtype, the block's positions, and the scales' strides."""
+    code = _CODES.get(k_pages.dtype)
+    if k_scales is None or v_scales is None or code is None or v_pages.dtype != k_pages.dtype:
+        raise ValueError(f"{what}: a cache in 8 bits has pages of one dtype, float8_e4m3fn or int8, and k_scales and v_scales")
+    pool, page, hk, _ = k_pages.shape
+    shape = k_scales.shape
+    if (k_scales.dtype is not torch.float8_e8m0fnu or v_scales.dtype is not torch.float8_e8m0fnu or len(shape) != 3
+            or v_scales.shape != shape or shape[0] != pool or shape[2] != hk or shape[1] < 1 or page % shape[1]):
+        raise ValueError(f"{what}: the scales must be float8_e8m0fnu [pages, blocks of a page, Hk], keys and values alike")
+    return code, page // shape[1], k_scales.stride(), v_scales.stride()
+
+
+def _aligned(what: str, k_pages: torch.Tensor, v_pages: torch.Tensor, unit: int) -> None:
+    """Refuses caches whose rows do not lie on multiples of 8 elements (of `unit` bytes in all)."""
+    kst, vst = k_pages.stride(), v_pages.stride()
+    if (k_pages.data_ptr() | v_pages.data_ptr()) & (unit - 1) or (
+            kst[0] | kst[1] | kst[2] | vst[0] | vst[1] | vst[2]) & 7 and any(
+            n > 1 and (a | b) & 7 for n, a, b in zip(k_pages.shape[:3], kst, vst)):
+        raise ValueError(f"{what}: the caches must be {unit}-byte aligned, with strides of whole multiples of 8 elements")
+
+
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor,
-                    cu: torch.Tensor, *, scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+                    cu: torch.Tensor, *, k_scales: torch.Tensor | None = None, v_scales: torch.Tensor | None = None,
+                    scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of chunks of new tokens over a cache in pages: q [tokens, Hq, D] with the chunks one after another (cu
     [sequences + 1]), caches [pages, page size, Hk, D], table [sequences, most pages] (position p of sequence b in page
     table[b, p // page size]; entries past its length are not read), lengths [sequences]: a sequence's positions in the
     cache, its chunk's among them (append first). A chunk's tokens are the last positions; each sees all up to its own. Rows
     that no chunk covers come out as zeros. A row that sees a position whose page id is outside the cache is NaN; so may other
-    rows of its chunk be.
+    rows of its chunk be. With k_scales and v_scales the caches are 8-bit codes, in blocks of a multiple of 4 positions; they
+    become values of q's dtype exactly (fp16: those past its range become its greatest, 65504).
     Returns [tokens, Hq, D], in `out` when given: q itself or a tensor apart from q and the caches."""
+    if k_scales is not None or v_scales is not None:
+        return _paged_attention8(q, k_pages, v_pages, table, lengths, cu, k_scales, v_scales, scale, out)
     what = "paged_attention"
     if q.dim() != 3:
         raise ValueError(f"{what}: q must be [tokens, Hq, D]")
@@ -218,13 +254,51 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     return y
 
 
+def _paged_attention8(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor,
+                      cu: torch.Tensor, k_scales: torch.Tensor | None, v_scales: torch.Tensor | None, scale: float | None,
+                      out: torch.Tensor | None) -> torch.Tensor:
+    what = "paged_attention"
+    if q.dim() != 3:
+        raise ValueError(f"{what}: q must be [tokens, Hq, D]")
+    (pool, page, hk, dk), kst, vst, seqs, most, row = _pages(what, k_pages, v_pages, table, lengths, cu)
+    code, block, ksst, vsst = _codes(what, k_pages, v_pages, k_scales, v_scales)
+    if block % 4:
+        raise ValueError(f"{what}: a block must have a multiple of 4 positions, not {block}")
+    tokens, hq, d = q.shape
+    dtype = _FLOATS.get(q.dtype)
+    if dtype is None:
+        raise ValueError(f"{what}: q must be bfloat16 or float16")
+    _heads(what, hq, hk, d, dk)
+    _aligned(what, k_pages, v_pages, 8)
+    index = _same_device(what, q, k_pages, v_pages, k_scales, v_scales, table, lengths, cu, out)
+    if q.requires_grad or k_pages.requires_grad or v_pages.requires_grad or forward_ad._current_level >= 0:
+        _no_derivative(what, q, k_pages, v_pages)
+    scale = _scale(what, scale, d)
+    q = _rows(q)
+    y = _output(what, q, out, k_pages, v_pages, k_scales, v_scales)
+    if tokens == 0:
+        return y
+    ws, need = _workspace(tokens, seqs, hq, hk, d, page * most, q.device)
+    q_t, q_h, _ = q.stride()
+    _launch(index, "bp_attn_paged8", dtype, code, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), k_scales.data_ptr(),
+            v_scales.data_ptr(), y.data_ptr(), table.data_ptr(), row, lengths.data_ptr(), cu.data_ptr(), tokens, seqs, pool, page,
+            block, most, hq, hk, d, q_t, q_h, kst[0], kst[1], kst[2], vst[0], vst[1], vst[2], *ksst, *vsst, scale, _lib.ptr(ws),
+            need)
+    return y
+
+
 def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor,
-                 lengths: torch.Tensor, cu: torch.Tensor) -> None:
+                 lengths: torch.Tensor, cu: torch.Tensor, *, k_scales: torch.Tensor | None = None,
+                 v_scales: torch.Tensor | None = None) -> None:
     """The chunks' keys and values k, v [tokens, Hk, D] (any strides with the last dimension contiguous) into the caches, at
     the last positions of each sequence: token i of a chunk of c at position lengths[b] - c + i. Tokens of no chunk, positions
     outside the table (also where lengths[b] is past it, which paged_attention takes as the table's end) and pages outside the
-    cache are left out. Any dtype of 1, 2 or 4 bytes; the caches' dtype is k's."""
+    cache are left out. Any dtype of 1, 2 or 4 bytes; the caches' dtype is k's. With k_scales and v_scales (which it writes, too)
+    the caches are 8-bit codes and k and v bf16, fp16 or fp32: the codes are the nearest, ties to even, infinities the greatest,
+    NaN stays NaN in e4m3 and is 0 in int8. A block that a chunk writes to must be no other sequence's of the call."""
     what = "paged_append"
+    if k_scales is not None or v_scales is not None:
+        return _paged_append8(k, v, k_pages, v_pages, table, lengths, cu, k_scales, v_scales)
     if k.dim() != 3 or v.shape != k.shape:
         raise ValueError(f"{what}: k and v must be [tokens, Hk, D]")
     (pool, page, hk, d), kst, vst, seqs, most, row = _pages(what, k_pages, v_pages, table, lengths, cu)
@@ -247,3 +321,69 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
             table.data_ptr(), row, lengths.data_ptr(), cu.data_ptr(), tokens, seqs, pool, page, most, hk, d, k_t, k_h, v_t, v_h,
             kst[0], kst[1], kst[2], vst[0], vst[1], vst[2])
     increment_version((k_pages, v_pages))
+
+
+def _paged_append8(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor,
+                   lengths: torch.Tensor, cu: torch.Tensor, k_scales: torch.Tensor | None, v_scales: torch.Tensor | None) -> None:
+    what = "paged_append"
+    if k.dim() != 3 or v.shape != k.shape:
+        raise ValueError(f"{what}: k and v must be [tokens, Hk, D]")
+    (pool, page, hk, d), kst, vst, seqs, most, row = _pages(what, k_pages, v_pages, table, lengths, cu)
+    code, block, ksst, vsst = _codes(what, k_pages, v_pages, k_scales, v_scales)
+    tokens, heads, dim = k.shape
+    if heads != hk or dim != d:
+        raise ValueError(f"{what}: the caches hold {hk} heads of {d}, k and v {heads} of {dim}")
+    dtype = _VALUES.get(k.dtype)
+    if dtype is None or v.dtype != k.dtype:
+        raise ValueError(f"{what}: k and v must share one dtype, bfloat16, float16 or float32")
+    k_t, k_h, k_d = k.stride()
+    v_t, v_h, v_d = v.stride()
+    if (k_d != 1 or v_d != 1) and k.numel():
+        raise ValueError(f"{what}: k and v must be contiguous in the head dimension")
+    index = _same_device(what, k, v, k_pages, v_pages, k_scales, v_scales, table, lengths, cu)
+    if k.requires_grad or v.requires_grad or k_pages.requires_grad or v_pages.requires_grad or forward_ad._current_level >= 0:
+        _no_derivative(what, k, v, k_pages, v_pages)
+    if tokens == 0 or hk == 0 or d == 0:
+        return
+    _launch(index, "bp_paged_append8", dtype, code, k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
+            k_scales.data_ptr(), v_scales.data_ptr(), table.data_ptr(), row, lengths.data_ptr(), cu.data_ptr(), tokens, seqs, pool,
+            page, block, most, hk, d, k_t, k_h, v_t, v_h, kst[0], kst[1], kst[2], vst[0], vst[1], vst[2], *ksst, *vsst)
+    increment_version((k_pages, v_pages, k_scales, v_scales))
+
+
+def paged_read(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, cu: torch.Tensor,
+               tokens: int, *, k_scales: torch.Tensor | None = None, v_scales: torch.Tensor | None = None,
+               dtype: torch.dtype | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """The way back of paged_append: of each sequence b its last cu[b + 1] - cu[b] positions, as (k, v) [tokens, Hk, D], new
+    tensors. A 16-bit cache (bf16 or fp16) gives its values in its own dtype; an 8-bit one (with k_scales and v_scales) code x
+    scale in `dtype`: bf16 (by default; exact), fp16 (past its range 65504) or fp32. Tokens of no sequence and positions outside the table come out as
+    zeros, those of a page outside the cache as NaN."""
+    what = "paged_read"
+    (pool, page, hk, d), kst, vst, seqs, most, row = _pages(what, k_pages, v_pages, table, lengths, cu)
+    ks = vs = None
+    block, ksst, vsst = page, (0, 0, 0), (0, 0, 0)
+    if k_scales is not None or v_scales is not None:
+        code, block, ksst, vsst = _codes(what, k_pages, v_pages, k_scales, v_scales)
+        dtype = torch.bfloat16 if dtype is None else dtype
+        kind = _VALUES.get(dtype)
+        if kind is None:
+            raise ValueError(f"{what}: dtype must be bfloat16, float16 or float32")
+        ks, vs = k_scales.data_ptr(), v_scales.data_ptr()
+    else:
+        dtype = k_pages.dtype if dtype is None else dtype
+        kind = code = _FLOATS.get(dtype)
+        if code is None or k_pages.dtype != dtype or v_pages.dtype != dtype:
+            raise ValueError(f"{what}: a cache without scales is bfloat16 or float16 and is read in its own dtype")
+    if tokens < 0 or d % 8:
+        raise ValueError(f"{what}: tokens must not be negative, and head_dim must be a multiple of 8")
+    _aligned(what, k_pages, v_pages, 8 * k_pages.element_size())
+    index = _same_device(what, k_pages, v_pages, k_scales, v_scales, table, lengths, cu)
+    if k_pages.requires_grad or v_pages.requires_grad or forward_ad._current_level >= 0:
+        _no_derivative(what, k_pages, v_pages)
+    k = torch.empty((tokens, hk, d), dtype=dtype, device=k_pages.device)
+    v = torch.empty((tokens, hk, d), dtype=dtype, device=k_pages.device)
+    if k.numel():
+        _launch(index, "bp_paged_read", kind, code, k_pages.data_ptr(), v_pages.data_ptr(), ks, vs, k.data_ptr(), v.data_ptr(),
+                table.data_ptr(), row, lengths.data_ptr(), cu.data_ptr(), tokens, seqs, pool, page, block, most, hk, d, kst[0],
+                kst[1], kst[2], vst[0], vst[1], vst[2], *ksst, *vsst)
+    return k, v

@@ -36,6 +36,7 @@ extern "C" {
 #define BP_DT_F16 1
 #define BP_DT_F32 2
 #define BP_DT_I8 3
+#define BP_DT_E4M3 4 /* codes of a cache only: 4 exponent and 3 mantissa bits, no infinities, greatest 448 */
 
 /* Library version (major * 10000 + minor * 100 + patch). */
 int bp_version(void);
@@ -455,6 +456,59 @@ int bp_paged_append(int element_bytes, const void* k, const void* v, void* k_pag
                     int64_t table_stride, const int32_t* lengths, const int32_t* cu, int tokens, int seqs, int pool, int page,
                     int max_pages, int hk, int head_dim, int64_t k_t, int64_t k_h, int64_t v_t, int64_t v_h, int64_t kp_p,
                     int64_t kp_t, int64_t kp_h, int64_t vp_p, int64_t vp_t, int64_t vp_h, void* stream);
+
+/*
+ * The same cache held in 8 bits: codes (cache_dtype BP_DT_E4M3 or BP_DT_I8) [pool, page, hk, head_dim] and, for each block of
+ * `block` positions of a page and each head, the exponent of a power of two, [pool, page / block, hk] (uint8, bias 127, 255: NaN):
+ * a value is code x 2^(byte - 127). Strides in elements (bytes); the innermost of the codes is 1. page a multiple of block.
+ *
+ * append8: k, v [tokens, hk, head_dim] (dtype BP_DT_BF16, F16 or F32) to the positions that bp_paged_append gives them. A block's
+ * scale becomes the least power of two s with |x| <= 448 s (E4M3) or 127 s (I8) for all its new values (infinities and NaN aside);
+ * where the block holds positions from before the chunk, no less than it was, and if it grows their codes are rounded to it again.
+ * A code is x / s to the nearest, ties to even; infinities give the greatest code, NaN gives NaN (E4M3) or 0 (I8). The other
+ * positions of a block keep their codes. A block must belong to one sequence of the call only.
+ *
+ * paged8: bp_attn_paged over codes, which become values of q's dtype exactly (BP_DT_F16: those past fp16's range become its
+ * greatest, 65504, those below its least are rounded; E4M3 scales past 2^22 count as 2^22). block a multiple of 4; the codes' bases and the strides of dimensions of more than one entry
+ * multiples of 8. The workspace is bp_attn_workspace_bytes' for page x max_pages keys.
+ *
+ * read: the positions of bp_paged_append out of the cache, into k, v [tokens, hk, head_dim] (dtype, contiguous, 16-byte aligned):
+ * codes x scale (in BP_DT_F16 as for paged8), or (cache_dtype = dtype BP_DT_BF16 or F16; block and scales unused) a 16-bit cache's values. head_dim a multiple
+ * of 8, rows on multiples of 8 elements. Tokens of no sequence and positions outside the table give zeros, pages outside the cache
+ * NaN.
+ * No counterpart in the reference.
+ */
+int bp_paged_append8(int dtype, int cache_dtype, const void* k, const void* v, void* k_pages, void* v_pages, uint8_t* k_scales,
+                     uint8_t* v_scales, const int32_t* table, int64_t table_stride, const int32_t* lengths, const int32_t* cu,
+                     int tokens, int seqs, int pool, int page, int block, int max_pages, int hk, int head_dim, int64_t k_t,
+                     int64_t k_h, int64_t v_t, int64_t v_h, int64_t kp_p, int64_t kp_t, int64_t kp_h, int64_t vp_p, int64_t vp_t,
+                     int64_t vp_h, int64_t ks_p, int64_t ks_b, int64_t ks_h, int64_t vs_p, int64_t vs_b, int64_t vs_h,
+                     void* stream);
+int bp_attn_paged8(int dtype, int cache_dtype, const void* q, const void* k_pages, const void* v_pages, const uint8_t* k_scales,
+                   const uint8_t* v_scales, void* out, const int32_t* table, int64_t table_stride, const int32_t* lengths,
+                   const int32_t* cu, int tokens, int seqs, int pool, int page, int block, int max_pages, int hq, int hk,
+                   int head_dim, int64_t q_t, int64_t q_h, int64_t k_p, int64_t k_t, int64_t k_h, int64_t v_p, int64_t v_t,
+                   int64_t v_h, int64_t ks_p, int64_t ks_b, int64_t ks_h, int64_t vs_p, int64_t vs_b, int64_t vs_h, float scale,
+                   void* workspace, size_t workspace_bytes, void* stream);
+int bp_paged_read(int dtype, int cache_dtype, const void* k_pages, const void* v_pages, const uint8_t* k_scales,
+                  const uint8_t* v_scales, void* k, void* v, const int32_t* table, int64_t table_stride, const int32_t* lengths,
+                  const int32_t* cu, int tokens, int seqs, int pool, int page, int block, int max_pages, int hk, int head_dim,
+                  int64_t kp_p, int64_t kp_t, int64_t kp_h, int64_t vp_p, int64_t vp_t, int64_t vp_h, int64_t ks_p, int64_t ks_b,
+                  int64_t ks_h, int64_t vs_p, int64_t vs_b, int64_t vs_h, void* stream);
+
+/*
+ * Rotary positions: of every head of q [tokens, hq, head_dim] and k [tokens, hk, head_dim] (BP_DT_BF16, F16 or F32; hq or hk may
+ * be 0), the first rot columns as rot / 2 pairs, (i, i + rot / 2) or, interleaved, (2 i, 2 i + 1), become
+ * factor (x1 cos a - x2 sin a, x2 cos a + x1 sin a) with a = positions[token] inv_freq[i]; the other columns are copied. The angle
+ * is reduced in 64 bits, the rest in fp32, the result rounded once. positions [tokens] of position_bytes 4 or 8 (signed), inv_freq
+ * [rot / 2]. head_dim at most 1024. Strides in elements, the innermost 1; an output is its own input (with its strides) or apart
+ * from everything else; slices of one projection are apart. 16 bytes at a time where all rows and halves allow.
+ * No counterpart in the reference (its decode step's rotation is inside bp_decode_qk_rope_cache).
+ */
+int bp_rotary(int dtype, const void* q, const void* k, void* q_out, void* k_out, const void* positions, int position_bytes,
+              const float* inv_freq, int64_t tokens, int hq, int hk, int head_dim, int rot, int interleaved, float factor,
+              int64_t q_t, int64_t q_h, int64_t k_t, int64_t k_h, int64_t qo_t, int64_t qo_h, int64_t ko_t, int64_t ko_h,
+              void* stream);
 
 /*
  * Of every row of logits [rows, vocab] (BP_DT_BF16 / F16 / F32, row_stride elements apart, rows contiguous): logprob [rows] =

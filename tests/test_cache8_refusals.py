@@ -1,0 +1,219 @@
+"""What the operators of the 8-bit cache and rotary refuse, at their Python names and at their C entries, and the frequencies of
+rotary_frequencies. CPU only: every call here returns or raises before anything is enqueued."""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+import pytest
+import torch
+
+from byteprof_amd.optim import attention as A
+from byteprof_amd.optim.rotary import rotary, rotary_frequencies
+
+BF, FP = torch.bfloat16, torch.float16
+E4M3, E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+CU = torch.tensor([0, 4], dtype=torch.int32)
+
+
+def z(*shape, dtype=BF):
+    return torch.zeros(*shape, dtype=dtype)
+
+
+@pytest.fixture(scope="module")
+def L():
+    from byteprof_amd import _lib
+
+    return _lib.lib()
+
+
+def cache(**kw):
+    args = {"k_pages": z(3, 16, 1, 64, dtype=E4M3), "v_pages": z(3, 16, 1, 64, dtype=E4M3),
+            "table": torch.zeros(1, 2, dtype=torch.int32), "lengths": torch.tensor([4], dtype=torch.int32), "cu": CU,
+            "k_scales": z(3, 2, 1, dtype=E8M0), "v_scales": z(3, 2, 1, dtype=E8M0)}
+    args.update(kw)
+    return args
+
+
+BAD_CACHE = [
+    ({"k_scales": None}, "8 bits"),
+    ({"v_scales": None}, "8 bits"),
+    ({"k_pages": z(3, 16, 1, 64), "v_pages": z(3, 16, 1, 64)}, "8 bits"),
+    ({"v_pages": z(3, 16, 1, 64, dtype=torch.int8)}, "8 bits"),
+    ({"k_pages": z(3, 16, 1, 64, dtype=torch.uint8), "v_pages": z(3, 16, 1, 64, dtype=torch.uint8)}, "8 bits"),
+    ({"k_scales": z(3, 2, 1, dtype=torch.float32)}, "scales must be"),
+    ({"k_scales": z(3, 2, 1, dtype=torch.uint8)}, "scales must be"),
+    ({"v_scales": z(3, 4, 1, dtype=E8M0)}, "scales must be"),
+    ({"k_scales": z(3, 3, 1, dtype=E8M0), "v_scales": z(3, 3, 1, dtype=E8M0)}, "scales must be"),
+    ({"k_scales": z(3, 0, 1, dtype=E8M0), "v_scales": z(3, 0, 1, dtype=E8M0)}, "scales must be"),
+    ({"k_scales": z(2, 2, 1, dtype=E8M0), "v_scales": z(2, 2, 1, dtype=E8M0)}, "scales must be"),
+    ({"k_scales": z(3, 2, dtype=E8M0), "v_scales": z(3, 2, dtype=E8M0)}, "scales must be"),
+    ({"table": torch.zeros(1, 2, dtype=torch.int64)}, "int32"),
+    ({"table": torch.zeros(2, 2, dtype=torch.int32)}, "disagree"),
+    ({}, "on a GPU"),
+]
+
+
+@pytest.mark.parametrize("change,match", BAD_CACHE + [
+    ({"q": z(4, 64)}, "q must be"),
+    ({"q": z(4, 2, 64, dtype=torch.float32)}, "bfloat16 or float16"),
+    ({"q": z(4, 2, 128)}, "head_dim"),
+    ({"k_scales": z(3, 8, 1, dtype=E8M0), "v_scales": z(3, 8, 1, dtype=E8M0)}, "multiple of 4"),
+    ({"k_pages": z(3, 16, 1, 72, dtype=E4M3).as_strided((3, 16, 1, 64), (16 * 72, 72, 68, 1), 4)}, "8-byte aligned"),
+    ({"k_pages": z(3, 16, 2, 64, dtype=E4M3).as_strided((3, 16, 1, 64), (2000, 68, 64, 1))}, "8-byte aligned"),
+])
+def test_attention_refusals(change, match):
+    with pytest.raises(ValueError, match=match):
+        A.paged_attention(**{"q": z(4, 2, 64), **cache(**change)})
+
+
+@pytest.mark.parametrize("change,match", BAD_CACHE + [
+    ({"k": z(4, 64)}, "k and v must be"),
+    ({"v": z(5, 1, 64)}, "k and v must be"),
+    ({"k": z(4, 2, 64), "v": z(4, 2, 64)}, "the caches hold"),
+    ({"v": z(4, 1, 64, dtype=FP)}, "share one dtype"),
+    ({"k": z(4, 1, 64, dtype=E4M3), "v": z(4, 1, 64, dtype=E4M3)}, "share one dtype"),
+    ({"k": z(4, 1, 128)[..., ::2]}, "contiguous in the head"),
+])
+def test_append_refusals(change, match):
+    with pytest.raises(ValueError, match=match):
+        A.paged_append(**{"k": z(4, 1, 64), "v": z(4, 1, 64), **cache(**change)})
+
+
+@pytest.mark.parametrize("change,match", BAD_CACHE + [
+    ({"dtype": E4M3}, "dtype must be"),
+    ({"tokens": -1}, "must not be negative"),
+    ({"k_pages": z(3, 16, 1, 60, dtype=E4M3), "v_pages": z(3, 16, 1, 60, dtype=E4M3)}, "multiple of 8"),
+    ({"k_scales": None, "v_scales": None}, "without scales"),
+    ({"k_scales": None, "v_scales": None, "k_pages": z(3, 16, 1, 64), "v_pages": z(3, 16, 1, 64), "dtype": FP}, "own dtype"),
+    ({"k_scales": None, "v_scales": None, "k_pages": z(3, 16, 1, 64), "v_pages": z(3, 16, 1, 64, dtype=FP)}, "own dtype"),
+])
+def test_read_refusals(change, match):
+    with pytest.raises(ValueError, match=match):
+        A.paged_read(**{"tokens": 4, **cache(**change)})
+
+
+POS, INV = torch.arange(4), torch.ones(32)
+
+
+@pytest.mark.parametrize("change,match", [
+    ({"q": z(4, 64)}, "q must be"),
+    ({"k": z(5, 1, 64)}, "q must be"),
+    ({"k": z(4, 1, 72)}, "q must be"),
+    ({"k": z(4, 1, 64, dtype=FP)}, "share one dtype"),
+    ({"q": z(4, 2, 64, dtype=torch.float64), "k": None}, "share one dtype"),
+    ({"q": z(4, 1, 1032), "k": None}, "1024 columns"),
+    ({"positions": POS.float()}, "positions must be"),
+    ({"positions": POS[:3]}, "positions must be"),
+    ({"inv_freq": INV.double()}, "inv_freq must be"),
+    ({"inv_freq": torch.ones(33)}, "inv_freq must be"),
+    ({"inv_freq": INV[None]}, "inv_freq must be"),
+    ({"factor": math.inf}, "factor must be"),
+    ({"factor": math.nan}, "factor must be"),
+    ({"q": z(4, 2, 128)[..., ::2]}, "contiguous in the head"),
+    ({"out": (z(4, 2, 64),)}, "out must be"),
+    ({"out": (z(4, 2, 64), None)}, "out must be"),
+    ({}, "on a GPU"),
+])
+def test_rotary_refusals(change, match):
+    args = {"q": z(4, 2, 64), "k": z(4, 1, 64), "positions": POS, "inv_freq": INV}
+    args.update(change)
+    with pytest.raises(ValueError, match=match):
+        rotary(**args)
+
+
+def test_outputs_of_rotary_that_are_apart():
+    from byteprof_amd.optim.rotary import _disjoint, _writable
+
+    x = torch.zeros(6, 5, 8)
+    assert _disjoint(x[:, :2], x[:, 2:]) and _disjoint(x[:, 2:], x[:, :2]) and _disjoint(x[:3], x[3:])
+    assert not _disjoint(x[:, :3], x[:, 2:]) and not _disjoint(x[:4], x[3:]) and not _disjoint(x, x)
+    assert _disjoint(x[..., :4], x[..., 4:]) is False  # columns of every head: not looked into
+    assert not _disjoint(x[1:, :2], x[:5, 1:3]) and _disjoint(x[1:, :2], x[:5, 2:4])
+    assert _writable(x) and _writable(x.transpose(0, 1)) and _writable(x[:, :2]) and _writable(x[:1])
+    assert not _writable(torch.zeros(6, 1, 8).expand(6, 5, 8)) and not _writable(torch.zeros(1, 5, 8).expand(6, 5, 8))
+    assert not _writable(x.view(-1).as_strided((6, 2, 8), (10, 8, 1)))
+
+
+def test_rotary_frequencies():
+    inv, by = rotary_frequencies(8, 10000.0)
+    assert torch.allclose(inv.double(), torch.tensor([1.0, 0.1, 0.01, 0.001], dtype=torch.float64), rtol=2.0 ** -23) and by == 1.0
+    assert torch.equal(rotary_frequencies(8, scaling="linear", factor=4.0)[0], inv / 4)
+    base, by = rotary_frequencies(8, scaling="base", factor=4.0)
+    assert base[0] == 1.0 and abs(base[-1].item() / (0.001 / 4) - 1) < 1e-6 and by == 1.0
+    # 10000 positions: 1591.5, 159.2, 15.9 and 1.59 turns
+    parts, by = rotary_frequencies(8, scaling="parts", factor=8.0, trained=10000, slow=2.0, fast=100.0)
+    ramp = (10000 * 0.01 / (2 * math.pi) - 2) / 98
+    want = [1.0, 0.1, 0.01 * ramp + 0.01 / 8 * (1 - ramp), 0.001 / 8]
+    assert torch.allclose(parts.double(), torch.tensor(want, dtype=torch.float64), rtol=2.0 ** -22)
+    assert by == 0.1 * math.log(8.0) + 1.0
+    assert torch.equal(rotary_frequencies(64, scaling="parts", factor=1.0, trained=100)[0], rotary_frequencies(64)[0])
+    for bad in ({"dim": 7}, {"dim": 0}, {"dim": 8, "theta": 0.0}, {"dim": 8, "factor": 0.5}, {"dim": 8, "scaling": "other"},
+                {"dim": 8, "scaling": "parts", "factor": 2.0}, {"dim": 2, "scaling": "base", "factor": 2.0},
+                {"dim": 8, "scaling": "parts", "factor": 2.0, "trained": 100, "slow": 3.0, "fast": 3.0}):
+        with pytest.raises(ValueError, match="rotary_frequencies"):
+            rotary_frequencies(**bad)
+
+
+def test_attention_entry_refuses_before_any_launch(L):
+    p, odd = ctypes.c_void_p(64), ctypes.c_void_p(68)  # never dereferenced
+
+    def attn(dtype=0, kind=4, q=p, k=p, ks=p, out=ctypes.c_void_p(1 << 20), table=p, lengths=p, cu=p, tokens=4, seqs=1, pool=4, page=16, block=16,
+             pages=4, hq=2, hk=1, d=64, k_t=64, scale=0.1, ws=None, n=0):
+        return L.bp_attn_paged8(dtype, kind, q, k, p, ks, p, out, table, 4, lengths, cu, tokens, seqs, pool, page, block, pages, hq,
+                                hk, d, 128, 64, 1024, k_t, 64, 1024, 64, 64, 1, 1, 1, 1, 1, 1, scale, ws, n, None)
+
+    assert attn(tokens=0) == 0
+    assert attn(dtype=2) == -2 and attn(kind=0) == -2 and attn(kind=2) == -2 and attn(d=60) == -2 and attn(d=264) == -2
+    assert attn(q=None) == -1 and attn(k=None) == -1 and attn(ks=None) == -1 and attn(table=None) == -1 and attn(cu=None) == -1
+    assert attn(lengths=None) == -1 and attn(pool=0) == -1 and attn(pool=-1) == -1 and attn(pages=-1) == -1 and attn(page=0) == -1
+    assert attn(block=0) == -1 and attn(block=2) == -1 and attn(block=12) == -1 and attn(page=18, block=6) == -1
+    assert attn(k=odd) == -1 and attn(k_t=68) == -1 and attn(hq=3, hk=2) == -1 and attn(scale=0.0) == -1
+    assert attn(page=1 << 20, block=16, pages=1 << 12) == -1
+    assert attn(tokens=1 << 29) == -2
+    assert attn(page=64, block=64, pages=100) == -3  # 6400 positions may be divided: no workspace
+    assert attn(out=p) == -1  # overlaps the codes
+
+
+def test_append_and_read_entries_refuse_before_any_launch(L):
+    p, odd = ctypes.c_void_p(64), ctypes.c_void_p(68)
+
+    def append(dtype=0, kind=4, k=p, ks=p, table=p, tokens=4, seqs=1, pool=4, page=16, block=8, pages=4, hk=1, d=64):
+        return L.bp_paged_append8(dtype, kind, k, p, p, p, ks, p, table, 4, p, p, tokens, seqs, pool, page, block, pages, hk, d,
+                                  *([64] * 16), None)
+
+    assert append(dtype=3) == -2 and append(kind=0) == -2 and append(k=None) == -1 and append(ks=None) == -1
+    assert append(table=None) == -1 and append(tokens=-1) == -1 and append(page=0) == -1 and append(block=0) == -1
+    assert append(block=5) == -1 and append(page=1 << 20, block=16, pages=1 << 10) == -1
+    assert append(tokens=0) == 0 and append(seqs=0) == 0 and append(pool=0) == 0 and append(pages=0) == 0 and append(d=0) == 0
+    assert append(hk=1 << 29) == -2 and append(page=1 << 16, block=1 << 16, d=1 << 15) == -2
+
+    def read(dtype=0, kind=4, kp=p, ks=p, k=p, table=p, cu=p, tokens=4, seqs=1, pool=4, page=16, block=8, pages=4, hk=2, d=64, p_t=64):
+        return L.bp_paged_read(dtype, kind, kp, p, ks, p, k, p, table, 4, p, cu, tokens, seqs, pool, page, block, pages, hk, d, 64,
+                               p_t, *([64] * 10), None)
+
+    assert read(dtype=3) == -2 and read(kind=0, dtype=1) == -2 and read(kind=2, dtype=2) == -2 and read(d=60) == -2
+    assert read(kp=None) == -1 and read(ks=None) == -1 and read(k=None) == -1 and read(table=None) == -1 and read(cu=None) == -1
+    assert read(block=5) == -1 and read(block=0) == -1 and read(page=0) == -1 and read(tokens=-1) == -1
+    assert read(k=odd) == -1 and read(kp=odd) == -1 and read(p_t=68) == -1
+    assert read(tokens=0) == 0 and read(hk=0) == 0
+    assert read(tokens=1 << 28, hk=8) == -2
+
+
+def test_rotary_entry_refuses_before_any_launch(L):
+    q, k, pos, inv = (ctypes.c_void_p(n << 20) for n in (1, 2, 3, 4))
+
+    def rot(dtype=0, q=q, qo=ctypes.c_void_p(5 << 20), k=k, ko=ctypes.c_void_p(6 << 20), pos=pos, size=8, inv=inv, tokens=4, hq=2, hk=1,
+            d=64, r=64, factor=1.0, q_t=128, qo_t=128, qo_h=64):
+        return L.bp_rotary(dtype, q, k, qo, ko, pos, size, inv, tokens, hq, hk, d, r, 0, factor, q_t, 64, 64, 64, qo_t, qo_h, 64, 64,
+                           None)
+
+    assert rot(tokens=0) == 0 and rot(d=0, r=0) == 0 and rot(hq=0, hk=0) == 0
+    assert rot(dtype=3) == -2 and rot(d=1032) == -2
+    assert rot(r=63) == -1 and rot(r=66) == -1 and rot(r=-2) == -1 and rot(size=2) == -1 and rot(factor=math.nan) == -1
+    assert rot(tokens=-1) == -1 and rot(hq=-1) == -1 and rot(q=None) == -1 and rot(ko=None) == -1 and rot(pos=None) == -1
+    assert rot(inv=None) == -1 and rot(qo_t=100) == -1 and rot(qo_h=32) == -1
+    assert rot(qo=ctypes.c_void_p((1 << 20) + 64)) == -1  # shifted within its own input
+    assert rot(qo=k) == -1 and rot(qo=ctypes.c_void_p(6 << 20)) == -1 and rot(qo=pos) == -1 and rot(qo=inv) == -1
+    assert rot(q_t=256, qo=q) == -1  # its own input's place, but not its strides
