@@ -7,6 +7,10 @@ probabilities (token_logprobs). The single-sequence loops of olmo.py are not tou
   scores = batch.score([ids_a, ids_b], top=5)             # of every prompt token after the first
   outs = batch.generate([ids_a, ids_b], max_new_tokens=32, top=5)
 
+The cache may be held in 8 bits (cache=torch.float8_e4m3fn or torch.int8: half the memory, and the steps' attention reads half as
+much; prompts still run over their own 16-bit keys and values), and positions may turn by frequencies of the program's own
+(rotary=rotary_frequencies(...), made for contexts longer than the decoder's).
+
 Greedy; a sequence ends after an EOS id or max_new_tokens. Pages are taken when a call begins and given back when it ends.
 """
 
@@ -21,6 +25,7 @@ from . import skinny as S
 from .attention import packed_attention, paged_append, paged_attention
 from .logprobs import MAX_TOP, TokenLogprobs, token_logprobs
 from .olmo import OlmoDecoder, OptimizeError
+from .rotary import rotary as rotate
 
 
 class Generated(NamedTuple):
@@ -35,15 +40,30 @@ class Generated(NamedTuple):
 
 
 class OlmoBatch:
-    """pages x page positions of cache for every layer of `dec`."""
+    """pages x page positions of cache for every layer of `dec`, of dtype `cache`: bfloat16, or (pages of a multiple of 4 positions)
+    8-bit codes with a scale for each head and block of 16 positions (12, 8 or 4 where 16 does not divide a page). rotary: (inv_freq [head_dim / 2], factor) on the decoder's device; by default the decoder's own frequencies,
+    their angles rounded to float32 as its own loops have them where the cache is bfloat16."""
 
-    def __init__(self, dec: OlmoDecoder, pages: int, page: int = 16):
+    def __init__(self, dec: OlmoDecoder, pages: int, page: int = 16, *, cache: torch.dtype = torch.bfloat16,
+                 rotary: tuple[torch.Tensor, float] | None = None):
         if pages < 1 or page < 1:
             raise ValueError("the cache needs at least one page of at least one position")
+        if cache not in (torch.bfloat16, torch.float8_e4m3fn, torch.int8):
+            raise ValueError(f"the cache is held in bfloat16, float8_e4m3fn or int8, not {cache}")
+        if cache != torch.bfloat16 and page % 4:
+            raise ValueError(f"an 8-bit cache needs pages of a multiple of 4 positions, not {page}")
         cfg = dec.cfg
         self.dec, self.page = dec, page
         shape = (cfg.layers, pages, page, cfg.heads, cfg.head_dim)
-        self.k_pages, self.v_pages = (torch.zeros(shape, dtype=torch.bfloat16, device=dec.device) for _ in range(2))
+        self.k_pages, self.v_pages = (torch.zeros(shape, dtype=cache, device=dec.device) for _ in range(2))
+        self.scales: list[dict] = [{}] * cfg.layers
+        if cache != torch.bfloat16:
+            block = next(b for b in (16, 12, 8, 4) if page % b == 0)
+            shape = (2, cfg.layers, pages, page // block, cfg.heads)
+            k_scales, v_scales = torch.zeros(shape, dtype=torch.uint8, device=dec.device).view(torch.float8_e8m0fnu)
+            self.scales = [{"k_scales": k, "v_scales": v} for k, v in zip(k_scales, v_scales)]
+            rotary = rotary or (dec.inv_freq, 1.0)
+        self.rotary = rotary
         self.free = list(range(pages))
 
     def _ints(self, xs: list) -> torch.Tensor:
@@ -77,13 +97,18 @@ class OlmoBatch:
         attention of a layer, [tokens, heads, head_dim] each."""
         dec, cfg = self.dec, self.dec.cfg
         st = _lib.stream_ptr(dec.device)
-        angle = positions[:, None].float() * dec.inv_freq[None, :]
-        cos, sin = angle.cos()[:, None], angle.sin()[:, None]
+        if self.rotary is None:
+            angle = positions[:, None].float() * dec.inv_freq[None, :]
+            cos, sin = angle.cos()[:, None], angle.sin()[:, None]
         x = dec.embed[ids]
         for i, w in enumerate(dec.layers):
             q, k, v = S.skinny_mm(x, *w["qkv"]).split(cfg.hidden, dim=1)
-            q = self._rope(self._norm(q.contiguous(), w["q_norm"]), cos, sin)
-            k = self._rope(self._norm(k.contiguous(), w["k_norm"]), cos, sin)
+            q, k = self._norm(q.contiguous(), w["q_norm"]), self._norm(k.contiguous(), w["k_norm"])
+            if self.rotary is None:
+                q, k = self._rope(q, cos, sin), self._rope(k, cos, sin)
+            else:
+                q, k = (t.view(-1, cfg.heads, cfg.head_dim) for t in (q, k))
+                rotate(q, k, positions, self.rotary[0], factor=self.rotary[1], out=(q, k))
             a = attend(i, q, k, v.unflatten(1, (cfg.heads, cfg.head_dim)))
             x = self._norm(S.skinny_mm(a.view(-1, cfg.hidden), *w["o"]), w["post_attn"], x)
             gate_up = S.skinny_mm(x, *w["gate_up"])
@@ -142,12 +167,12 @@ class OlmoBatch:
         lengths = self._ints([len(i) for i in ids])
 
         def prompt(i: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> torch.Tensor:
-            paged_append(k, v, self.k_pages[i], self.v_pages[i], table, lengths, cu)
+            paged_append(k, v, self.k_pages[i], self.v_pages[i], table, lengths, cu, **self.scales[i])
             return packed_attention(q, k, v, cu)
 
         def step(i: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> torch.Tensor:
-            paged_append(k, v, self.k_pages[i], self.v_pages[i], table, lengths, ones)
-            return paged_attention(q, self.k_pages[i], self.v_pages[i], table, lengths, ones)
+            paged_append(k, v, self.k_pages[i], self.v_pages[i], table, lengths, ones, **self.scales[i])
+            return paged_attention(q, self.k_pages[i], self.v_pages[i], table, lengths, ones, **self.scales[i])
 
         n = len(ids)
         ones = torch.arange(n + 1, dtype=torch.int32, device=self.dec.device)
