@@ -340,7 +340,7 @@ __device__ __forceinline__ void merge_rows(const Args& a, const Item& it, int kv
 // Joins the partials of a unit's rows: the parts' sums, each times exp2 of its maximum less the greatest. Few parts or many
 // rows: merge_rows. Few rows of many parts: the workgroup has one row, whose parts its groups of d / 4 threads share (one
 // thread after another part took 30 us for 80 parts of 36 rows).
-template <class T, int DP>
+template <class T, int DP, class P>
 __global__ __launch_bounds__(kThreads) void merge_kernel(Args a) {
   __shared__ float red[kWaves];
   __shared__ f32x4 sums[kThreads];
@@ -349,7 +349,7 @@ __global__ __launch_bounds__(kThreads) void merge_kernel(Args a) {
   const int tid = threadIdx.x, pieces = a.d / 4;
   const int64_t step = static_cast<int64_t>(a.hk.d) * a.ws_rows * (DP + 2);
   for (int unit = index;; unit += a.hk(gridDim.x)) {
-    const Item it = find_item<true>(a, unit);
+    const Item it = find_item<true, P>(a, unit);
     if (it.b < 0) return;
     if (it.slot + it.splits > a.slots) continue;
     const float* ws = slot_at<DP>(a, it.slot, kvh);
@@ -452,7 +452,7 @@ int launch(const Args& a, const Launch& n, hipStream_t st) {
   else attention_kernel<T, DP, PAGED, false><<<grid, kThreads, 0, st>>>(a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return static_cast<int>(e);
-  return n.merges > 0 ? launch_merge(std::is_same<T, Bf16>::value ? BP_DT_BF16 : BP_DT_F16, a, n, st) : BP_OK;
+  return n.merges > 0 ? launch_merge<Tiles32>(std::is_same<T, Bf16>::value ? BP_DT_BF16 : BP_DT_F16, a, n, st) : BP_OK;
 }
 
 template <class T, bool PAGED>
@@ -510,18 +510,26 @@ int run(int dtype, Args& a, bool paged, size_t ws_bytes, hipStream_t st) {
 
 }  // namespace
 
+template <class T, class P>
+void merge(const Args& a, unsigned grid, hipStream_t st) {
+  switch (padded_dim(a.d)) {
+    case 64: merge_kernel<T, 64, P><<<grid, kThreads, 0, st>>>(a); break;
+    case 96: merge_kernel<T, 96, P><<<grid, kThreads, 0, st>>>(a); break;
+    case 128: merge_kernel<T, 128, P><<<grid, kThreads, 0, st>>>(a); break;
+    default: merge_kernel<T, 256, P><<<grid, kThreads, 0, st>>>(a);
+  }
+}
+
+template <class P>
 int launch_merge(int dtype, const Args& a, const Launch& n, hipStream_t st) {
   const unsigned grid = static_cast<unsigned>(n.merges * a.hk.d);
-  const bool bf16 = dtype == BP_DT_BF16;
-  switch (padded_dim(a.d)) {
-    case 64: bf16 ? merge_kernel<Bf16, 64><<<grid, kThreads, 0, st>>>(a) : merge_kernel<F16, 64><<<grid, kThreads, 0, st>>>(a); break;
-    case 96: bf16 ? merge_kernel<Bf16, 96><<<grid, kThreads, 0, st>>>(a) : merge_kernel<F16, 96><<<grid, kThreads, 0, st>>>(a); break;
-    case 128: bf16 ? merge_kernel<Bf16, 128><<<grid, kThreads, 0, st>>>(a) : merge_kernel<F16, 128><<<grid, kThreads, 0, st>>>(a); break;
-    default: bf16 ? merge_kernel<Bf16, 256><<<grid, kThreads, 0, st>>>(a) : merge_kernel<F16, 256><<<grid, kThreads, 0, st>>>(a);
-  }
+  if (dtype == BP_DT_BF16) merge<Bf16, P>(a, grid, st);
+  else merge<F16, P>(a, grid, st);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? BP_OK : static_cast<int>(e);
 }
+template int launch_merge<Tiles32>(int, const Args&, const Launch&, hipStream_t);
+template int launch_merge<Tiles16>(int, const Args&, const Launch&, hipStream_t);
 
 }  // namespace attn
 }  // namespace bp

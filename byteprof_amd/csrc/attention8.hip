@@ -21,6 +21,7 @@ struct Args8 : Args {
   int64_t ks_p, ks_b, ks_h, vs_p, vs_b, vs_h;
   Div block;
   int wide;  // 16 codes at a time: all rows lie on 16 bytes and are made of them
+  int even;  // pages of whole 16 positions, blocks that are whole 16s or parts of one, and keys and values laid out alike
 };
 
 namespace {
@@ -57,6 +58,34 @@ struct Cache {
     vo = n * a.v_p + slot * a.v_t;
     kso = n * a.ks_p + blk * a.ks_b;
     vso = n * a.vs_p + blk * a.vs_b;
+  }
+};
+
+// 16 keys from a multiple of 16 on, where the cache is even (Args8::even): they lie in one page, and in one block or in whole blocks,
+// so that their addresses are a wave's, with offsets of the lanes that do not change. Of the item's last keys, those that there are:
+// `rest` of them after the first.
+struct Sixteen {
+  const uint8_t* k;
+  const uint8_t* v;
+  const uint8_t* ks;
+  const uint8_t* vs;
+  int rest;
+
+  __device__ __forceinline__ Sixteen(const Args8& a, Cache& c, int key, int id) {
+    key = min(key, c.last & ~15);
+    rest = c.last - key;
+    const uint32_t slot = key - a.page(key) * a.page.d, blk = a.block(slot);
+    uint32_t n = __builtin_amdgcn_readfirstlane(id);
+    if (n >= static_cast<uint32_t>(a.pool)) {
+      c.bad = true;
+      n = 0;
+    }
+    const uint64_t at = static_cast<uint64_t>(n) * static_cast<uint32_t>(a.k_p) + slot * static_cast<uint32_t>(a.k_t);
+    const uint64_t sat = static_cast<uint64_t>(n) * static_cast<uint32_t>(a.ks_p) + blk * static_cast<uint32_t>(a.ks_b);
+    k = c.k + at;
+    v = c.v + at;
+    ks = c.ks + sat;
+    vs = c.vs + sat;
   }
 };
 
@@ -149,40 +178,54 @@ __device__ __forceinline__ void small_tile8(const Args8& a, const Item& it, int 
   Cache cache(a, it, kvh);
   u32x4* img = smem + wave * 32 * (DP / 16);
   constexpr int STEP = 32 * kWaves;
-  u32x4 kc[DP / 32], vc[DP / 32];
-  int ks = 0, vs = 0, next = 0;
-  const auto load = [&](int key) {
-    int64_t ko, vo, kso, vso;
-    cache.at(a, key, next, ko, vo, kso, vso);
-    ks = cache.ks[kso];
-#pragma unroll
-    for (int c = 0; c < DP / 32; ++c) kc[c] = codes16<FULL>(a, cache.k + ko, 2 * c + half);
-    vs = cache.vs[vso];
-#pragma unroll
-    for (int c = 0; c < DP / 32; ++c) vc[c] = codes16<FULL>(a, cache.v + vo, 2 * c + half);
-    next = cache.id(a, key + STEP);
-  };
-  int key = it.key0 + 32 * wave;
   const int sub = lane & 31;
-  if (key < it.key1) {
-    next = cache.id(a, key + sub);
-    load(key + sub);
-  }
-  for (; key < it.key1; key += STEP) {
+  int key = it.key0 + 32 * wave;
+  // Two blocks ahead: every load is sent, past the item's keys from its last row over again (with a branch around them the
+  // compiler would wait for all loads that are out).
+  struct Block {
+    u32x4 k[DP / 32], v[DP / 32];
+    int ks, vs, id;
+  } even, odd;
+  const auto load = [&](Block& x, int at) {
+    int64_t ko, vo, kso, vso;
+    cache.at(a, at, x.id, ko, vo, kso, vso);
+    x.ks = cache.ks[kso];
+#pragma unroll
+    for (int c = 0; c < DP / 32; ++c) x.k[c] = codes16<FULL>(a, cache.k + ko, 2 * c + half);
+    x.vs = cache.vs[vso];
+#pragma unroll
+    for (int c = 0; c < DP / 32; ++c) x.v[c] = codes16<FULL>(a, cache.v + vo, 2 * c + half);
+    x.id = cache.id(a, at + 2 * STEP);
+  };
+  const auto step = [&](Block& x, int at) {
     f32x16 s[1] = {};
-    const typename C::Scale kscale = C::scale(ks);
+    const typename C::Scale kscale = C::scale(x.ks);
 #pragma unroll
     for (int c = 0; c < DP / 32; ++c) {
-      s[0] = T::mfma(cache8::eight<C>(kc[c][0], kc[c][1], kscale), q[2 * c], s[0]);
-      s[0] = T::mfma(cache8::eight<C>(kc[c][2], kc[c][3], kscale), q[2 * c + 1], s[0]);
+      s[0] = T::mfma(cache8::eight<C>(x.k[c][0], x.k[c][1], kscale), q[2 * c], s[0]);
+      s[0] = T::mfma(cache8::eight<C>(x.k[c][2], x.k[c][3], kscale), q[2 * c + 1], s[0]);
     }
 #pragma unroll
-    for (int c = 0; c < DP / 32; ++c) img[place8<DP>(sub, 2 * c + half)] = vc[c];
-    const int now = vs;
-    if (key + STEP < it.key1) load(key + STEP + sub);
+    for (int c = 0; c < DP / 32; ++c) img[place8<DP>(sub, 2 * c + half)] = x.v[c];
+    const int vs = x.vs;
+    load(x, at + 2 * STEP + sub);
     u32x4 p[1][2];
-    softmax_step<T, DP, 1>(s, p, r, a.scale_log2, key, min(limit, cache.last), key + 31 > min(least, cache.last), lane);
-    weighted8<T, C, DP>(img, now, p[0], r.o, lane);
+    softmax_step<T, DP, 1>(s, p, r, a.scale_log2, at, min(limit, cache.last), at + 31 > min(least, cache.last), lane);
+    weighted8<T, C, DP>(img, vs, p[0], r.o, lane);
+  };
+  if (key < it.key1) {
+    even.id = cache.id(a, key + sub);
+    odd.id = cache.id(a, key + STEP + sub);
+    load(even, key + sub);
+    load(odd, key + STEP + sub);
+    while (true) {
+      step(even, key);
+      key += STEP;
+      if (key >= it.key1) break;
+      step(odd, key);
+      key += STEP;
+      if (key >= it.key1) break;
+    }
   }
   if (__any(cache.bad)) r.l = NAN;
   join_waves<T, DP, Shape8<DP>::G>(a, it, kvh, r, smem, stats);
@@ -284,6 +327,277 @@ __device__ __forceinline__ void large_tile8(const Args8& a, const Item& it, int 
   if (active) write_rows<T, DP>(a, it, kvh, row, r, lane);
 }
 
+// Launches of few rows a sequence (decode steps): tiles of 16 rows. Half the softmax and matrix work of a 32-row tile for each key,
+// and so few registers that four workgroups are on a CU (256 columns: two), whose loads are what fills the memory's queue.
+
+__device__ __forceinline__ f32x4 mfma16(Bf16, u32x4 a, u32x4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma16(F16, u32x4 a, u32x4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// Place of 16-code chunk `chunk` of a row in a wave's image of 32 value rows: 8 rows written, and the 16 rows that two 16-lane groups
+// read transposed (4 and 4, 16 apart, of either), lie in different banks.
+template <int DP>
+__device__ __forceinline__ int place16(int row, int chunk) {
+  constexpr int CH = DP / 16;
+  const int high = row >> 4 & 1;
+  if constexpr (CH == 4) return row * CH + (chunk ^ ((row >> 2 & 1) | high << 1));
+  else if constexpr (CH == 8) return row * CH + (chunk ^ ((row >> 1 & 3) | high << 2));
+  else return row * CH + (chunk ^ ((row & 7) | high << 3));
+}
+
+template <int DP>
+struct Shape16 {
+  static constexpr int NB = 2;                                    // 16-key blocks of a wave's step
+  static constexpr int kImages = kWaves * 2 * 16 * NB * DP / 16;  // a wave's keys and values
+  static constexpr int G = DP < 128 ? DP : 128;              // columns of a round of the waves' join
+  static constexpr int kJoin = kWaves * 16 * G / 4;
+  static constexpr int kChunks = kImages > kJoin ? kImages : kJoin;
+};
+
+// A lane has row lane % 16: of 16 keys' scores (S^T = K Q^T, 16 x 16) four, keys 4 (lane / 16) + 0..3; those of 32 keys are the
+// operand of O^T = V^T P^T where they lie, whose values come transposed from LDS in the same order of the keys.
+template <class T, class C, int DP, bool FULL>
+__global__ __launch_bounds__(kThreads, DP > 128 ? 2 : DP > 64 ? 3 : 4) void attention8_few_kernel(Args8 a) {
+  constexpr int NC = DP / 64, NB = Shape16<DP>::NB, KEYS = 16 * NB, STEP = KEYS * kWaves;
+  __shared__ __align__(16) u32x4 smem[Shape16<DP>::kChunks];
+  __shared__ float stats[16 * (2 * kWaves + 1)];
+  if constexpr (std::is_same<T, F16>::value) cache8::saturate_f16();
+  // Workgroup b runs on XCD b % 8: a part's key heads, whose rows lie side by side, go to one XCD.
+  const int place = blockIdx.x / kXcds, part = a.hk(place), kvh = place - part * a.hk.d;
+  const int index = part * kXcds + blockIdx.x % kXcds;
+  const Item it = find_item<false, Tiles16>(a, index);
+  if (it.b < 0) {
+    fill_rest(a, kvh, it.extra, a.hk(gridDim.x) - (index - it.extra));
+    return;
+  }
+  if (it.key0 >= it.key1 && it.split > 0) return;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), row = lane & 15, g = lane >> 4;
+  const int top = it.row0 + it.rows - 1, mine = min(it.row0 + row, top);
+  u32x4 q[2 * NC];
+  {
+    const int n = a.group(mine);
+    const uint16_t* p = static_cast<const uint16_t*>(a.q) + static_cast<int64_t>(it.begin + n) * a.q_t +
+                        static_cast<int64_t>(kvh * a.group.d + mine - n * a.group.d) * a.q_h;
+#pragma unroll
+    for (int i = 0; i < 2 * NC; ++i) {
+      const int col = 64 * (i / 2) + 16 * g + 8 * (i % 2);
+      q[i] = FULL || col < a.d ? *reinterpret_cast<const u32x4*>(p + col) : u32x4{};
+    }
+  }
+  const int limit = min(it.first + a.group(mine), it.keys - 1);
+  const int least = __builtin_amdgcn_readfirstlane(limit);
+  const float c = a.scale_log2;
+  f32x4 o[DP / 16];
+#pragma unroll
+  for (int d = 0; d < DP / 16; ++d) o[d] = f32x4{};
+  float m = -INFINITY, l = 0.f;
+  Cache cache(a, it, kvh);
+  // Rows of codes go from memory to registers as they lie, a row's 16-byte chunks on neighbouring lanes, a step ahead; through LDS
+  // they become operands. (Keys straight in their operand's layout, a row to a lane: every lane then asks for a line of its own, and
+  // the address unit is busy half of the time.)
+  constexpr int CH = DP / 16, RPI = kWave / CH, N = KEYS / RPI, M = 16 / RPI;  // rows of a load, loads of a step and of 16 keys
+  u32x4* kimg = smem + wave * 2 * KEYS * CH;
+  u32x4* vimg = kimg + KEYS * CH;
+  const int lr = lane / CH, lc = lane % CH;
+  u32x4 kc[N], vc[N];
+  int ks[NB], vs[NB], id[NB];
+  const uint32_t k_t = static_cast<uint32_t>(a.k_t);
+  const auto part_of = [&](int r) { return static_cast<uint32_t>(a.block(r)) * static_cast<uint32_t>(a.ks_b); };
+  const int k_key = C::kPlainK ? 4 * g : row;  // the first product's operand is of key `row` of 16, its result of 4 g + 0..3
+  const uint32_t at_lane = lr * k_t + 16 * lc, ks_lane = FULL ? part_of(k_key) : 0, vs_lane = FULL ? part_of(4 * g) : 0;
+  // Every load is sent, past the item's keys from its last ones over again. Scales: of key k_key of 16, and of keys 4 g + 0..3 (the
+  // second product's operand); not FULL: of key lane % 32, to be fetched from there.
+  const auto load = [&](int at) {
+    if constexpr (FULL) {
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        const Sixteen x(a, cache, at + 16 * b, id[b]);
+        if (x.rest >= 15) {
+          ks[b] = x.ks[ks_lane];
+          vs[b] = x.vs[vs_lane];
+#pragma unroll
+          for (int j = 0; j < M; ++j) kc[b * M + j] = *reinterpret_cast<const u32x4*>(x.k + j * RPI * k_t + at_lane);
+#pragma unroll
+          for (int j = 0; j < M; ++j) vc[b * M + j] = *reinterpret_cast<const u32x4*>(x.v + j * RPI * k_t + at_lane);
+        } else {
+          ks[b] = x.ks[part_of(min(k_key, x.rest))];
+          vs[b] = x.vs[part_of(min(4 * g, x.rest))];
+#pragma unroll
+          for (int j = 0; j < M; ++j) {
+            const uint32_t off = min(j * RPI + lr, x.rest) * k_t + 16 * lc;
+            kc[b * M + j] = *reinterpret_cast<const u32x4*>(x.k + off);
+            vc[b * M + j] = *reinterpret_cast<const u32x4*>(x.v + off);
+          }
+        }
+        id[b] = cache.id(a, at + STEP + 16 * b);
+      }
+    } else {
+      int64_t ko, vo, kso, vso;
+      cache.at(a, at + lane % KEYS, id[0], ko, vo, kso, vso);
+      ks[0] = cache.ks[kso];
+      vs[0] = cache.vs[vso];
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        kc[j] = codes16<false>(a, cache.k + __shfl(ko, j * RPI + lr), lc);
+        vc[j] = codes16<false>(a, cache.v + __shfl(vo, j * RPI + lr), lc);
+      }
+      id[0] = cache.id(a, at + STEP + lane % KEYS);
+    }
+  };
+  int key = it.key0 + KEYS * wave;
+  if (key < it.key1) {
+    if constexpr (FULL) {
+#pragma unroll
+      for (int b = 0; b < NB; ++b) id[b] = cache.id(a, key + 16 * b);
+    } else {
+      id[0] = cache.id(a, key + lane % KEYS);
+    }
+    load(key);
+  }
+  for (; key < it.key1; key += STEP) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) kimg[place16<DP>(j * RPI + lr, lc)] = kc[j];
+#pragma unroll
+    for (int j = 0; j < N; ++j) vimg[place16<DP>(j * RPI + lr, lc)] = vc[j];
+    using K = cache8::Outside<C, C::kPlainK>;
+    using V = cache8::Outside<C, C::kPlainV>;
+    typename K::Scale k_scale[NB];
+    typename V::Scale v_scale[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      k_scale[b] = K::scale(FULL ? ks[b] : __shfl(ks[0], 16 * b + k_key));
+      v_scale[b] = V::scale(FULL ? vs[b] : __shfl(vs[0], 16 * b + 4 * g));
+    }
+    load(key + STEP);
+    f32x4 s[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      s[b] = f32x4{};
+#pragma unroll
+      for (int i = 0; i < NC; ++i) {
+        const u32x4 w = kimg[place16<DP>(16 * b + row, 4 * i + g)];
+        s[b] = mfma16(T(), cache8::eight<K>(w[0], w[1], k_scale[b]), q[2 * i], s[b]);
+        s[b] = mfma16(T(), cache8::eight<K>(w[2], w[3], k_scale[b]), q[2 * i + 1], s[b]);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[b][i] = K::times(s[b][i], k_scale[b]);
+    }
+    const int last = cache.last;
+    if (key + KEYS - 1 > min(least, last)) {
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (key + 16 * b + 4 * g + i > min(limit, last)) s[b][i] = -INFINITY;
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[b][i]);
+    mx = fmaxf(m, xor_stage<32>(xor_stage<16>(mx, MaxOp()), MaxOp()));
+    if (__any(mx > m)) {
+      const float f = rescaled(m, mx, c);
+      m = mx;
+      l *= f;
+#pragma unroll
+      for (int d = 0; d < DP / 16; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[d][i] *= f;
+    }
+    // as in softmax_step: far from zero the difference is taken first
+    float shift = m == -INFINITY ? 0.f : -(m * c);
+    if (__any(!(fabsf(shift) < kFar))) {
+      const float less = fabsf(shift) < kFar ? 0.f : m;
+      shift = fabsf(shift) < kFar ? shift : 0.f;
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[b][i] -= less;
+    }
+    u32x4 p[NB / 2];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        s[b][i] = __builtin_amdgcn_exp2f(fmaf(s[b][i], c, shift));
+        l += s[b][i];
+      }
+      const auto weight = [&](int i) { return V::times(s[b][i], v_scale[b]); };
+      p[b / 2][2 * (b % 2)] = T::pack(weight(0), weight(1));
+      p[b / 2][2 * (b % 2) + 1] = T::pack(weight(2), weight(3));
+    }
+    typedef int i32x2 __attribute__((ext_vector_type(2)));
+    typedef __attribute__((address_space(3))) i32x2* lds2;
+    const int j = row >> 1, from = 16 * (j >> 2) + 4 * g + (j & 3);
+#pragma unroll
+    for (int b = 0; b < NB; b += 2)
+#pragma unroll
+      for (int d = 0; d < DP / 16; ++d) {
+        const char* at = reinterpret_cast<const char*>(vimg + place16<DP>(16 * b + from, d)) + 8 * (row & 1);
+        const i32x2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds2)(__attribute__((address_space(3))) void*)at);
+        const u32x2 x = V::four(w[0], v_scale[b]), y = V::four(w[1], v_scale[b + 1]);
+        o[d] = mfma16(T(), u32x4{x[0], x[1], y[0], y[1]}, p[b / 2], o[d]);
+      }
+  }
+  if (__any(cache.bad)) l = NAN;
+  l = xor_stage<32>(xor_stage<16>(l, AddOp()), AddOp());
+  // the waves' parts are joined: stats: [wave][16] maxima, [wave][16] sums, [16] factors of the result
+  if (lane < 16) {
+    stats[16 * wave + lane] = m;
+    stats[16 * (kWaves + wave) + lane] = l;
+  }
+  __syncthreads();
+  float whole_m = -INFINITY, whole_l = 0.f;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) whole_m = fmaxf(whole_m, stats[16 * w + row]);
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w)
+    whole_l += stats[16 * (kWaves + w) + row] * rescaled(stats[16 * w + row], whole_m, c);
+  const float f = rescaled(m, whole_m, c);
+  const bool whole = !it.divided, keep = whole || it.slot + it.split < a.slots;
+  const int wd = a.d <= 64 ? 64 : a.d <= 96 ? 96 : DP;  // columns of a slot
+  float* ws = whole ? nullptr : a.ws + (static_cast<int64_t>(it.slot + it.split) * a.hk.d + kvh) * a.ws_rows * (wd + 2);
+  if (wave == 0 && lane < 16) {
+    stats[16 * 2 * kWaves + lane] = whole ? inverse(whole_l) : 1.f;
+    if (!whole && keep && lane < it.rows) {
+      ws[a.ws_rows * wd + lane] = whole_m;
+      ws[a.ws_rows * (wd + 1) + lane] = whole_l;
+    }
+  }
+  f32x4* parts = reinterpret_cast<f32x4*>(smem);  // [wave][4 columns][16 rows]
+  constexpr int G = Shape16<DP>::G;
+#pragma unroll
+  for (int r = 0; r < DP / G; ++r) {
+    if (row < it.rows) {
+#pragma unroll
+      for (int d = 0; d < G / 16; ++d) {
+        const f32x4 x = o[r * (G / 16) + d];
+        parts[(wave * (G / 4) + 4 * d + g) * 16 + row] = f32x4{x[0] * f, x[1] * f, x[2] * f, x[3] * f};
+      }
+    }
+    __syncthreads();
+    for (int i = tid; i < it.rows * (G / 4); i += kThreads) {
+      const int rw = i / (G / 4), piece = i % (G / 4), col = 4 * piece + r * G;
+      f32x4 x = parts[piece * 16 + rw];
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) x += parts[(w * (G / 4) + piece) * 16 + rw];
+      if (whole) {
+        const float inv = stats[16 * 2 * kWaves + rw];
+        if (col < a.d)
+          *reinterpret_cast<u32x2*>(out_row(a, it, kvh, it.row0 + rw) + col) =
+              u32x2{T::pack(x[0] * inv, x[1] * inv), T::pack(x[2] * inv, x[3] * inv)};
+      } else if (keep && col < wd) {
+        *reinterpret_cast<f32x4*>(ws + rw * wd + col) = x;
+      }
+    }
+    if (r + 1 < DP / G) __syncthreads();
+  }
+}
+
 template <class T, class C, int DP, bool FULL>
 __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void attention8_kernel(Args8 a) {
   __shared__ __align__(16) u32x4 smem[Shape8<DP>::kChunks];
@@ -301,25 +615,39 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void attention8_kernel(
 }
 
 template <class T, int KIND, int DP>
-int launch8(const Args8& a, const Launch& n, hipStream_t st) {
-  constexpr bool bf16 = std::is_same<T, Bf16>::value;
-  using C = cache8::Codes<KIND, bf16>;
+void launch8(const Args8& a, const Launch& n, hipStream_t st) {
+  using C = cache8::Codes<KIND, std::is_same<T, Bf16>::value>;
   const unsigned grid = static_cast<unsigned>(n.index * a.hk.d);
   if (a.d == DP && a.wide) attention8_kernel<T, C, DP, true><<<grid, kThreads, 0, st>>>(a);
   else attention8_kernel<T, C, DP, false><<<grid, kThreads, 0, st>>>(a);
-  const hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return static_cast<int>(e);
-  return n.merges > 0 ? launch_merge(bf16 ? BP_DT_BF16 : BP_DT_F16, a, n, st) : BP_OK;
+}
+
+template <class T, int KIND, int DP>
+void launch8_few(const Args8& a, const Launch& n, hipStream_t st) {
+  using C = cache8::Codes<KIND, std::is_same<T, Bf16>::value>;
+  const unsigned grid = static_cast<unsigned>((n.index + kXcds - 1) / kXcds * kXcds * a.hk.d);
+  if (a.d == DP && a.wide && a.even) attention8_few_kernel<T, C, DP, true><<<grid, kThreads, 0, st>>>(a);
+  else attention8_few_kernel<T, C, DP, false><<<grid, kThreads, 0, st>>>(a);
 }
 
 template <class T, int KIND>
-int launch8_dim(const Args8& a, const Launch& n, hipStream_t st) {
-  switch (padded_dim(a.d)) {
-    case 64: return launch8<T, KIND, 64>(a, n, st);
-    case 96: return launch8<T, KIND, 96>(a, n, st);
-    case 128: return launch8<T, KIND, 128>(a, n, st);
-    default: return launch8<T, KIND, 256>(a, n, st);
+int launch8_dim(const Args8& a, const Launch& n, bool few, hipStream_t st) {
+  const int padded = padded_dim(a.d);
+  if (few) {
+    if (padded == 64) launch8_few<T, KIND, 64>(a, n, st);
+    else if (padded <= 128) launch8_few<T, KIND, 128>(a, n, st);
+    else launch8_few<T, KIND, 256>(a, n, st);
+  } else {
+    if (padded == 64) launch8<T, KIND, 64>(a, n, st);
+    else if (padded == 96) launch8<T, KIND, 96>(a, n, st);
+    else if (padded == 128) launch8<T, KIND, 128>(a, n, st);
+    else launch8<T, KIND, 256>(a, n, st);
   }
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return static_cast<int>(e);
+  if (n.merges == 0) return BP_OK;
+  const int dtype = std::is_same<T, Bf16>::value ? BP_DT_BF16 : BP_DT_F16;
+  return few ? launch_merge<Tiles16>(dtype, a, n, st) : launch_merge<Tiles32>(dtype, a, n, st);
 }
 
 bool aligned(const void* p, int n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
@@ -345,10 +673,18 @@ int run8(int dtype, int kind, Args8& a, size_t ws_bytes, hipStream_t st) {
       (strides & 7) != 0)
     return BP_E_INVALID_ARG;
   a.wide = aligned(a.k, 16) && aligned(a.v, 16) && (strides & 15) == 0 && a.d % 16 == 0;
+  // (and a page's strides, and offsets inside a page, in 32 bits)
+  a.even = a.page.d % 16 == 0 && (a.block.d % 16 == 0 || 16 % a.block.d == 0) && a.k_p == a.v_p && a.k_t == a.v_t &&
+           a.ks_p == a.vs_p && a.ks_b == a.vs_b && ((a.k_p | a.ks_p) & ~0x7fffffffll) == 0 && a.k_t >= 0 && a.ks_b >= 0 &&
+           a.k_t * a.page.d < (1ll << 31) && a.ks_b * blocks < (1ll << 31);
   // rows of a sequence, and keys plus a split, in 32 bits
   if (static_cast<int64_t>(a.tokens) * a.hq >= (1ll << 30) || a.max_keys >= (1 << 29)) return BP_E_UNSUPPORTED;
+  // Few rows a sequence, as far as the host can tell (the offsets are the device's; any are right): tiles of 16 rows. Their
+  // workspace is no larger: at most twice the tiles, or parts, of half the rows.
+  const int group = a.hq / hk;
+  const bool few = group <= 16 && static_cast<int64_t>(a.tokens) * group <= 16ll * a.seqs;
   Launch n;
-  if (!plan_launch(a, n)) return BP_E_UNSUPPORTED;
+  if (!(few ? plan_launch<Tiles16>(a, n) : plan_launch<Tiles32>(a, n))) return BP_E_UNSUPPORTED;
   if (n.workspace > 0 && (a.ws == nullptr || ws_bytes < n.workspace || !aligned(a.ws, 16))) return BP_E_WORKSPACE;
   if (n.workspace == 0) a.ws = nullptr;
   // A row of q is read by the tile that writes its result and by no other, so out may be q itself.
@@ -365,8 +701,8 @@ int run8(int dtype, int kind, Args8& a, size_t ws_bytes, hipStream_t st) {
     return BP_E_INVALID_ARG;
   const bool e4m3 = kind == BP_DT_E4M3;
   if (dtype == BP_DT_BF16)
-    return e4m3 ? launch8_dim<Bf16, cache8::kE4m3>(a, n, st) : launch8_dim<Bf16, cache8::kInt8>(a, n, st);
-  return e4m3 ? launch8_dim<F16, cache8::kE4m3>(a, n, st) : launch8_dim<F16, cache8::kInt8>(a, n, st);
+    return e4m3 ? launch8_dim<Bf16, cache8::kE4m3>(a, n, few, st) : launch8_dim<Bf16, cache8::kInt8>(a, n, few, st);
+  return e4m3 ? launch8_dim<F16, cache8::kE4m3>(a, n, few, st) : launch8_dim<F16, cache8::kInt8>(a, n, few, st);
 }
 
 }  // namespace

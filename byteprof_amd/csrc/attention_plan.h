@@ -18,6 +18,30 @@ constexpr int kTileLarge = 128;  // 32 rows a wave, all keys
 constexpr int kSharedMin = 512;  // least keys of a split where the parts are more than that
 constexpr int kKeyStep = 128;    // a split's keys are a multiple of this: whole steps of either kind of tile
 
+constexpr int kCus = 256;
+
+// How a launch cuts sequences into tiles. Tiles32: the kernels of attention.hip, and over a cache in 8 bits wherever sequences have
+// many rows. Tiles16: the kernel of attention8.hip for launches of few rows a sequence.
+struct Tiles32 {
+  static constexpr int kFew = kSmallRows;    // sequences of at most this many rows have the small tiles
+  static constexpr int kSmall = kTileSmall;
+  static constexpr bool kFit = true;         // parts that all fit the card at once, if that many do (split_keys)
+  static constexpr int kMergeRows = 32;      // rows of a unit of the merge; of up to kFew rows with more than kMergeParts parts, one
+  static constexpr int kTarget = 1024;       // bound of what splitting aims at (twice the workgroups that the card holds at once:
+                                             // 1024, for 256 columns 512)
+  // By the registers of attention_kernel: 256 columns leave one wave a SIMD, 128 two (fewer columns three, but planning for three
+  // made heads of 96 no faster and cached ones slower, 97 us against 90).
+  static int workgroups_a_cu(int padded) { return padded > 128 ? 1 : 2; }
+};
+struct Tiles16 {
+  static constexpr int kFew = 1 << 30;
+  static constexpr int kSmall = 16;
+  static constexpr bool kFit = false;
+  static constexpr int kMergeRows = 16;
+  static constexpr int kTarget = 2048;
+  static int workgroups_a_cu(int padded) { return padded > 128 ? 2 : padded > 64 ? 3 : 4; }
+};
+
 // n / d for n below 2^30 without a division: magic = floor(2^(32 + shift) / d) + 1 with 2^shift < d <= 2^(shift + 1).
 struct Div {
   uint32_t magic;
@@ -62,6 +86,7 @@ struct Seq {
   int begin, count, rows, keys, tiles;
 };
 
+template <class P>
 __device__ __forceinline__ Seq sequence(const Args& a, int b) {
   Seq s;
   s.begin = min(max(a.cu[b], 0), a.tokens);
@@ -69,7 +94,7 @@ __device__ __forceinline__ Seq sequence(const Args& a, int b) {
   s.count = end - s.begin;
   s.rows = s.count * a.group.d;
   s.keys = a.lengths ? min(max(a.lengths[b], 0), a.max_keys) : s.count;
-  s.tiles = s.rows <= kSmallRows ? (s.rows + kTileSmall - 1) / kTileSmall : (s.rows + kTileLarge - 1) / kTileLarge;
+  s.tiles = s.rows <= P::kFew ? (s.rows + P::kSmall - 1) / P::kSmall : (s.rows + kTileLarge - 1) / kTileLarge;
   return s;
 }
 
@@ -93,10 +118,11 @@ __device__ __forceinline__ int scan_add(int v) {
 // than those; else over `target`, so that ragged parts share the card evenly; never under chunk_min. (A verify round of 36 rows
 // over 41k keys: 39 us in 480 parts, 53 in 660; a decode batch of 64 ragged sequences: 219 us by the first rule, 204 to 210 by
 // the second.) Every workgroup adds the same numbers in the same order, so all of them find the same value.
+template <class P>
 __device__ __forceinline__ int split_keys(const Args& a, const Seq& own, int lane) {
   float units = 0.f;
   for (int b = lane; b < a.seqs; b += kWave) {
-    const Seq s = b < kWave ? own : sequence(a, b);
+    const Seq s = b < kWave ? own : sequence<P>(a, b);
     units += static_cast<float>(s.tiles) * static_cast<float>(s.keys);
   }
   units = xor_butterfly<true>(units, AddOp()) * static_cast<float>(a.hk.d) * 1.001f;
@@ -105,10 +131,11 @@ __device__ __forceinline__ int split_keys(const Args& a, const Seq& own, int lan
     const int chunk = want < 1e9f ? static_cast<int>(want) + 1 : 0x3fffff00;
     return __builtin_amdgcn_readfirstlane((max(chunk, a.chunk_min) + kKeyStep - 1) / kKeyStep * kKeyStep);
   };
+  if constexpr (!P::kFit) return max(chunk_of(a.target), kSharedMin);
   const int chunk = chunk_of(a.resident);
   int items = 0;
   for (int b = lane; b < a.seqs; b += kWave) {
-    const Seq s = b < kWave ? own : sequence(a, b);
+    const Seq s = b < kWave ? own : sequence<P>(a, b);
     items += s.tiles * max(1, static_cast<int>(static_cast<unsigned>(s.keys + chunk / 2) / static_cast<unsigned>(chunk)));
   }
   return wave_sum(items) <= a.resident / a.hk.d ? chunk : max(chunk_of(a.target), kSharedMin);
@@ -122,27 +149,26 @@ struct Item {
   bool small, divided;
 };
 
-constexpr int kMergeRows = 32;  // rows of a unit of the merge; of up to 64 rows with more than kMergeParts parts, one
 constexpr int kMergeParts = 8;
 constexpr int kLevel = 128;  // keys of a level, of which the order of the tiles is made
 constexpr int kUndivided = 0x3fffffff;
 
 // The tile of index `index` (per key head); or, of the sequences whose keys are divided, the unit of rows of index `index` with
 // what its tile's parts are.
-template <bool MERGE>
+template <bool MERGE, class P = Tiles32>
 __device__ __forceinline__ Item find_item(const Args& a, int index) {
   const int lane = static_cast<int>(threadIdx.x) & 63;
   Seq own = {0, 0, 0, 0, 0};  // the lane's of the first 64 sequences: read once
-  if (lane < a.seqs) own = sequence(a, lane);
+  if (lane < a.seqs) own = sequence<P>(a, lane);
   const bool divide = a.ws != nullptr;
-  const int chunk = divide ? split_keys(a, own, lane) : 0;
+  const int chunk = divide ? split_keys<P>(a, own, lane) : 0;
   Item it;
   it.b = -1;
   int items = 0, slots = 0;
   for (int b0 = 0; b0 < a.seqs; b0 += kWave) {
     const int b = b0 + lane;
     Seq s = own;
-    if (b0 > 0) s = b < a.seqs ? sequence(a, b) : Seq{0, 0, 0, 0, 0};
+    if (b0 > 0) s = b < a.seqs ? sequence<P>(a, b) : Seq{0, 0, 0, 0, 0};
     int splits = 1, part = kUndivided, parts = 0, slot_upto = 0;
     if (divide) {
       splits = max(1u, static_cast<unsigned>(s.keys + chunk / 2) / static_cast<unsigned>(chunk));
@@ -159,7 +185,7 @@ __device__ __forceinline__ Item find_item(const Args& a, int index) {
       // Tiles by level, the number of keys in steps, from the greatest down; within a level by sequence. later(x): how many
       // tiles of the lane's sequence have level x or more. A causal tile's level grows with its place, others' are alike. No
       // tile has level hi: a causal one has it only if its sequence's last token is that far, whatever the rows of a token.
-      const bool ladder = a.causal && s.rows > kSmallRows && splits == 1;
+      const bool ladder = a.causal && s.rows > P::kFew && splits == 1;
       const int flat = min(s.keys, part) / kLevel, first = max(s.keys - s.count, 0);
       const auto later = [&](int x) {
         if (!ladder) return flat >= x ? s.tiles : 0;
@@ -184,8 +210,8 @@ __device__ __forceinline__ Item find_item(const Args& a, int index) {
       at = from - __builtin_amdgcn_readlane(upto - count, l);
       above = __builtin_amdgcn_readlane(before, l);
     } else {
-      const bool single = splits > kMergeParts && s.rows <= kSmallRows;
-      const int count = !MERGE ? all : splits == 1 ? 0 : single ? s.rows : (s.rows + kMergeRows - 1) / kMergeRows;
+      const bool single = splits > kMergeParts && s.rows <= P::kFew;
+      const int count = !MERGE ? all : splits == 1 ? 0 : single ? s.rows : (s.rows + P::kMergeRows - 1) / P::kMergeRows;
       const int upto = scan_add(count);
       const uint64_t over = __ballot(items + upto > index);
       if (over == 0) {
@@ -203,11 +229,11 @@ __device__ __forceinline__ Item find_item(const Args& a, int index) {
     it.keys = __builtin_amdgcn_readlane(s.keys, l);
     it.splits = __builtin_amdgcn_readlane(splits, l);
     it.divided = it.splits > 1;
-    it.small = rows <= kSmallRows;
-    const int tile_rows = it.small ? kTileSmall : kTileLarge;
+    it.small = rows <= P::kFew;
+    const int tile_rows = it.small ? P::kSmall : kTileLarge;
     // the last rows first: under a causal mask they have the most keys
     const int done = it.divided && !MERGE ? static_cast<unsigned>(at) / static_cast<unsigned>(it.splits) : at;
-    const int unit = MERGE && (it.splits <= kMergeParts || !it.small) ? kMergeRows : 1;
+    const int unit = MERGE && (it.splits <= kMergeParts || !it.small) ? P::kMergeRows : 1;
     const int tile = MERGE ? at * unit / tile_rows : tiles - 1 - above - done;
     it.split = it.divided ? at - done * it.splits : 0;
     it.slot = slots + __builtin_amdgcn_readlane(slot_upto - parts, l) + tile * it.splits;
@@ -228,42 +254,41 @@ __device__ __forceinline__ Item find_item(const Args& a, int index) {
   return it;
 }
 
-constexpr int kCus = 256;
-constexpr int kTarget = 1024;    // bound of what splitting aims at (twice the workgroups that the card holds at once: 1024, for 256
-                                 // columns 512)
 constexpr int kChunkMin = BP_ATTN_UNDIVIDED_KEYS;  // least keys of a split
 constexpr int kMergeGrid = 1024;  // workgroups of a merge launch; each takes every such unit
 
-// Row tiles of a key head that any offsets can give: sequences of up to 64 rows have 32-row tiles.
-inline int64_t tiles_bound(int64_t tokens, int64_t seqs, int64_t group) {
+// Row tiles of a key head that any offsets can give: sequences of up to kFew rows (64, or all) have small tiles.
+template <class P = Tiles32>
+int64_t tiles_bound(int64_t tokens, int64_t seqs, int64_t group) {
   const int64_t rows = tokens * group, some = seqs < tokens ? seqs : tokens;
-  const int64_t a = rows / kTileLarge + 2 * some, b = rows / kTileSmall + some;
-  return a < b ? a : b;
+  const int64_t a = rows / kTileLarge + 2 * some, b = rows / P::kSmall + some;
+  return P::kFew > kSmallRows || b <= a ? b : a;
 }
 
 inline bool may_split(int64_t max_keys) { return max_keys > kChunkMin; }
 
 inline int padded_dim(int d) { return d <= 64 ? 64 : d <= 96 ? 96 : d <= 128 ? 128 : 256; }
 
-// By the registers of attention_kernel: 256 columns leave one wave a SIMD, 128 two (fewer columns three, but planning for three
-// made heads of 96 no faster and cached ones slower, 97 us against 90).
-inline int workgroups_a_cu(int padded) { return padded > 128 ? 1 : 2; }
-
-inline int slot_rows(int64_t tokens, int64_t group) { return tokens * group <= kSmallRows ? kTileSmall : kTileLarge; }
+template <class P = Tiles32>
+int slot_rows(int64_t tokens, int64_t group) {
+  return tokens * group <= P::kFew ? P::kSmall : kTileLarge;
+}
 
 // Partials that any offsets can give. A split's keys are at least the whole work over the target, and a sequence is divided
 // into as many parts as its keys come to, rounded to the nearest, from 1.5 on: at most a third more parts than the target. Nor
 // are they more than every tile's most.
-inline int64_t slots_bound(int64_t tokens, int64_t seqs, int64_t group, int64_t hk, int64_t max_keys) {
-  const int64_t most = tiles_bound(tokens, seqs, group) * hk * ((max_keys + kChunkMin - 1) / kChunkMin);
-  const int64_t aim = kTarget + kTarget / 3 + 1 + hk;
+template <class P = Tiles32>
+int64_t slots_bound(int64_t tokens, int64_t seqs, int64_t group, int64_t hk, int64_t max_keys) {
+  const int64_t most = tiles_bound<P>(tokens, seqs, group) * hk * ((max_keys + kChunkMin - 1) / kChunkMin);
+  const int64_t aim = P::kTarget + P::kTarget / 3 + 1 + hk;
   return most < aim ? most : aim;
 }
 
-inline size_t workspace_bytes(int64_t tokens, int64_t seqs, int64_t hq, int64_t hk, int64_t d, int64_t max_keys) {
+template <class P = Tiles32>
+size_t workspace_bytes(int64_t tokens, int64_t seqs, int64_t hq, int64_t hk, int64_t d, int64_t max_keys) {
   if (tokens <= 0 || seqs <= 0 || hk <= 0 || hq % hk != 0 || d <= 0 || d > 256 || !may_split(max_keys)) return 0;
   const int64_t group = hq / hk;
-  return static_cast<size_t>(slots_bound(tokens, seqs, group, hk, max_keys)) * slot_rows(tokens, group) *
+  return static_cast<size_t>(slots_bound<P>(tokens, seqs, group, hk, max_keys)) * slot_rows<P>(tokens, group) *
          (padded_dim(static_cast<int>(d)) + 2) * sizeof(float);
 }
 
@@ -275,22 +300,23 @@ struct Launch {
 };
 
 // Completes the arguments (hk.d, page and the sizes are set) and gives the launch's. False: more workgroups than a launch has.
-inline bool plan_launch(Args& a, Launch& n) {
+template <class P = Tiles32>
+bool plan_launch(Args& a, Launch& n) {
   const int hk = a.hk.d, group = a.hq / hk;
   a.hk = Div::of(hk);
   a.group = Div::of(group);
-  a.resident = kCus * workgroups_a_cu(padded_dim(a.d));
+  a.resident = kCus * P::workgroups_a_cu(padded_dim(a.d));
   a.target = 2 * a.resident;
   a.chunk_min = kChunkMin;
-  a.ws_rows = slot_rows(a.tokens, group);
-  const int64_t tiles = tiles_bound(a.tokens, a.seqs, group);
+  a.ws_rows = slot_rows<P>(a.tokens, group);
+  const int64_t tiles = tiles_bound<P>(a.tokens, a.seqs, group);
   n.index = tiles;
   n.merges = 0;
-  n.workspace = workspace_bytes(a.tokens, a.seqs, a.hq, hk, a.d, a.max_keys);
+  n.workspace = workspace_bytes<P>(a.tokens, a.seqs, a.hq, hk, a.d, a.max_keys);
   a.slots = 0;
   if (n.workspace > 0) {
-    a.slots = static_cast<int>(slots_bound(a.tokens, a.seqs, group, hk, a.max_keys) / hk);
-    const int64_t most = tiles * ((a.max_keys + kChunkMin - 1) / kChunkMin - 1), aim = kTarget / hk + 1;
+    a.slots = static_cast<int>(slots_bound<P>(a.tokens, a.seqs, group, hk, a.max_keys) / hk);
+    const int64_t most = tiles * ((a.max_keys + kChunkMin - 1) / kChunkMin - 1), aim = P::kTarget / hk + 1;
     n.index += most < aim ? most : aim;
     const int64_t units = static_cast<int64_t>(a.tokens) * group, wanted = kMergeGrid / hk + 1;
     n.merges = units < wanted ? units : wanted;

@@ -152,6 +152,7 @@ __device__ __forceinline__ void join_waves(const Args& a, const Item& it, int kv
 }
 
 // Joins the partial sums of divided tiles (n.merges > 0). dtype: BP_DT_BF16 or BP_DT_F16.
+template <class P>
 int launch_merge(int dtype, const Args& a, const Launch& n, hipStream_t st);
 
 }  // namespace attn

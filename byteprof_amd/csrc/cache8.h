@@ -30,12 +30,15 @@ __device__ __forceinline__ float scale_value(uint32_t byte) {
   return __uint_as_float(byte == 255 ? 0x7fc00000u : byte == 0 ? 0x00400000u : byte << 23);
 }
 
-// Four codes times a scale as four values of T (two registers), exact but for values that T cannot hold.
+// Four codes times a scale as four values of T (two registers), exact but for values that T cannot hold; plain(): without the scale,
+// which a sum over keys then takes outside: that of a score's key (kPlainK), that of a probability's (kPlainV, where T has the
+// range). e4m3's conversion has it for nothing.
 template <int KIND, bool BF16>
 struct Codes;
 
 template <>
 struct Codes<kE4m3, true> {
+  static constexpr bool kPlainK = false, kPlainV = false;
   typedef float Scale;
   static __device__ __forceinline__ Scale scale(uint32_t byte) { return scale_field(byte); }
   static __device__ __forceinline__ u32x2 four(uint32_t w, Scale s) {
@@ -46,6 +49,7 @@ struct Codes<kE4m3, true> {
 
 template <>
 struct Codes<kE4m3, false> {
+  static constexpr bool kPlainK = false, kPlainV = false;
   // The conversion's own overflow does not saturate: it takes scales up to 2^7, which 448 stands, and a product the rest (scales
   // past 2^22 count as 2^22).
   struct Scale {
@@ -65,6 +69,7 @@ struct Codes<kE4m3, false> {
 
 template <>
 struct Codes<kInt8, true> {
+  static constexpr bool kPlainK = true, kPlainV = true;
   typedef float Scale;
   static __device__ __forceinline__ Scale scale(uint32_t byte) { return scale_value(byte); }
   static __device__ __forceinline__ u32x2 four(uint32_t w, Scale s) {
@@ -75,23 +80,47 @@ struct Codes<kInt8, true> {
     return u32x2{__builtin_amdgcn_perm(__float_as_uint(f[1]), __float_as_uint(f[0]), 0x07060302u),
                  __builtin_amdgcn_perm(__float_as_uint(f[3]), __float_as_uint(f[2]), 0x07060302u)};
   }
+  static __device__ __forceinline__ u32x2 plain(uint32_t w) { return u32x2{i8pair_to_bf16x2(w, 0), i8pair_to_bf16x2(w, 16)}; }
 };
 
 template <>
 struct Codes<kInt8, false> {
+  static constexpr bool kPlainK = true, kPlainV = false;
   typedef f16x2 Scale;
   static __device__ __forceinline__ Scale scale(uint32_t byte) {
     const _Float16 h = static_cast<_Float16>(scale_value(byte));
     return f16x2{h, h};
   }
-  static __device__ __forceinline__ u32x2 four(uint32_t w, Scale s) {
+  static __device__ __forceinline__ u32x2 plain(uint32_t w) {
     // a byte u under the exponent of 1024 is 1024 + u; u = code + 128
     const uint32_t u = w ^ 0x80808080u;
     const f16x2 bias = {static_cast<_Float16>(-1152.f), static_cast<_Float16>(-1152.f)};
-    const f16x2 lo = (__builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) + bias) * s;
-    const f16x2 hi = (__builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) + bias) * s;
+    const f16x2 lo = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) + bias;
+    const f16x2 hi = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) + bias;
     return u32x2{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
   }
+  static __device__ __forceinline__ u32x2 four(uint32_t w, Scale s) {
+    const u32x2 x = plain(w);
+    const uint32_t lo = x[0], hi = x[1];  // (a bit cast of a vector's element takes the vector's first)
+    return u32x2{__builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, lo) * s),
+                 __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, hi) * s)};
+  }
+};
+
+// What a factor outside the sum is, and four codes as the sum's operand with it (PLAIN) or without.
+template <class C, bool PLAIN>
+struct Outside {
+  typedef typename C::Scale Scale;
+  static __device__ __forceinline__ Scale scale(uint32_t byte) { return C::scale(byte); }
+  static __device__ __forceinline__ float times(float x, Scale) { return x; }
+  static __device__ __forceinline__ u32x2 four(uint32_t w, Scale s) { return C::four(w, s); }
+};
+template <class C>
+struct Outside<C, true> {
+  typedef float Scale;
+  static __device__ __forceinline__ Scale scale(uint32_t byte) { return scale_value(byte); }
+  static __device__ __forceinline__ float times(float x, Scale s) { return x * s; }
+  static __device__ __forceinline__ u32x2 four(uint32_t w, Scale) { return C::plain(w); }
 };
 
 // Eight codes as eight values.
