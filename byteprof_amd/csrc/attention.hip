@@ -529,7 +529,9 @@ int launch_merge(int dtype, const Args& a, const Launch& n, hipStream_t st) {
   return e == hipSuccess ? BP_OK : static_cast<int>(e);
 }
 template int launch_merge<Tiles32>(int, const Args&, const Launch&, hipStream_t);
-template int launch_merge<Tiles16>(int, const Args&, const Launch&, hipStream_t);
+template int launch_merge<FewTiles<1>>(int, const Args&, const Launch&, hipStream_t);
+template int launch_merge<FewTiles<2>>(int, const Args&, const Launch&, hipStream_t);
+template int launch_merge<FewTiles<3>>(int, const Args&, const Launch&, hipStream_t);
 
 }  // namespace attn
 }  // namespace bp

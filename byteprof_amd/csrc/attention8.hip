@@ -107,137 +107,346 @@ __device__ __forceinline__ u32x4 codes16(const Args8& a, const uint8_t* row, int
   return r;
 }
 
-// Place of 16-code chunk `chunk` of a row in a wave's image of 32 value rows: turned, so that 8 rows written and the 8 rows that
-// a transposed read takes (4 and 4, 8 apart) lie in different banks.
-template <int DP>
-__device__ __forceinline__ int place8(int row, int chunk) {
-  constexpr int CH = DP / 16;
-  const int turn = (row & 7) ^ ((row >> 3 & 1) << 2);
-  if constexpr (CH == 4) return row * CH + (chunk ^ ((row >> 2 & 1) | (row >> 2 & 2)));
-  else if constexpr (CH == 8) return row * CH + (chunk ^ turn);
-  else if constexpr (CH == 16) return row * CH + (chunk ^ 2 * turn);
-  else return row * CH + chunk;
-}
-
-template <int DP>
-struct Shape8 {
-  static constexpr int BN = DP <= 128 ? 64 : 32;  // keys of a step of a large tile
-  static constexpr int kLarge = 4 * BN * DP / 8;  // 16-byte chunks: two images of keys and two of values, as values
-  static constexpr int kSmall = kWaves * 32 * DP / 16;  // a wave's value codes
-  static constexpr int G = DP / 32 < 4 ? DP / 32 : 4;
-  static constexpr int kMerge = kWaves * G * 8 * 32;
-  static constexpr int kChunks = kLarge > kSmall ? (kLarge > kMerge ? kLarge : kMerge) : (kSmall > kMerge ? kSmall : kMerge);
+// How few rows a tile has: 16 RB of them, for launches whose sequences have no more (RB: 1, 2 or 3), and RB = 2 for the small
+// sequences beside large ones.
+template <int DP, int RB>
+struct Few {
+  static constexpr int kImages = kWaves * 2 * 32 * DP / 16;        // a wave's keys and values of a step, 16-byte chunks
+  static constexpr int kMost = RB == 1 ? 128 : RB == 2 ? 64 : 32;  // columns of a round of the waves' join: 32 KB at most
+  static constexpr int G = DP < kMost ? DP : kMost;
+  static constexpr int kJoin = kWaves * 16 * RB * G / 4;
+  // The queries of 48 rows are operands in LDS, 64 lanes' 16 bytes each, behind the images: beside the sums there are no registers
+  // for them, and what the compiler then puts aside is fetched behind the loads that are out (a verify round of six sequences, fp16
+  // over int8, 38.6 us in place of XX).
+  static constexpr bool kQueries = RB > 2;
+  static constexpr int kAhead = kImages + (kQueries ? RB * DP / 32 * kWave : 0);
+  static constexpr int kChunks = kAhead > kJoin ? kAhead : kJoin;
+  static constexpr int kStats = 16 * RB * (2 * kWaves + 1);
 };
 
-// O^T += V^T P^T over 32 keys whose codes lie in a wave's image; scale: the lane's key's.
-template <class T, class C, int DP>
-__device__ __forceinline__ void weighted8(const u32x4* img, int scale, const u32x4 (&p)[2], f32x16 (&o)[DP / 32], int lane) {
-  typedef int i32x2 __attribute__((ext_vector_type(2)));
-  typedef __attribute__((address_space(3))) i32x2* lds2;
-  const int half = lane >> 5, sub = (lane >> 4) & 1, j = (lane & 15) >> 1, e = lane & 1;
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    // a scale holds for aligned groups of 4 keys at least
-    const typename C::Scale s0 = C::scale(__shfl(scale, 16 * t + 4 * half)), s1 = C::scale(__shfl(scale, 16 * t + 8 + 4 * half));
-    const int key = 16 * t + 8 * (j >> 2) + 4 * half + (j & 3);
-#pragma unroll
-    for (int db = 0; db < DP / 32; ++db) {
-      // a 16-lane group reads 8 keys x 16 columns, 8 columns a lane, and gets them transposed: its column's 8 keys
-      const char* at = reinterpret_cast<const char*>(img + place8<DP>(key, 2 * db + sub)) + 8 * e;
-      const i32x2 r = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds2)(__attribute__((address_space(3))) void*)at);
-      const u32x2 x = C::four(r[0], s0), y = C::four(r[1], s1);
-      o[db] = T::mfma(u32x4{x[0], x[1], y[0], y[1]}, p[t], o[db]);
-    }
-  }
+__device__ __forceinline__ f32x4 mfma16(Bf16, u32x4 a, u32x4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma16(F16, u32x4 a, u32x4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-// Up to 32 rows: every wave has all rows and takes every fourth block of 32 keys; then the waves' parts are joined. Keys go from
-// memory to registers, 16 codes a lane of the lane's own key, and become the first product's operand there (its order of the
-// columns is the queries', too); values go through an image in LDS, which is read transposed. A block's loads are sent as soon as
-// the last block's registers are free.
-template <class T, class C, int DP, bool FULL>
-__device__ __forceinline__ void small_tile8(const Args8& a, const Item& it, int kvh, u32x4* smem, float* stats) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
+// Place of 16-code chunk `chunk` of a row in a wave's image of 32 rows: 8 rows written, and the 16 rows that two 16-lane groups
+// read transposed (4 and 4, 16 apart, of either), lie in different banks.
+template <int DP>
+__device__ __forceinline__ int place16(int row, int chunk) {
+  constexpr int CH = DP / 16;
+  const int high = row >> 4 & 1;
+  if constexpr (CH == 4) return row * CH + (chunk ^ ((row >> 2 & 1) | high << 1));
+  else if constexpr (CH == 8) return row * CH + (chunk ^ ((row >> 1 & 3) | high << 2));
+  else return row * CH + (chunk ^ ((row & 7) | high << 3));
+}
+
+// 16 RB rows; every wave has all of them and takes every fourth block of 32 keys, then the waves' parts are joined. A lane has rows
+// lane % 16 of each 16: of 16 keys' scores (S^T = K Q^T, 16 x 16) four, keys 4 (lane / 16) + 0..3; those of 32 keys are the operand
+// of O^T = V^T P^T where they lie, whose values come transposed from LDS in the same order of the keys. Codes become operands
+// once for all rows.
+template <class T, class C, int DP, bool FULL, int RB>
+__device__ __forceinline__ void few_rows(const Args8& a, const Item& it, int kvh, u32x4* smem, float* stats) {
+  using S = Few<DP, RB>;
+  using K = cache8::Outside<C, C::kPlainK>;
+  using V = cache8::Outside<C, C::kPlainV>;
+  constexpr int NC = DP / 64, STEP = 32 * kWaves;
+  // Rows of codes go from memory to registers as they lie, a row's 16-byte chunks on neighbouring lanes, a step ahead; through LDS
+  // they become operands. (Keys straight in their operand's layout, a row to a lane: every lane then asks for a line of its own, and
+  // the address unit is busy half of the time.)
+  constexpr int CH = DP / 16, RPI = kWave / CH, N = 32 / RPI, M = 16 / RPI;  // rows of a load, loads of a step and of 16 keys
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), row = lane & 15, g = lane >> 4;
   const int top = it.row0 + it.rows - 1;
-  const int mine = min(it.row0 + (lane & 31), top);
-  u32x4 q[DP / 16];
-  {
-    const int n = a.group(mine);
+  u32x4 q[S::kQueries ? 1 : RB][2 * NC];
+  u32x4* queries = smem + S::kImages;
+  int limit[RB];
+#pragma unroll
+  for (int x = 0; x < RB; ++x) {
+    const int mine = min(it.row0 + 16 * x + row, top), n = a.group(mine);
+    limit[x] = min(it.first + n, it.keys - 1);
+    if (S::kQueries && wave != x) continue;
     const uint16_t* p = static_cast<const uint16_t*>(a.q) + static_cast<int64_t>(it.begin + n) * a.q_t +
                         static_cast<int64_t>(kvh * a.group.d + mine - n * a.group.d) * a.q_h;
 #pragma unroll
-    for (int i = 0; i < DP / 16; ++i) {
-      const int col = 32 * (i / 2) + 16 * half + 8 * (i % 2);
-      q[i] = FULL || col < a.d ? *reinterpret_cast<const u32x4*>(p + col) : u32x4{};
+    for (int i = 0; i < 2 * NC; ++i) {
+      const int col = 64 * (i / 2) + 16 * g + 8 * (i % 2);
+      const u32x4 y = FULL || col < a.d ? *reinterpret_cast<const u32x4*>(p + col) : u32x4{};
+      if constexpr (S::kQueries) queries[(x * 2 * NC + i) * kWave + lane] = y;
+      else q[x][i] = y;
     }
   }
-  const int limit = min(it.first + a.group(mine), it.keys - 1);
-  const int least = __builtin_amdgcn_readfirstlane(limit);
-  Running<DP> r;
-  r.clear();
+  const auto query = [&](int x, int i) {
+    if constexpr (S::kQueries) return queries[(x * 2 * NC + i) * kWave + lane];
+    else return q[x][i];
+  };
+  const int least = __builtin_amdgcn_readfirstlane(limit[0]);
+  const float c = a.scale_log2;
+  f32x4 o[RB][DP / 16];
+  float m[RB], l[RB];
+#pragma unroll
+  for (int x = 0; x < RB; ++x) {
+    m[x] = -INFINITY;
+    l[x] = 0.f;
+#pragma unroll
+    for (int d = 0; d < DP / 16; ++d) o[x][d] = f32x4{};
+  }
   Cache cache(a, it, kvh);
-  u32x4* img = smem + wave * 32 * (DP / 16);
-  constexpr int STEP = 32 * kWaves;
-  const int sub = lane & 31;
-  int key = it.key0 + 32 * wave;
-  // Two blocks ahead: every load is sent, past the item's keys from its last row over again (with a branch around them the
-  // compiler would wait for all loads that are out).
-  struct Block {
-    u32x4 k[DP / 32], v[DP / 32];
-    int ks, vs, id;
-  } even, odd;
-  const auto load = [&](Block& x, int at) {
-    int64_t ko, vo, kso, vso;
-    cache.at(a, at, x.id, ko, vo, kso, vso);
-    x.ks = cache.ks[kso];
+  u32x4* kimg = smem + wave * 2 * 32 * CH;
+  u32x4* vimg = kimg + 32 * CH;
+  const int lr = lane / CH, lc = lane % CH;
+  u32x4 kc[N], vc[N];
+  int ks[2], vs[2], id[2];
+  const uint32_t k_t = static_cast<uint32_t>(a.k_t);
+  const auto part_of = [&](int r) { return static_cast<uint32_t>(a.block(r)) * static_cast<uint32_t>(a.ks_b); };
+  const int k_key = C::kPlainK ? 4 * g : row;  // the first product's operand is of key `row` of 16, its result of 4 g + 0..3
+  const uint32_t at_lane = lr * k_t + 16 * lc, ks_lane = FULL ? part_of(k_key) : 0, vs_lane = FULL ? part_of(4 * g) : 0;
+  // Every load is sent, past the item's keys from its last ones over again. Scales: of key k_key of 16, and of keys 4 g + 0..3 (the
+  // second product's operand); not FULL: of key lane % 32, to be fetched from there.
+  const auto load = [&](int at) {
+    if constexpr (FULL) {
 #pragma unroll
-    for (int c = 0; c < DP / 32; ++c) x.k[c] = codes16<FULL>(a, cache.k + ko, 2 * c + half);
-    x.vs = cache.vs[vso];
+      for (int b = 0; b < 2; ++b) {
+        const Sixteen x(a, cache, at + 16 * b, id[b]);
+        if (x.rest >= 15) {
+          ks[b] = x.ks[ks_lane];
+          vs[b] = x.vs[vs_lane];
 #pragma unroll
-    for (int c = 0; c < DP / 32; ++c) x.v[c] = codes16<FULL>(a, cache.v + vo, 2 * c + half);
-    x.id = cache.id(a, at + 2 * STEP);
+          for (int j = 0; j < M; ++j) kc[b * M + j] = *reinterpret_cast<const u32x4*>(x.k + j * RPI * k_t + at_lane);
+#pragma unroll
+          for (int j = 0; j < M; ++j) vc[b * M + j] = *reinterpret_cast<const u32x4*>(x.v + j * RPI * k_t + at_lane);
+        } else {
+          ks[b] = x.ks[part_of(min(k_key, x.rest))];
+          vs[b] = x.vs[part_of(min(4 * g, x.rest))];
+#pragma unroll
+          for (int j = 0; j < M; ++j) {
+            const uint32_t off = min(j * RPI + lr, x.rest) * k_t + 16 * lc;
+            kc[b * M + j] = *reinterpret_cast<const u32x4*>(x.k + off);
+            vc[b * M + j] = *reinterpret_cast<const u32x4*>(x.v + off);
+          }
+        }
+        id[b] = cache.id(a, at + STEP + 16 * b);
+      }
+    } else {
+      int64_t ko, vo, kso, vso;
+      cache.at(a, at + lane % 32, id[0], ko, vo, kso, vso);
+      ks[0] = cache.ks[kso];
+      vs[0] = cache.vs[vso];
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        kc[j] = codes16<false>(a, cache.k + __shfl(ko, j * RPI + lr), lc);
+        vc[j] = codes16<false>(a, cache.v + __shfl(vo, j * RPI + lr), lc);
+      }
+      id[0] = cache.id(a, at + STEP + lane % 32);
+    }
   };
-  const auto step = [&](Block& x, int at) {
-    f32x16 s[1] = {};
-    const typename C::Scale kscale = C::scale(x.ks);
+  int key = it.key0 + 32 * wave;
+  if (key < it.key1) {
+    id[0] = cache.id(a, FULL ? key : key + lane % 32);
+    if constexpr (FULL) id[1] = cache.id(a, key + 16);
+    load(key);
+  }
+  if constexpr (S::kQueries) __syncthreads();
+  for (; key < it.key1; key += STEP) {
 #pragma unroll
-    for (int c = 0; c < DP / 32; ++c) {
-      s[0] = T::mfma(cache8::eight<C>(x.k[c][0], x.k[c][1], kscale), q[2 * c], s[0]);
-      s[0] = T::mfma(cache8::eight<C>(x.k[c][2], x.k[c][3], kscale), q[2 * c + 1], s[0]);
+    for (int j = 0; j < N; ++j) kimg[place16<DP>(j * RPI + lr, lc)] = kc[j];
+#pragma unroll
+    for (int j = 0; j < N; ++j) vimg[place16<DP>(j * RPI + lr, lc)] = vc[j];
+    typename K::Scale k_scale[2];
+    typename V::Scale v_scale[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      k_scale[b] = K::scale(FULL ? ks[b] : __shfl(ks[0], 16 * b + k_key));
+      v_scale[b] = V::scale(FULL ? vs[b] : __shfl(vs[0], 16 * b + 4 * g));
+    }
+    load(key + STEP);
+    f32x4 s[RB][2];
+#pragma unroll
+    for (int x = 0; x < RB; ++x) s[x][0] = s[x][1] = f32x4{};
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      u32x4 k[2][2];
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const u32x4 w = kimg[place16<DP>(16 * b + row, 4 * i + g)];
+        k[b][0] = cache8::eight<K>(w[0], w[1], k_scale[b]);
+        k[b][1] = cache8::eight<K>(w[2], w[3], k_scale[b]);
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int x = 0; x < RB; ++x) {
+          const u32x4 y = query(x, 2 * i + h);
+#pragma unroll
+          for (int b = 0; b < 2; ++b) s[x][b] = mfma16(T(), k[b][h], y, s[x][b]);
+        }
     }
 #pragma unroll
-    for (int c = 0; c < DP / 32; ++c) img[place8<DP>(sub, 2 * c + half)] = x.v[c];
-    const int vs = x.vs;
-    load(x, at + 2 * STEP + sub);
-    u32x4 p[1][2];
-    softmax_step<T, DP, 1>(s, p, r, a.scale_log2, at, min(limit, cache.last), at + 31 > min(least, cache.last), lane);
-    weighted8<T, C, DP>(img, vs, p[0], r.o, lane);
-  };
-  if (key < it.key1) {
-    even.id = cache.id(a, key + sub);
-    odd.id = cache.id(a, key + STEP + sub);
-    load(even, key + sub);
-    load(odd, key + STEP + sub);
-    while (true) {
-      step(even, key);
-      key += STEP;
-      if (key >= it.key1) break;
-      step(odd, key);
-      key += STEP;
-      if (key >= it.key1) break;
+    for (int x = 0; x < RB; ++x)
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[x][b][i] = K::times(s[x][b][i], k_scale[b]);
+    if (key + 31 > min(least, cache.last)) {
+#pragma unroll
+      for (int x = 0; x < RB; ++x)
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (key + 16 * b + 4 * g + i > min(limit[x], cache.last)) s[x][b][i] = -INFINITY;
+    }
+    u32x4 p[RB];
+#pragma unroll
+    for (int x = 0; x < RB; ++x) {
+      float mx = s[x][0][0];
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[x][b][i]);
+      mx = fmaxf(m[x], xor_stage<32>(xor_stage<16>(mx, MaxOp()), MaxOp()));
+      if (__any(mx > m[x])) {
+        const float f = rescaled(m[x], mx, c);
+        m[x] = mx;
+        l[x] *= f;
+#pragma unroll
+        for (int d = 0; d < DP / 16; ++d)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[x][d][i] *= f;
+      }
+      // as in softmax_step: far from zero the difference is taken first
+      float shift = m[x] == -INFINITY ? 0.f : -(m[x] * c);
+      if (__any(!(fabsf(shift) < kFar))) {
+        const float less = fabsf(shift) < kFar ? 0.f : m[x];
+        shift = fabsf(shift) < kFar ? shift : 0.f;
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[x][b][i] -= less;
+      }
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          s[x][b][i] = __builtin_amdgcn_exp2f(fmaf(s[x][b][i], c, shift));
+          l[x] += s[x][b][i];
+        }
+        const auto weight = [&](int i) { return V::times(s[x][b][i], v_scale[b]); };
+        p[x][2 * b] = T::pack(weight(0), weight(1));
+        p[x][2 * b + 1] = T::pack(weight(2), weight(3));
+      }
+    }
+    typedef int i32x2 __attribute__((ext_vector_type(2)));
+    typedef __attribute__((address_space(3))) i32x2* lds2;
+    const int j = row >> 1, from = 16 * (j >> 2) + 4 * g + (j & 3);
+#pragma unroll
+    for (int d = 0; d < DP / 16; ++d) {
+      // a 16-lane group reads 8 keys x 16 columns, 8 columns a lane, and gets them transposed: its column's 8 keys
+      const char* at = reinterpret_cast<const char*>(vimg + place16<DP>(from, d)) + 8 * (row & 1);
+      const i32x2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds2)(__attribute__((address_space(3))) void*)at);
+      const u32x2 v0 = V::four(w[0], v_scale[0]), v1 = V::four(w[1], v_scale[1]);
+#pragma unroll
+      for (int x = 0; x < RB; ++x) o[x][d] = mfma16(T(), u32x4{v0[0], v0[1], v1[0], v1[1]}, p[x], o[x][d]);
     }
   }
-  if (__any(cache.bad)) r.l = NAN;
-  join_waves<T, DP, Shape8<DP>::G>(a, it, kvh, r, smem, stats);
+  const bool bad = __any(cache.bad);
+  // The waves' parts are joined. stats: [wave][rows] maxima, [wave][rows] sums, [rows] factors of the result.
+  constexpr int R = 16 * RB;
+#pragma unroll
+  for (int x = 0; x < RB; ++x) {
+    l[x] = bad ? NAN : xor_stage<32>(xor_stage<16>(l[x], AddOp()), AddOp());
+    if (lane < 16) {
+      stats[R * wave + 16 * x + lane] = m[x];
+      stats[R * (kWaves + wave) + 16 * x + lane] = l[x];
+    }
+  }
+  __syncthreads();
+  const bool whole = !it.divided, keep = whole || it.slot + it.split < a.slots;
+  const int wd = a.d <= 64 ? 64 : a.d <= 96 ? 96 : DP;  // columns of a slot
+  float* ws = whole ? nullptr : a.ws + (static_cast<int64_t>(it.slot + it.split) * a.hk.d + kvh) * a.ws_rows * (wd + 2);
+  float f[RB];
+#pragma unroll
+  for (int x = 0; x < RB; ++x) {
+    float all_m = -INFINITY, all_l = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) all_m = fmaxf(all_m, stats[R * w + 16 * x + row]);
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w)
+      all_l += stats[R * (kWaves + w) + 16 * x + row] * rescaled(stats[R * w + 16 * x + row], all_m, c);
+    f[x] = rescaled(m[x], all_m, c);
+    if (wave == 0 && lane < 16) {
+      stats[R * 2 * kWaves + 16 * x + lane] = whole ? inverse(all_l) : 1.f;
+      if (!whole && keep && 16 * x + lane < it.rows) {
+        ws[a.ws_rows * wd + 16 * x + lane] = all_m;
+        ws[a.ws_rows * (wd + 1) + 16 * x + lane] = all_l;
+      }
+    }
+  }
+  f32x4* parts = reinterpret_cast<f32x4*>(smem);  // [wave][4 columns][rows]
+  constexpr int G = S::G;
+#pragma unroll
+  for (int r = 0; r < DP / G; ++r) {
+#pragma unroll
+    for (int x = 0; x < RB; ++x) {
+      if (16 * x + row < it.rows) {
+#pragma unroll
+        for (int d = 0; d < G / 16; ++d) {
+          const f32x4 y = o[x][r * (G / 16) + d];
+          parts[(wave * (G / 4) + 4 * d + g) * R + 16 * x + row] = f32x4{y[0] * f[x], y[1] * f[x], y[2] * f[x], y[3] * f[x]};
+        }
+      }
+    }
+    __syncthreads();
+    for (int i = tid; i < it.rows * (G / 4); i += kThreads) {
+      const int rw = i / (G / 4), piece = i % (G / 4), col = 4 * piece + r * G;
+      f32x4 y = parts[piece * R + rw];
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) y += parts[(w * (G / 4) + piece) * R + rw];
+      if (whole) {
+        const float inv = stats[R * 2 * kWaves + rw];
+        if (col < a.d)
+          *reinterpret_cast<u32x2*>(out_row(a, it, kvh, it.row0 + rw) + col) =
+              u32x2{T::pack(y[0] * inv, y[1] * inv), T::pack(y[2] * inv, y[3] * inv)};
+      } else if (keep && col < wd) {
+        *reinterpret_cast<f32x4*>(ws + rw * wd + col) = y;
+      }
+    }
+    if (r + 1 < DP / G) __syncthreads();
+  }
 }
 
-// 128 rows, 32 a wave; the keys in steps of BN that all waves share. The workgroup turns a step's codes into values once, in
-// registers, and writes them to the images that the 16-bit kernel's tiles have (two of each in turn); their loads are sent a step
-// before.
+// Launches of few rows a sequence.
+template <class T, class C, int DP, bool FULL, int RB>
+__global__ __launch_bounds__(kThreads, FewTiles<RB>::workgroups_a_cu(DP)) void attention8_few_kernel(Args8 a) {
+  __shared__ __align__(16) u32x4 smem[Few<DP, RB>::kChunks];
+  __shared__ float stats[Few<DP, RB>::kStats];
+  if constexpr (std::is_same<T, F16>::value) cache8::saturate_f16();
+  // Workgroup b runs on XCD b % 8: a part's key heads, whose rows lie side by side, go to one XCD. (With a head to an XCD, as
+  // b % hk deals them where hk is 8 or 16, an XCD asks for every eighth 128 bytes only, and those are in 2 of the 16 channels of
+  // its L2: a decode batch of 64 sequences took 149 us in place of 137.)
+  const int place = blockIdx.x / kXcds, part = a.hk(place), kvh = place - part * a.hk.d;
+  const int index = part * kXcds + blockIdx.x % kXcds;
+  const Item it = find_item<false, FewTiles<RB>>(a, index);
+  if (it.b < 0) {
+    fill_rest(a, kvh, it.extra, a.hk(gridDim.x) - (index - it.extra));
+    return;
+  }
+  if (it.key0 >= it.key1 && it.split > 0) return;
+  few_rows<T, C, DP, FULL, RB>(a, it, kvh, smem, stats);
+}
+
+// A large tile's steps: BN keys, whose codes the workgroup turns into values once, in registers, and writes to the images that the
+// 16-bit kernel's tiles have (two of keys and two of values in turn).
+template <int DP>
+struct Large {
+  static constexpr int BN = DP <= 128 ? 64 : 32;
+  static constexpr int kImages = 4 * BN * DP / 8;
+};
+
+// 128 rows, 32 a wave; the keys in steps of BN that all waves share; a step's loads are sent a step before it is turned.
 template <class T, class C, int DP, bool FULL>
 __device__ __forceinline__ void large_tile8(const Args8& a, const Item& it, int kvh, u32x4* smem) {
-  using S = Shape8<DP>;
-  constexpr int BN = S::BN, NB = BN / 32, CH = DP / 16, IMG = BN * DP / 8;
+  constexpr int BN = Large<DP>::BN, NB = BN / 32, CH = DP / 16, IMG = BN * DP / 8;
   constexpr int N = (BN * CH + kThreads - 1) / kThreads;  // 16-code pieces of a thread
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int top = it.row0 + it.rows - 1;
@@ -254,22 +463,38 @@ __device__ __forceinline__ void large_tile8(const Args8& a, const Item& it, int 
   u32x4 kc[N], vc[N];
   int ks[N], vs[N], next[N];
   const auto mine_of = [&](int n) { return BN * CH % kThreads == 0 || tid + n * kThreads < BN * CH; };
+  // FULL: a wave's piece is rows of one 16-key block, its first at `first_row`.
+  constexpr int RPI = kWave / CH;
+  const auto first_row = [&](int n) { return RPI * (wave + kWaves * n); };
+  const uint32_t k_t = static_cast<uint32_t>(a.k_t);
   const auto look = [&](int key) {
 #pragma unroll
-    for (int n = 0; n < N; ++n)
-      if (mine_of(n)) next[n] = cache.id(a, key + (tid + n * kThreads) / CH);
+    for (int n = 0; n < N; ++n) {
+      if constexpr (FULL) next[n] = cache.id(a, key + (first_row(n) & ~15));
+      else if (mine_of(n)) next[n] = cache.id(a, key + (tid + n * kThreads) / CH);
+    }
   };
   const auto load = [&](int key) {
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-      if (!mine_of(n)) continue;
-      const int i = tid + n * kThreads;
-      int64_t ko, vo, kso, vso;
-      cache.at(a, key + i / CH, next[n], ko, vo, kso, vso);
-      ks[n] = cache.ks[kso];
-      vs[n] = cache.vs[vso];
-      kc[n] = codes16<FULL>(a, cache.k + ko, i % CH);
-      vc[n] = codes16<FULL>(a, cache.v + vo, i % CH);
+      if constexpr (FULL) {
+        const Sixteen x(a, cache, key + (first_row(n) & ~15), next[n]);
+        const int r = min((first_row(n) & 15) + lane / CH, x.rest);
+        const uint32_t off = r * k_t + 16 * (lane % CH), part = static_cast<uint32_t>(a.block(r)) * static_cast<uint32_t>(a.ks_b);
+        ks[n] = x.ks[part];
+        vs[n] = x.vs[part];
+        kc[n] = *reinterpret_cast<const u32x4*>(x.k + off);
+        vc[n] = *reinterpret_cast<const u32x4*>(x.v + off);
+      } else {
+        if (!mine_of(n)) continue;
+        const int i = tid + n * kThreads;
+        int64_t ko, vo, kso, vso;
+        cache.at(a, key + i / CH, next[n], ko, vo, kso, vso);
+        ks[n] = cache.ks[kso];
+        vs[n] = cache.vs[vso];
+        kc[n] = codes16<false>(a, cache.k + ko, i % CH);
+        vc[n] = codes16<false>(a, cache.v + vo, i % CH);
+      }
     }
   };
   const auto turn = [&](int to) {
@@ -327,281 +552,12 @@ __device__ __forceinline__ void large_tile8(const Args8& a, const Item& it, int 
   if (active) write_rows<T, DP>(a, it, kvh, row, r, lane);
 }
 
-// Launches of few rows a sequence (decode steps): tiles of 16 rows. Half the softmax and matrix work of a 32-row tile for each key,
-// and so few registers that four workgroups are on a CU (256 columns: two), whose loads are what fills the memory's queue.
-
-__device__ __forceinline__ f32x4 mfma16(Bf16, u32x4 a, u32x4 b, f32x4 c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
-__device__ __forceinline__ f32x4 mfma16(F16, u32x4 a, u32x4 b, f32x4 c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-}
-
-// Place of 16-code chunk `chunk` of a row in a wave's image of 32 value rows: 8 rows written, and the 16 rows that two 16-lane groups
-// read transposed (4 and 4, 16 apart, of either), lie in different banks.
-template <int DP>
-__device__ __forceinline__ int place16(int row, int chunk) {
-  constexpr int CH = DP / 16;
-  const int high = row >> 4 & 1;
-  if constexpr (CH == 4) return row * CH + (chunk ^ ((row >> 2 & 1) | high << 1));
-  else if constexpr (CH == 8) return row * CH + (chunk ^ ((row >> 1 & 3) | high << 2));
-  else return row * CH + (chunk ^ ((row & 7) | high << 3));
-}
-
-template <int DP>
-struct Shape16 {
-  static constexpr int NB = 2;                                    // 16-key blocks of a wave's step
-  static constexpr int kImages = kWaves * 2 * 16 * NB * DP / 16;  // a wave's keys and values
-  static constexpr int G = DP < 128 ? DP : 128;              // columns of a round of the waves' join
-  static constexpr int kJoin = kWaves * 16 * G / 4;
-  static constexpr int kChunks = kImages > kJoin ? kImages : kJoin;
-};
-
-// A lane has row lane % 16: of 16 keys' scores (S^T = K Q^T, 16 x 16) four, keys 4 (lane / 16) + 0..3; those of 32 keys are the
-// operand of O^T = V^T P^T where they lie, whose values come transposed from LDS in the same order of the keys.
-template <class T, class C, int DP, bool FULL>
-__global__ __launch_bounds__(kThreads, DP > 128 ? 2 : DP > 64 ? 3 : 4) void attention8_few_kernel(Args8 a) {
-  constexpr int NC = DP / 64, NB = Shape16<DP>::NB, KEYS = 16 * NB, STEP = KEYS * kWaves;
-  __shared__ __align__(16) u32x4 smem[Shape16<DP>::kChunks];
-  __shared__ float stats[16 * (2 * kWaves + 1)];
-  if constexpr (std::is_same<T, F16>::value) cache8::saturate_f16();
-  // Workgroup b runs on XCD b % 8: a part's key heads, whose rows lie side by side, go to one XCD.
-  const int place = blockIdx.x / kXcds, part = a.hk(place), kvh = place - part * a.hk.d;
-  const int index = part * kXcds + blockIdx.x % kXcds;
-  const Item it = find_item<false, Tiles16>(a, index);
-  if (it.b < 0) {
-    fill_rest(a, kvh, it.extra, a.hk(gridDim.x) - (index - it.extra));
-    return;
-  }
-  if (it.key0 >= it.key1 && it.split > 0) return;
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), row = lane & 15, g = lane >> 4;
-  const int top = it.row0 + it.rows - 1, mine = min(it.row0 + row, top);
-  u32x4 q[2 * NC];
-  {
-    const int n = a.group(mine);
-    const uint16_t* p = static_cast<const uint16_t*>(a.q) + static_cast<int64_t>(it.begin + n) * a.q_t +
-                        static_cast<int64_t>(kvh * a.group.d + mine - n * a.group.d) * a.q_h;
-#pragma unroll
-    for (int i = 0; i < 2 * NC; ++i) {
-      const int col = 64 * (i / 2) + 16 * g + 8 * (i % 2);
-      q[i] = FULL || col < a.d ? *reinterpret_cast<const u32x4*>(p + col) : u32x4{};
-    }
-  }
-  const int limit = min(it.first + a.group(mine), it.keys - 1);
-  const int least = __builtin_amdgcn_readfirstlane(limit);
-  const float c = a.scale_log2;
-  f32x4 o[DP / 16];
-#pragma unroll
-  for (int d = 0; d < DP / 16; ++d) o[d] = f32x4{};
-  float m = -INFINITY, l = 0.f;
-  Cache cache(a, it, kvh);
-  // Rows of codes go from memory to registers as they lie, a row's 16-byte chunks on neighbouring lanes, a step ahead; through LDS
-  // they become operands. (Keys straight in their operand's layout, a row to a lane: every lane then asks for a line of its own, and
-  // the address unit is busy half of the time.)
-  constexpr int CH = DP / 16, RPI = kWave / CH, N = KEYS / RPI, M = 16 / RPI;  // rows of a load, loads of a step and of 16 keys
-  u32x4* kimg = smem + wave * 2 * KEYS * CH;
-  u32x4* vimg = kimg + KEYS * CH;
-  const int lr = lane / CH, lc = lane % CH;
-  u32x4 kc[N], vc[N];
-  int ks[NB], vs[NB], id[NB];
-  const uint32_t k_t = static_cast<uint32_t>(a.k_t);
-  const auto part_of = [&](int r) { return static_cast<uint32_t>(a.block(r)) * static_cast<uint32_t>(a.ks_b); };
-  const int k_key = C::kPlainK ? 4 * g : row;  // the first product's operand is of key `row` of 16, its result of 4 g + 0..3
-  const uint32_t at_lane = lr * k_t + 16 * lc, ks_lane = FULL ? part_of(k_key) : 0, vs_lane = FULL ? part_of(4 * g) : 0;
-  // Every load is sent, past the item's keys from its last ones over again. Scales: of key k_key of 16, and of keys 4 g + 0..3 (the
-  // second product's operand); not FULL: of key lane % 32, to be fetched from there.
-  const auto load = [&](int at) {
-    if constexpr (FULL) {
-#pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        const Sixteen x(a, cache, at + 16 * b, id[b]);
-        if (x.rest >= 15) {
-          ks[b] = x.ks[ks_lane];
-          vs[b] = x.vs[vs_lane];
-#pragma unroll
-          for (int j = 0; j < M; ++j) kc[b * M + j] = *reinterpret_cast<const u32x4*>(x.k + j * RPI * k_t + at_lane);
-#pragma unroll
-          for (int j = 0; j < M; ++j) vc[b * M + j] = *reinterpret_cast<const u32x4*>(x.v + j * RPI * k_t + at_lane);
-        } else {
-          ks[b] = x.ks[part_of(min(k_key, x.rest))];
-          vs[b] = x.vs[part_of(min(4 * g, x.rest))];
-#pragma unroll
-          for (int j = 0; j < M; ++j) {
-            const uint32_t off = min(j * RPI + lr, x.rest) * k_t + 16 * lc;
-            kc[b * M + j] = *reinterpret_cast<const u32x4*>(x.k + off);
-            vc[b * M + j] = *reinterpret_cast<const u32x4*>(x.v + off);
-          }
-        }
-        id[b] = cache.id(a, at + STEP + 16 * b);
-      }
-    } else {
-      int64_t ko, vo, kso, vso;
-      cache.at(a, at + lane % KEYS, id[0], ko, vo, kso, vso);
-      ks[0] = cache.ks[kso];
-      vs[0] = cache.vs[vso];
-#pragma unroll
-      for (int j = 0; j < N; ++j) {
-        kc[j] = codes16<false>(a, cache.k + __shfl(ko, j * RPI + lr), lc);
-        vc[j] = codes16<false>(a, cache.v + __shfl(vo, j * RPI + lr), lc);
-      }
-      id[0] = cache.id(a, at + STEP + lane % KEYS);
-    }
-  };
-  int key = it.key0 + KEYS * wave;
-  if (key < it.key1) {
-    if constexpr (FULL) {
-#pragma unroll
-      for (int b = 0; b < NB; ++b) id[b] = cache.id(a, key + 16 * b);
-    } else {
-      id[0] = cache.id(a, key + lane % KEYS);
-    }
-    load(key);
-  }
-  for (; key < it.key1; key += STEP) {
-#pragma unroll
-    for (int j = 0; j < N; ++j) kimg[place16<DP>(j * RPI + lr, lc)] = kc[j];
-#pragma unroll
-    for (int j = 0; j < N; ++j) vimg[place16<DP>(j * RPI + lr, lc)] = vc[j];
-    using K = cache8::Outside<C, C::kPlainK>;
-    using V = cache8::Outside<C, C::kPlainV>;
-    typename K::Scale k_scale[NB];
-    typename V::Scale v_scale[NB];
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      k_scale[b] = K::scale(FULL ? ks[b] : __shfl(ks[0], 16 * b + k_key));
-      v_scale[b] = V::scale(FULL ? vs[b] : __shfl(vs[0], 16 * b + 4 * g));
-    }
-    load(key + STEP);
-    f32x4 s[NB];
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      s[b] = f32x4{};
-#pragma unroll
-      for (int i = 0; i < NC; ++i) {
-        const u32x4 w = kimg[place16<DP>(16 * b + row, 4 * i + g)];
-        s[b] = mfma16(T(), cache8::eight<K>(w[0], w[1], k_scale[b]), q[2 * i], s[b]);
-        s[b] = mfma16(T(), cache8::eight<K>(w[2], w[3], k_scale[b]), q[2 * i + 1], s[b]);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) s[b][i] = K::times(s[b][i], k_scale[b]);
-    }
-    const int last = cache.last;
-    if (key + KEYS - 1 > min(least, last)) {
-#pragma unroll
-      for (int b = 0; b < NB; ++b)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (key + 16 * b + 4 * g + i > min(limit, last)) s[b][i] = -INFINITY;
-    }
-    float mx = s[0][0];
-#pragma unroll
-    for (int b = 0; b < NB; ++b)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[b][i]);
-    mx = fmaxf(m, xor_stage<32>(xor_stage<16>(mx, MaxOp()), MaxOp()));
-    if (__any(mx > m)) {
-      const float f = rescaled(m, mx, c);
-      m = mx;
-      l *= f;
-#pragma unroll
-      for (int d = 0; d < DP / 16; ++d)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[d][i] *= f;
-    }
-    // as in softmax_step: far from zero the difference is taken first
-    float shift = m == -INFINITY ? 0.f : -(m * c);
-    if (__any(!(fabsf(shift) < kFar))) {
-      const float less = fabsf(shift) < kFar ? 0.f : m;
-      shift = fabsf(shift) < kFar ? shift : 0.f;
-#pragma unroll
-      for (int b = 0; b < NB; ++b)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s[b][i] -= less;
-    }
-    u32x4 p[NB / 2];
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        s[b][i] = __builtin_amdgcn_exp2f(fmaf(s[b][i], c, shift));
-        l += s[b][i];
-      }
-      const auto weight = [&](int i) { return V::times(s[b][i], v_scale[b]); };
-      p[b / 2][2 * (b % 2)] = T::pack(weight(0), weight(1));
-      p[b / 2][2 * (b % 2) + 1] = T::pack(weight(2), weight(3));
-    }
-    typedef int i32x2 __attribute__((ext_vector_type(2)));
-    typedef __attribute__((address_space(3))) i32x2* lds2;
-    const int j = row >> 1, from = 16 * (j >> 2) + 4 * g + (j & 3);
-#pragma unroll
-    for (int b = 0; b < NB; b += 2)
-#pragma unroll
-      for (int d = 0; d < DP / 16; ++d) {
-        const char* at = reinterpret_cast<const char*>(vimg + place16<DP>(16 * b + from, d)) + 8 * (row & 1);
-        const i32x2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds2)(__attribute__((address_space(3))) void*)at);
-        const u32x2 x = V::four(w[0], v_scale[b]), y = V::four(w[1], v_scale[b + 1]);
-        o[d] = mfma16(T(), u32x4{x[0], x[1], y[0], y[1]}, p[b / 2], o[d]);
-      }
-  }
-  if (__any(cache.bad)) l = NAN;
-  l = xor_stage<32>(xor_stage<16>(l, AddOp()), AddOp());
-  // the waves' parts are joined: stats: [wave][16] maxima, [wave][16] sums, [16] factors of the result
-  if (lane < 16) {
-    stats[16 * wave + lane] = m;
-    stats[16 * (kWaves + wave) + lane] = l;
-  }
-  __syncthreads();
-  float whole_m = -INFINITY, whole_l = 0.f;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) whole_m = fmaxf(whole_m, stats[16 * w + row]);
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w)
-    whole_l += stats[16 * (kWaves + w) + row] * rescaled(stats[16 * w + row], whole_m, c);
-  const float f = rescaled(m, whole_m, c);
-  const bool whole = !it.divided, keep = whole || it.slot + it.split < a.slots;
-  const int wd = a.d <= 64 ? 64 : a.d <= 96 ? 96 : DP;  // columns of a slot
-  float* ws = whole ? nullptr : a.ws + (static_cast<int64_t>(it.slot + it.split) * a.hk.d + kvh) * a.ws_rows * (wd + 2);
-  if (wave == 0 && lane < 16) {
-    stats[16 * 2 * kWaves + lane] = whole ? inverse(whole_l) : 1.f;
-    if (!whole && keep && lane < it.rows) {
-      ws[a.ws_rows * wd + lane] = whole_m;
-      ws[a.ws_rows * (wd + 1) + lane] = whole_l;
-    }
-  }
-  f32x4* parts = reinterpret_cast<f32x4*>(smem);  // [wave][4 columns][16 rows]
-  constexpr int G = Shape16<DP>::G;
-#pragma unroll
-  for (int r = 0; r < DP / G; ++r) {
-    if (row < it.rows) {
-#pragma unroll
-      for (int d = 0; d < G / 16; ++d) {
-        const f32x4 x = o[r * (G / 16) + d];
-        parts[(wave * (G / 4) + 4 * d + g) * 16 + row] = f32x4{x[0] * f, x[1] * f, x[2] * f, x[3] * f};
-      }
-    }
-    __syncthreads();
-    for (int i = tid; i < it.rows * (G / 4); i += kThreads) {
-      const int rw = i / (G / 4), piece = i % (G / 4), col = 4 * piece + r * G;
-      f32x4 x = parts[piece * 16 + rw];
-#pragma unroll
-      for (int w = 1; w < kWaves; ++w) x += parts[(w * (G / 4) + piece) * 16 + rw];
-      if (whole) {
-        const float inv = stats[16 * 2 * kWaves + rw];
-        if (col < a.d)
-          *reinterpret_cast<u32x2*>(out_row(a, it, kvh, it.row0 + rw) + col) =
-              u32x2{T::pack(x[0] * inv, x[1] * inv), T::pack(x[2] * inv, x[3] * inv)};
-      } else if (keep && col < wd) {
-        *reinterpret_cast<f32x4*>(ws + rw * wd + col) = x;
-      }
-    }
-    if (r + 1 < DP / G) __syncthreads();
-  }
-}
-
+// Heads of up to 96 columns: the large tiles are made for 96, the few rows' for 128.
 template <class T, class C, int DP, bool FULL>
 __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void attention8_kernel(Args8 a) {
-  __shared__ __align__(16) u32x4 smem[Shape8<DP>::kChunks];
-  __shared__ float stats[32 * (2 * kWaves + 1)];
+  using F = Few<DP == 96 ? 128 : DP, 2>;
+  __shared__ __align__(16) u32x4 smem[F::kChunks > Large<DP>::kImages ? F::kChunks : Large<DP>::kImages];
+  __shared__ float stats[F::kStats];
   if constexpr (std::is_same<T, F16>::value) cache8::saturate_f16();
   const int index = a.hk(blockIdx.x), kvh = blockIdx.x - index * a.hk.d;
   const Item it = find_item<false>(a, index);
@@ -610,44 +566,71 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void attention8_kernel(
     return;
   }
   if (it.key0 >= it.key1 && it.split > 0) return;
-  if (it.small) small_tile8<T, C, DP, FULL>(a, it, kvh, smem, stats);
+  if (it.small) few_rows<T, C, DP == 96 ? 128 : DP, FULL, 2>(a, it, kvh, smem, stats);
   else large_tile8<T, C, DP, FULL>(a, it, kvh, smem);
 }
 
-template <class T, int KIND, int DP>
-void launch8(const Args8& a, const Launch& n, hipStream_t st) {
-  using C = cache8::Codes<KIND, std::is_same<T, Bf16>::value>;
-  const unsigned grid = static_cast<unsigned>(n.index * a.hk.d);
-  if (a.d == DP && a.wide) attention8_kernel<T, C, DP, true><<<grid, kThreads, 0, st>>>(a);
-  else attention8_kernel<T, C, DP, false><<<grid, kThreads, 0, st>>>(a);
-}
-
-template <class T, int KIND, int DP>
-void launch8_few(const Args8& a, const Launch& n, hipStream_t st) {
+// What a launch is made for: tiles of 16 rb rows, or (rb 0) the large ones beside small ones of 32.
+template <class T, int KIND, int RB>
+int launch8_few(const Args8& a, const Launch& n, hipStream_t st) {
   using C = cache8::Codes<KIND, std::is_same<T, Bf16>::value>;
   const unsigned grid = static_cast<unsigned>((n.index + kXcds - 1) / kXcds * kXcds * a.hk.d);
-  if (a.d == DP && a.wide && a.even) attention8_few_kernel<T, C, DP, true><<<grid, kThreads, 0, st>>>(a);
-  else attention8_few_kernel<T, C, DP, false><<<grid, kThreads, 0, st>>>(a);
-}
-
-template <class T, int KIND>
-int launch8_dim(const Args8& a, const Launch& n, bool few, hipStream_t st) {
-  const int padded = padded_dim(a.d);
-  if (few) {
-    if (padded == 64) launch8_few<T, KIND, 64>(a, n, st);
-    else if (padded <= 128) launch8_few<T, KIND, 128>(a, n, st);
-    else launch8_few<T, KIND, 256>(a, n, st);
-  } else {
-    if (padded == 64) launch8<T, KIND, 64>(a, n, st);
-    else if (padded == 96) launch8<T, KIND, 96>(a, n, st);
-    else if (padded == 128) launch8<T, KIND, 128>(a, n, st);
-    else launch8<T, KIND, 256>(a, n, st);
+  const bool full = a.wide && a.even;
+  if (a.d == 64 && full) attention8_few_kernel<T, C, 64, true, RB><<<grid, kThreads, 0, st>>>(a);
+  else if (a.d <= 64) attention8_few_kernel<T, C, 64, false, RB><<<grid, kThreads, 0, st>>>(a);
+  else if (a.d == 128 && full) attention8_few_kernel<T, C, 128, true, RB><<<grid, kThreads, 0, st>>>(a);
+  else if (a.d <= 128) attention8_few_kernel<T, C, 128, false, RB><<<grid, kThreads, 0, st>>>(a);
+  else if constexpr (RB < 3) {
+    if (a.d == 256 && full) attention8_few_kernel<T, C, 256, true, RB><<<grid, kThreads, 0, st>>>(a);
+    else attention8_few_kernel<T, C, 256, false, RB><<<grid, kThreads, 0, st>>>(a);
   }
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return static_cast<int>(e);
-  if (n.merges == 0) return BP_OK;
-  const int dtype = std::is_same<T, Bf16>::value ? BP_DT_BF16 : BP_DT_F16;
-  return few ? launch_merge<Tiles16>(dtype, a, n, st) : launch_merge<Tiles32>(dtype, a, n, st);
+  return n.merges > 0 ? launch_merge<FewTiles<RB>>(std::is_same<T, Bf16>::value ? BP_DT_BF16 : BP_DT_F16, a, n, st) : BP_OK;
+}
+
+template <class T, int KIND>
+int launch8_large(const Args8& a, const Launch& n, hipStream_t st) {
+  using C = cache8::Codes<KIND, std::is_same<T, Bf16>::value>;
+  const unsigned grid = static_cast<unsigned>(n.index * a.hk.d);
+  const bool full = a.wide && a.even;
+  if (a.d == 64 && full) attention8_kernel<T, C, 64, true><<<grid, kThreads, 0, st>>>(a);
+  else if (a.d <= 64) attention8_kernel<T, C, 64, false><<<grid, kThreads, 0, st>>>(a);
+  else if (a.d <= 96) attention8_kernel<T, C, 96, false><<<grid, kThreads, 0, st>>>(a);
+  else if (a.d == 128 && full) attention8_kernel<T, C, 128, true><<<grid, kThreads, 0, st>>>(a);
+  else if (a.d <= 128) attention8_kernel<T, C, 128, false><<<grid, kThreads, 0, st>>>(a);
+  else if (a.d == 256 && full) attention8_kernel<T, C, 256, true><<<grid, kThreads, 0, st>>>(a);
+  else attention8_kernel<T, C, 256, false><<<grid, kThreads, 0, st>>>(a);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return static_cast<int>(e);
+  return n.merges > 0 ? launch_merge<Tiles32>(std::is_same<T, Bf16>::value ? BP_DT_BF16 : BP_DT_F16, a, n, st) : BP_OK;
+}
+
+template <class T, int KIND>
+int launch8(const Args8& a, const Launch& n, int rb, hipStream_t st) {
+  switch (rb) {
+    case 1: return launch8_few<T, KIND, 1>(a, n, st);
+    case 2: return launch8_few<T, KIND, 2>(a, n, st);
+    case 3: return launch8_few<T, KIND, 3>(a, n, st);
+    default: return launch8_large<T, KIND>(a, n, st);
+  }
+}
+
+// Few rows a sequence, as far as the host can tell (the offsets are the device's; any are right): 16-row blocks of a tile, 0: none.
+int few_of(int64_t tokens, int64_t seqs, int64_t group, int d) {
+  const int most = d > 128 ? 2 : 3;
+  for (int rb = 1; rb <= most; ++rb)
+    if (group <= 16 * rb && tokens * group <= 16 * rb * seqs) return rb;
+  return 0;
+}
+
+bool plan8(Args8& a, Launch& n, int rb) {
+  switch (rb) {
+    case 1: return plan_launch<FewTiles<1>>(a, n);
+    case 2: return plan_launch<FewTiles<2>>(a, n);
+    case 3: return plan_launch<FewTiles<3>>(a, n);
+    default: return plan_launch<Tiles32>(a, n);
+  }
 }
 
 bool aligned(const void* p, int n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
@@ -679,12 +662,9 @@ int run8(int dtype, int kind, Args8& a, size_t ws_bytes, hipStream_t st) {
            a.k_t * a.page.d < (1ll << 31) && a.ks_b * blocks < (1ll << 31);
   // rows of a sequence, and keys plus a split, in 32 bits
   if (static_cast<int64_t>(a.tokens) * a.hq >= (1ll << 30) || a.max_keys >= (1 << 29)) return BP_E_UNSUPPORTED;
-  // Few rows a sequence, as far as the host can tell (the offsets are the device's; any are right): tiles of 16 rows. Their
-  // workspace is no larger: at most twice the tiles, or parts, of half the rows.
-  const int group = a.hq / hk;
-  const bool few = group <= 16 && static_cast<int64_t>(a.tokens) * group <= 16ll * a.seqs;
+  const int rb = few_of(a.tokens, a.seqs, a.hq / hk, a.d);
   Launch n;
-  if (!(few ? plan_launch<Tiles16>(a, n) : plan_launch<Tiles32>(a, n))) return BP_E_UNSUPPORTED;
+  if (!plan8(a, n, rb)) return BP_E_UNSUPPORTED;
   if (n.workspace > 0 && (a.ws == nullptr || ws_bytes < n.workspace || !aligned(a.ws, 16))) return BP_E_WORKSPACE;
   if (n.workspace == 0) a.ws = nullptr;
   // A row of q is read by the tile that writes its result and by no other, so out may be q itself.
@@ -701,13 +681,25 @@ int run8(int dtype, int kind, Args8& a, size_t ws_bytes, hipStream_t st) {
     return BP_E_INVALID_ARG;
   const bool e4m3 = kind == BP_DT_E4M3;
   if (dtype == BP_DT_BF16)
-    return e4m3 ? launch8_dim<Bf16, cache8::kE4m3>(a, n, few, st) : launch8_dim<Bf16, cache8::kInt8>(a, n, few, st);
-  return e4m3 ? launch8_dim<F16, cache8::kE4m3>(a, n, few, st) : launch8_dim<F16, cache8::kInt8>(a, n, few, st);
+    return e4m3 ? launch8<Bf16, cache8::kE4m3>(a, n, rb, st) : launch8<Bf16, cache8::kInt8>(a, n, rb, st);
+  return e4m3 ? launch8<F16, cache8::kE4m3>(a, n, rb, st) : launch8<F16, cache8::kInt8>(a, n, rb, st);
 }
 
 }  // namespace
 }  // namespace attn
 }  // namespace bp
+
+extern "C" size_t bp_attn_paged8_workspace_bytes(int64_t tokens, int64_t seqs, int64_t hq, int64_t hk, int64_t head_dim,
+                                                 int64_t max_keys) {
+  using namespace bp::attn;
+  if (hk <= 0 || hq % hk != 0) return 0;
+  switch (few_of(tokens, seqs, hq / hk, static_cast<int>(head_dim))) {
+    case 1: return workspace_bytes<FewTiles<1>>(tokens, seqs, hq, hk, head_dim, max_keys);
+    case 2: return workspace_bytes<FewTiles<2>>(tokens, seqs, hq, hk, head_dim, max_keys);
+    case 3: return workspace_bytes<FewTiles<3>>(tokens, seqs, hq, hk, head_dim, max_keys);
+    default: return workspace_bytes<Tiles32>(tokens, seqs, hq, hk, head_dim, max_keys);
+  }
+}
 
 extern "C" int bp_attn_paged8(int dtype, int cache_dtype, const void* q, const void* k_pages, const void* v_pages,
                               const uint8_t* k_scales, const uint8_t* v_scales, void* out, const int32_t* table,

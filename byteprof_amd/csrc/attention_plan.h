@@ -21,7 +21,7 @@ constexpr int kKeyStep = 128;    // a split's keys are a multiple of this: whole
 constexpr int kCus = 256;
 
 // How a launch cuts sequences into tiles. Tiles32: the kernels of attention.hip, and over a cache in 8 bits wherever sequences have
-// many rows. Tiles16: the kernel of attention8.hip for launches of few rows a sequence.
+// many rows. FewTiles: the kernel of attention8.hip for launches of few rows a sequence.
 struct Tiles32 {
   static constexpr int kFew = kSmallRows;    // sequences of at most this many rows have the small tiles
   static constexpr int kSmall = kTileSmall;
@@ -33,13 +33,18 @@ struct Tiles32 {
   // made heads of 96 no faster and cached ones slower, 97 us against 90).
   static int workgroups_a_cu(int padded) { return padded > 128 ? 1 : 2; }
 };
-struct Tiles16 {
+// All tiles of 16 RB rows.
+template <int RB>
+struct FewTiles {
   static constexpr int kFew = 1 << 30;
-  static constexpr int kSmall = 16;
+  static constexpr int kSmall = 16 * RB;
   static constexpr bool kFit = false;
   static constexpr int kMergeRows = 16;
   static constexpr int kTarget = 2048;
-  static int workgroups_a_cu(int padded) { return padded > 128 ? 2 : padded > 64 ? 3 : 4; }
+  // By the registers of attention8_few_kernel, a workgroup's four waves on the four SIMDs.
+  __host__ __device__ static constexpr int workgroups_a_cu(int padded) {
+    return RB == 1 ? (padded > 128 ? 2 : padded > 64 ? 3 : 4) : padded > 128 ? 1 : 2;
+  }
 };
 
 // n / d for n below 2^30 without a division: magic = floor(2^(32 + shift) / d) + 1 with 2^shift < d <= 2^(shift + 1).

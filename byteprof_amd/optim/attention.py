@@ -119,10 +119,11 @@ def _output(what: str, q: torch.Tensor, out: torch.Tensor | None, *read: torch.T
     return out
 
 
-def _workspace(tokens: int, seqs: int, hq: int, hk: int, d: int, max_keys: int, device: torch.device):
+def _workspace(tokens: int, seqs: int, hq: int, hk: int, d: int, max_keys: int, device: torch.device,
+               of: str = "bp_attn_workspace_bytes"):
     if max_keys <= UNDIVIDED_KEYS:
         return None, 0
-    need = _lib.lib().bp_attn_workspace_bytes(tokens, seqs, hq, hk, d, max_keys)
+    need = getattr(_lib.lib(), of)(tokens, seqs, hq, hk, d, max_keys)
     return (torch.empty(need, dtype=torch.uint8, device=device), need) if need else (None, 0)
 
 
@@ -278,7 +279,7 @@ def _paged_attention8(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Ten
     y = _output(what, q, out, k_pages, v_pages, k_scales, v_scales)
     if tokens == 0:
         return y
-    ws, need = _workspace(tokens, seqs, hq, hk, d, page * most, q.device)
+    ws, need = _workspace(tokens, seqs, hq, hk, d, page * most, q.device, "bp_attn_paged8_workspace_bytes")
     q_t, q_h, _ = q.stride()
     _launch(index, "bp_attn_paged8", dtype, code, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), k_scales.data_ptr(),
             v_scales.data_ptr(), y.data_ptr(), table.data_ptr(), row, lengths.data_ptr(), cu.data_ptr(), tokens, seqs, pool, page,

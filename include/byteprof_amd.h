@@ -470,7 +470,7 @@ int bp_paged_append(int element_bytes, const void* k, const void* v, void* k_pag
  *
  * paged8: bp_attn_paged over codes, which become values of q's dtype exactly (BP_DT_F16: those past fp16's range become its
  * greatest, 65504, those below its least are rounded; E4M3 scales past 2^22 count as 2^22). block a multiple of 4; the codes' bases and the strides of dimensions of more than one entry
- * multiples of 8. The workspace is bp_attn_workspace_bytes' for page x max_pages keys.
+ * multiples of 8. workspace: bp_attn_paged8_workspace_bytes(tokens, seqs, hq, hk, head_dim, page x max_pages), 16-byte aligned.
  *
  * read: the positions of bp_paged_append out of the cache, into k, v [tokens, hk, head_dim] (dtype, contiguous, 16-byte aligned):
  * codes x scale (in BP_DT_F16 as for paged8), or (cache_dtype = dtype BP_DT_BF16 or F16; block and scales unused) a 16-bit cache's values. head_dim a multiple
@@ -484,6 +484,7 @@ int bp_paged_append8(int dtype, int cache_dtype, const void* k, const void* v, v
                      int64_t k_h, int64_t v_t, int64_t v_h, int64_t kp_p, int64_t kp_t, int64_t kp_h, int64_t vp_p, int64_t vp_t,
                      int64_t vp_h, int64_t ks_p, int64_t ks_b, int64_t ks_h, int64_t vs_p, int64_t vs_b, int64_t vs_h,
                      void* stream);
+size_t bp_attn_paged8_workspace_bytes(int64_t tokens, int64_t seqs, int64_t hq, int64_t hk, int64_t head_dim, int64_t max_keys);
 int bp_attn_paged8(int dtype, int cache_dtype, const void* q, const void* k_pages, const void* v_pages, const uint8_t* k_scales,
                    const uint8_t* v_scales, void* out, const int32_t* table, int64_t table_stride, const int32_t* lengths,
                    const int32_t* cu, int tokens, int seqs, int pool, int page, int block, int max_pages, int hq, int hk,
