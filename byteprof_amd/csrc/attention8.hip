@@ -701,29 +701,27 @@ extern "C" size_t bp_attn_paged8_workspace_bytes(int64_t tokens, int64_t seqs, i
   }
 }
 
-extern "C" int bp_attn_paged8(int dtype, int cache_dtype, const void* q, const void* k_pages, const void* v_pages,
-                              const uint8_t* k_scales, const uint8_t* v_scales, void* out, const int32_t* table,
-                              int64_t table_stride, const int32_t* lengths, const int32_t* cu, int tokens, int seqs, int pool,
-                              int page, int block, int max_pages, int hq, int hk, int head_dim, int64_t q_t, int64_t q_h,
-                              int64_t k_p, int64_t k_t, int64_t k_h, int64_t v_p, int64_t v_t, int64_t v_h, int64_t ks_p,
-                              int64_t ks_b, int64_t ks_h, int64_t vs_p, int64_t vs_b, int64_t vs_h, float scale, void* workspace,
-                              size_t workspace_bytes, void* stream) {
-  if (page <= 0 || pool < 0 || max_pages < 0 || static_cast<int64_t>(page) * max_pages >= (1ll << 29)) return BP_E_INVALID_ARG;
-  if (block <= 0 || block % 4 != 0 || page % block != 0) return BP_E_INVALID_ARG;
-  if (tokens > 0 && seqs > 0 &&
-      (lengths == nullptr || (max_pages > 0 && (table == nullptr || k_pages == nullptr || v_pages == nullptr ||
-                                                k_scales == nullptr || v_scales == nullptr || pool == 0))))
+extern "C" int bp_attn_paged8(const BpPagedCache* cache, int dtype, const void* q, void* out, const int32_t* cu, int tokens, int hq,
+                              int64_t q_t, int64_t q_h, float scale, void* workspace, size_t workspace_bytes, void* stream) {
+  if (cache == nullptr) return BP_E_INVALID_ARG;
+  const BpPagedCache& c = *cache;
+  if (c.page <= 0 || c.pool < 0 || c.seqs < 0 || c.max_pages < 0 || static_cast<int64_t>(c.page) * c.max_pages >= (1ll << 29))
+    return BP_E_INVALID_ARG;
+  if (c.block <= 0 || c.block % 4 != 0 || c.page % c.block != 0) return BP_E_INVALID_ARG;
+  if (tokens > 0 && c.seqs > 0 &&
+      (c.lengths == nullptr || (c.max_pages > 0 && (c.table == nullptr || c.k_pages == nullptr || c.v_pages == nullptr ||
+                                                    c.k_scales == nullptr || c.v_scales == nullptr || c.pool == 0))))
     return BP_E_INVALID_ARG;
   bp::attn::Args8 a = {};
-  a.q = q, a.k = k_pages, a.v = v_pages, a.out = out, a.cu = cu, a.lengths = lengths, a.table = table;
-  a.ks = k_scales, a.vs = v_scales;
+  a.q = q, a.k = c.k_pages, a.v = c.v_pages, a.out = out, a.cu = cu, a.lengths = c.lengths, a.table = c.table;
+  a.ks = static_cast<const uint8_t*>(c.k_scales), a.vs = static_cast<const uint8_t*>(c.v_scales);
   a.ws = static_cast<float*>(workspace);
-  a.q_t = q_t, a.q_h = q_h, a.k_p = k_p, a.k_t = k_t, a.k_h = k_h, a.v_p = v_p, a.v_t = v_t, a.v_h = v_h;
-  a.ks_p = ks_p, a.ks_b = ks_b, a.ks_h = ks_h, a.vs_p = vs_p, a.vs_b = vs_b, a.vs_h = vs_h;
-  a.table_stride = table_stride;
-  a.tokens = tokens, a.seqs = seqs, a.hq = hq, a.hk.d = hk, a.d = head_dim, a.causal = 1;
-  a.pool = pool, a.page = bp::attn::Div::of(page), a.block = bp::attn::Div::of(block);
-  a.max_keys = page * max_pages;
+  a.q_t = q_t, a.q_h = q_h, a.k_p = c.kp[0], a.k_t = c.kp[1], a.k_h = c.kp[2], a.v_p = c.vp[0], a.v_t = c.vp[1], a.v_h = c.vp[2];
+  a.ks_p = c.ks[0], a.ks_b = c.ks[1], a.ks_h = c.ks[2], a.vs_p = c.vs[0], a.vs_b = c.vs[1], a.vs_h = c.vs[2];
+  a.table_stride = c.table_stride;
+  a.tokens = tokens, a.seqs = c.seqs, a.hq = hq, a.hk.d = c.hk, a.d = c.head_dim, a.causal = 1;
+  a.pool = c.pool, a.page = bp::attn::Div::of(c.page), a.block = bp::attn::Div::of(c.block);
+  a.max_keys = c.page * c.max_pages;
   a.scale_log2 = scale * 1.44269504088896340736f;
-  return bp::attn::run8(dtype, cache_dtype, a, workspace_bytes, static_cast<hipStream_t>(stream));
+  return bp::attn::run8(dtype, c.dtype, a, workspace_bytes, static_cast<hipStream_t>(stream));
 }

@@ -318,10 +318,12 @@ void read_kind(const Read& a, int kind, unsigned grid, hipStream_t st) {
   else read_kernel<T, 2><<<grid, kThreads, 0, st>>>(a);
 }
 
-bool cache_sizes(int tokens, int seqs, int pool, int page, int max_pages, int hk, int head_dim) {
-  return tokens >= 0 && seqs >= 0 && pool >= 0 && page > 0 && max_pages >= 0 &&
-         static_cast<int64_t>(page) * max_pages < (1ll << 29) && hk >= 0 && head_dim >= 0;
+bool sizes_fit(const BpPagedCache* c, int tokens) {
+  return c != nullptr && tokens >= 0 && c->seqs >= 0 && c->pool >= 0 && c->page > 0 && c->max_pages >= 0 &&
+         static_cast<int64_t>(c->page) * c->max_pages < (1ll << 29) && c->hk >= 0 && c->head_dim >= 0;
 }
+
+bool has_codes(const BpPagedCache& c) { return c.dtype == BP_DT_E4M3 || c.dtype == BP_DT_I8; }
 
 }  // namespace
 }  // namespace cache8
@@ -329,91 +331,89 @@ bool cache_sizes(int tokens, int seqs, int pool, int page, int max_pages, int hk
 
 extern "C" {
 
-int bp_paged_append8(int dtype, int cache_dtype, const void* k, const void* v, void* k_pages, void* v_pages, uint8_t* k_scales,
-                     uint8_t* v_scales, const int32_t* table, int64_t table_stride, const int32_t* lengths, const int32_t* cu,
-                     int tokens, int seqs, int pool, int page, int block, int max_pages, int hk, int head_dim, int64_t k_t,
-                     int64_t k_h, int64_t v_t, int64_t v_h, int64_t kp_p, int64_t kp_t, int64_t kp_h, int64_t vp_p, int64_t vp_t,
-                     int64_t vp_h, int64_t ks_p, int64_t ks_b, int64_t ks_h, int64_t vs_p, int64_t vs_b, int64_t vs_h,
-                     void* stream) {
+int bp_paged_append8(const BpPagedCache* cache, int dtype, const void* k, const void* v, const int32_t* cu, int tokens, int64_t k_t,
+                     int64_t k_h, int64_t v_t, int64_t v_h, void* stream) {
   using namespace bp::cache8;
-  if ((dtype != BP_DT_BF16 && dtype != BP_DT_F16 && dtype != BP_DT_F32) || (cache_dtype != BP_DT_E4M3 && cache_dtype != BP_DT_I8))
-    return BP_E_UNSUPPORTED;
-  if (!cache_sizes(tokens, seqs, pool, page, max_pages, hk, head_dim) || block <= 0 || page % block != 0) return BP_E_INVALID_ARG;
-  if (tokens == 0 || seqs == 0 || pool == 0 || max_pages == 0 || hk == 0 || head_dim == 0) return BP_OK;
-  if (k == nullptr || v == nullptr || k_pages == nullptr || v_pages == nullptr || k_scales == nullptr || v_scales == nullptr ||
-      table == nullptr || lengths == nullptr || cu == nullptr)
+  if (!sizes_fit(cache, tokens)) return BP_E_INVALID_ARG;
+  const BpPagedCache& c = *cache;
+  if ((dtype != BP_DT_BF16 && dtype != BP_DT_F16 && dtype != BP_DT_F32) || !has_codes(c)) return BP_E_UNSUPPORTED;
+  if (c.block <= 0 || c.page % c.block != 0) return BP_E_INVALID_ARG;
+  if (tokens == 0 || c.seqs == 0 || c.pool == 0 || c.max_pages == 0 || c.hk == 0 || c.head_dim == 0) return BP_OK;
+  if (k == nullptr || v == nullptr || c.k_pages == nullptr || c.v_pages == nullptr || c.k_scales == nullptr ||
+      c.v_scales == nullptr || c.table == nullptr || c.lengths == nullptr || cu == nullptr)
     return BP_E_INVALID_ARG;
   Append a = {};
+  const void *pages[2] = {c.k_pages, c.v_pages}, *scales[2] = {c.k_scales, c.v_scales};
+  const int64_t *page_strides[2] = {c.kp, c.vp}, *scale_strides[2] = {c.ks, c.vs};
   a.in[0] = k, a.in[1] = v;
-  a.pages[0] = static_cast<uint8_t*>(k_pages), a.pages[1] = static_cast<uint8_t*>(v_pages);
-  a.scales[0] = k_scales, a.scales[1] = v_scales;
-  a.cu = cu, a.lengths = lengths, a.table = table, a.table_stride = table_stride;
   a.in_t[0] = k_t, a.in_t[1] = v_t, a.in_h[0] = k_h, a.in_h[1] = v_h;
-  a.p_p[0] = kp_p, a.p_p[1] = vp_p, a.p_t[0] = kp_t, a.p_t[1] = vp_t, a.p_h[0] = kp_h, a.p_h[1] = vp_h;
-  a.s_p[0] = ks_p, a.s_p[1] = vs_p, a.s_b[0] = ks_b, a.s_b[1] = vs_b, a.s_h[0] = ks_h, a.s_h[1] = vs_h;
-  a.page = bp::attn::Div::of(page), a.block = bp::attn::Div::of(block), a.heads = bp::attn::Div::of(hk);
-  a.tokens = tokens, a.seqs = seqs, a.pool = pool, a.max_keys = page * max_pages, a.hk = hk, a.d = head_dim;
   const int size = dtype == BP_DT_F32 ? 4 : 2;
-  const bool wide = head_dim % 8 == 0 && aligned(k, 16) && aligned(v, 16) && aligned(k_pages, 8) && aligned(v_pages, 8) &&
-                    ((k_t | k_h | v_t | v_h) * size & 15) == 0 && ((kp_p | kp_t | kp_h | vp_p | vp_t | vp_h) & 7) == 0;
-  a.row = bp::attn::Div::of(wide ? head_dim / 8 : head_dim);
-  const int64_t units = tokens / block + 2ll * seqs;
+  bool wide = c.head_dim % 8 == 0 && aligned(k, 16) && aligned(v, 16) && ((k_t | k_h | v_t | v_h) * size & 15) == 0;
+  for (int w = 0; w < 2; ++w) {
+    a.pages[w] = static_cast<uint8_t*>(const_cast<void*>(pages[w]));
+    a.scales[w] = static_cast<uint8_t*>(const_cast<void*>(scales[w]));
+    a.p_p[w] = page_strides[w][0], a.p_t[w] = page_strides[w][1], a.p_h[w] = page_strides[w][2];
+    a.s_p[w] = scale_strides[w][0], a.s_b[w] = scale_strides[w][1], a.s_h[w] = scale_strides[w][2];
+    wide = wide && aligned(pages[w], 8) && ((a.p_p[w] | a.p_t[w] | a.p_h[w]) & 7) == 0;
+  }
+  a.cu = cu, a.lengths = c.lengths, a.table = c.table, a.table_stride = c.table_stride;
+  a.page = bp::attn::Div::of(c.page), a.block = bp::attn::Div::of(c.block), a.heads = bp::attn::Div::of(c.hk);
+  a.row = bp::attn::Div::of(wide ? c.head_dim / 8 : c.head_dim);
+  a.tokens = tokens, a.seqs = c.seqs, a.pool = c.pool, a.max_keys = c.page * c.max_pages, a.hk = c.hk, a.d = c.head_dim;
+  const int64_t units = tokens / c.block + 2ll * c.seqs;
   // a unit's pieces, the units with their heads, and positions in 32 bits
-  if (static_cast<int64_t>(block) * head_dim >= (1ll << 30) || 2 * units * hk >= (1ll << 30) || tokens >= (1 << 30))
+  if (static_cast<int64_t>(c.block) * c.head_dim >= (1ll << 30) || 2 * units * c.hk >= (1ll << 30) || tokens >= (1 << 30))
     return BP_E_UNSUPPORTED;
   a.units = static_cast<int>(units);
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  if (dtype == BP_DT_BF16) append_kind<Bf16>(a, cache_dtype, wide, st);
-  else if (dtype == BP_DT_F16) append_kind<F16>(a, cache_dtype, wide, st);
-  else append_kind<F32>(a, cache_dtype, wide, st);
+  if (dtype == BP_DT_BF16) append_kind<Bf16>(a, c.dtype, wide, st);
+  else if (dtype == BP_DT_F16) append_kind<F16>(a, c.dtype, wide, st);
+  else append_kind<F32>(a, c.dtype, wide, st);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? BP_OK : static_cast<int>(e);
 }
 
-int bp_paged_read(int dtype, int cache_dtype, const void* k_pages, const void* v_pages, const uint8_t* k_scales,
-                  const uint8_t* v_scales, void* k, void* v, const int32_t* table, int64_t table_stride, const int32_t* lengths,
-                  const int32_t* cu, int tokens, int seqs, int pool, int page, int block, int max_pages, int hk, int head_dim,
-                  int64_t kp_p, int64_t kp_t, int64_t kp_h, int64_t vp_p, int64_t vp_t, int64_t vp_h, int64_t ks_p, int64_t ks_b,
-                  int64_t ks_h, int64_t vs_p, int64_t vs_b, int64_t vs_h, void* stream) {
+int bp_paged_read(const BpPagedCache* cache, int dtype, void* k, void* v, const int32_t* cu, int tokens, void* stream) {
   using namespace bp::cache8;
-  const bool codes = cache_dtype == BP_DT_E4M3 || cache_dtype == BP_DT_I8;
+  if (!sizes_fit(cache, tokens)) return BP_E_INVALID_ARG;
+  const BpPagedCache& c = *cache;
+  const bool codes = has_codes(c);
   if (dtype != BP_DT_BF16 && dtype != BP_DT_F16 && dtype != BP_DT_F32) return BP_E_UNSUPPORTED;
-  if (!codes && (cache_dtype != dtype || dtype == BP_DT_F32)) return BP_E_UNSUPPORTED;
-  if (!cache_sizes(tokens, seqs, pool, page, max_pages, hk, head_dim) || (codes && (block <= 0 || page % block != 0)))
+  if (!codes && (c.dtype != dtype || dtype == BP_DT_F32)) return BP_E_UNSUPPORTED;
+  if (codes && (c.block <= 0 || c.page % c.block != 0)) return BP_E_INVALID_ARG;
+  if (c.head_dim % 8 != 0) return BP_E_UNSUPPORTED;
+  if (tokens == 0 || c.hk == 0 || c.head_dim == 0) return BP_OK;
+  const bool empty = c.seqs == 0 || c.pool == 0 || c.max_pages == 0;
+  if (k == nullptr || v == nullptr || (c.seqs > 0 && (c.lengths == nullptr || cu == nullptr)) ||
+      (!empty && (c.k_pages == nullptr || c.v_pages == nullptr || c.table == nullptr ||
+                  (codes && (c.k_scales == nullptr || c.v_scales == nullptr)))))
     return BP_E_INVALID_ARG;
-  if (head_dim % 8 != 0) return BP_E_UNSUPPORTED;
-  if (tokens == 0 || hk == 0 || head_dim == 0) return BP_OK;
-  const bool empty = seqs == 0 || pool == 0 || max_pages == 0;
-  if (k == nullptr || v == nullptr || (seqs > 0 && (lengths == nullptr || cu == nullptr)) ||
-      (!empty && (k_pages == nullptr || v_pages == nullptr || table == nullptr ||
-                  (codes && (k_scales == nullptr || v_scales == nullptr)))))
-    return BP_E_INVALID_ARG;
-  const int size = codes ? 1 : 2, unit = 8 * size;
-  // a stride that nothing is multiplied with may be anything
-  if (pool == 1) kp_p = vp_p = 0;
-  if (page == 1) kp_t = vp_t = 0;
-  if (hk == 1) kp_h = vp_h = 0;
-  if (!aligned(k, 16) || !aligned(v, 16) || !aligned(k_pages, unit) || !aligned(v_pages, unit) ||
-      ((kp_p | kp_t | kp_h | vp_p | vp_t | vp_h) & 7) != 0)
-    return BP_E_INVALID_ARG;
-  if (static_cast<int64_t>(tokens) * hk * (head_dim / 8) >= (1ll << 30)) return BP_E_UNSUPPORTED;
+  const int size = codes ? 1 : 2;
   Read a = {};
-  a.pages[0] = static_cast<const uint8_t*>(k_pages), a.pages[1] = static_cast<const uint8_t*>(v_pages);
-  a.scales[0] = k_scales, a.scales[1] = v_scales;
   a.out[0] = k, a.out[1] = v;
-  a.cu = cu, a.lengths = lengths, a.table = table, a.table_stride = table_stride;
-  a.p_p[0] = kp_p * size, a.p_p[1] = vp_p * size, a.p_t[0] = kp_t * size, a.p_t[1] = vp_t * size;
-  a.p_h[0] = kp_h * size, a.p_h[1] = vp_h * size;
-  a.s_p[0] = ks_p, a.s_p[1] = vs_p, a.s_b[0] = ks_b, a.s_b[1] = vs_b, a.s_h[0] = ks_h, a.s_h[1] = vs_h;
-  a.page = bp::attn::Div::of(page), a.block = bp::attn::Div::of(codes ? block : page);
-  a.row = bp::attn::Div::of(head_dim / 8), a.token = bp::attn::Div::of(hk * (head_dim / 8));
-  a.tokens = tokens, a.seqs = seqs, a.pool = pool, a.max_keys = page * max_pages;
+  const void *pages[2] = {c.k_pages, c.v_pages}, *scales[2] = {c.k_scales, c.v_scales};
+  const int64_t *page_strides[2] = {c.kp, c.vp}, *scale_strides[2] = {c.ks, c.vs};
+  for (int w = 0; w < 2; ++w) {
+    // a stride that nothing is multiplied with may be anything
+    const int64_t p = c.pool == 1 ? 0 : page_strides[w][0], t = c.page == 1 ? 0 : page_strides[w][1],
+                  h = c.hk == 1 ? 0 : page_strides[w][2];
+    if (!aligned(a.out[w], 16) || !aligned(pages[w], 8 * size) || ((p | t | h) & 7) != 0) return BP_E_INVALID_ARG;
+    a.pages[w] = static_cast<const uint8_t*>(pages[w]);
+    a.scales[w] = static_cast<const uint8_t*>(scales[w]);
+    a.p_p[w] = p * size, a.p_t[w] = t * size, a.p_h[w] = h * size;
+    a.s_p[w] = scale_strides[w][0], a.s_b[w] = scale_strides[w][1], a.s_h[w] = scale_strides[w][2];
+  }
+  if (static_cast<int64_t>(tokens) * c.hk * (c.head_dim / 8) >= (1ll << 30)) return BP_E_UNSUPPORTED;
+  a.cu = cu, a.lengths = c.lengths, a.table = c.table, a.table_stride = c.table_stride;
+  a.page = bp::attn::Div::of(c.page), a.block = bp::attn::Div::of(codes ? c.block : c.page);
+  a.row = bp::attn::Div::of(c.head_dim / 8), a.token = bp::attn::Div::of(c.hk * (c.head_dim / 8));
+  a.tokens = tokens, a.seqs = c.seqs, a.pool = c.pool, a.max_keys = c.page * c.max_pages;
   const int64_t total = static_cast<int64_t>(tokens) * a.token.d, blocks = (total + kThreads - 1) / kThreads;
   const unsigned grid = static_cast<unsigned>(blocks < 16384 ? blocks : 16384);
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  if (dtype == BP_DT_BF16) read_kind<Bf16>(a, cache_dtype, grid, st);
-  else if (dtype == BP_DT_F16) read_kind<F16>(a, cache_dtype, grid, st);
-  else if (cache_dtype == BP_DT_E4M3) read_kernel<F32, kE4m3><<<grid, kThreads, 0, st>>>(a);
+  if (dtype == BP_DT_BF16) read_kind<Bf16>(a, c.dtype, grid, st);
+  else if (dtype == BP_DT_F16) read_kind<F16>(a, c.dtype, grid, st);
+  else if (c.dtype == BP_DT_E4M3) read_kernel<F32, kE4m3><<<grid, kThreads, 0, st>>>(a);
   else read_kernel<F32, kInt8><<<grid, kThreads, 0, st>>>(a);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? BP_OK : static_cast<int>(e);

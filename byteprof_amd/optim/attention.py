@@ -25,6 +25,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 
 import torch
 from torch.autograd import forward_ad
@@ -192,27 +193,54 @@ def _pages(what: str, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch
     return shape, kst, vst, seqs, most, row
 
 
-def _codes(what: str, k_pages: torch.Tensor, v_pages: torch.Tensor, k_scales: torch.Tensor | None,
-           v_scales: torch.Tensor | None) -> tuple:
-    """Of an 8-bit cache: the code of its dtype, the block's positions, and the scales' strides."""
-    code = _CODES.get(k_pages.dtype)
-    if k_scales is None or v_scales is None or code is None or v_pages.dtype != k_pages.dtype:
-        raise ValueError(f"{what}: a cache in 8 bits has pages of one dtype, float8_e4m3fn or int8, and k_scales and v_scales")
-    pool, page, hk, _ = k_pages.shape
-    shape = k_scales.shape
-    if (k_scales.dtype is not torch.float8_e8m0fnu or v_scales.dtype is not torch.float8_e8m0fnu or len(shape) != 3
-            or v_scales.shape != shape or shape[0] != pool or shape[2] != hk or shape[1] < 1 or page % shape[1]):
-        raise ValueError(f"{what}: the scales must be float8_e8m0fnu [pages, blocks of a page, Hk], keys and values alike")
-    return code, page // shape[1], k_scales.stride(), v_scales.stride()
+_DESCRIPTION = struct.Struct("6Q13q8i")  # BpPagedCache of byteprof_amd.h
+_I32 = torch.int32
 
 
-def _aligned(what: str, k_pages: torch.Tensor, v_pages: torch.Tensor, unit: int) -> None:
-    """Refuses caches whose rows do not lie on multiples of 8 elements (of `unit` bytes in all)."""
-    kst, vst = k_pages.stride(), v_pages.stride()
-    if (k_pages.data_ptr() | v_pages.data_ptr()) & (unit - 1) or (
-            kst[0] | kst[1] | kst[2] | vst[0] | vst[1] | vst[2]) & 7 and any(
-            n > 1 and (a | b) & 7 for n, a, b in zip(k_pages.shape[:3], kst, vst)):
-        raise ValueError(f"{what}: the caches must be {unit}-byte aligned, with strides of whole multiples of 8 elements")
+def _cache(what: str, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, cu: torch.Tensor,
+           k_scales: torch.Tensor | None, v_scales: torch.Tensor | None, unit: int) -> tuple:
+    """(the cache's description, pages, page size, Hk, D, positions of a block, sequences, most pages) of a cache in 8 bits, or
+    without scales in 16. unit: rows of codes lie on multiples of so many elements (1: anywhere)."""
+    shape, kst, vst = k_pages.shape, k_pages.stride(), v_pages.stride()
+    if len(shape) != 4 or v_pages.shape != shape or shape[1] < 1:
+        raise ValueError(f"{what}: the caches must be [pages, page size, Hk, D], keys and values alike")
+    pool, page, hk, d = shape
+    dtype = k_pages.dtype
+    if k_scales is None and v_scales is None:
+        code, size, block, scales = _FLOATS.get(dtype), 2, page, (None, None, (0, 0, 0), (0, 0, 0))
+        if code is None or v_pages.dtype is not dtype:
+            raise ValueError(f"{what}: a cache without scales is bfloat16 or float16")
+    else:
+        code, size = _CODES.get(dtype), 1
+        if k_scales is None or v_scales is None or code is None or v_pages.dtype is not dtype:
+            raise ValueError(f"{what}: a cache in 8 bits has pages of one dtype, float8_e4m3fn or int8, and k_scales and v_scales")
+        blocks = k_scales.shape
+        if (k_scales.dtype is not torch.float8_e8m0fnu or v_scales.dtype is not torch.float8_e8m0fnu or len(blocks) != 3
+                or v_scales.shape != blocks or blocks[0] != pool or blocks[2] != hk or blocks[1] < 1 or page % blocks[1]):
+            raise ValueError(f"{what}: the scales must be float8_e8m0fnu [pages, blocks of a page, Hk], keys and values alike")
+        block, scales = page // blocks[1], (k_scales.data_ptr(), v_scales.data_ptr(), k_scales.stride(), v_scales.stride())
+    (k_p, k_t, k_h, k_d), (v_p, v_t, v_h, v_d) = kst, vst
+    if k_d != 1 or v_d != 1:
+        raise ValueError(f"{what}: the caches must be contiguous in the head dimension")
+    k_at, v_at = k_pages.data_ptr(), v_pages.data_ptr()
+    if unit > 1 and ((k_at | v_at) & (unit * size - 1) or (k_p | k_t | k_h | v_p | v_t | v_h) & (unit - 1) and any(
+            n > 1 and (a | b) & (unit - 1) for n, a, b in zip(shape, kst[:3], vst))):
+        raise ValueError(f"{what}: the caches must be {unit * size}-byte aligned, with strides of whole multiples of {unit} elements")
+    if table.dtype is not _I32 or table.dim() != 2 or not (table.is_contiguous() or table.stride(1) == 1):
+        _ints(what, "table", table, 2)
+    if lengths.dtype is not _I32 or lengths.dim() != 1 or not lengths.is_contiguous():
+        _ints(what, "lengths", lengths, 1)
+    if cu.dtype is not _I32 or cu.dim() != 1 or not cu.is_contiguous():
+        _ints(what, "cu", cu, 1)
+    seqs, most = table.shape
+    if lengths.numel() != seqs or cu.numel() != seqs + 1:
+        raise ValueError(f"{what}: table [sequences, pages], lengths [sequences] and cu [sequences + 1] disagree")
+    if most * page >= 1 << 29:
+        raise ValueError(f"{what}: a sequence may have fewer than 2 ** 29 positions")
+    ks, vs, ks_st, vs_st = scales
+    described = _DESCRIPTION.pack(k_at, v_at, ks or 0, vs or 0, table.data_ptr(), lengths.data_ptr(), table.stride()[0], k_p, k_t, k_h,
+                                  v_p, v_t, v_h, *ks_st, *vs_st, code, seqs, pool, page, block, most, hk, d)
+    return described, pool, page, hk, d, block, seqs, most
 
 
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor,
@@ -261,8 +289,7 @@ def _paged_attention8(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Ten
     what = "paged_attention"
     if q.dim() != 3:
         raise ValueError(f"{what}: q must be [tokens, Hq, D]")
-    (pool, page, hk, dk), kst, vst, seqs, most, row = _pages(what, k_pages, v_pages, table, lengths, cu)
-    code, block, ksst, vsst = _codes(what, k_pages, v_pages, k_scales, v_scales)
+    cache, _, page, hk, dk, block, seqs, most = _cache(what, k_pages, v_pages, table, lengths, cu, k_scales, v_scales, 8)
     if block % 4:
         raise ValueError(f"{what}: a block must have a multiple of 4 positions, not {block}")
     tokens, hq, d = q.shape
@@ -270,7 +297,6 @@ def _paged_attention8(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Ten
     if dtype is None:
         raise ValueError(f"{what}: q must be bfloat16 or float16")
     _heads(what, hq, hk, d, dk)
-    _aligned(what, k_pages, v_pages, 8)
     index = _same_device(what, q, k_pages, v_pages, k_scales, v_scales, table, lengths, cu, out)
     if q.requires_grad or k_pages.requires_grad or v_pages.requires_grad or forward_ad._current_level >= 0:
         _no_derivative(what, q, k_pages, v_pages)
@@ -281,10 +307,8 @@ def _paged_attention8(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Ten
         return y
     ws, need = _workspace(tokens, seqs, hq, hk, d, page * most, q.device, "bp_attn_paged8_workspace_bytes")
     q_t, q_h, _ = q.stride()
-    _launch(index, "bp_attn_paged8", dtype, code, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), k_scales.data_ptr(),
-            v_scales.data_ptr(), y.data_ptr(), table.data_ptr(), row, lengths.data_ptr(), cu.data_ptr(), tokens, seqs, pool, page,
-            block, most, hq, hk, d, q_t, q_h, kst[0], kst[1], kst[2], vst[0], vst[1], vst[2], *ksst, *vsst, scale, _lib.ptr(ws),
-            need)
+    _launch(index, "bp_attn_paged8", cache, dtype, q.data_ptr(), y.data_ptr(), cu.data_ptr(), tokens, hq, q_t, q_h, scale,
+            _lib.ptr(ws), need)
     return y
 
 
@@ -329,16 +353,14 @@ def _paged_append8(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pa
     what = "paged_append"
     if k.dim() != 3 or v.shape != k.shape:
         raise ValueError(f"{what}: k and v must be [tokens, Hk, D]")
-    (pool, page, hk, d), kst, vst, seqs, most, row = _pages(what, k_pages, v_pages, table, lengths, cu)
-    code, block, ksst, vsst = _codes(what, k_pages, v_pages, k_scales, v_scales)
+    cache, _, _, hk, d, _, _, _ = _cache(what, k_pages, v_pages, table, lengths, cu, k_scales, v_scales, 1)
     tokens, heads, dim = k.shape
     if heads != hk or dim != d:
         raise ValueError(f"{what}: the caches hold {hk} heads of {d}, k and v {heads} of {dim}")
     dtype = _VALUES.get(k.dtype)
     if dtype is None or v.dtype != k.dtype:
         raise ValueError(f"{what}: k and v must share one dtype, bfloat16, float16 or float32")
-    k_t, k_h, k_d = k.stride()
-    v_t, v_h, v_d = v.stride()
+    (k_t, k_h, k_d), (v_t, v_h, v_d) = k.stride(), v.stride()
     if (k_d != 1 or v_d != 1) and k.numel():
         raise ValueError(f"{what}: k and v must be contiguous in the head dimension")
     index = _same_device(what, k, v, k_pages, v_pages, k_scales, v_scales, table, lengths, cu)
@@ -346,9 +368,7 @@ def _paged_append8(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pa
         _no_derivative(what, k, v, k_pages, v_pages)
     if tokens == 0 or hk == 0 or d == 0:
         return
-    _launch(index, "bp_paged_append8", dtype, code, k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
-            k_scales.data_ptr(), v_scales.data_ptr(), table.data_ptr(), row, lengths.data_ptr(), cu.data_ptr(), tokens, seqs, pool,
-            page, block, most, hk, d, k_t, k_h, v_t, v_h, kst[0], kst[1], kst[2], vst[0], vst[1], vst[2], *ksst, *vsst)
+    _launch(index, "bp_paged_append8", cache, dtype, k.data_ptr(), v.data_ptr(), cu.data_ptr(), tokens, k_t, k_h, v_t, v_h)
     increment_version((k_pages, v_pages, k_scales, v_scales))
 
 
@@ -357,34 +377,26 @@ def paged_read(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor
                dtype: torch.dtype | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """The way back of paged_append: of each sequence b its last cu[b + 1] - cu[b] positions, as (k, v) [tokens, Hk, D], new
     tensors. A 16-bit cache (bf16 or fp16) gives its values in its own dtype; an 8-bit one (with k_scales and v_scales) code x
-    scale in `dtype`: bf16 (by default; exact), fp16 (past its range 65504) or fp32. Tokens of no sequence and positions outside the table come out as
-    zeros, those of a page outside the cache as NaN."""
+    scale in `dtype`: bf16 (by default; exact), fp16 (past its range 65504) or fp32. Tokens of no sequence and positions outside the
+    table come out as zeros, those of a page outside the cache as NaN."""
     what = "paged_read"
-    (pool, page, hk, d), kst, vst, seqs, most, row = _pages(what, k_pages, v_pages, table, lengths, cu)
-    ks = vs = None
-    block, ksst, vsst = page, (0, 0, 0), (0, 0, 0)
-    if k_scales is not None or v_scales is not None:
-        code, block, ksst, vsst = _codes(what, k_pages, v_pages, k_scales, v_scales)
-        dtype = torch.bfloat16 if dtype is None else dtype
-        kind = _VALUES.get(dtype)
-        if kind is None:
-            raise ValueError(f"{what}: dtype must be bfloat16, float16 or float32")
-        ks, vs = k_scales.data_ptr(), v_scales.data_ptr()
-    else:
-        dtype = k_pages.dtype if dtype is None else dtype
-        kind = code = _FLOATS.get(dtype)
-        if code is None or k_pages.dtype != dtype or v_pages.dtype != dtype:
-            raise ValueError(f"{what}: a cache without scales is bfloat16 or float16 and is read in its own dtype")
+    cache, _, _, hk, d, _, _, _ = _cache(what, k_pages, v_pages, table, lengths, cu, k_scales, v_scales, 8)
+    if k_scales is None:
+        if dtype is not None and dtype is not k_pages.dtype:
+            raise ValueError(f"{what}: a cache without scales is read in its own dtype")
+        dtype = k_pages.dtype
+    elif dtype is None:
+        dtype = torch.bfloat16
+    kind = _VALUES.get(dtype)
+    if kind is None:
+        raise ValueError(f"{what}: dtype must be bfloat16, float16 or float32")
     if tokens < 0 or d % 8:
         raise ValueError(f"{what}: tokens must not be negative, and head_dim must be a multiple of 8")
-    _aligned(what, k_pages, v_pages, 8 * k_pages.element_size())
     index = _same_device(what, k_pages, v_pages, k_scales, v_scales, table, lengths, cu)
     if k_pages.requires_grad or v_pages.requires_grad or forward_ad._current_level >= 0:
         _no_derivative(what, k_pages, v_pages)
     k = torch.empty((tokens, hk, d), dtype=dtype, device=k_pages.device)
-    v = torch.empty((tokens, hk, d), dtype=dtype, device=k_pages.device)
-    if k.numel():
-        _launch(index, "bp_paged_read", kind, code, k_pages.data_ptr(), v_pages.data_ptr(), ks, vs, k.data_ptr(), v.data_ptr(),
-                table.data_ptr(), row, lengths.data_ptr(), cu.data_ptr(), tokens, seqs, pool, page, block, most, hk, d, kst[0],
-                kst[1], kst[2], vst[0], vst[1], vst[2], *ksst, *vsst)
+    v = torch.empty_like(k)
+    if tokens and hk and d:
+        _launch(index, "bp_paged_read", cache, kind, k.data_ptr(), v.data_ptr(), cu.data_ptr(), tokens)
     return k, v

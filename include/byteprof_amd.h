@@ -458,44 +458,45 @@ int bp_paged_append(int element_bytes, const void* k, const void* v, void* k_pag
                     int64_t kp_t, int64_t kp_h, int64_t vp_p, int64_t vp_t, int64_t vp_h, void* stream);
 
 /*
- * The same cache held in 8 bits: codes (cache_dtype BP_DT_E4M3 or BP_DT_I8) [pool, page, hk, head_dim] and, for each block of
- * `block` positions of a page and each head, the exponent of a power of two, [pool, page / block, hk] (uint8, bias 127, 255: NaN):
- * a value is code x 2^(byte - 127). Strides in elements (bytes); the innermost of the codes is 1. page a multiple of block.
+ * A cache of bp_attn_paged, described once for the functions below: 16 bits (dtype BP_DT_BF16 or F16) or 8 (BP_DT_E4M3 or BP_DT_I8).
+ * In 8 bits, k_pages and v_pages hold codes, and k_scales, v_scales, for each block of `block` positions of a page (page a multiple of
+ * block) and each head, the exponent of a power of two, [pool, page / block, hk] (uint8, bias 127; 255: NaN): a value is
+ * code x 2^(byte - 127). Strides in elements (kp, vp: between pages, positions and heads; ks, vs: between pages, blocks and heads);
+ * head_dim is contiguous. A 16-bit cache has neither scales nor block (both ignored).
+ */
+typedef struct BpPagedCache {
+  const void *k_pages, *v_pages, *k_scales, *v_scales; /* written by bp_paged_append8 */
+  const int32_t *table, *lengths;                       /* [seqs, table_stride], [seqs] */
+  int64_t table_stride;
+  int64_t kp[3], vp[3], ks[3], vs[3];
+  int32_t dtype, seqs, pool, page, block, max_pages, hk, head_dim;
+} BpPagedCache;
+
+/*
+ * append8 (a cache in 8 bits): k, v [tokens, hk, head_dim] (dtype BP_DT_BF16, F16 or F32) to the positions that bp_paged_append gives
+ * them. A block's scale becomes the least power of two s with |x| <= 448 s (E4M3) or 127 s (I8) for all its new values (infinities
+ * and NaN aside); where the block holds positions from before the chunk, no less than it was, and if it grows their codes are
+ * rounded to it again. A code is x / s to the nearest, ties to even; infinities give the greatest code, NaN gives NaN (E4M3) or 0
+ * (I8). The other positions of a block keep their codes. A block must belong to one sequence of the call only.
  *
- * append8: k, v [tokens, hk, head_dim] (dtype BP_DT_BF16, F16 or F32) to the positions that bp_paged_append gives them. A block's
- * scale becomes the least power of two s with |x| <= 448 s (E4M3) or 127 s (I8) for all its new values (infinities and NaN aside);
- * where the block holds positions from before the chunk, no less than it was, and if it grows their codes are rounded to it again.
- * A code is x / s to the nearest, ties to even; infinities give the greatest code, NaN gives NaN (E4M3) or 0 (I8). The other
- * positions of a block keep their codes. A block must belong to one sequence of the call only.
+ * paged8 (a cache in 8 bits): bp_attn_paged over codes, which become values of q's dtype exactly (BP_DT_F16: those past fp16's range
+ * become its greatest, 65504, those below its least are rounded; E4M3 scales past 2^22 count as 2^22). block a multiple of 4; the
+ * codes' bases and the strides of dimensions of more than one entry multiples of 8. workspace:
+ * bp_attn_paged8_workspace_bytes(tokens, seqs, hq, hk, head_dim, page x max_pages), 16-byte aligned.
  *
- * paged8: bp_attn_paged over codes, which become values of q's dtype exactly (BP_DT_F16: those past fp16's range become its
- * greatest, 65504, those below its least are rounded; E4M3 scales past 2^22 count as 2^22). block a multiple of 4; the codes' bases and the strides of dimensions of more than one entry
- * multiples of 8. workspace: bp_attn_paged8_workspace_bytes(tokens, seqs, hq, hk, head_dim, page x max_pages), 16-byte aligned.
- *
- * read: the positions of bp_paged_append out of the cache, into k, v [tokens, hk, head_dim] (dtype, contiguous, 16-byte aligned):
- * codes x scale (in BP_DT_F16 as for paged8), or (cache_dtype = dtype BP_DT_BF16 or F16; block and scales unused) a 16-bit cache's values. head_dim a multiple
+ * read (either cache): the positions of bp_paged_append out of the cache, into k, v [tokens, hk, head_dim] (contiguous, 16-byte
+ * aligned): codes x scale in dtype BP_DT_BF16, F16 (as for paged8) or F32, or a 16-bit cache's values in its own. head_dim a multiple
  * of 8, rows on multiples of 8 elements. Tokens of no sequence and positions outside the table give zeros, pages outside the cache
  * NaN.
- * No counterpart in the reference.
+ *
+ * cu [seqs + 1] as in bp_attn_paged. No counterpart in the reference.
  */
-int bp_paged_append8(int dtype, int cache_dtype, const void* k, const void* v, void* k_pages, void* v_pages, uint8_t* k_scales,
-                     uint8_t* v_scales, const int32_t* table, int64_t table_stride, const int32_t* lengths, const int32_t* cu,
-                     int tokens, int seqs, int pool, int page, int block, int max_pages, int hk, int head_dim, int64_t k_t,
-                     int64_t k_h, int64_t v_t, int64_t v_h, int64_t kp_p, int64_t kp_t, int64_t kp_h, int64_t vp_p, int64_t vp_t,
-                     int64_t vp_h, int64_t ks_p, int64_t ks_b, int64_t ks_h, int64_t vs_p, int64_t vs_b, int64_t vs_h,
-                     void* stream);
+int bp_paged_append8(const BpPagedCache* cache, int dtype, const void* k, const void* v, const int32_t* cu, int tokens, int64_t k_t,
+                     int64_t k_h, int64_t v_t, int64_t v_h, void* stream);
 size_t bp_attn_paged8_workspace_bytes(int64_t tokens, int64_t seqs, int64_t hq, int64_t hk, int64_t head_dim, int64_t max_keys);
-int bp_attn_paged8(int dtype, int cache_dtype, const void* q, const void* k_pages, const void* v_pages, const uint8_t* k_scales,
-                   const uint8_t* v_scales, void* out, const int32_t* table, int64_t table_stride, const int32_t* lengths,
-                   const int32_t* cu, int tokens, int seqs, int pool, int page, int block, int max_pages, int hq, int hk,
-                   int head_dim, int64_t q_t, int64_t q_h, int64_t k_p, int64_t k_t, int64_t k_h, int64_t v_p, int64_t v_t,
-                   int64_t v_h, int64_t ks_p, int64_t ks_b, int64_t ks_h, int64_t vs_p, int64_t vs_b, int64_t vs_h, float scale,
-                   void* workspace, size_t workspace_bytes, void* stream);
-int bp_paged_read(int dtype, int cache_dtype, const void* k_pages, const void* v_pages, const uint8_t* k_scales,
-                  const uint8_t* v_scales, void* k, void* v, const int32_t* table, int64_t table_stride, const int32_t* lengths,
-                  const int32_t* cu, int tokens, int seqs, int pool, int page, int block, int max_pages, int hk, int head_dim,
-                  int64_t kp_p, int64_t kp_t, int64_t kp_h, int64_t vp_p, int64_t vp_t, int64_t vp_h, int64_t ks_p, int64_t ks_b,
-                  int64_t ks_h, int64_t vs_p, int64_t vs_b, int64_t vs_h, void* stream);
+int bp_attn_paged8(const BpPagedCache* cache, int dtype, const void* q, void* out, const int32_t* cu, int tokens, int hq, int64_t q_t,
+                   int64_t q_h, float scale, void* workspace, size_t workspace_bytes, void* stream);
+int bp_paged_read(const BpPagedCache* cache, int dtype, void* k, void* v, const int32_t* cu, int tokens, void* stream);
 
 /*
  * Rotary positions: of every head of q [tokens, hq, head_dim] and k [tokens, hk, head_dim] (BP_DT_BF16, F16 or F32; hq or hk may

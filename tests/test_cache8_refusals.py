@@ -84,10 +84,11 @@ def test_append_refusals(change, match):
 @pytest.mark.parametrize("change,match", BAD_CACHE + [
     ({"dtype": E4M3}, "dtype must be"),
     ({"tokens": -1}, "must not be negative"),
-    ({"k_pages": z(3, 16, 1, 60, dtype=E4M3), "v_pages": z(3, 16, 1, 60, dtype=E4M3)}, "multiple of 8"),
+    ({"k_pages": z(3, 16, 1, 60, dtype=E4M3), "v_pages": z(3, 16, 1, 60, dtype=E4M3)}, "multiple"),
+    ({"k_pages": z(3, 16, 1, 64, dtype=E4M3)[..., :60], "v_pages": z(3, 16, 1, 64, dtype=E4M3)[..., :60]}, "head_dim must be"),
     ({"k_scales": None, "v_scales": None}, "without scales"),
     ({"k_scales": None, "v_scales": None, "k_pages": z(3, 16, 1, 64), "v_pages": z(3, 16, 1, 64), "dtype": FP}, "own dtype"),
-    ({"k_scales": None, "v_scales": None, "k_pages": z(3, 16, 1, 64), "v_pages": z(3, 16, 1, 64, dtype=FP)}, "own dtype"),
+    ({"k_scales": None, "v_scales": None, "k_pages": z(3, 16, 1, 64), "v_pages": z(3, 16, 1, 64, dtype=FP)}, "without scales"),
 ])
 def test_read_refusals(change, match):
     with pytest.raises(ValueError, match=match):
@@ -156,49 +157,75 @@ def test_rotary_frequencies():
             rotary_frequencies(**bad)
 
 
-def test_attention_entry_refuses_before_any_launch(L):
-    p, odd = ctypes.c_void_p(64), ctypes.c_void_p(68)  # never dereferenced
+class Cache(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k_pages", "v_pages", "k_scales", "v_scales", "table", "lengths")] + [
+        ("table_stride", ctypes.c_int64)] + [(n, ctypes.c_int64 * 3) for n in ("kp", "vp", "ks", "vs")] + [
+        (n, ctypes.c_int32) for n in ("dtype", "seqs", "pool", "page", "block", "max_pages", "hk", "head_dim")]
 
-    def attn(dtype=0, kind=4, q=p, k=p, ks=p, out=ctypes.c_void_p(1 << 20), table=p, lengths=p, cu=p, tokens=4, seqs=1, pool=4, page=16, block=16,
-             pages=4, hq=2, hk=1, d=64, k_t=64, scale=0.1, ws=None, n=0):
-        return L.bp_attn_paged8(dtype, kind, q, k, p, ks, p, out, table, 4, lengths, cu, tokens, seqs, pool, page, block, pages, hq,
-                                hk, d, 128, 64, 1024, k_t, 64, 1024, 64, 64, 1, 1, 1, 1, 1, 1, scale, ws, n, None)
+
+def described(**kw):
+    """A cache whose addresses are never dereferenced."""
+    c = Cache(64, 64, 64, 64, 64, 64, 4, (1024, 64, 64), (1024, 64, 64), (1, 1, 1), (1, 1, 1), 4, 1, 4, 16, 16, 4, 1, 64)
+    for name, value in kw.items():
+        setattr(c, name, (ctypes.c_int64 * 3)(*value) if isinstance(value, tuple) else value)
+    return ctypes.byref(c)
+
+
+def test_the_description_is_the_headers():
+    assert ctypes.sizeof(Cache) == A._DESCRIPTION.size == 6 * 8 + 13 * 8 + 8 * 4
+    packed = A._DESCRIPTION.pack(*range(1, 28))
+    c = Cache.from_buffer_copy(packed)
+    assert (c.k_pages, c.lengths, c.table_stride, list(c.kp), list(c.vs), c.dtype, c.head_dim) == (1, 6, 7, [8, 9, 10], [17, 18, 19], 20, 27)
+
+
+def test_attention_entry_refuses_before_any_launch(L):
+    p = ctypes.c_void_p(64)
+
+    def attn(dtype=0, q=p, out=ctypes.c_void_p(1 << 20), cu=p, tokens=4, hq=2, scale=0.1, ws=None, n=0, cache=None, **kw):
+        return L.bp_attn_paged8(described(**kw), dtype, q, out, cu, tokens, hq, 128, 64, scale, ws, n, None)
 
     assert attn(tokens=0) == 0
-    assert attn(dtype=2) == -2 and attn(kind=0) == -2 and attn(kind=2) == -2 and attn(d=60) == -2 and attn(d=264) == -2
-    assert attn(q=None) == -1 and attn(k=None) == -1 and attn(ks=None) == -1 and attn(table=None) == -1 and attn(cu=None) == -1
-    assert attn(lengths=None) == -1 and attn(pool=0) == -1 and attn(pool=-1) == -1 and attn(pages=-1) == -1 and attn(page=0) == -1
-    assert attn(block=0) == -1 and attn(block=2) == -1 and attn(block=12) == -1 and attn(page=18, block=6) == -1
-    assert attn(k=odd) == -1 and attn(k_t=68) == -1 and attn(hq=3, hk=2) == -1 and attn(scale=0.0) == -1
-    assert attn(page=1 << 20, block=16, pages=1 << 12) == -1
-    assert attn(tokens=1 << 29) == -2
-    assert attn(page=64, block=64, pages=100) == -3  # 6400 positions may be divided: no workspace
-    assert attn(out=p) == -1  # overlaps the codes
+    assert L.bp_attn_paged8(None, 0, p, p, p, 4, 2, 128, 64, 0.1, None, 0, None) == -1
+    for kw in ({"dtype": 2}, {"head_dim": 60}, {"head_dim": 264}, {"tokens": 1 << 29}):
+        assert attn(**kw) == -2, kw
+    for kind in (0, 2):
+        assert L.bp_attn_paged8(described(dtype=kind), 0, p, ctypes.c_void_p(1 << 20), p, 4, 2, 128, 64, 0.1, None, 0, None) == -2
+    for kw in ({"q": None}, {"cu": None}, {"k_pages": None}, {"k_scales": None}, {"table": None}, {"lengths": None}, {"pool": 0},
+               {"pool": -1}, {"seqs": -1}, {"max_pages": -1}, {"page": 0}, {"block": 0}, {"block": 2}, {"block": 12},
+               {"page": 18, "block": 6}, {"k_pages": 68}, {"kp": (1024, 68, 64)}, {"hq": 3, "hk": 2}, {"hk": 0}, {"scale": 0.0},
+               {"page": 1 << 20, "max_pages": 1 << 12}, {"out": p}):
+        assert attn(**kw) == -1, kw
+    assert attn(page=64, block=64, max_pages=100) == -3  # 6400 positions may be divided: no workspace
+    need = L.bp_attn_paged8_workspace_bytes(4, 1, 2, 1, 64, 6400)
+    assert need > 0 and attn(page=64, block=64, max_pages=100, ws=p, n=need - 1) == -3
+    assert L.bp_attn_paged8_workspace_bytes(4, 1, 2, 1, 64, 256) == 0 and L.bp_attn_paged8_workspace_bytes(4, 1, 3, 2, 64, 6400) == 0
 
 
 def test_append_and_read_entries_refuse_before_any_launch(L):
     p, odd = ctypes.c_void_p(64), ctypes.c_void_p(68)
 
-    def append(dtype=0, kind=4, k=p, ks=p, table=p, tokens=4, seqs=1, pool=4, page=16, block=8, pages=4, hk=1, d=64):
-        return L.bp_paged_append8(dtype, kind, k, p, p, p, ks, p, table, 4, p, p, tokens, seqs, pool, page, block, pages, hk, d,
-                                  *([64] * 16), None)
+    def append(dtype=0, k=p, tokens=4, cu=p, **kw):
+        return L.bp_paged_append8(described(**kw), dtype, k, p, cu, tokens, 64, 64, 64, 64, None)
 
-    assert append(dtype=3) == -2 and append(kind=0) == -2 and append(k=None) == -1 and append(ks=None) == -1
-    assert append(table=None) == -1 and append(tokens=-1) == -1 and append(page=0) == -1 and append(block=0) == -1
-    assert append(block=5) == -1 and append(page=1 << 20, block=16, pages=1 << 10) == -1
-    assert append(tokens=0) == 0 and append(seqs=0) == 0 and append(pool=0) == 0 and append(pages=0) == 0 and append(d=0) == 0
-    assert append(hk=1 << 29) == -2 and append(page=1 << 16, block=1 << 16, d=1 << 15) == -2
+    assert append(dtype=3) == -2 and append(hk=1 << 29) == -2 and append(page=1 << 16, block=1 << 16, head_dim=1 << 15) == -2
+    assert L.bp_paged_append8(described(dtype=0), 0, p, p, p, 4, 64, 64, 64, 64, None) == -2
+    assert L.bp_paged_append8(None, 0, p, p, p, 4, 64, 64, 64, 64, None) == -1
+    for kw in ({"k": None}, {"k_scales": None}, {"table": None}, {"cu": None}, {"tokens": -1}, {"page": 0}, {"block": 0}, {"block": 5},
+               {"page": 1 << 20, "max_pages": 1 << 10}, {"seqs": -1}):
+        assert append(**kw) == -1, kw
+    for kw in ({"tokens": 0}, {"seqs": 0}, {"pool": 0}, {"max_pages": 0}, {"head_dim": 0}, {"hk": 0}):
+        assert append(**kw) == 0, kw
 
-    def read(dtype=0, kind=4, kp=p, ks=p, k=p, table=p, cu=p, tokens=4, seqs=1, pool=4, page=16, block=8, pages=4, hk=2, d=64, p_t=64):
-        return L.bp_paged_read(dtype, kind, kp, p, ks, p, k, p, table, 4, p, cu, tokens, seqs, pool, page, block, pages, hk, d, 64,
-                               p_t, *([64] * 10), None)
+    def read(dtype=0, k=p, cu=p, tokens=4, **kw):
+        return L.bp_paged_read(described(**kw), dtype, k, p, cu, tokens, None)
 
-    assert read(dtype=3) == -2 and read(kind=0, dtype=1) == -2 and read(kind=2, dtype=2) == -2 and read(d=60) == -2
-    assert read(kp=None) == -1 and read(ks=None) == -1 and read(k=None) == -1 and read(table=None) == -1 and read(cu=None) == -1
-    assert read(block=5) == -1 and read(block=0) == -1 and read(page=0) == -1 and read(tokens=-1) == -1
-    assert read(k=odd) == -1 and read(kp=odd) == -1 and read(p_t=68) == -1
+    assert read(dtype=3) == -2 and read(head_dim=60) == -2 and read(tokens=1 << 28, hk=8) == -2
+    assert L.bp_paged_read(described(dtype=0), 1, p, p, p, 4, None) == -2 and L.bp_paged_read(described(dtype=2), 2, p, p, p, 4, None) == -2
+    assert L.bp_paged_read(None, 0, p, p, p, 4, None) == -1
+    for kw in ({"k_pages": None}, {"k_scales": None}, {"k": None}, {"table": None}, {"cu": None}, {"block": 5}, {"block": 0}, {"page": 0},
+               {"tokens": -1}, {"k": odd}, {"k_pages": 68}, {"kp": (1024, 68, 64)}):
+        assert read(**kw) == -1, kw
     assert read(tokens=0) == 0 and read(hk=0) == 0
-    assert read(tokens=1 << 28, hk=8) == -2
 
 
 def test_rotary_entry_refuses_before_any_launch(L):
