@@ -110,7 +110,7 @@ SIGNATURES: dict[str, tuple] = {
     "bp_attn_paged8_workspace_bytes": (_c_size, [_c_i64] * 6),
     "bp_attn_paged8": (_c_int, [_c_vp, _c_int] + [_c_vp] * 3 + [_c_int] * 2 + [_c_i64] * 2 + [_c_float, _c_vp, _c_size, _c_vp]),
     "bp_paged_read": (_c_int, [_c_vp, _c_int] + [_c_vp] * 3 + [_c_int, _c_vp]),
-    "bp_rotary": (_c_int, [_c_int] + [_c_vp] * 5 + [_c_int, _c_vp, _c_i64] + [_c_int] * 5 + [_c_float] + [_c_i64] * 8 + [_c_vp]),
+    "bp_rotary": (_c_int, [_c_vp, _c_vp]),
     "bp_logprobs_workspace_bytes": (_c_size, [_c_int, _c_i64, _c_i64, _c_int]),
     "bp_logprobs": (_c_int, [_c_int, _c_vp, _c_i64] + [_c_vp] * 5 + [_c_i64, _c_i64, _c_int, _c_vp, _c_size, _c_vp]),
 }

@@ -52,21 +52,28 @@ struct Args {
   float factor;
 };
 
-// V elements as a vector of 16 bytes, or one.
+// V elements: 16, 8 or 4 bytes, or one element.
 template <class T, int V>
 struct Piece {
-  uint32_t w[V == 1 ? 1 : 4];
+  static constexpr int BYTES = V * static_cast<int>(sizeof(typename T::Bits)), W = BYTES < 4 ? 1 : BYTES / 4;
+  typedef uint32_t Words __attribute__((ext_vector_type(W)));
+  uint32_t w[W];
   __device__ __forceinline__ void load(const typename T::Bits* p) {
-    if constexpr (V == 1) w[0] = *p;
+    if constexpr (BYTES < 4) w[0] = *p;
     else {
-      const u32x4 x = *reinterpret_cast<const u32x4*>(p);
+      const Words x = *reinterpret_cast<const Words*>(p);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = x[i];
+      for (int i = 0; i < W; ++i) w[i] = x[i];
     }
   }
   __device__ __forceinline__ void store(typename T::Bits* p) const {
-    if constexpr (V == 1) *p = static_cast<typename T::Bits>(w[0]);
-    else *reinterpret_cast<u32x4*>(p) = u32x4{w[0], w[1], w[2], w[3]};
+    if constexpr (BYTES < 4) *p = static_cast<typename T::Bits>(w[0]);
+    else {
+      Words x;
+#pragma unroll
+      for (int i = 0; i < W; ++i) x[i] = w[i];
+      *reinterpret_cast<Words*>(p) = x;
+    }
   }
   __device__ __forceinline__ float get(int e) const {
     if constexpr (V == 1 || sizeof(typename T::Bits) == 4) return T::value(w[e]);
@@ -78,8 +85,8 @@ struct Piece {
   }
 };
 
-// A piece of work: V pairs of a head (two vectors, V columns apart by rot / 2; interleaved: two neighbouring vectors, or one pair of
-// elements), or V columns (interleaved: 2 V) that do not turn.
+// A piece of work: V pairs of a head (two vectors, rot / 2 columns apart; interleaved: two neighbouring ones), or V columns that do
+// not turn.
 template <class T, int V, bool INTER>
 __global__ __launch_bounds__(kThreads) void rotary_kernel(Args a) {
   __shared__ float2 turns[kPairs];  // cosine and sine, times factor
@@ -129,18 +136,19 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(Args a) {
   }
 }
 
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+template <class T, int V>
+void launch_of(const Args& a, bool inter, unsigned grid, hipStream_t st) {
+  if (inter) rotary_kernel<T, V, true><<<grid, kThreads, 0, st>>>(a);
+  else rotary_kernel<T, V, false><<<grid, kThreads, 0, st>>>(a);
+}
 
 template <class T>
 void launch(const Args& a, int v, bool inter, unsigned grid, hipStream_t st) {
   constexpr int V = 16 / sizeof(typename T::Bits);
-  if (v == 1) {
-    if (inter) rotary_kernel<T, 1, true><<<grid, kThreads, 0, st>>>(a);
-    else rotary_kernel<T, 1, false><<<grid, kThreads, 0, st>>>(a);
-  } else {
-    if (inter) rotary_kernel<T, V, true><<<grid, kThreads, 0, st>>>(a);
-    else rotary_kernel<T, V, false><<<grid, kThreads, 0, st>>>(a);
-  }
+  if (v == V) launch_of<T, V>(a, inter, grid, st);
+  else if (v == V / 2) launch_of<T, V / 2>(a, inter, grid, st);
+  else if (V / 4 > 1 && v == V / 4) launch_of<T, V / 4>(a, inter, grid, st);
+  else launch_of<T, 1>(a, inter, grid, st);
 }
 
 // Whether the elements of two tensors [tokens, heads, d] are apart: their ranges are, or they have one token stride and lie in
@@ -157,14 +165,14 @@ bool apart(const void* p, int64_t p_t, int64_t p_row, const void* q, int64_t q_t
 }  // namespace rotary
 }  // namespace bp
 
-extern "C" int bp_rotary(int dtype, const void* q, const void* k, void* q_out, void* k_out, const void* positions,
-                         int position_bytes, const float* inv_freq, int64_t tokens, int hq, int hk, int head_dim, int rot,
-                         int interleaved, float factor, int64_t q_t, int64_t q_h, int64_t k_t, int64_t k_h, int64_t qo_t,
-                         int64_t qo_h, int64_t ko_t, int64_t ko_h, void* stream) {
+extern "C" int bp_rotary(const BpRotary* rotary, void* stream) {
   using namespace bp::rotary;
+  if (rotary == nullptr) return BP_E_INVALID_ARG;
+  const auto [q, k, q_out, k_out, positions, inv_freq, tokens, q_st, k_st, qo_st, ko_st, dtype, position_bytes, hq, hk, head_dim, rot,
+              interleaved, factor] = *rotary;
   if (dtype != BP_DT_BF16 && dtype != BP_DT_F16 && dtype != BP_DT_F32) return BP_E_UNSUPPORTED;
   if (tokens < 0 || hq < 0 || hk < 0 || head_dim < 0 || rot < 0 || rot % 2 != 0 || rot > head_dim ||
-      (position_bytes != 4 && position_bytes != 8) || !(fabsf(factor) <= 3.0e38f) || (q_t | q_h | k_t | k_h) < 0)
+      (position_bytes != 4 && position_bytes != 8) || !(fabsf(factor) <= 3.0e38f) || (q_st[0] | q_st[1] | k_st[0] | k_st[1]) < 0)
     return BP_E_INVALID_ARG;
   if (head_dim > kMaxDim) return BP_E_UNSUPPORTED;
   if (tokens == 0 || hq + hk == 0 || head_dim == 0) return BP_OK;
@@ -174,11 +182,12 @@ extern "C" int bp_rotary(int dtype, const void* q, const void* k, void* q_out, v
   Args a = {};
   const int heads[2] = {hq, hk};
   a.in[0] = q, a.in[1] = k, a.out[0] = q_out, a.out[1] = k_out;
-  a.in_t[0] = q_t, a.in_t[1] = k_t, a.in_h[0] = q_h, a.in_h[1] = k_h;
-  a.out_t[0] = qo_t, a.out_t[1] = ko_t, a.out_h[0] = qo_h, a.out_h[1] = ko_h;
+  a.in_t[0] = q_st[0], a.in_t[1] = k_st[0], a.in_h[0] = q_st[1], a.in_h[1] = k_st[1];
+  a.out_t[0] = qo_st[0], a.out_t[1] = ko_st[0], a.out_h[0] = qo_st[1], a.out_h[1] = ko_st[1];
   const int size = dtype == BP_DT_F32 ? 4 : 2, V = 16 / size;
   int64_t odd = 0;
-  bool base = true, in_place = true;
+  uintptr_t at = 0;
+  bool in_place = true;
   for (int w = 0; w < 2; ++w) {
     if (heads[w] == 0) continue;
     // a stride that nothing is multiplied with may be anything
@@ -190,10 +199,11 @@ extern "C" int bp_rotary(int dtype, const void* q, const void* k, void* q_out, v
     const bool by_head = t >= head_dim && h >= (tokens - 1) * t + head_dim;
     if (!by_token && !by_head) return BP_E_INVALID_ARG;
     odd |= a.in_t[w] | a.in_h[w] | t | h;
-    base = base && aligned16(a.in[w]) && aligned16(a.out[w]);
+    at |= reinterpret_cast<uintptr_t>(a.in[w]) | reinterpret_cast<uintptr_t>(a.out[w]);
     in_place = in_place && a.in[w] == a.out[w] && a.in_t[w] == t && a.in_h[w] == h;
   }
-  const auto row = [&](int w, int64_t h) { return size * ((heads[w] - 1) * h + head_dim); };
+  const int64_t dim = head_dim;
+  const auto row = [&](int w, int64_t h) { return size * ((heads[w] - 1) * h + dim); };
   for (int o = 0; o < 2; ++o) {
     if (heads[o] == 0) continue;
     for (int i = 0; i < 4; ++i) {
@@ -212,8 +222,10 @@ extern "C" int bp_rotary(int dtype, const void* q, const void* k, void* q_out, v
   a.positions = positions, a.wide_positions = position_bytes == 8, a.inv_freq = inv_freq;
   a.tokens = tokens, a.hq = hq, a.rot = rot, a.factor = factor;
   const bool inter = interleaved != 0;
-  const int step = 2 * V;  // of the columns that turn, in vectors
-  const int v = base && odd % V == 0 && head_dim % V == 0 && rot % step == 0 ? V : 1;
+  // The widest vectors that rows, halves and heads are made of. (5000 tokens of 40 heads of 128: halves of 64 or 32 17 to 19 us, of 36 21, of 45,
+  // an element at a time, 49.)
+  int v = V;
+  while (v > 1 && !(at % (v * size) == 0 && odd % v == 0 && head_dim % v == 0 && rot % (2 * v) == 0)) v /= 2;
   a.turned = rot / 2 / v;
   a.head = bp::attn::Div::of(a.turned + (in_place ? 0 : (head_dim - rot) / v) > 0 ? a.turned + (in_place ? 0 : (head_dim - rot) / v) : 1);
   if (a.turned + (in_place ? 0 : (head_dim - rot) / v) == 0) return BP_OK;

@@ -4,6 +4,7 @@ frequencies, scaled for contexts longer than a model was trained on."""
 from __future__ import annotations
 
 import math
+import struct
 
 import torch
 from torch.autograd import forward_ad
@@ -13,6 +14,7 @@ from .. import _lib
 from .attention import _VALUES, _launch, _no_derivative, _same_device, _span
 
 MAX_HEAD_DIM = 1024
+_DESCRIPTION = struct.Struct("6Q9q7if")  # BpRotary of byteprof_amd.h
 
 
 def rotary_frequencies(dim: int, theta: float = 10000.0, *, scaling: str = "none", factor: float = 1.0, trained: int | None = None,
@@ -70,6 +72,33 @@ def _writable(t: torch.Tensor) -> bool:
     return sh >= d and st >= (h - 1) * sh + d or st >= d and sh >= (n - 1) * st + d
 
 
+_POSITIONS = {torch.int64: 8, torch.int32: 4}
+
+
+def _outputs(what: str, q: torch.Tensor, k: torch.Tensor | None, out: tuple) -> tuple:
+    """out as (q_out, k_out), each like its input and of elements of its own."""
+    out = tuple(out)
+    if len(out) != 2 or out[0] is None or (out[1] is None) != (k is None):
+        raise ValueError(f"{what}: out must be (q_out, k_out), as q and k are given")
+    for x, y in zip((q, k), out):
+        if y is not None and (y.shape != x.shape or y.dtype != x.dtype or (
+                y.numel() and (y.stride(2) != 1 and y.shape[2] > 1 or not _writable(y)))):
+            raise ValueError(f"{what}: an output must be like its input, contiguous in the head dimension, each element its own")
+    return out
+
+
+def _apart(what: str, q: torch.Tensor, k: torch.Tensor | None, q_out: torch.Tensor, k_out: torch.Tensor | None,
+           *read: torch.Tensor) -> None:
+    """Refuses outputs that are neither their own input nor apart from everything else."""
+    for y, own, others in ((q_out, q, (k, k_out)), (k_out, k, (q, q_out))):
+        if y is None or not y.numel():
+            continue
+        a, b = _span(y)
+        if not (y.data_ptr() == own.data_ptr() and y.stride() == own.stride()) and not _disjoint(y, own) or not all(
+                t is None or _disjoint(y, t) for t in others) or any(c < b and a < e for c, e in map(_span, read)):
+            raise ValueError(f"{what}: an output must be its own input or apart from everything else")
+
+
 def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv_freq: torch.Tensor, *, interleaved: bool = False,
            factor: float = 1.0, out: tuple | None = None) -> tuple[torch.Tensor, torch.Tensor | None]:
     """q [tokens, Hq, D] and k [tokens, Hk, D] (or None) at positions [tokens] (int64 or int32): of every head, the first
@@ -80,55 +109,44 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv
     of any such strides apart from everything else. Forward only: tensors that require a gradient or carry a forward-mode tangent
     are refused."""
     what = "rotary"
-    if q.dim() != 3 or (k is not None and (k.dim() != 3 or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2])):
+    shape, dtype = q.shape, _VALUES.get(q.dtype)
+    if len(shape) != 3:
         raise ValueError(f"{what}: q must be [tokens, Hq, D] and k [tokens, Hk, D]")
-    tokens, hq, d = q.shape
-    dtype = _VALUES.get(q.dtype)
-    if dtype is None or (k is not None and k.dtype != q.dtype):
+    tokens, hq, d = shape
+    q_st, hk, k_st = q.stride(), 0, (0, 0, 1)
+    if k is not None:
+        k_shape, k_st = k.shape, k.stride()
+        if len(k_shape) != 3 or k_shape[0] != tokens or k_shape[2] != d:
+            raise ValueError(f"{what}: q must be [tokens, Hq, D] and k [tokens, Hk, D]")
+        hk = k_shape[1]
+    if dtype is None or (k is not None and k.dtype is not q.dtype):
         raise ValueError(f"{what}: q and k must share one dtype, bfloat16, float16 or float32")
     if d > MAX_HEAD_DIM:
         raise ValueError(f"{what}: a head may have {MAX_HEAD_DIM} columns, not {d}")
-    if positions.dtype not in (torch.int64, torch.int32) or positions.shape != (tokens,):
+    if positions.dtype not in _POSITIONS or positions.dim() != 1 or positions.numel() != tokens:
         raise ValueError(f"{what}: positions must be int64 or int32 [tokens]")
-    if inv_freq.dtype is not torch.float32 or inv_freq.dim() != 1 or 2 * inv_freq.shape[0] > d:
+    if inv_freq.dtype is not torch.float32 or inv_freq.dim() != 1 or 2 * inv_freq.numel() > d:
         raise ValueError(f"{what}: inv_freq must be float32 [pairs], of at most half of a head's columns")
-    if not math.isfinite(factor) or abs(factor) > 3e38:
+    if not -3e38 <= factor <= 3e38:
         raise ValueError(f"{what}: factor must be finite in float32")
-    given = [t for t in (q, k) if t is not None]
-    if any(t.stride(2) != 1 and d > 1 and t.numel() for t in given):
+    if (q_st[2] != 1 or k_st[2] != 1) and d > 1 and (q.numel() if q_st[2] != 1 else k.numel()):
         raise ValueError(f"{what}: q and k must be contiguous in the head dimension")
-    outs = (None, None) if out is None else tuple(out)
-    if len(outs) != 2 or (out is not None and (outs[0] is None or (outs[1] is None) != (k is None))):
-        raise ValueError(f"{what}: out must be (q_out, k_out), as q and k are given")
-    index = _same_device(what, q, k, positions, inv_freq, *outs)
-    if any(t.requires_grad for t in given) or inv_freq.requires_grad or forward_ad._current_level >= 0:
-        _no_derivative(what, *given, inv_freq)
+    q_out, k_out = (None, None) if out is None else _outputs(what, q, k, out)
+    index = _same_device(what, q, k, positions, inv_freq, q_out, k_out)
+    if q.requires_grad or inv_freq.requires_grad or (k is not None and k.requires_grad) or forward_ad._current_level >= 0:
+        _no_derivative(what, q, inv_freq, *(() if k is None else (k,)))
     positions, inv_freq = positions.contiguous(), inv_freq.contiguous()
     if out is None:
-        outs = tuple(None if t is None else torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k))
+        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        if k is not None:
+            k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
     else:
-        for i, (t, y) in enumerate(zip((q, k), outs)):
-            if y is None:
-                continue
-            if y.shape != t.shape or y.dtype != t.dtype or (y.stride(2) != 1 and d > 1) or (y.numel() and not _writable(y)):
-                raise ValueError(f"{what}: an output must be like its input, contiguous in the head dimension, each element its own")
-            others = [x for j, x in enumerate((q, k)) if x is not None
-                      and not (i == j and x.data_ptr() == y.data_ptr() and x.stride() == y.stride())]
-            others += [x for j, x in enumerate(outs) if x is not None and j != i]
-            a, b = _span(y)
-            apart = all(_disjoint(y, x) for x in others) and all(
-                b <= c or e <= a for c, e in map(_span, (positions, inv_freq)))
-            if y.numel() and not apart:
-                raise ValueError(f"{what}: an output must be its own input or apart from everything else")
-        increment_version([y for y in outs if y is not None])
-    if tokens == 0 or d == 0:
-        return outs
-    (q_t, q_h, _), (qo_t, qo_h, _) = q.stride(), outs[0].stride()
-    hk = k_t = k_h = ko_t = ko_h = 0
-    if k is not None:
-        hk, (k_t, k_h, _), (ko_t, ko_h, _) = k.shape[1], k.stride(), outs[1].stride()
-    if hq + hk:
-        _launch(index, "bp_rotary", dtype, q.data_ptr(), _lib.ptr(k), outs[0].data_ptr(), _lib.ptr(outs[1]), positions.data_ptr(),
-                positions.element_size(), inv_freq.data_ptr(), tokens, hq, hk, d, 2 * inv_freq.shape[0], interleaved, factor, q_t, q_h,
-                k_t, k_h, qo_t, qo_h, ko_t, ko_h)
-    return outs
+        _apart(what, q, k, q_out, k_out, positions, inv_freq)
+        increment_version([y for y in (q_out, k_out) if y is not None])
+    if tokens and d and (hq or hk):
+        k_at, k_out_at, k_out_st = (0, 0, k_st) if k is None else (k.data_ptr(), k_out.data_ptr(), k_out.stride())
+        _launch(index, "bp_rotary", _DESCRIPTION.pack(
+            q.data_ptr(), k_at, q_out.data_ptr(), k_out_at, positions.data_ptr(), inv_freq.data_ptr(), tokens, *q_st[:2], *k_st[:2],
+            *q_out.stride()[:2], *k_out_st[:2], dtype, _POSITIONS[positions.dtype], hq, hk, d, 2 * inv_freq.numel(), interleaved,
+            factor))
+    return q_out, k_out

@@ -507,10 +507,17 @@ int bp_paged_read(const BpPagedCache* cache, int dtype, void* k, void* v, const 
  * from everything else; slices of one projection are apart. 16 bytes at a time where all rows and halves allow.
  * No counterpart in the reference (its decode step's rotation is inside bp_decode_qk_rope_cache).
  */
-int bp_rotary(int dtype, const void* q, const void* k, void* q_out, void* k_out, const void* positions, int position_bytes,
-              const float* inv_freq, int64_t tokens, int hq, int hk, int head_dim, int rot, int interleaved, float factor,
-              int64_t q_t, int64_t q_h, int64_t k_t, int64_t k_h, int64_t qo_t, int64_t qo_h, int64_t ko_t, int64_t ko_h,
-              void* stream);
+typedef struct BpRotary {
+  const void *q, *k;
+  void *q_out, *k_out;
+  const void* positions;
+  const float* inv_freq;
+  int64_t tokens;
+  int64_t q_st[2], k_st[2], q_out_st[2], k_out_st[2]; /* between tokens and between heads */
+  int32_t dtype, position_bytes, hq, hk, head_dim, rot, interleaved;
+  float factor;
+} BpRotary;
+int bp_rotary(const BpRotary* rotary, void* stream);
 
 /*
  * Of every row of logits [rows, vocab] (BP_DT_BF16 / F16 / F32, row_stride elements apart, rows contiguous): logprob [rows] =

@@ -10,6 +10,7 @@ import pytest
 import torch
 
 from byteprof_amd.optim import attention as A
+from byteprof_amd.optim import rotary as R
 from byteprof_amd.optim.rotary import rotary, rotary_frequencies
 
 BF, FP = torch.bfloat16, torch.float16
@@ -233,9 +234,11 @@ def test_rotary_entry_refuses_before_any_launch(L):
 
     def rot(dtype=0, q=q, qo=ctypes.c_void_p(5 << 20), k=k, ko=ctypes.c_void_p(6 << 20), pos=pos, size=8, inv=inv, tokens=4, hq=2, hk=1,
             d=64, r=64, factor=1.0, q_t=128, qo_t=128, qo_h=64):
-        return L.bp_rotary(dtype, q, k, qo, ko, pos, size, inv, tokens, hq, hk, d, r, 0, factor, q_t, 64, 64, 64, qo_t, qo_h, 64, 64,
-                           None)
+        at = lambda p: (p.value if p is not None else 0) or 0  # noqa: E731
+        return L.bp_rotary(R._DESCRIPTION.pack(at(q), at(k), at(qo), at(ko), at(pos), at(inv), tokens, q_t, 64, 64, 64, qo_t, qo_h, 64, 64,
+                                               dtype, size, hq, hk, d, r, 0, factor), None)
 
+    assert L.bp_rotary(None, None) == -1 and R._DESCRIPTION.size == 6 * 8 + 9 * 8 + 8 * 4
     assert rot(tokens=0) == 0 and rot(d=0, r=0) == 0 and rot(hq=0, hk=0) == 0
     assert rot(dtype=3) == -2 and rot(d=1032) == -2
     assert rot(r=63) == -1 and rot(r=66) == -1 and rot(r=-2) == -1 and rot(size=2) == -1 and rot(factor=math.nan) == -1
