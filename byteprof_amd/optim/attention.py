@@ -252,7 +252,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     cache, its chunk's among them (append first). A chunk's tokens are the last positions; each sees all up to its own. Rows
     that no chunk covers come out as zeros. A row that sees a position whose page id is outside the cache is NaN; so may other
     rows of its chunk be. With k_scales and v_scales the caches are 8-bit codes, in blocks of a multiple of 4 positions; they
-    become values of q's dtype exactly (fp16: those past its range become its greatest, 65504).
+    become values of q's dtype exactly (fp16: those past its range become its greatest, 65504, int8 scales below 2 ** -24 count
+    as 0), queries over int8 codes below 2 ** 112.
     Returns [tokens, Hq, D], in `out` when given: q itself or a tensor apart from q and the caches."""
     if k_scales is not None or v_scales is not None:
         return _paged_attention8(q, k_pages, v_pages, table, lengths, cu, k_scales, v_scales, scale, out)
@@ -320,7 +321,7 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     outside the table (also where lengths[b] is past it, which paged_attention takes as the table's end) and pages outside the
     cache are left out. Any dtype of 1, 2 or 4 bytes; the caches' dtype is k's. With k_scales and v_scales (which it writes, too)
     the caches are 8-bit codes and k and v bf16, fp16 or fp32: the codes are the nearest, ties to even, infinities the greatest,
-    NaN stays NaN in e4m3 and is 0 in int8. A block that a chunk writes to must be no other sequence's of the call."""
+    NaN stays NaN in e4m3 and is 0 in int8. A block that a chunk writes to must be its sequence's only, and once in its table."""
     what = "paged_append"
     if k_scales is not None or v_scales is not None:
         return _paged_append8(k, v, k_pages, v_pages, table, lengths, cu, k_scales, v_scales)

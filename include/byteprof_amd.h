@@ -477,11 +477,12 @@ typedef struct BpPagedCache {
  * them. A block's scale becomes the least power of two s with |x| <= 448 s (E4M3) or 127 s (I8) for all its new values (infinities
  * and NaN aside); where the block holds positions from before the chunk, no less than it was, and if it grows their codes are
  * rounded to it again. A code is x / s to the nearest, ties to even; infinities give the greatest code, NaN gives NaN (E4M3) or 0
- * (I8). The other positions of a block keep their codes. A block must belong to one sequence of the call only.
+ * (I8). The other positions of a block keep their codes. A block that is written to must be one sequence's only, and once in its table.
  *
  * paged8 (a cache in 8 bits): bp_attn_paged over codes, which become values of q's dtype exactly (BP_DT_F16: those past fp16's range
- * become its greatest, 65504, those below its least are rounded; E4M3 scales past 2^22 count as 2^22). block a multiple of 4; the
- * codes' bases and the strides of dimensions of more than one entry multiples of 8. workspace:
+ * become its greatest, 65504, those below its least are rounded; E4M3 scales past 2^22 count as 2^22, I8 scales below 2^-24 as 0.
+ * BP_DT_BF16: a value past bf16's range is infinite). I8 codes are multiplied with the queries before their scale: |q| below 2^112.
+ * block a multiple of 4; the codes' bases and the strides of dimensions of more than one entry multiples of 8. workspace:
  * bp_attn_paged8_workspace_bytes(tokens, seqs, hq, hk, head_dim, page x max_pages), 16-byte aligned.
  *
  * read (either cache): the positions of bp_paged_append out of the cache, into k, v [tokens, hk, head_dim] (contiguous, 16-byte
