@@ -12,7 +12,8 @@ product, fused multi-step mLSTM recurrence) as hand-written gfx950 (MI355X) HIP 
 
 and, for several sequences at once (no counterpart in the reference):
 
-  byteprof_amd.optim.attention      packed_attention, paged_append, paged_attention
+  byteprof_amd.optim.attention      packed_attention, paged_append, paged_attention, paged_read
+  byteprof_amd.optim.rotary         rotary, rotary_frequencies
   byteprof_amd.optim.logprobs       token_logprobs
   byteprof_amd.optim.olmo_batch     OlmoBatch
 """

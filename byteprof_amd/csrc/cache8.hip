@@ -241,7 +241,7 @@ struct Read {
 // 16 bits. Positions that the table does not have are zeros, a page outside the pool gives NaN. Where the workgroup's tokens lie is
 // found once for a token, then all of a thread's pieces are asked for before the first is written. Bound by memory: 24 441 positions of
 // 12 heads of 64 columns from int8 to fp16, 113 MB in 25.5 us (4.4 TB/s), two pieces a thread; one 29.5, four 26.5; with the bisection
-// and the table ahead of every piece 34.6. 161 positions 3 us.
+// and the table ahead of every piece 34.6. 161 positions 4 us.
 template <class T, int KIND>
 __global__ __launch_bounds__(kThreads) void read_kernel(Read a) {
   constexpr int kCopy = 2, CHUNKS = std::is_same<T, F32>::value ? 2 : 1, SPAN = kThreads * kPieces;

@@ -4,9 +4,9 @@
 //
 // Angles: at position 10^6 a float32 product is off by up to 0.03, so position x frequency / 2 pi is formed in 64 bits, whole turns are
 // taken off, and the rest goes into sine and cosine in 32 bits. That is done once for a token and frequency, through LDS, and used by
-// all heads. Bound by memory: 8192 tokens of 32 + 8 heads of 128 columns in bf16, 168 MB in 29 us (5.8 TB/s, some of it from the last
-// level's cache); one token 2.4 us, as long as any launch. Vectors are as wide as the halves and the alignment allow, 16 bytes down to an
-// element: 5000 such tokens of 128 turned columns 17 us, of 90 (an odd half, elements) 49.
+// all heads. Bound by memory: 8192 tokens of 32 + 8 heads of 128 columns in bf16, 168 MB in 34.5 us (4.9 TB/s; 29 us where a part is
+// still in the last level's cache); one token 2.2 us, as long as any launch. Vectors are as wide as the halves and the alignment allow,
+// 16 bytes down to an element: 5000 such tokens of 128 turned columns 17 us, of 90 (an odd half, elements) 49.
 
 #include <hip/hip_runtime.h>
 #include <math.h>

@@ -41,8 +41,9 @@ class Generated(NamedTuple):
 
 class OlmoBatch:
     """pages x page positions of cache for every layer of `dec`, of dtype `cache`: bfloat16, or (pages of a multiple of 4 positions)
-    8-bit codes with a scale for each head and block of 16 positions (12, 8 or 4 where 16 does not divide a page). rotary: (inv_freq [head_dim / 2], factor) on the decoder's device; by default the decoder's own frequencies,
-    their angles rounded to float32 as its own loops have them where the cache is bfloat16."""
+    8-bit codes with a scale for each head and block of 16 positions (12, 8 or 4 where 16 does not divide a page). rotary:
+    (inv_freq [head_dim / 2], factor) on the decoder's device; by default the decoder's own frequencies, their angles rounded to
+    float32 as its own loops have them where the cache is bfloat16."""
 
     def __init__(self, dec: OlmoDecoder, pages: int, page: int = 16, *, cache: torch.dtype = torch.bfloat16,
                  rotary: tuple[torch.Tensor, float] | None = None):

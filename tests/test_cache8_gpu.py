@@ -254,6 +254,8 @@ READ = [
     ([500] * 70, [i % 9 for i in range(70)], 64, 32, 1, 64, I8, BF),
     ([600, 20], [600, 20], 256, 64, 2, 256, E4M3, FP),
     ([90, 3], [80, 3], 32, 8, 1, 8, I8, F32),
+    ([1500, 0, 700], [1500, 0, 690], 16, 16, 1, 8, I8, BF),  # a piece a token
+    ([40, 3], [2, 3], 16, 16, 40, 256, E4M3, BF),  # a token of more pieces than a workgroup has
 ]
 
 
