@@ -327,11 +327,13 @@ __global__ __launch_bounds__(kThreads) void read_kernel(Read a) {
 
 bool aligned(const void* p, int n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
+constexpr int64_t kHeld = 8 * kWave;
+
 template <class T, int KIND, int V>
 void append_launch(const Append& a, hipStream_t st) {
   const int64_t pieces = static_cast<int64_t>(a.block.d) * a.row.d, waves = 2ll * a.units * a.hk;
   // a wave holds 512 pieces; past those a workgroup takes the unit, and what is held is still read once
-  if (pieces <= 8 * kWave)
+  if (pieces <= kHeld)
     append8_kernel<T, KIND, V, kWave><<<static_cast<unsigned>((waves + 3) / 4), kThreads, 0, st>>>(a);
   else append8_kernel<T, KIND, V, kThreads><<<static_cast<unsigned>(waves), kThreads, 0, st>>>(a);
 }
@@ -398,8 +400,9 @@ int bp_paged_append8(const BpPagedCache* cache, int dtype, const void* k, const 
   a.row = bp::attn::Div::of(wide ? c.head_dim / 8 : c.head_dim);
   a.tokens = tokens, a.seqs = c.seqs, a.pool = c.pool, a.max_keys = c.page * c.max_pages, a.hk = c.hk, a.d = c.head_dim;
   const int64_t units = tokens / c.block + 2ll * c.seqs;
-  // a unit's pieces, the units with their heads, and positions in 32 bits
-  if (static_cast<int64_t>(c.block) * c.head_dim >= (1ll << 30) || 2 * units * c.hk >= (1ll << 30) || tokens >= (1 << 30))
+  const int64_t threads = static_cast<int64_t>(c.block) * a.row.d <= kHeld ? bp::kWave : kThreads;
+  // a unit's pieces, positions, and a launch's threads in 32 bits
+  if (static_cast<int64_t>(c.block) * c.head_dim >= (1ll << 30) || 2 * units * c.hk >= (1ll << 32) / threads || tokens >= (1 << 30))
     return BP_E_UNSUPPORTED;
   a.units = static_cast<int>(units);
   const hipStream_t st = static_cast<hipStream_t>(stream);
@@ -441,6 +444,16 @@ int bp_paged_read(const BpPagedCache* cache, int dtype, void* k, void* v, const 
     a.s_p[w] = scale_strides[w][0], a.s_b[w] = scale_strides[w][1], a.s_h[w] = scale_strides[w][2];
   }
   if (static_cast<int64_t>(tokens) * c.hk * (c.head_dim / 8) >= (1ll << 30)) return BP_E_UNSUPPORTED;
+  const int64_t out = static_cast<int64_t>(tokens) * c.hk * c.head_dim * (dtype == BP_DT_F32 ? 4 : 2);
+  const auto reach = [&](const int64_t* st, int rows, int last, int bytes) {
+    return bytes * ((c.pool - 1) * st[0] + (rows - 1) * st[1] + (c.hk - 1) * st[2] + last);
+  };
+  if (bp::ranges_overlap(k, out, v, out)) return BP_E_INVALID_ARG;
+  for (int w = 0; w < 2 && !empty; ++w)
+    for (int o = 0; o < 2; ++o)
+      if (bp::ranges_overlap(a.out[o], out, pages[w], reach(page_strides[w], c.page, c.head_dim, size)) ||
+          (codes && bp::ranges_overlap(a.out[o], out, scales[w], reach(scale_strides[w], c.page / c.block, 1, 1))))
+        return BP_E_INVALID_ARG;
   a.cu = cu, a.lengths = c.lengths, a.table = c.table, a.table_stride = c.table_stride;
   a.page = bp::attn::Div::of(c.page), a.block = bp::attn::Div::of(codes ? c.block : c.page);
   a.row = bp::attn::Div::of(c.head_dim / 8), a.token = bp::attn::Div::of(c.hk * (c.head_dim / 8));

@@ -177,7 +177,8 @@ extern "C" int bp_rotary(const BpRotary* rotary, void* stream) {
       (position_bytes != 4 && position_bytes != 8) || !(fabsf(factor) <= 3.0e38f) || (q_st[0] | q_st[1] | k_st[0] | k_st[1]) < 0)
     return BP_E_INVALID_ARG;
   if (head_dim > kMaxDim) return BP_E_UNSUPPORTED;
-  if (tokens == 0 || hq + hk == 0 || head_dim == 0) return BP_OK;
+  const int64_t all = static_cast<int64_t>(hq) + hk;
+  if (tokens == 0 || all == 0 || head_dim == 0) return BP_OK;
   if ((hq > 0 && (q == nullptr || q_out == nullptr)) || (hk > 0 && (k == nullptr || k_out == nullptr)) ||
       (rot > 0 && (positions == nullptr || inv_freq == nullptr)))
     return BP_E_INVALID_ARG;
@@ -224,14 +225,15 @@ extern "C" int bp_rotary(const BpRotary* rotary, void* stream) {
   a.positions = positions, a.wide_positions = position_bytes == 8, a.inv_freq = inv_freq;
   a.tokens = tokens, a.hq = hq, a.rot = rot, a.factor = factor;
   const bool inter = interleaved != 0;
-  // The widest vectors that rows, halves and heads are made of. (5000 tokens of 40 heads of 128: halves of 64 or 32 17 to 19 us, of 36 21, of 45,
-  // an element at a time, 49.)
+  // The widest vectors that rows, halves and heads are made of. (5000 tokens of 40 heads of 128: halves of 64 or 32 17 to 19 us, of 36
+  // 21, of 45, an element at a time, 49.)
   int v = V;
   while (v > 1 && !(at % (v * size) == 0 && odd % v == 0 && head_dim % v == 0 && rot % (2 * v) == 0)) v /= 2;
   a.turned = rot / 2 / v;
-  a.head = bp::attn::Div::of(a.turned + (in_place ? 0 : (head_dim - rot) / v) > 0 ? a.turned + (in_place ? 0 : (head_dim - rot) / v) : 1);
-  if (a.turned + (in_place ? 0 : (head_dim - rot) / v) == 0) return BP_OK;
-  const int64_t pieces = static_cast<int64_t>(a.head.d) * (hq + hk);
+  const int of_head = a.turned + (in_place ? 0 : (head_dim - rot) / v);
+  if (of_head == 0) return BP_OK;
+  a.head = bp::attn::Div::of(of_head);
+  const int64_t pieces = of_head * all;
   if (pieces >= (1 << 24)) return BP_E_UNSUPPORTED;
   a.token = bp::attn::Div::of(static_cast<int>(pieces));
   a.pairs = bp::attn::Div::of(rot > 0 ? rot / 2 : 1);
@@ -241,7 +243,7 @@ extern "C" int bp_rotary(const BpRotary* rotary, void* stream) {
   while (group > 1 && tokens / group < 1024) group /= 2;
   a.group = group < 1 ? 1 : group;
   const int64_t grid = (tokens + a.group - 1) / a.group;
-  if (grid >= (1ll << 31)) return BP_E_UNSUPPORTED;
+  if (grid >= (1ll << 24)) return BP_E_UNSUPPORTED;  // threads in 32 bits
   const hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype == BP_DT_BF16) launch<Bf16>(a, v, inter, static_cast<unsigned>(grid), st);
   else if (dtype == BP_DT_F16) launch<F16>(a, v, inter, static_cast<unsigned>(grid), st);

@@ -253,7 +253,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     that no chunk covers come out as zeros. A row that sees a position whose page id is outside the cache is NaN; so may other
     rows of its chunk be. With k_scales and v_scales the caches are 8-bit codes, in blocks of a multiple of 4 positions; they
     become values of q's dtype exactly (fp16: those past its range become its greatest, 65504, int8 scales below 2 ** -24 count
-    as 0), queries over int8 codes below 2 ** 112.
+    as 0), queries over int8 codes below 2 ** 112. A NaN among the values of a chunk's own positions may reach its earlier rows.
     Returns [tokens, Hq, D], in `out` when given: q itself or a tensor apart from q and the caches."""
     if k_scales is not None or v_scales is not None:
         return _paged_attention8(q, k_pages, v_pages, table, lengths, cu, k_scales, v_scales, scale, out)

@@ -104,7 +104,7 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv
     """q [tokens, Hq, D] and k [tokens, Hk, D] (or None) at positions [tokens] (int64 or int32): of every head, the first
     2 len(inv_freq) columns in pairs (i, i + len(inv_freq)), interleaved (2 i, 2 i + 1), become
     factor (x1 cos a - x2 sin a, x2 cos a + x1 sin a), a = position x inv_freq[i] (float32); the other columns stay as they are.
-    Angles are right at any position (reduced in 64 bits). bf16, fp16 or fp32, any strides with the last dimension contiguous
+    Angles are reduced in 64 bits (right to float32 up to positions of 2 ** 28). bf16, fp16 or fp32, any strides with the last dimension contiguous
     (slices of one projection as they lie). Returns (q, k), contiguous, or in `out` = (q_out, k_out): q and k themselves, or tensors
     of any such strides apart from everything else. Forward only: tensors that require a gradient or carry a forward-mode tangent
     are refused."""

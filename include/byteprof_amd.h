@@ -482,13 +482,14 @@ typedef struct BpPagedCache {
  * paged8 (a cache in 8 bits): bp_attn_paged over codes, which become values of q's dtype exactly (BP_DT_F16: those past fp16's range
  * become its greatest, 65504, those below its least are rounded; E4M3 scales past 2^22 count as 2^22, I8 scales below 2^-24 as 0.
  * BP_DT_BF16: a value past bf16's range is infinite). I8 codes are multiplied with the queries before their scale: |q| below 2^112.
+ * A NaN among a sequence's own tokens' values may reach the rows of its earlier tokens, as in a cache in 16 bits.
  * block a multiple of 4; the codes' bases and the strides of dimensions of more than one entry multiples of 8. workspace:
  * bp_attn_paged8_workspace_bytes(tokens, seqs, hq, hk, head_dim, page x max_pages), 16-byte aligned.
  *
  * read (either cache): the positions of bp_paged_append out of the cache, into k, v [tokens, hk, head_dim] (contiguous, 16-byte
  * aligned): codes x scale in dtype BP_DT_BF16, F16 (as for paged8) or F32, or a 16-bit cache's values in its own. head_dim a multiple
- * of 8, rows on multiples of 8 elements. Tokens of no sequence and positions outside the table give zeros, pages outside the cache
- * NaN.
+ * of 8, rows on multiples of 8 elements, k and v apart from each other and from the cache. Tokens of no sequence and positions outside
+ * the table give zeros, pages outside the cache NaN.
  *
  * cu [seqs + 1] as in bp_attn_paged. No counterpart in the reference.
  */

@@ -208,6 +208,7 @@ def test_append_and_read_entries_refuse_before_any_launch(L):
     def append(dtype=0, k=p, tokens=4, cu=p, **kw):
         return L.bp_paged_append8(described(**kw), dtype, k, p, cu, tokens, 64, 64, 64, 64, None)
 
+    assert append(page=4096, block=4096, head_dim=8, hk=1 << 23) == -2  # threads past 32 bits
     assert append(dtype=3) == -2 and append(hk=1 << 29) == -2 and append(page=1 << 16, block=1 << 16, head_dim=1 << 15) == -2
     assert L.bp_paged_append8(described(dtype=0), 0, p, p, p, 4, 64, 64, 64, 64, None) == -2
     assert L.bp_paged_append8(None, 0, p, p, p, 4, 64, 64, 64, 64, None) == -1
@@ -217,8 +218,10 @@ def test_append_and_read_entries_refuse_before_any_launch(L):
     for kw in ({"tokens": 0}, {"seqs": 0}, {"pool": 0}, {"max_pages": 0}, {"head_dim": 0}, {"hk": 0}):
         assert append(**kw) == 0, kw
 
-    def read(dtype=0, k=p, cu=p, tokens=4, **kw):
-        return L.bp_paged_read(described(**kw), dtype, k, p, cu, tokens, None)
+    far = ctypes.c_void_p(1 << 40)
+
+    def read(dtype=0, k=ctypes.c_void_p(1 << 30), v=far, cu=p, tokens=4, **kw):
+        return L.bp_paged_read(described(**kw), dtype, k, v, cu, tokens, None)
 
     assert read(dtype=3) == -2 and read(head_dim=60) == -2 and read(tokens=1 << 28, hk=8) == -2
     assert L.bp_paged_read(described(dtype=0), 1, p, p, p, 4, None) == -2 and L.bp_paged_read(described(dtype=2), 2, p, p, p, 4, None) == -2
@@ -227,6 +230,10 @@ def test_append_and_read_entries_refuse_before_any_launch(L):
                {"tokens": -1}, {"k": odd}, {"k_pages": 68}, {"kp": (1024, 68, 64)}):
         assert read(**kw) == -1, kw
     assert read(tokens=0) == 0 and read(hk=0) == 0
+    # k and v apart from each other and from the cache: codes of 4 pages of 1024 bytes from 1 << 35, 19 bytes of scales from 1 << 36
+    apart = dict(k_pages=1 << 35, v_pages=1 << 35, k_scales=1 << 36, v_scales=1 << 36, ks=(6, 3, 1), vs=(6, 3, 1))
+    for at in ((1 << 40) + 496, (1 << 40) - 496, (1 << 35) - 496, (1 << 35) + 4080, (1 << 36) - 496, (1 << 36) + 16):
+        assert read(k=ctypes.c_void_p(at), **apart) == -1 and read(k=far, v=ctypes.c_void_p(at), **apart) == -1, at
 
 
 def test_rotary_entry_refuses_before_any_launch(L):
@@ -241,6 +248,9 @@ def test_rotary_entry_refuses_before_any_launch(L):
     assert L.bp_rotary(None, None) == -1 and R._DESCRIPTION.size == 6 * 8 + 9 * 8 + 8 * 4
     assert rot(tokens=0) == 0 and rot(d=0, r=0) == 0 and rot(hq=0, hk=0) == 0
     assert rot(dtype=3) == -2 and rot(d=1032) == -2
+    far = dict(zip(("q", "k", "qo", "ko"), (ctypes.c_void_p(1 << n) for n in (40, 41, 42, 43))))
+    assert rot(**far, tokens=1, hq=1 << 30, hk=1 << 30, d=8, r=8) == -2  # heads past 32 bits
+    assert rot(**far, tokens=1 << 24, hq=1, hk=0, d=1024, r=1024, q_t=1024, qo_t=1024) == -2  # threads past 32 bits
     assert rot(r=63) == -1 and rot(r=66) == -1 and rot(r=-2) == -1 and rot(size=2) == -1 and rot(factor=math.nan) == -1
     assert rot(tokens=-1) == -1 and rot(hq=-1) == -1 and rot(q=None) == -1 and rot(ko=None) == -1 and rot(pos=None) == -1
     assert rot(inv=None) == -1 and rot(qo_t=100) == -1 and rot(qo_h=32) == -1
