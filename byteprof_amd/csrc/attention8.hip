@@ -146,9 +146,11 @@ __device__ __forceinline__ int place16(int row, int chunk) {
 // lane % 16 of each 16: of 16 keys' scores (S^T = K Q^T, 16 x 16) four, keys 4 (lane / 16) + 0..3; those of 32 keys are the operand
 // of O^T = V^T P^T where they lie, whose values come transposed from LDS in the same order of the keys. Codes become operands
 // once for all rows.
-template <class T, class C, int DP, bool FULL, int RB>
+template <class T, int KIND, int DP, bool FULL, int RB>
 __device__ __forceinline__ void few_rows(const Args8& a, const Item& it, int kvh, u32x4* smem, float* stats) {
   using S = Few<DP, RB>;
+  using C = cache8::Codes<KIND, std::is_same<T, Bf16>::value>;
+  using E = cache8::Ends<KIND>;
   using K = cache8::Outside<C, C::kPlainK>;
   using V = cache8::Outside<C, C::kPlainV>;
   constexpr int NC = DP / 64, STEP = 32 * kWaves;
@@ -252,6 +254,27 @@ __device__ __forceinline__ void few_rows(const Args8& a, const Item& it, int kvh
     for (int j = 0; j < N; ++j) kimg[place16<DP>(j * RPI + lr, lc)] = kc[j];
 #pragma unroll
     for (int j = 0; j < N; ++j) vimg[place16<DP>(j * RPI + lr, lc)] = vc[j];
+    if constexpr (std::is_same<T, F16>::value) {  // codes at scales near fp16's ends become others
+      if (__any(E::beyond(ks[0]) | E::beyond(vs[0]) | (FULL ? E::beyond(ks[1]) | E::beyond(vs[1]) : 0))) {
+        // (a row's scales lie in the lanes that load() says)
+#pragma unroll 1
+        for (int i = lane; i < 32 * CH; i += kWave) {
+          const int r = i / CH, at = place16<DP>(r, i % CH), four = FULL ? (r & 15) / 4 * 16 : r, k_lane = FULL && !C::kPlainK ? r & 15 : four;
+          int kb = __shfl(ks[0], k_lane), vb = __shfl(vs[0], four);
+          if constexpr (FULL) {
+            const int k_high = __shfl(ks[1], k_lane), v_high = __shfl(vs[1], four);
+            kb = r < 16 ? kb : k_high, vb = r < 16 ? vb : v_high;
+          }
+          u32x4 k = kimg[at], v = vimg[at];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) k[e] = E::codes(k[e], kb), v[e] = E::codes(v[e], vb);
+          kimg[at] = k;
+          vimg[at] = v;
+        }
+#pragma unroll
+        for (int b = 0; b < (FULL ? 2 : 1); ++b) ks[b] = E::byte(ks[b]), vs[b] = E::byte(vs[b]);
+      }
+    }
     typename K::Scale k_scale[2];
     typename V::Scale v_scale[2];
 #pragma unroll
@@ -419,7 +442,7 @@ __device__ __forceinline__ void few_rows(const Args8& a, const Item& it, int kvh
 // 540 MB in 119 us with the merge of their parts (4.5 TB/s; the kernel alone 112 us, 4.8 TB/s), against 201 us over the same positions
 // in 16 bits; three contexts of 9000 to 65537 keys, 16 heads of 64 columns in int8, 235 MB in 65 us (the kernel alone 57, the merge
 // 7). A launch of one token is 6 us, finding the item, the first load and the join of the waves one behind the other.
-template <class T, class C, int DP, bool FULL, int RB>
+template <class T, int KIND, int DP, bool FULL, int RB>
 __global__ __launch_bounds__(kThreads, FewTiles<RB>::workgroups_a_cu(DP)) void attention8_few_kernel(Args8 a) {
   __shared__ __align__(16) u32x4 smem[Few<DP, RB>::kChunks];
   __shared__ float stats[Few<DP, RB>::kStats];
@@ -435,7 +458,7 @@ __global__ __launch_bounds__(kThreads, FewTiles<RB>::workgroups_a_cu(DP)) void a
     return;
   }
   if (it.key0 >= it.key1 && it.split > 0) return;
-  few_rows<T, C, DP, FULL, RB>(a, it, kvh, smem, stats);
+  few_rows<T, KIND, DP, FULL, RB>(a, it, kvh, smem, stats);
 }
 
 // A large tile's steps: BN keys, whose codes the workgroup turns into values once, in registers, and writes to the images that the
@@ -452,8 +475,11 @@ struct Large {
 // columns, 106 GFLOP in 156 us (0.68 PFLOP/s), 19 of them the merge of 68 MB of parts; in 16 bits 162 us. (Of 64 rows a wave, one
 // workgroup a CU, the next step's scores between the exponentials: heads of 64 columns 194 us in place of 101; steps of 32 keys for
 // three workgroups a CU: 259 us in place of 162, what the registers do not hold is put aside.)
-template <class T, class C, int DP, bool FULL>
+template <class T, int KIND, int DP, bool FULL>
 __device__ __forceinline__ void large_tile8(const Args8& a, const Item& it, int kvh, u32x4* smem) {
+  constexpr bool F = std::is_same<T, F16>::value;
+  using C = typename std::conditional<F && KIND == cache8::kInt8, cache8::TwoFactors, cache8::Codes<KIND, !F>>::type;
+  using E = cache8::Ends<KIND>;
   constexpr int BN = Large<DP>::BN, NB = BN / 32, CH = DP / 16, IMG = BN * DP / 8;
   constexpr int N = (BN * CH + kThreads - 1) / kThreads;  // 16-code pieces of a thread
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -505,6 +531,24 @@ __device__ __forceinline__ void large_tile8(const Args8& a, const Item& it, int 
       }
     }
   };
+  // e4m3 to fp16: codes at scales past 2^22 become others. A branch, behind the barrier where the step has one anyway (chunks of 128
+  // columns 164 us to 166, of 64 101 to 103; inside turn() 170 and 109, and by a second factor 169 and 104).
+  const auto settle = [&] {
+    if constexpr (F && KIND == cache8::kE4m3) {
+      uint32_t beyond = 0;
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+        if (mine_of(n)) beyond |= E::beyond(ks[n]) | E::beyond(vs[n]);
+      if (!__any(beyond)) return;
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        if (!mine_of(n)) continue;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) kc[n][e] = E::codes(kc[n][e], ks[n]), vc[n][e] = E::codes(vc[n][e], vs[n]);
+        ks[n] = E::byte(ks[n]), vs[n] = E::byte(vs[n]);
+      }
+    }
+  };
   const auto turn = [&](int to) {
     u32x4* kimg = smem + to * IMG;
     u32x4* vimg = smem + (2 + to) * IMG;
@@ -524,6 +568,7 @@ __device__ __forceinline__ void large_tile8(const Args8& a, const Item& it, int 
     look(it.key0);
     load(it.key0);
     look(it.key0 + BN);
+    settle();
     turn(0);
     if (it.key0 + BN < it.key1) load(it.key0 + BN);
     look(it.key0 + 2 * BN);
@@ -542,6 +587,7 @@ __device__ __forceinline__ void large_tile8(const Args8& a, const Item& it, int 
   const int mine_end = active ? min(it.key1, most + 1) : it.key0;
   for (; key < mine_end; key += BN) {
     __syncthreads();
+    settle();
     f32x16 s[NB];
     u32x4 p[NB][2];
 #pragma unroll
@@ -555,6 +601,7 @@ __device__ __forceinline__ void large_tile8(const Args8& a, const Item& it, int 
   }
   for (; key < it.key1; key += BN) {
     __syncthreads();
+    settle();
     turn(buf ^ 1);
     send(key);
     buf ^= 1;
@@ -584,7 +631,7 @@ __device__ __forceinline__ Item found_once(const Args& a, int index, int (&words
 }
 
 // Heads of up to 96 columns: the large tiles are made for 96, the few rows' for 128.
-template <class T, class C, int DP, bool FULL>
+template <class T, int KIND, int DP, bool FULL>
 __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void attention8_kernel(Args8 a) {
   using F = Few<DP == 96 ? 128 : DP, 2>;
   __shared__ __align__(16) u32x4 smem[F::kChunks > Large<DP>::kImages ? F::kChunks : Large<DP>::kImages];
@@ -598,23 +645,22 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void attention8_kernel(
     return;
   }
   if (it.key0 >= it.key1 && it.split > 0) return;
-  if (it.small) few_rows<T, C, DP == 96 ? 128 : DP, FULL, 2>(a, it, kvh, smem, stats);
-  else large_tile8<T, C, DP, FULL>(a, it, kvh, smem);
+  if (it.small) few_rows<T, KIND, DP == 96 ? 128 : DP, FULL, 2>(a, it, kvh, smem, stats);
+  else large_tile8<T, KIND, DP, FULL>(a, it, kvh, smem);
 }
 
 // What a launch is made for: tiles of 16 rb rows, or (rb 0) the large ones beside small ones of 32.
 template <class T, int KIND, int RB>
 int launch8_few(const Args8& a, const Launch& n, hipStream_t st) {
-  using C = cache8::Codes<KIND, std::is_same<T, Bf16>::value>;
   const unsigned grid = static_cast<unsigned>((n.index + kXcds - 1) / kXcds * kXcds * a.hk.d);
   const bool full = a.wide && a.even;
-  if (a.d == 64 && full) attention8_few_kernel<T, C, 64, true, RB><<<grid, kThreads, 0, st>>>(a);
-  else if (a.d <= 64) attention8_few_kernel<T, C, 64, false, RB><<<grid, kThreads, 0, st>>>(a);
-  else if (a.d == 128 && full) attention8_few_kernel<T, C, 128, true, RB><<<grid, kThreads, 0, st>>>(a);
-  else if (a.d <= 128) attention8_few_kernel<T, C, 128, false, RB><<<grid, kThreads, 0, st>>>(a);
+  if (a.d == 64 && full) attention8_few_kernel<T, KIND, 64, true, RB><<<grid, kThreads, 0, st>>>(a);
+  else if (a.d <= 64) attention8_few_kernel<T, KIND, 64, false, RB><<<grid, kThreads, 0, st>>>(a);
+  else if (a.d == 128 && full) attention8_few_kernel<T, KIND, 128, true, RB><<<grid, kThreads, 0, st>>>(a);
+  else if (a.d <= 128) attention8_few_kernel<T, KIND, 128, false, RB><<<grid, kThreads, 0, st>>>(a);
   else if constexpr (RB < 3) {
-    if (a.d == 256 && full) attention8_few_kernel<T, C, 256, true, RB><<<grid, kThreads, 0, st>>>(a);
-    else attention8_few_kernel<T, C, 256, false, RB><<<grid, kThreads, 0, st>>>(a);
+    if (a.d == 256 && full) attention8_few_kernel<T, KIND, 256, true, RB><<<grid, kThreads, 0, st>>>(a);
+    else attention8_few_kernel<T, KIND, 256, false, RB><<<grid, kThreads, 0, st>>>(a);
   }
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return static_cast<int>(e);
@@ -623,16 +669,15 @@ int launch8_few(const Args8& a, const Launch& n, hipStream_t st) {
 
 template <class T, int KIND>
 int launch8_large(const Args8& a, const Launch& n, hipStream_t st) {
-  using C = cache8::Codes<KIND, std::is_same<T, Bf16>::value>;
   const unsigned grid = static_cast<unsigned>(n.index * a.hk.d);
   const bool full = a.wide && a.even;
-  if (a.d == 64 && full) attention8_kernel<T, C, 64, true><<<grid, kThreads, 0, st>>>(a);
-  else if (a.d <= 64) attention8_kernel<T, C, 64, false><<<grid, kThreads, 0, st>>>(a);
-  else if (a.d <= 96) attention8_kernel<T, C, 96, false><<<grid, kThreads, 0, st>>>(a);
-  else if (a.d == 128 && full) attention8_kernel<T, C, 128, true><<<grid, kThreads, 0, st>>>(a);
-  else if (a.d <= 128) attention8_kernel<T, C, 128, false><<<grid, kThreads, 0, st>>>(a);
-  else if (a.d == 256 && full) attention8_kernel<T, C, 256, true><<<grid, kThreads, 0, st>>>(a);
-  else attention8_kernel<T, C, 256, false><<<grid, kThreads, 0, st>>>(a);
+  if (a.d == 64 && full) attention8_kernel<T, KIND, 64, true><<<grid, kThreads, 0, st>>>(a);
+  else if (a.d <= 64) attention8_kernel<T, KIND, 64, false><<<grid, kThreads, 0, st>>>(a);
+  else if (a.d <= 96) attention8_kernel<T, KIND, 96, false><<<grid, kThreads, 0, st>>>(a);
+  else if (a.d == 128 && full) attention8_kernel<T, KIND, 128, true><<<grid, kThreads, 0, st>>>(a);
+  else if (a.d <= 128) attention8_kernel<T, KIND, 128, false><<<grid, kThreads, 0, st>>>(a);
+  else if (a.d == 256 && full) attention8_kernel<T, KIND, 256, true><<<grid, kThreads, 0, st>>>(a);
+  else attention8_kernel<T, KIND, 256, false><<<grid, kThreads, 0, st>>>(a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return static_cast<int>(e);
   return n.merges > 0 ? launch_merge<Tiles32>(std::is_same<T, Bf16>::value ? BP_DT_BF16 : BP_DT_F16, a, n, st) : BP_OK;

@@ -2,8 +2,8 @@
 // of two for each block of tokens and head, kept as its exponent with bias 127 (255: not a number). A power of two costs e4m3
 // nothing (a floating code is as exact at any scale) and int8 half a bit in the mean; in return x / scale and code x scale are
 // exact, so a code is the correct rounding of its definition and code x scale, of 8 significant bits at most, is exact in bf16
-// (in fp16 from its least subnormal to its greatest value; saturate_f16 has those past it become the greatest: an infinity
-// would turn the probabilities 0 of the keys beside it into NaN, and 65504 rounded to e4m3 is 65536).
+// (in fp16 rounded once below its normal values; saturate_f16 has those past its range become its greatest: an infinity would turn
+// the probabilities 0 of the keys beside it into NaN, and 65504 rounded to e4m3 is 65536).
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -50,8 +50,8 @@ struct Codes<kE4m3, true> {
 template <>
 struct Codes<kE4m3, false> {
   static constexpr bool kPlainK = false, kPlainV = false;
-  // The conversion's own overflow does not saturate: it takes scales up to 2^7, which 448 stands, and a product the rest (scales
-  // past 2^22 count as 2^22).
+  // The conversion's own overflow does not saturate: it takes scales up to 2^7, which 448 stands, and a product the rest, up to 2^15
+  // (Ends has no scale be greater than that).
   struct Scale {
     float field;
     f16x2 rest;
@@ -71,6 +71,7 @@ template <>
 struct Codes<kInt8, true> {
   static constexpr bool kPlainK = true, kPlainV = true;
   typedef float Scale;
+  static __device__ __forceinline__ float outside(uint32_t byte) { return scale_value(byte); }
   static __device__ __forceinline__ Scale scale(uint32_t byte) { return scale_value(byte); }
   static __device__ __forceinline__ u32x2 four(uint32_t w, Scale s) {
     float f[4];
@@ -87,6 +88,8 @@ template <>
 struct Codes<kInt8, false> {
   static constexpr bool kPlainK = true, kPlainV = false;
   typedef f16x2 Scale;
+  // (below 2^-31 every code rounds to 0 in fp16)
+  static __device__ __forceinline__ float outside(uint32_t byte) { return byte < 96 ? 0.f : scale_value(byte); }
   static __device__ __forceinline__ Scale scale(uint32_t byte) {
     const _Float16 h = static_cast<_Float16>(scale_value(byte));
     return f16x2{h, h};
@@ -107,6 +110,68 @@ struct Codes<kInt8, false> {
   }
 };
 
+// The ends of fp16: one factor, rounded to fp16 itself, is right for a scale in the middle only. Codes at a scale that beyond() names are
+// replaced by codes() at the scale byte(), which stand for the same fp16 values. (That happens for blocks of values below 2^-18 or past
+// 2^15. A second factor in every product instead costs a verify round over int8 33.1 us to 34.4, a decode batch of int8 heads of 200
+// columns, whose registers do not suffice then, 374 to 451; the look at the scales costs them 33.7 and 384.)
+template <int KIND>
+struct Ends;
+
+// Past 2^22 all normal codes are past fp16's range, there as at 2^22, and a code m below them, m 2^-9, times 2^n is m << n.
+template <>
+struct Ends<kE4m3> {
+  static __device__ __forceinline__ uint32_t beyond(uint32_t byte) { return byte > 149 && byte < 255; }
+  static __device__ __forceinline__ uint32_t byte(uint32_t byte) { return beyond(byte) ? 149 : byte; }
+  static __device__ __forceinline__ uint32_t codes(uint32_t w, uint32_t byte) {
+    const uint32_t n = beyond(byte) ? min(byte - 149, 3u) : 0;
+    const uint32_t normal = (((w & 0x78787878u) + 0x78787878u) >> 7 & 0x01010101u) * 0xff;
+    return (w & (normal | 0x80808080u)) | (w & 0x07070707u & ~normal) << n;
+  }
+};
+
+// From 2^-31 to 2^-25 a value is a whole multiple of fp16's least, 2^-24, to the nearest: that multiple is its code at 2^-24. Past 2^9, a
+// code whose value is past fp16's range becomes that of 2^16 (as a factor outside of a sum takes it; inside, it is the greatest).
+template <>
+struct Ends<kInt8> {
+  static __device__ __forceinline__ uint32_t beyond(uint32_t byte) { return (byte > 136 && byte < 255) || byte - 96u <= 102u - 96u; }
+  static __device__ __forceinline__ uint32_t byte(uint32_t byte) { return beyond(byte) ? byte > 136 ? min(byte, 143u) : 103 : byte; }
+  static __device__ __forceinline__ uint32_t codes(uint32_t w, uint32_t byte) {
+    const float f = beyond(byte) && byte < 103 ? scale_field(byte + 24) : 1.f;
+    const float most = beyond(byte) && byte > 136 ? scale_field(127 + 143 - min(byte, 143u)) : 128.f;
+    uint32_t y = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float x = rintf(static_cast<float>(static_cast<int8_t>(w >> (8 * i))) * f);
+      y |= (static_cast<uint32_t>(static_cast<int>(fminf(fmaxf(x, -most), most))) & 0xffu) << (8 * i);
+    }
+    return y;
+  }
+};
+
+// int8 codes as fp16 by two factors, 2^e = first x rest, first from 2^-14 to 2^5: a code times first is exact, so that the last product
+// alone rounds or saturates. As many products as with one factor (the code's bias goes into the first), and right for every scale: the
+// large tiles' form (chunks of 128 columns 169 us to 172, of 64 102 to 105).
+struct TwoFactors {
+  struct Scale {
+    f16x2 factors, bias;  // first and rest; -1152 x first
+  };
+  static __device__ __forceinline__ Scale scale(uint32_t byte) {
+    const int e = static_cast<int>(byte) - 127, n = min(max(e, -14), 5);
+    const _Float16 first = __builtin_bit_cast(f16x2, (15 + n) << 10)[0], bias = first * static_cast<_Float16>(-1152.f);
+    // (of the rest, below 2^-24 and past 2^15 nothing changes: 127 x 2^-38 rounds to 0, 2^20 is past the greatest)
+    const _Float16 rest = byte == 255 ? static_cast<_Float16>(NAN) : static_cast<_Float16>(scale_field(min(max(e - n, -24), 15) + 127));
+    return Scale{{first, rest}, {bias, bias}};
+  }
+  static __device__ __forceinline__ u32x2 four(uint32_t w, Scale s) {
+    const uint32_t u = w ^ 0x80808080u;  // as in Codes
+    const f16x2 lo = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u));
+    const f16x2 hi = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u));
+    const f16x2 first = s.factors.xx, rest = s.factors.yy;
+    const f16x2 x = __builtin_elementwise_fma(lo, first, s.bias) * rest, y = __builtin_elementwise_fma(hi, first, s.bias) * rest;
+    return u32x2{__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, y)};
+  }
+};
+
 // What a factor outside the sum is, and four codes as the sum's operand with it (PLAIN) or without.
 template <class C, bool PLAIN>
 struct Outside {
@@ -118,7 +183,7 @@ struct Outside {
 template <class C>
 struct Outside<C, true> {
   typedef float Scale;
-  static __device__ __forceinline__ Scale scale(uint32_t byte) { return scale_value(byte); }
+  static __device__ __forceinline__ Scale scale(uint32_t byte) { return C::outside(byte); }
   static __device__ __forceinline__ float times(float x, Scale s) { return x * s; }
   static __device__ __forceinline__ u32x2 four(uint32_t w, Scale) { return C::plain(w); }
 };

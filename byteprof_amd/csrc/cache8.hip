@@ -310,7 +310,14 @@ __global__ __launch_bounds__(kThreads) void read_kernel(Read a) {
             for (int e = 0; e < 8; ++e) y[e / 4][e % 4] = T::bits(decode<KIND>(w[e / 4] >> (8 * (e % 4)) & 0xff) * s);
           } else {
             using C = Codes<KIND, std::is_same<T, Bf16>::value>;
-            y[0] = eight<C>(w[0], w[1], C::scale(byte[u][kv]));
+            if constexpr (std::is_same<T, F16>::value) {
+              using E = Ends<KIND>;
+              const uint32_t b = byte[u][kv];
+              if (E::beyond(b)) y[0] = eight<C>(E::codes(w[0], b), E::codes(w[1], b), C::scale(E::byte(b)));
+              else y[0] = eight<C>(w[0], w[1], C::scale(b));
+            } else {
+              y[0] = eight<C>(w[0], w[1], C::scale(byte[u][kv]));
+            }
           }
         } else if (id[u] == kOutside) {
           const uint32_t nan = T::bits(NAN), two = CHUNKS == 2 ? nan : nan | nan << 16;

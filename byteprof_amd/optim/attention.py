@@ -252,8 +252,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     cache, its chunk's among them (append first). A chunk's tokens are the last positions; each sees all up to its own. Rows
     that no chunk covers come out as zeros. A row that sees a position whose page id is outside the cache is NaN; so may other
     rows of its chunk be. With k_scales and v_scales the caches are 8-bit codes, in blocks of a multiple of 4 positions; they
-    become values of q's dtype exactly (fp16: those past its range become its greatest, 65504, int8 scales below 2 ** -24 count
-    as 0), queries over int8 codes below 2 ** 112. A NaN among the values of a chunk's own positions may reach its earlier rows.
+    become values of q's dtype, those that paged_read gives (an int8 key past fp16's range may count as 65536 in place of 65504),
+    bf16 queries over int8 codes below 2 ** 112. A NaN among the values of a chunk's own positions may reach its earlier rows.
     Returns [tokens, Hq, D], in `out` when given: q itself or a tensor apart from q and the caches."""
     if k_scales is not None or v_scales is not None:
         return _paged_attention8(q, k_pages, v_pages, table, lengths, cu, k_scales, v_scales, scale, out)
@@ -378,8 +378,8 @@ def paged_read(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor
                dtype: torch.dtype | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """The way back of paged_append: of each sequence b its last cu[b + 1] - cu[b] positions, as (k, v) [tokens, Hk, D], new
     tensors. A 16-bit cache (bf16 or fp16) gives its values in its own dtype; an 8-bit one (with k_scales and v_scales) code x
-    scale in `dtype`: bf16 (by default; exact), fp16 (past its range 65504) or fp32. Tokens of no sequence and positions outside the
-    table come out as zeros, those of a page outside the cache as NaN."""
+    scale in `dtype`: bf16 (by default; exact), fp16 (rounded below its normal values, past its range 65504) or fp32. Tokens of no
+    sequence and positions outside the table come out as zeros, those of a page outside the cache as NaN."""
     what = "paged_read"
     cache, _, _, hk, d, _, _, _ = _cache(what, k_pages, v_pages, table, lengths, cu, k_scales, v_scales, 8)
     if k_scales is None:

@@ -479,9 +479,10 @@ typedef struct BpPagedCache {
  * rounded to it again. A code is x / s to the nearest, ties to even; infinities give the greatest code, NaN gives NaN (E4M3) or 0
  * (I8). The other positions of a block keep their codes. A block that is written to must be one sequence's only, and once in its table.
  *
- * paged8 (a cache in 8 bits): bp_attn_paged over codes, which become values of q's dtype exactly (BP_DT_F16: those past fp16's range
- * become its greatest, 65504, those below its least are rounded; E4M3 scales past 2^22 count as 2^22, I8 scales below 2^-24 as 0.
- * BP_DT_BF16: a value past bf16's range is infinite). I8 codes are multiplied with the queries before their scale: |q| below 2^112.
+ * paged8 (a cache in 8 bits): bp_attn_paged over codes, which become values of q's dtype exactly (BP_DT_F16: rounded once below its normal
+ * values, its greatest, 65504, where they are past its range, but I8 keys past it may count as 65536. BP_DT_BF16: past its range they
+ * are infinite, and so, or NaN, is what sees them). In BP_DT_BF16, I8 codes are multiplied with the queries before their scale: |q| below
+ * 2^112.
  * A NaN among a sequence's own tokens' values may reach the rows of its earlier tokens, as in a cache in 16 bits.
  * block a multiple of 4; the codes' bases and the strides of dimensions of more than one entry multiples of 8. workspace:
  * bp_attn_paged8_workspace_bytes(tokens, seqs, hq, hk, head_dim, page x max_pages), 16-byte aligned.
