@@ -431,9 +431,9 @@ int bp_paged_read(const BpPagedCache* cache, int dtype, void* k, void* v, const 
   if (c.head_dim % 8 != 0) return BP_E_UNSUPPORTED;
   if (tokens == 0 || c.hk == 0 || c.head_dim == 0) return BP_OK;
   const bool empty = c.seqs == 0 || c.pool == 0 || c.max_pages == 0;
-  if (k == nullptr || v == nullptr || (c.seqs > 0 && (c.lengths == nullptr || cu == nullptr)) ||
-      (!empty && (c.k_pages == nullptr || c.v_pages == nullptr || c.table == nullptr ||
-                  (codes && (c.k_scales == nullptr || c.v_scales == nullptr)))))
+  // (a pool without pages still has its table read)
+  if (k == nullptr || v == nullptr || (c.seqs > 0 && (c.lengths == nullptr || cu == nullptr || (c.max_pages > 0 && c.table == nullptr))) ||
+      (!empty && (c.k_pages == nullptr || c.v_pages == nullptr || (codes && (c.k_scales == nullptr || c.v_scales == nullptr)))))
     return BP_E_INVALID_ARG;
   const int size = codes ? 1 : 2;
   Read a = {};

@@ -257,3 +257,14 @@ def test_rotary_entry_refuses_before_any_launch(L):
     assert rot(qo=ctypes.c_void_p((1 << 20) + 64)) == -1  # shifted within its own input
     assert rot(qo=k) == -1 and rot(qo=ctypes.c_void_p(6 << 20)) == -1 and rot(qo=pos) == -1 and rot(qo=inv) == -1
     assert rot(q_t=256, qo=q) == -1  # its own input's place, but not its strides
+
+
+def test_read_entry_needs_a_table_wherever_it_looks_one_up(L):
+    """Also with no page in the pool: every position of the table is looked up before its page is found to be outside."""
+    p = ctypes.c_void_p(64)
+
+    def read(**kw):
+        return L.bp_paged_read(described(**kw), 0, ctypes.c_void_p(1 << 30), ctypes.c_void_p(1 << 40), p, 4, None)
+
+    assert read(pool=0, table=None) == -1 and read(pool=0, lengths=None) == -1
+    assert L.bp_paged_read(described(dtype=0, pool=0, table=None), 0, ctypes.c_void_p(1 << 30), ctypes.c_void_p(1 << 40), p, 4, None) == -1
