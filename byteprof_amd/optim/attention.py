@@ -299,8 +299,9 @@ def _paged_attention8(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Ten
         raise ValueError(f"{what}: q must be bfloat16 or float16")
     _heads(what, hq, hk, d, dk)
     index = _same_device(what, q, k_pages, v_pages, k_scales, v_scales, table, lengths, cu, out)
-    if q.requires_grad or k_pages.requires_grad or v_pages.requires_grad or forward_ad._current_level >= 0:
-        _no_derivative(what, q, k_pages, v_pages)
+    if (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad or k_scales.requires_grad or v_scales.requires_grad
+            or forward_ad._current_level >= 0):
+        _no_derivative(what, q, k_pages, v_pages, k_scales, v_scales)
     scale = _scale(what, scale, d)
     q = _rows(q)
     y = _output(what, q, out, k_pages, v_pages, k_scales, v_scales)
@@ -365,8 +366,9 @@ def _paged_append8(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pa
     if (k_d != 1 or v_d != 1) and k.numel():
         raise ValueError(f"{what}: k and v must be contiguous in the head dimension")
     index = _same_device(what, k, v, k_pages, v_pages, k_scales, v_scales, table, lengths, cu)
-    if k.requires_grad or v.requires_grad or k_pages.requires_grad or v_pages.requires_grad or forward_ad._current_level >= 0:
-        _no_derivative(what, k, v, k_pages, v_pages)
+    if (k.requires_grad or v.requires_grad or k_pages.requires_grad or v_pages.requires_grad or k_scales.requires_grad
+            or v_scales.requires_grad or forward_ad._current_level >= 0):
+        _no_derivative(what, k, v, k_pages, v_pages, k_scales, v_scales)
     if tokens == 0 or hk == 0 or d == 0:
         return
     _launch(index, "bp_paged_append8", cache, dtype, k.data_ptr(), v.data_ptr(), cu.data_ptr(), tokens, k_t, k_h, v_t, v_h)
@@ -394,8 +396,9 @@ def paged_read(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor
     if tokens < 0 or d % 8:
         raise ValueError(f"{what}: tokens must not be negative, and head_dim must be a multiple of 8")
     index = _same_device(what, k_pages, v_pages, k_scales, v_scales, table, lengths, cu)
-    if k_pages.requires_grad or v_pages.requires_grad or forward_ad._current_level >= 0:
-        _no_derivative(what, k_pages, v_pages)
+    scales = () if k_scales is None else (k_scales, v_scales)
+    if k_pages.requires_grad or v_pages.requires_grad or any(s.requires_grad for s in scales) or forward_ad._current_level >= 0:
+        _no_derivative(what, k_pages, v_pages, *scales)
     k = torch.empty((tokens, hk, d), dtype=dtype, device=k_pages.device)
     v = torch.empty_like(k)
     if tokens and hk and d:

@@ -268,3 +268,15 @@ def test_read_entry_needs_a_table_wherever_it_looks_one_up(L):
 
     assert read(pool=0, table=None) == -1 and read(pool=0, lengths=None) == -1
     assert L.bp_paged_read(described(dtype=0, pool=0, table=None), 0, ctypes.c_void_p(1 << 30), ctypes.c_void_p(1 << 40), p, 4, None) == -1
+
+
+@pytest.mark.parametrize("name", ["k_scales", "v_scales"])
+def test_scales_that_require_a_gradient_are_refused(monkeypatch, name):
+    """As the codes are: scales made of something that does are part of its graph."""
+    monkeypatch.setattr(A, "_same_device", lambda *args: 0)
+    scales = torch.ones(3, 2, 1, requires_grad=True).to(E8M0)
+    assert scales.requires_grad
+    for call in (lambda c: A.paged_attention(q=z(4, 2, 64), **c), lambda c: A.paged_append(k=z(4, 1, 64), v=z(4, 1, 64), **c),
+                 lambda c: A.paged_read(tokens=4, **c)):
+        with pytest.raises(ValueError, match="no backward"):
+            call(cache(**{name: scales}))
