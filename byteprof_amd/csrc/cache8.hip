@@ -411,6 +411,7 @@ int bp_paged_append8(const BpPagedCache* cache, int dtype, const void* k, const 
   // a unit's pieces, positions, and a launch's threads in 32 bits
   if (static_cast<int64_t>(c.block) * c.head_dim >= (1ll << 30) || 2 * units * c.hk >= (1ll << 32) / threads || tokens >= (1 << 30))
     return BP_E_UNSUPPORTED;
+  if (c.k_pages == c.v_pages || c.k_scales == c.v_scales) return BP_E_INVALID_ARG;
   a.units = static_cast<int>(units);
   const hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype == BP_DT_BF16) append_kind<Bf16>(a, c.dtype, wide, st);

@@ -194,6 +194,7 @@ def _pages(what: str, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch
 
 
 _DESCRIPTION = struct.Struct("6Q13q8i")  # BpPagedCache of byteprof_amd.h
+_ADDRESSES = struct.Struct("4Q")  # its first: pages and scales
 _I32 = torch.int32
 
 
@@ -356,6 +357,9 @@ def _paged_append8(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pa
     if k.dim() != 3 or v.shape != k.shape:
         raise ValueError(f"{what}: k and v must be [tokens, Hk, D]")
     cache, _, _, hk, d, _, _, _ = _cache(what, k_pages, v_pages, table, lengths, cu, k_scales, v_scales, 1)
+    k_at, v_at, ks_at, vs_at = _ADDRESSES.unpack_from(cache)
+    if k_at == v_at != 0 or ks_at == vs_at != 0:
+        raise ValueError(f"{what}: keys and values need pages and scales in memory of their own")
     tokens, heads, dim = k.shape
     if heads != hk or dim != d:
         raise ValueError(f"{what}: the caches hold {hk} heads of {d}, k and v {heads} of {dim}")

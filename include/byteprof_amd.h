@@ -477,7 +477,8 @@ typedef struct BpPagedCache {
  * them. A block's scale becomes the least power of two s with |x| <= 448 s (E4M3) or 127 s (I8) for all its new values (infinities
  * and NaN aside); where the block holds positions from before the chunk, no less than it was, and if it grows their codes are
  * rounded to it again. A code is x / s to the nearest, ties to even; infinities give the greatest code, NaN gives NaN (E4M3) or 0
- * (I8). The other positions of a block keep their codes. A block that is written to must be one sequence's only, and once in its table.
+ * (I8). The other positions of a block keep their codes. A block that is written to must be one sequence's only, and once in its table;
+ * keys and values have pages and scales of their own.
  *
  * paged8 (a cache in 8 bits): bp_attn_paged over codes, which become values of q's dtype exactly (BP_DT_F16: rounded once below its normal
  * values, its greatest, 65504, where they are past its range, but I8 keys past it may count as 65536. BP_DT_BF16: past its range they

@@ -280,3 +280,16 @@ def test_scales_that_require_a_gradient_are_refused(monkeypatch, name):
                  lambda c: A.paged_read(tokens=4, **c)):
         with pytest.raises(ValueError, match="no backward"):
             call(cache(**{name: scales}))
+
+
+def test_append_refuses_keys_and_values_in_one_place(monkeypatch, L):
+    """One tensor for both scales (or both caches) would hold whichever was written last."""
+    monkeypatch.setattr(A, "_same_device", lambda *args: 0)
+    c, k = cache(), z(4, 1, 64)
+    for same in ({"v_scales": c["k_scales"]}, {"v_pages": c["k_pages"]}, {"v_scales": c["k_scales"].view(torch.uint8).view(E8M0)}):
+        with pytest.raises(ValueError, match="memory of their own"):
+            A.paged_append(k=k, v=k, **{**c, **same})
+    p = ctypes.c_void_p(64)
+    apart = dict(k_pages=1 << 20, v_pages=2 << 20, k_scales=3 << 20, v_scales=4 << 20)
+    for same in ({"v_scales": 3 << 20}, {"v_pages": 1 << 20}):
+        assert L.bp_paged_append8(described(**{**apart, **same}), 0, p, p, p, 4, 64, 64, 64, 64, None) == -1, same
