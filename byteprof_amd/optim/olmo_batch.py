@@ -54,6 +54,11 @@ class OlmoBatch:
         if cache != torch.bfloat16 and page % 4:
             raise ValueError(f"an 8-bit cache needs pages of a multiple of 4 positions, not {page}")
         cfg = dec.cfg
+        if rotary is not None:
+            inv_freq, factor = rotary if isinstance(rotary, (tuple, list)) and len(rotary) == 2 else (None, 0.0)
+            if (not isinstance(inv_freq, torch.Tensor) or inv_freq.dtype is not torch.float32 or inv_freq.shape != (cfg.head_dim // 2,)
+                    or inv_freq.device != dec.inv_freq.device or not -3e38 <= factor <= 3e38):
+                raise ValueError(f"rotary must be (inv_freq, factor): float32 [{cfg.head_dim // 2}] on {dec.inv_freq.device}, a finite number")
         self.dec, self.page = dec, page
         shape = (cfg.layers, pages, page, cfg.heads, cfg.head_dim)
         self.k_pages, self.v_pages = (torch.zeros(shape, dtype=cache, device=dec.device) for _ in range(2))

@@ -293,3 +293,20 @@ def test_append_refuses_keys_and_values_in_one_place(monkeypatch, L):
     apart = dict(k_pages=1 << 20, v_pages=2 << 20, k_scales=3 << 20, v_scales=4 << 20)
     for same in ({"v_scales": 3 << 20}, {"v_pages": 1 << 20}):
         assert L.bp_paged_append8(described(**{**apart, **same}), 0, p, p, p, 4, 64, 64, 64, 64, None) == -1, same
+
+
+def test_a_batch_refuses_frequencies_that_are_not_its_heads():
+    """Fewer pairs would turn a part of each head only, and tensors elsewhere would be found out in the middle of a pass."""
+    from types import SimpleNamespace
+
+    from byteprof_amd.optim.olmo import OlmoConfig
+    from byteprof_amd.optim.olmo_batch import OlmoBatch
+
+    cfg = OlmoConfig(hidden=128, ffn=64, layers=1, heads=2, vocab=20)
+    dec = SimpleNamespace(cfg=cfg, device=torch.device("cpu"), inv_freq=torch.ones(32))
+    assert OlmoBatch(dec, pages=2, rotary=(torch.ones(32), 1.25)).rotary[1] == 1.25
+    for bad in ((torch.ones(16), 1.0), (torch.ones(64), 1.0), (torch.ones(32, dtype=torch.float64), 1.0), (torch.ones(1, 32), 1.0),
+                (torch.ones(32, device="meta"), 1.0), (torch.ones(32), math.inf), (torch.ones(32), math.nan), (torch.ones(32),),
+                torch.ones(32)):
+        with pytest.raises(ValueError, match="rotary must be"):
+            OlmoBatch(dec, pages=2, rotary=bad)
