@@ -15,7 +15,7 @@ constexpr int kWaves = kThreads / kWave;
 constexpr int kSmallRows = 64;   // sequences of at most this many rows: 32-row tiles whose waves share the keys
 constexpr int kTileSmall = 32;
 constexpr int kTileLarge = 128;  // 32 rows a wave, all keys
-constexpr int kSharedMin = 512;  // least keys of a split where the parts are more than that
+constexpr int kSharedMin = 512;  // least keys of a split of few rows, and of others where the parts are more than the card holds
 constexpr int kKeyStep = 128;    // a split's keys are a multiple of this: whole steps of either kind of tile
 
 constexpr int kCus = 256;
@@ -29,6 +29,8 @@ struct Tiles32 {
   static constexpr int kMergeRows = 32;      // rows of a unit of the merge; of up to kFew rows with more than kMergeParts parts, one
   static constexpr int kTarget = 1024;       // bound of what splitting aims at (twice the workgroups that the card holds at once:
                                              // 1024, for 256 columns 512)
+  static constexpr int kLeast = BP_ATTN_UNDIVIDED_KEYS;  // least keys of a split
+  static constexpr int kWhole = BP_ATTN_UNDIVIDED_KEYS;  // where no sequence can have more keys, none is divided
   // By the registers of attention_kernel: 256 columns leave one wave a SIMD, 128 two (fewer columns three, but planning for three
   // made heads of 96 no faster and cached ones slower, 97 us against 90).
   static int workgroups_a_cu(int padded) { return padded > 128 ? 1 : 2; }
@@ -42,6 +44,10 @@ struct FewTiles {
   static constexpr bool kFit = false;
   static constexpr int kMergeRows = 16;
   static constexpr int kTarget = 2048;
+  static constexpr int kLeast = kSharedMin;
+  // find_item divides from one and a half least splits on. (With a launch of the merge that had no unit, from 257 on: a decode step over a
+  // table of 300 or 600 positions 17 us, now 12.)
+  static constexpr int kWhole = kLeast + kLeast / 2 - 1;
   // By the registers of attention8_few_kernel, a workgroup's four waves on the four SIMDs. (128 columns and 16 rows with room for
   // four: what the compiler puts aside in the loop is waited for with the loads, a decode batch 162 us in place of 119.)
   __host__ __device__ static constexpr int workgroups_a_cu(int padded) {
@@ -138,7 +144,7 @@ __device__ __forceinline__ int split_keys(const Args& a, const Seq& own, int lan
     const int chunk = want < 1e9f ? static_cast<int>(want) + 1 : 0x3fffff00;
     return __builtin_amdgcn_readfirstlane((max(chunk, a.chunk_min) + kKeyStep - 1) / kKeyStep * kKeyStep);
   };
-  if constexpr (!P::kFit) return max(chunk_of(a.target), kSharedMin);
+  if constexpr (!P::kFit) return chunk_of(a.target);
   const int chunk = chunk_of(a.resident);
   int items = 0;
   for (int b = lane; b < a.seqs; b += kWave) {
@@ -261,7 +267,6 @@ __device__ __forceinline__ Item find_item(const Args& a, int index) {
   return it;
 }
 
-constexpr int kChunkMin = BP_ATTN_UNDIVIDED_KEYS;  // least keys of a split
 constexpr int kMergeGrid = 1024;  // workgroups of a merge launch; each takes every such unit
 
 // Row tiles of a key head that any offsets can give: sequences of up to kFew rows (64, or all) have small tiles.
@@ -272,7 +277,10 @@ int64_t tiles_bound(int64_t tokens, int64_t seqs, int64_t group) {
   return P::kFew > kSmallRows || b <= a ? b : a;
 }
 
-inline bool may_split(int64_t max_keys) { return max_keys > kChunkMin; }
+template <class P = Tiles32>
+bool may_split(int64_t max_keys) {
+  return max_keys > P::kWhole;
+}
 
 inline int padded_dim(int d) { return d <= 64 ? 64 : d <= 96 ? 96 : d <= 128 ? 128 : 256; }
 
@@ -286,14 +294,14 @@ int slot_rows(int64_t tokens, int64_t group) {
 // are they more than every tile's most.
 template <class P = Tiles32>
 int64_t slots_bound(int64_t tokens, int64_t seqs, int64_t group, int64_t hk, int64_t max_keys) {
-  const int64_t most = tiles_bound<P>(tokens, seqs, group) * hk * ((max_keys + kChunkMin - 1) / kChunkMin);
+  const int64_t most = tiles_bound<P>(tokens, seqs, group) * hk * ((max_keys + P::kLeast - 1) / P::kLeast);
   const int64_t aim = P::kTarget + P::kTarget / 3 + 1 + hk;
   return most < aim ? most : aim;
 }
 
 template <class P = Tiles32>
 size_t workspace_bytes(int64_t tokens, int64_t seqs, int64_t hq, int64_t hk, int64_t d, int64_t max_keys) {
-  if (tokens <= 0 || seqs <= 0 || hk <= 0 || hq % hk != 0 || d <= 0 || d > 256 || !may_split(max_keys)) return 0;
+  if (tokens <= 0 || seqs <= 0 || hk <= 0 || hq % hk != 0 || d <= 0 || d > 256 || !may_split<P>(max_keys)) return 0;
   const int64_t group = hq / hk;
   return static_cast<size_t>(slots_bound<P>(tokens, seqs, group, hk, max_keys)) * slot_rows<P>(tokens, group) *
          (padded_dim(static_cast<int>(d)) + 2) * sizeof(float);
@@ -314,7 +322,7 @@ bool plan_launch(Args& a, Launch& n) {
   a.group = Div::of(group);
   a.resident = kCus * P::workgroups_a_cu(padded_dim(a.d));
   a.target = 2 * a.resident;
-  a.chunk_min = kChunkMin;
+  a.chunk_min = P::kLeast;
   a.ws_rows = slot_rows<P>(a.tokens, group);
   const int64_t tiles = tiles_bound<P>(a.tokens, a.seqs, group);
   n.index = tiles;
@@ -323,7 +331,7 @@ bool plan_launch(Args& a, Launch& n) {
   a.slots = 0;
   if (n.workspace > 0) {
     a.slots = static_cast<int>(slots_bound<P>(a.tokens, a.seqs, group, hk, a.max_keys) / hk);
-    const int64_t most = tiles * ((a.max_keys + kChunkMin - 1) / kChunkMin - 1), aim = P::kTarget / hk + 1;
+    const int64_t most = tiles * ((a.max_keys + P::kLeast - 1) / P::kLeast - 1), aim = P::kTarget / hk + 1;
     n.index += most < aim ? most : aim;
     const int64_t units = static_cast<int64_t>(a.tokens) * group, wanted = kMergeGrid / hk + 1;
     n.merges = units < wanted ? units : wanted;
