@@ -49,7 +49,8 @@ struct FewTiles {
   // table of 300 or 600 positions 17 us, now 12.)
   static constexpr int kWhole = kLeast + kLeast / 2 - 1;
   // By the registers of attention8_few_kernel, a workgroup's four waves on the four SIMDs. (128 columns and 16 rows with room for
-  // four: what the compiler puts aside in the loop is waited for with the loads, a decode batch 162 us in place of 119.)
+  // four: what the compiler puts aside in the loop is waited for with the loads, a decode batch 162 us in place of 119. 64 columns and 32
+  // or 48 rows would have room for three: planned so, verify rounds of 6 and of 24 sequences take the same, 24.4, 27.4 and 25.4 us.)
   __host__ __device__ static constexpr int workgroups_a_cu(int padded) {
     return RB == 1 ? (padded > 128 ? 2 : padded > 64 ? 3 : 4) : padded > 128 ? 1 : 2;
   }
@@ -128,9 +129,10 @@ __device__ __forceinline__ int scan_add(int v) {
 }
 
 // Keys of a split: the whole work in keys x tiles over the workgroups that the card holds at once, where the parts are no more
-// than those; else over `target`, so that ragged parts share the card evenly; never under chunk_min. (A verify round of 36 rows
-// over 41k keys: 39 us in 480 parts, 53 in 660; a decode batch of 64 ragged sequences: 219 us by the first rule, 204 to 210 by
-// the second.) Every workgroup adds the same numbers in the same order, so all of them find the same value.
+// than those (P::kFit); else over `target`, so that ragged parts share the card evenly; never under chunk_min, by `target` with
+// kFit not under kSharedMin. (A verify round of 36 rows over 41k keys: 39 us in 480 parts, 53 in 660; a decode batch of 64
+// ragged sequences: 219 us by the first rule, 204 to 210 by the second.) Every workgroup adds the same numbers in the same
+// order, so all of them find the same value.
 template <class P>
 __device__ __forceinline__ int split_keys(const Args& a, const Seq& own, int lane) {
   float units = 0.f;

@@ -11,7 +11,8 @@ The cache holds 16-bit values, or (with k_scales and v_scales) 8 bits: pages of 
 a page's positions and each head a power of two, float8_e8m0fnu [pages, blocks of a page, Hk]; a value is code x scale. The append
 takes the least power of two that all new values of a block fit under (448 times it for e4m3, 127 times it for int8); where a
 block holds earlier positions it never lowers their scale, and rounds their codes again when it grows. int8 holds normally
-distributed keys and values about three times as exactly as e4m3 does; e4m3 holds small values beside large ones.
+distributed keys and values about twice as exactly as e4m3 does (1.8 to 2.9 times, by where a block's greatest lies between two powers
+of two); e4m3 holds small values beside large ones.
 
 Offsets, lengths and page tables are int32 tensors on the GPU that the kernels read: the calls neither copy nor synchronise,
 and one captured graph serves whatever the tensors hold when it is replayed. bf16 or fp16, softmax and sums in fp32; any
