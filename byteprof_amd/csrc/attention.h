@@ -36,6 +36,7 @@ struct Bf16 {
     typedef float f2 __attribute__((ext_vector_type(2)));
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2){x, y}, bf16x2));
   }
+  static __device__ __forceinline__ uint32_t result(float x, float y) { return pack(x, y); }
 };
 struct F16 {
   static __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
@@ -45,6 +46,10 @@ struct F16 {
     typedef _Float16 h2 __attribute__((ext_vector_type(2)));
     return __builtin_bit_cast(uint32_t, (h2){static_cast<_Float16>(x), static_cast<_Float16>(y)});
   }
+  // The mean of values near fp16's greatest is no more than that, but rounded probabilities may add up to 1 + 2^-11, and from
+  // 65504 (1 + 2^-12) on a result would be infinite. Infinities (of infinite values) stay.
+  static __device__ __forceinline__ float finite(float x) { return fabsf(x) < INFINITY ? fminf(fmaxf(x, -65504.f), 65504.f) : x; }
+  static __device__ __forceinline__ uint32_t result(float x, float y) { return pack(finite(x), finite(y)); }
 };
 
 // LDS images of key and value rows: [row][DP / 8] chunks of 16 bytes, the chunk of a row at a place that the row turns, so

@@ -333,7 +333,7 @@ __device__ __forceinline__ void merge_rows(const Args& a, const Item& it, int kv
     }
     const float inv = inverse(sum);
     *reinterpret_cast<u32x2*>(out_row(a, it, kvh, it.row0 + row) + col) =
-        u32x2{T::pack(o[0] * inv, o[1] * inv), T::pack(o[2] * inv, o[3] * inv)};
+        u32x2{T::result(o[0] * inv, o[1] * inv), T::result(o[2] * inv, o[3] * inv)};
   }
 }
 
@@ -394,7 +394,7 @@ __global__ __launch_bounds__(kThreads) void merge_kernel(Args a) {
       }
       const float inv = inverse(sum);
       *reinterpret_cast<u32x2*>(out_row(a, it, kvh, it.row0 + row) + 4 * piece) =
-          u32x2{T::pack(o[0] * inv, o[1] * inv), T::pack(o[2] * inv, o[3] * inv)};
+          u32x2{T::result(o[0] * inv, o[1] * inv), T::result(o[2] * inv, o[3] * inv)};
     }
   }
 }

@@ -63,8 +63,8 @@ __device__ __forceinline__ void write_rows(const Args& a, const Item& it, int kv
         u32x2 x, y;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          x[e] = T::pack(r.o[db][8 * i + 2 * e] * inv, r.o[db][8 * i + 2 * e + 1] * inv);
-          y[e] = T::pack(r.o[db][8 * i + 4 + 2 * e] * inv, r.o[db][8 * i + 4 + 2 * e + 1] * inv);
+          x[e] = T::result(r.o[db][8 * i + 2 * e] * inv, r.o[db][8 * i + 2 * e + 1] * inv);
+          y[e] = T::result(r.o[db][8 * i + 4 + 2 * e] * inv, r.o[db][8 * i + 4 + 2 * e + 1] * inv);
         }
         const auto w0 = __builtin_amdgcn_permlane32_swap(x[0], y[0], false, false);
         const auto w1 = __builtin_amdgcn_permlane32_swap(x[1], y[1], false, false);
@@ -142,7 +142,7 @@ __device__ __forceinline__ void join_waves(const Args& a, const Item& it, int kv
         const float inv = stats[32 * 2 * kWaves + row];
         if (col < a.d)
           *reinterpret_cast<u32x2*>(out_row(a, it, kvh, it.row0 + row) + col) =
-              u32x2{T::pack(x[0] * inv, x[1] * inv), T::pack(x[2] * inv, x[3] * inv)};
+              u32x2{T::result(x[0] * inv, x[1] * inv), T::result(x[2] * inv, x[3] * inv)};
       } else if (keep) {
         *reinterpret_cast<f32x4*>(ws + row * DP + col) = x;
       }
