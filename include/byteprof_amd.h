@@ -481,9 +481,8 @@ typedef struct BpPagedCache {
  * keys and values have pages and scales of their own.
  *
  * paged8 (a cache in 8 bits): bp_attn_paged over codes, which become values of q's dtype exactly (BP_DT_F16: rounded once below its normal
- * values, its greatest, 65504, where they are past its range, but I8 keys past it may count as 65536. BP_DT_BF16: past its range they
- * are infinite, and so, or NaN, is what sees them). In BP_DT_BF16, I8 codes are multiplied with the queries before their scale: |q| below
- * 2^112.
+ * values, its greatest, 65504, where they are past its range, but I8 keys past it may count as 65536. BP_DT_BF16: what sees a value past
+ * bf16's range may be infinite or NaN). In BP_DT_BF16, I8 codes are multiplied with the queries before their scale: |q| below 2^112.
  * A NaN among a sequence's own tokens' values may reach the rows of its earlier tokens, as in a cache in 16 bits.
  * block a multiple of 4; the codes' bases and the strides of dimensions of more than one entry multiples of 8. workspace:
  * bp_attn_paged8_workspace_bytes(tokens, seqs, hq, hk, head_dim, page x max_pages), 16-byte aligned.
